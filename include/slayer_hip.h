@@ -633,6 +633,65 @@ int slayer_rf_limit(float *sin_decay, float *cos_decay, float gain_max, int64_t 
 int slayer_quantize_bwd(float *grad_in, const float *grad_out, const unsigned char *inside, float scale, int64_t n,
                         void *stream);
 
+/* ---- token mixing: leaky attention, group norm, dropout ---------------------------------------- */
+/* Not in the reference.  Tensors of float32 or bfloat16 (`dtype`), statistics and states float32. */
+
+#define SLAYER_FLOAT32  0
+#define SLAYER_BFLOAT16 1
+
+/* Leaky attention: for every sample and head, with a = 1 - decay / 4096,
+ *     S[t] = a S[t-1] + key[t] (outer) value[t],   out[t] = scale * query[t] S[t],
+ * S [keys][values], S[-1] = state.  query and key are [samples][tokens][heads][keys], value [samples][tokens][heads][values], with
+ * strides (in elements) of their first three axes and neighbouring elements on the last; out and the gradients are contiguous.
+ * Sample n has lengths[n] tokens: those behind it are not read, their outputs and gradients are 0, its last state is the one behind
+ * its last token (state itself for no tokens). */
+typedef struct slayer_attention {
+    int64_t samples, tokens, heads, keys, values;   /* keys and values up to 128 */
+    int64_t num_decays;                             /* 1 or heads */
+    const float *decay;
+    const void *lengths;                            /* samples integers on the device, or NULL: all of `tokens` */
+    int lengths_bytes;                              /* 4 or 8 */
+    int dtype;
+    double scale;
+    int64_t query_stride[3], key_stride[3], value_stride[3], grad_stride[3];   /* sample, token, head; grad_stride: of grad_out */
+} slayer_attention;
+
+/* Floats of workspace for a forward or a backward call, or a negative SLAYER_E*. */
+int64_t slayer_leaky_attention_workspace(const slayer_attention *a, int backward);
+/* state, last: [samples][heads][keys][values] floats or NULL (zeros; not wanted) */
+int slayer_leaky_attention_fwd(void *out, float *last, const void *query, const void *key, const void *value, const float *state,
+                               const slayer_attention *a, float *workspace, int64_t workspace_floats, void *stream);
+/* Gradients from those of out and of last (NULL: 0).  Any result may be NULL, grad_value only where grad_state is.  grad_decay:
+ * num_decays floats, the derivative with respect to the decay itself (the -1 / 4096 of a is in it). */
+int slayer_leaky_attention_bwd(void *grad_query, void *grad_key, void *grad_value, float *grad_decay, float *grad_state,
+                               const void *grad_out, const float *grad_last, const void *query, const void *key, const void *value,
+                               const float *state, const slayer_attention *a, float *workspace, int64_t workspace_floats, void *stream);
+/* One token a sample (tokens and the token strides are not looked at): state is updated in place. */
+int slayer_leaky_attention_step(void *out, float *state, const void *query, const void *key, const void *value,
+                                const slayer_attention *a, void *stream);
+
+/* Group norm with the channels last and an activation behind it, on contiguous [samples][pixels][channels]: groups of
+ * channels / groups neighbouring channels over all pixels of a sample, out = act((in - mean) * scale * weight + bias),
+ * scale = 1 / sqrt(var + eps).  weight, bias: channels floats or NULL (1, 0).  mean, scale: samples * groups floats for the backward
+ * call; both may be NULL where pixels is 1 and a group has at most 2048 (float32) or 4096 channels.
+ * activation: 0 none, 1 relu, 2 silu, 3 gelu (with the error function). */
+int64_t slayer_group_norm_workspace(int dtype, int64_t samples, int64_t pixels, int64_t channels, int64_t groups, int backward);
+int slayer_group_norm_fwd(void *out, float *mean, float *scale, const void *in, const float *weight, const float *bias, int dtype,
+                          int64_t samples, int64_t pixels, int64_t channels, int64_t groups, float eps, int activation,
+                          float *workspace, int64_t workspace_floats, void *stream);
+/* grad_weight, grad_bias: channels floats or NULL */
+int slayer_group_norm_bwd(void *grad_in, float *grad_weight, float *grad_bias, const void *grad_out, const void *in,
+                          const float *mean, const float *scale, const float *weight, const float *bias, int dtype,
+                          int64_t samples, int64_t pixels, int64_t channels, int64_t groups, int activation,
+                          float *workspace, int64_t workspace_floats, void *stream);
+
+/* Dropout with a mask that is a function of (seed, offset, index): out = keep ? in * scale : 0.  Decision i is half word i % 8 of
+ * the 128 bits of Philox-4x32-10 with key seed and counter (i / 8, offset), and says keep at or above `limit` (0 ... 65536).
+ * steps 0: a decision for each of the n elements; otherwise one for each `steps` neighbouring ones (a neuron's time steps).  The
+ * gradient is the same call on grad_out. */
+int slayer_dropout(void *out, const void *in, int dtype, int64_t n, int64_t steps, int limit, float scale, uint64_t seed,
+                   uint64_t offset, void *stream);
+
 /* ---- cross-check implementations (debug mode) ------------------------------------------------ */
 
 /* The reference's debug mode runs its CPU loop next to its kernel and raises on a difference

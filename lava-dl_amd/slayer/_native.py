@@ -36,6 +36,18 @@ class Delays(ctypes.Structure):
 
 _DP = ctypes.POINTER(Delays)
 
+
+class Attention(ctypes.Structure):
+    """struct slayer_attention of include/slayer_hip.h (device pointers as integers)."""
+    _fields_ = [('samples', _I64), ('tokens', _I64), ('heads', _I64), ('keys', _I64), ('values', _I64),
+                ('num_decays', _I64), ('decay', _P), ('lengths', _P), ('lengths_bytes', _INT), ('dtype', _INT),
+                ('scale', _D), ('query_stride', _I64 * 3), ('key_stride', _I64 * 3), ('value_stride', _I64 * 3),
+                ('grad_stride', _I64 * 3)]
+
+
+_AP = ctypes.POINTER(Attention)
+_U64 = ctypes.c_uint64
+
 _SIGNATURES = {
     'slayer_abi_version': (_INT, []),
     'slayer_error_string': (ctypes.c_char_p, [_INT]),
@@ -88,6 +100,14 @@ _SIGNATURES = {
     'slayer_rf_limit': (_INT, [_P] * 2 + [_F, _I64, _P]),
     'slayer_quantize_bwd': (_INT, [_P] * 3 + [_F, _I64, _P]),
     'slayer_recurrent_steps_bwd': (_INT, [_P] * 5 + [_F, _F, _F, _INT] + [_I64] * 3 + [_P, _I64, _P]),
+    'slayer_leaky_attention_workspace': (_I64, [_AP, _INT]),
+    'slayer_leaky_attention_fwd': (_INT, [_P] * 6 + [_AP, _P, _I64, _P]),
+    'slayer_leaky_attention_bwd': (_INT, [_P] * 11 + [_AP, _P, _I64, _P]),
+    'slayer_leaky_attention_step': (_INT, [_P] * 5 + [_AP, _P]),
+    'slayer_group_norm_workspace': (_I64, [_INT] + [_I64] * 4 + [_INT]),
+    'slayer_group_norm_fwd': (_INT, [_P] * 6 + [_INT] + [_I64] * 4 + [_F, _INT, _P, _I64, _P]),
+    'slayer_group_norm_bwd': (_INT, [_P] * 9 + [_INT] + [_I64] * 4 + [_INT, _P, _I64, _P]),
+    'slayer_dropout': (_INT, [_P, _P, _INT, _I64, _I64, _INT, _F, _U64, _U64, _P]),
     'slayer_li_fwd_naive': (_INT, [_P, _P, _P, _P, _D, _INT, _I64, _I64, _I64, _I64, _I64, _P]),
     'slayer_li_bwd_naive': (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _P]),
     'slayer_ath_fwd_naive': (_INT, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _INT,
@@ -216,6 +236,28 @@ def require_gpu(*tensors):
         elif t.device != dev:
             raise RuntimeError(f'tensors on different devices: {dev} and {t.device}')
     return dev
+
+
+#: The types of the token-mixing operators, as slayer_hip.h numbers them.
+ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def require_elements(*tensors):
+    """``require_gpu`` for the operators that also take bfloat16: (device, number of the type all tensors share)."""
+    first = tensors[0]
+    for t in tensors:
+        if not torch.is_tensor(t):
+            raise RuntimeError(f'expected a tensor, got {type(t)}')
+        if not t.is_cuda:
+            raise RuntimeError('slayer HIP kernels need tensors on an MI355X device; '
+                               'there is no CPU implementation in this package')
+        if t.dtype not in ELEMENT_TYPES:
+            raise RuntimeError(f'expected a float32 or bfloat16 tensor, got {t.dtype}')
+        if t.dtype != first.dtype:
+            raise RuntimeError(f'tensors of different types: {first.dtype} and {t.dtype}')
+        if t.device != first.device:
+            raise RuntimeError(f'tensors on different devices: {first.device} and {t.device}')
+    return first.device, ELEMENT_TYPES[first.dtype]
 
 
 def scan_tolerance(grad):

@@ -3,6 +3,7 @@ and ``neuron_params``), the dynamics operators they are built from, and the norm
 can be given."""
 from . import dynamics, cuba, alif, rf, rf_iz, adrf, adrf_iz, sigma_delta
 from . import norm
-from .dropout import Dropout
+from .dropout import Dropout, CounterDropout, counter_dropout
 
-__all__ = ['dynamics', 'cuba', 'alif', 'rf', 'rf_iz', 'adrf', 'adrf_iz', 'sigma_delta', 'norm', 'Dropout']
+__all__ = ['dynamics', 'cuba', 'alif', 'rf', 'rf_iz', 'adrf', 'adrf_iz', 'sigma_delta', 'norm', 'Dropout',
+           'CounterDropout', 'counter_dropout']

@@ -1,6 +1,9 @@
-"""Neuron dropout (counterpart of neuron/dropout.py:10-35 in the reference)."""
+"""Neuron dropout (counterpart of neuron/dropout.py:10-35 in the reference), and dropout whose mask comes from a counter
+and is never stored (slayer_dropout of libslayer_hip.so)."""
 import torch
 import torch.nn.functional as F
+
+from .. import _native as N
 
 
 class Dropout(torch.nn.Dropout3d):
@@ -11,3 +14,80 @@ class Dropout(torch.nn.Dropout3d):
         shape = input.shape
         per_neuron = input.reshape((shape[0], -1, 1, 1, shape[-1]))       # one channel per neuron, time last
         return F.dropout3d(per_neuron, self.p, self.training, self.inplace).reshape(shape)
+
+
+def counter_dropout(input, p, seed, offset=0, per_neuron=False):
+    """Sets elements of ``input`` to zero with probability ``p`` and scales the others by the inverse of the share that
+    stays.  Which ones is a function of ``seed``, ``offset`` and an element's place alone: the same call gives the same
+    mask again, on any layout and for either type, and the backward pass works it out anew instead of keeping it.
+
+    Parameters
+    ----------
+    input : torch.Tensor
+        float32 or bfloat16 GPU tensor of any shape.
+    p : float
+        probability in [0, 1], rounded to a multiple of 1/65536: a decision takes sixteen bits of the generator
+        (Philox-4x32 with ten rounds).  The scale is the inverse of what the rounded probability leaves.
+    seed, offset : int
+        0 <= seed, offset < 2**64.  Different offsets give masks that have nothing to do with each other: count it up
+        from call to call.  A captured graph replays the numbers it was captured with.
+    per_neuron : bool
+        one decision for all elements along the last axis (the time steps of a neuron).
+
+    Returns
+    -------
+    torch.Tensor, contiguous, of the shape and type of ``input``.
+    """
+    if not 0 <= p <= 1:
+        raise ValueError(f'dropout probability has to be between 0 and 1, got {p}')
+    if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
+        raise ValueError(f'seed and offset have to be between 0 and 2**64 - 1, got {seed} and {offset}')
+    if per_neuron and torch.is_tensor(input) and input.dim() == 0:
+        raise RuntimeError('per_neuron needs an axis of time steps, got a tensor without axes')
+    if N.wants_grad(input):
+        return _CounterDropout.apply(input, float(p), int(seed), int(offset), bool(per_neuron))
+    return _dropout(input, float(p), int(seed), int(offset), bool(per_neuron))
+
+
+def _dropout(input, p, seed, offset, per_neuron):
+    device, dtype = N.require_elements(input)
+    input = input.contiguous()
+    out = torch.empty_like(input)
+    limit = round(p * 65536)
+    scale = 65536 / (65536 - limit) if limit < 65536 else 0.0
+    with N.device_guard(device):
+        N.check(N.lib().slayer_dropout(N.ptr(out), N.ptr(input), dtype, input.numel(), input.shape[-1] if per_neuron else 0,
+                                       limit, scale, seed, offset, N.stream_handle()))
+    return out
+
+
+class _CounterDropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, input, p, seed, offset, per_neuron):
+        ctx.args = (p, seed, offset, per_neuron)
+        return _dropout(input, *ctx.args)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        p, seed, offset, per_neuron = ctx.args
+        return counter_dropout(grad_output, p, seed, offset, per_neuron), None, None, None, None
+
+
+class CounterDropout(torch.nn.Module):
+    """:func:`counter_dropout` while training, the identity otherwise.  ``offset`` counts the calls made while training;
+    set it (and ``seed``) to repeat them."""
+
+    def __init__(self, p=0.5, seed=0, per_neuron=False):
+        super().__init__()
+        if not 0 <= p <= 1:
+            raise ValueError(f'dropout probability has to be between 0 and 1, got {p}')
+        self.p, self.seed, self.per_neuron, self.offset = p, seed, per_neuron, 0
+
+    def forward(self, input):
+        if not self.training or self.p == 0:
+            return input
+        self.offset += 1
+        return counter_dropout(input, self.p, self.seed, self.offset - 1, self.per_neuron)
+
+    def extra_repr(self):
+        return f'p={self.p}, seed={self.seed}, per_neuron={self.per_neuron}'

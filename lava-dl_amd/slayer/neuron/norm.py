@@ -3,8 +3,13 @@
 
 Plain torch modules, as in the reference: they run once per call on the [N, C, ..., T] tensor and are not part
 of the time-sequential kernels.  A neuron that is given one of them hooks its weight quantiser into
-``pre_hook_fx`` (neuron/base.py:127-141 in the reference)."""
+``pre_hook_fx`` (neuron/base.py:127-141 in the reference).
+
+``group_norm`` and ``GroupNorm`` are for tensors with the channels last (tokens, images) and run in slayer_group_norm_fwd / bwd
+of libslayer_hip.so."""
 import torch
+
+from .. import _native as N
 
 
 def _identity(x, descale=False):
@@ -94,3 +99,124 @@ class WgtScaleBatchNorm(_FeatureNorm):
         else:
             var = self.running_var
         return (inp - self.pre_hook_fx(self._per_feature(mean, inp))) / self._per_feature(self.std(var), inp)
+
+
+ACTIVATIONS = {None: 0, 'none': 0, 'relu': 1, 'silu': 2, 'gelu': 3}
+
+
+def group_norm(input, num_groups, weight=None, bias=None, eps=1e-5, activation=None):
+    """Group norm over the last axis with an activation behind it, in one operator: for each sample (first axis) the
+    channels (last axis) are cut into ``num_groups`` groups of neighbours; a group is normalised over its channels and
+    all positions between first and last axis, scaled, shifted and activated.
+
+    Parameters
+    ----------
+    input : torch.Tensor
+        float32 or bfloat16 GPU tensor [N, ..., C].
+    num_groups : int
+        divides C.
+    weight, bias : torch.Tensor or None
+        C floating-point values each; None: 1 and 0.
+    eps : float
+    activation : None, 'none', 'relu', 'silu' or 'gelu' (with the error function)
+
+    Returns
+    -------
+    torch.Tensor, contiguous, of the shape and type of ``input``.  Statistics, weights and their gradients are float32.
+    """
+    if activation not in ACTIVATIONS:
+        raise ValueError(f'unknown activation {activation!r}: one of {list(ACTIVATIONS)}')
+    N.require_elements(input)
+    if input.dim() < 2:
+        raise RuntimeError(f'expected a tensor [N, ..., C], got {input.dim()} axes')
+    channels = input.shape[-1]
+    if num_groups < 1 or channels < 1 or channels % num_groups:
+        raise RuntimeError(f'{channels} channels cannot be cut into {num_groups} groups')
+    if not eps >= 0:
+        raise ValueError(f'eps has to be at least 0, got {eps}')
+    for name, t in (('weight', weight), ('bias', bias)):
+        if t is not None:
+            if not torch.is_tensor(t) or t.shape != (channels,) or not t.is_floating_point():
+                raise RuntimeError(f'{name}: expected {channels} floating-point values')
+            if t.device != input.device:
+                raise RuntimeError(f'tensors on different devices: {input.device} and {t.device}')
+    weight = weight if weight is None else weight.float().contiguous()
+    bias = bias if bias is None else bias.float().contiguous()
+    code = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, weight, bias)):
+        return _GroupNorm.apply(input, weight, bias, num_groups, eps, code)
+    return _norm_fwd(input.contiguous(), weight, bias, num_groups, eps, code, False)[0]
+
+
+def _norm_sizes(input, groups):
+    n, c = input.shape[0], input.shape[-1]
+    return n, (input.numel() // (n * c) if n else 0), c, groups
+
+
+def _norm_fwd(input, weight, bias, groups, eps, activation, keep):
+    dtype = N.ELEMENT_TYPES[input.dtype]
+    sizes = _norm_sizes(input, groups)
+    lib = N.lib()
+    floats = lib.slayer_group_norm_workspace(dtype, *sizes, 0)
+    if floats < 0:
+        N.check(int(floats))
+    out = torch.empty_like(input)
+    mean = scale = workspace = None
+    if keep or floats:
+        stats = torch.empty(2 * sizes[0] * groups + floats, dtype=torch.float32, device=input.device)
+        mean, scale, workspace = stats.split((sizes[0] * groups, sizes[0] * groups, floats))
+    with N.device_guard(input.device):
+        N.check(lib.slayer_group_norm_fwd(N.ptr(out), N.ptr(mean), N.ptr(scale), N.ptr(input), N.ptr(weight), N.ptr(bias),
+                                          dtype, *sizes, eps, activation, N.ptr(workspace), floats, N.stream_handle()))
+    return out, mean, scale
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, input, weight, bias, groups, eps, activation):
+        input = input.contiguous()
+        out, mean, scale = _norm_fwd(input, weight, bias, groups, eps, activation, True)
+        ctx.save_for_backward(input, weight, bias, mean, scale)
+        ctx.args = (groups, activation)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_output):
+        input, weight, bias, mean, scale = ctx.saved_tensors
+        groups, activation = ctx.args
+        grad_output = grad_output.contiguous()
+        dtype, sizes = N.ELEMENT_TYPES[input.dtype], _norm_sizes(input, groups)
+        grad = torch.empty_like(input)
+        wanted = [torch.empty_like(t) if t is not None and need else None
+                  for t, need in ((weight, ctx.needs_input_grad[1]), (bias, ctx.needs_input_grad[2]))]
+        lib = N.lib()
+        floats = lib.slayer_group_norm_workspace(dtype, *sizes, 1)
+        if floats < 0:
+            N.check(int(floats))
+        workspace = torch.empty(floats, dtype=torch.float32, device=input.device)
+        with N.device_guard(input.device):
+            N.check(lib.slayer_group_norm_bwd(N.ptr(grad), N.ptr(wanted[0]), N.ptr(wanted[1]), N.ptr(grad_output),
+                                              N.ptr(input), N.ptr(mean), N.ptr(scale), N.ptr(weight), N.ptr(bias), dtype,
+                                              *sizes, activation, N.ptr(workspace), floats, N.stream_handle()))
+        return grad, wanted[0], wanted[1], None, None, None
+
+
+class GroupNorm(torch.nn.Module):
+    """:func:`group_norm` with a trained weight and bias for each channel (``affine=False``: without)."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation=None):
+        super().__init__()
+        if num_groups < 1 or num_channels < 1 or num_channels % num_groups:
+            raise ValueError(f'{num_channels} channels cannot be cut into {num_groups} groups')
+        if activation not in ACTIVATIONS:
+            raise ValueError(f'unknown activation {activation!r}: one of {list(ACTIVATIONS)}')
+        self.num_groups, self.num_channels, self.eps, self.activation = num_groups, num_channels, eps, activation
+        self.weight = torch.nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = torch.nn.Parameter(torch.zeros(num_channels)) if affine else None
+
+    def forward(self, input):
+        return group_norm(input, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+
+    def extra_repr(self):
+        return f'{self.num_groups}, {self.num_channels}, eps={self.eps}, activation={self.activation}'
