@@ -661,11 +661,13 @@ int64_t slayer_leaky_attention_workspace(const slayer_attention *a, int backward
 /* state, last: [samples][heads][keys][values] floats or NULL (zeros; not wanted) */
 int slayer_leaky_attention_fwd(void *out, float *last, const void *query, const void *key, const void *value, const float *state,
                                const slayer_attention *a, float *workspace, int64_t workspace_floats, void *stream);
-/* Gradients from those of out and of last (NULL: 0).  Any result may be NULL, grad_value only where grad_state is.  grad_decay:
- * num_decays floats, the derivative with respect to the decay itself (the -1 / 4096 of a is in it). */
+/* Gradients from those of out and of last (NULL: 0).  Any result may be NULL, but grad_value only where grad_state is and
+ * grad_query only where grad_decay is.  grad_decay: num_decays floats, the derivative with respect to the decay itself (the
+ * -1 / 4096 of a is in it).  starts: the workspace of the forward call as that left it, or NULL. */
 int slayer_leaky_attention_bwd(void *grad_query, void *grad_key, void *grad_value, float *grad_decay, float *grad_state,
                                const void *grad_out, const float *grad_last, const void *query, const void *key, const void *value,
-                               const float *state, const slayer_attention *a, float *workspace, int64_t workspace_floats, void *stream);
+                               const float *state, const float *starts, const slayer_attention *a, float *workspace,
+                               int64_t workspace_floats, void *stream);
 /* One token a sample (tokens and the token strides are not looked at): state is updated in place. */
 int slayer_leaky_attention_step(void *out, float *state, const void *query, const void *key, const void *value,
                                 const slayer_attention *a, void *stream);

@@ -1,0 +1,524 @@
+// The kernel of leaky attention (attention.hip says what it computes), for attention_f32.hip and attention_bf16.hip.
+#pragma once
+#include "common.h"
+#include "elements.h"
+#include <type_traits>
+
+namespace slayer {
+
+constexpr int kChunk = 64;
+
+// One pass of the recurrence, as its kernels see it.  `query`, `key`, `value` are the tensors in the three places.
+struct LeakyPass {
+    void* out;
+    const void *query, *key, *value;
+    const float* decay;
+    const void* lengths;
+    const float* first;            // [samples][heads] states with strides first_k, first_v, or nullptr: zeros
+    float* starts;                 // states in front of the segments, [samples * heads][segments] of them
+    float* last;                   // state behind the last token, or nullptr
+    float* slope_starts;           // LEAKY_SLOPE: derivatives of the states in `starts`
+    const float* grad_last;        // LEAKY_SLOPE: gradient of the last state, or nullptr
+    const void* other;             // LEAKY_SLOPE: what the derivative of the results is multiplied with, laid out as they are
+    double* slopes;                // LEAKY_SLOPE: [samples][heads][segments][slices]
+    int64_t out_n, out_t, out_h, query_n, query_t, query_h, key_n, key_t, key_h, value_n, value_t, value_h, other_n, other_t, other_h;
+    int tokens, heads, keys, values, state_k, state_v;      // the strides of a state's axes
+    int units;                     // samples * heads
+    int one_decay, lengths64, segments, segment, slices, backwards;
+    int whole_out;                 // four results are a multiple of their size apart from the tensor's start
+    float out_scale, key_scale;    // of the results; of what `key` stands for, in scores and in the state
+};
+
+// ---- fragments of the matrix instructions.  A fragment holds kDepth terms of a product for 16 rows (or columns): lane l has
+// row l % 16 and, with g = l / 16,
+//   float32 : terms 4g ... 4g+3 of 16, one v_mfma_f32_16x16x4_f32 for each of the four;
+//   bfloat16: eight of 32, for one v_mfma_f32_16x16x32_bf16: 8g ... 8g+7 where both operands lie along the terms in LDS, or
+//             4g ... 4g+3 and 16+4g ... 16+4g+3 ("halves") where one of them is a pair of results (whose lane l has rows
+//             4g ... 4g+3 of column l % 16 of a 16 x 16 tile) or is read across its rows.
+template <typename T> struct Frag;
+template <> struct Frag<float> {
+    static constexpr int kDepth = 16;
+    typedef f4 Type;
+};
+template <> struct Frag<bf16> {
+    static constexpr int kDepth = 32;
+    typedef b8 Type;
+};
+__device__ __forceinline__ f4 mma(f4 a, f4 b, f4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ f4 mma(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// terms along the row of `tile`
+template <typename T>
+__device__ __forceinline__ typename Frag<T>::Type along(const T* tile, int pitch, int row, int term) {
+    const int lane = threadIdx.x & 63;
+    return *reinterpret_cast<const typename Frag<T>::Type*>(tile + (row + (lane & 15)) * pitch + term + (lane >> 4) * Elements<T>::kVec);
+}
+// terms across the rows of `tile`, the sixteen columns from `column` on
+__device__ __forceinline__ f4 across(const float* tile, int pitch, int column, int term) {
+    const int lane = threadIdx.x & 63;
+    const float* p = tile + (term + (lane >> 4) * 4) * pitch + column + (lane & 15);
+    return f4{p[0], p[pitch], p[2 * pitch], p[3 * pitch]};
+}
+typedef __attribute__((address_space(3))) short LdsShort;
+typedef short s4 __attribute__((ext_vector_type(4)));
+// ds_read_b64_tr_b16: the sixteen lanes of a group read four rows of sixteen columns, lane i gets column i of the four
+__device__ __forceinline__ b8 across(const bf16* tile, int pitch, int column, int term) {
+    const int lane = threadIdx.x & 63, i = lane & 15;
+    const bf16* p = tile + (term + (lane >> 4) * 4 + (i >> 2)) * pitch + column + (i & 3) * 4;
+    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(LdsShort*)p);
+    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(LdsShort*)(p + 16 * pitch));
+    const b4 a = __builtin_bit_cast(b4, lo), b = __builtin_bit_cast(b4, hi);
+    return b8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// A float32 operand: in float32, or as bfloat16 numbers that sum to it, so that what the kernel makes itself is not rounded to
+// the type of the tensors on the way: two for scores and states, which end in a result of that type (within 2^-17, a hundredth of
+// what rounding the result costs), three for the leaked keys, which end in a float32 state (within 2^-25).
+template <int PARTS> struct Split { b8 part[PARTS]; };
+template <int PARTS>
+__device__ __forceinline__ Split<PARTS> split(f8 v) {
+    Split<PARTS> o;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        o.part[i] = __builtin_convertvector(v, b8);
+        if (i + 1 < PARTS) v -= __builtin_convertvector(o.part[i], f8);
+    }
+    return o;
+}
+
+__device__ __forceinline__ double power(double a, int n) {
+    double p = 1;
+    for (; n > 0; n >>= 1) {
+        if (n & 1) p *= a;
+        a *= a;
+    }
+    return p;
+}
+
+__device__ __forceinline__ int sample_length(const LeakyPass& a, int n) {
+    if (!a.lengths) return a.tokens;
+    const int64_t l = a.lengths64 ? static_cast<const int64_t*>(a.lengths)[n] : static_cast<const int*>(a.lengths)[n];
+    return l < 0 ? 0 : (l > a.tokens ? a.tokens : (int)l);
+}
+
+
+enum { LEAKY_STATE, LEAKY_MAIN, LEAKY_STATE_SLOPE, LEAKY_SLOPE };
+
+// a^n and its derivative n a^(n-1); both 0 for n < 0
+__device__ __forceinline__ float power_at(const float* powers, int n) { return n >= 0 ? powers[n] : 0.f; }
+__device__ __forceinline__ float slope_at(const float* powers, int n) { return n >= 1 ? (float)n * powers[n - 1] : 0.f; }
+
+// A workgroup of four waves takes one segment of one head of one sample, chunk after chunk, and one slice of 16 VT values.
+// Wave w makes the outputs of places 16w ... 16w+15 (transposed: lane = place) and the rows of the state w, w+4, ... (16 each).
+// The first chunk is the one that is not full, with its tokens at the end, so that weights behind a token are the same in all.
+//   LEAKY_STATE: only the state, from zero, into `starts` behind the segment's place (for the segments but the last).
+//   LEAKY_SLOPE: results, and the derivative of each with respect to a, in which the state's derivative W takes the place of S:
+//       dout[i] = a^(i+1) query[i] W + (i+1) a^i query[i] S + sum over j of (i-j) a^(i-j-1) (query[i] . key[j]) value[j]
+//       W'      = a^64 W + 64 a^63 S + sum over j of (63-j) a^(62-j) key[j] (outer) value[j]
+//     of which the workgroup returns the sum of its products with `other`.  LEAKY_STATE_SLOPE: S and W from zero.
+//   WHOLE: the rows of all tensors are made of whole, aligned 16-byte pieces.
+#ifndef LEAKY_WAVES
+#define LEAKY_WAVES(T, KT, VT, MODE) 2
+#endif
+template <typename T, int KT, int VT, int MODE, bool WHOLE>
+__global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kernel(LeakyPass a) {
+    typedef typename Frag<T>::Type F;
+    typedef typename Elements<T>::Vec Vec;
+    constexpr bool MAIN = MODE == LEAKY_MAIN || MODE == LEAKY_SLOPE, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
+    constexpr int V = Elements<T>::kVec, D = Frag<T>::kDepth, P = F32 ? 1 : 2;       // parts of a state in LDS
+    constexpr int KP = KT * 16, VP = VT * 16, kPitch = KP + V, vPitch = VP + V;
+    constexpr int KV = KP / V, VV = VP / V;                                  // 16-byte pieces of a row
+    constexpr int kLoads = (kChunk * KV + 255) / 256, vLoads = (kChunk * VV + 255) / 256;
+    constexpr int ST = (KT + 3) / 4;                                         // strips of the state of a wave
+    constexpr int kStates = MAIN ? (SLOPE ? 2 : 1) : 0;                      // states in LDS
+    __shared__ __align__(16) T keys[kChunk * kPitch];
+    __shared__ __align__(16) T values[kChunk * vPitch];
+    __shared__ __align__(16) T state[kStates ? kStates * P * VP * kPitch : 8];       // transposed: [state][part][value][key]
+    __shared__ __align__(16) float powers[kChunk + 4];                       // a^i
+    __shared__ __align__(16) float behind[SLOPE ? 2 : 1][kChunk];            // what key j counts behind the chunk; its derivative
+    __shared__ double sums[4];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
+    const int segments = MAIN ? a.segments : a.segments - 1;
+    // the slices of a segment, which read the same queries and keys, eight workgroups apart: on the same XCD, with one L2
+    int slice, at_segment = blockIdx.x;
+    if (at_segment < (a.units * segments & ~7) * a.slices) {
+        slice = at_segment / 8 % a.slices;
+        at_segment = at_segment / (8 * a.slices) * 8 + at_segment % 8;
+    } else {
+        slice = at_segment % a.slices;
+        at_segment /= a.slices;
+    }
+    const int seg = at_segment % segments, unit = at_segment / segments;
+    const int n = unit / a.heads, h = unit % a.heads;
+    const int v0 = slice * VP, vleft = a.values - v0, length = sample_length(a, n);
+    const double leak = 1.0 - (double)a.decay[a.one_decay ? 0 : h] / 4096.0;
+    const int begin = seg * a.segment, end = min(begin + a.segment, a.tokens), stop = min(end, length);
+    if (!MAIN && end > length) return;                                       // no segment behind it needs this one's state
+    const int64_t state_size = (int64_t)a.keys * a.values;
+    T* out = (T*)a.out + n * a.out_n + h * a.out_h + v0;
+    if (threadIdx.x <= kChunk) powers[threadIdx.x] = (float)power(leak, threadIdx.x);
+    __syncthreads();
+    if (threadIdx.x < kChunk) {
+        const int left = kChunk - 1 - (int)threadIdx.x;
+        behind[0][threadIdx.x] = powers[left + (a.backwards ? 1 : 0)] * a.key_scale;
+        if (SLOPE) behind[SLOPE ? 1 : 0][threadIdx.x] = slope_at(powers, left);
+    }
+    const double whole_leak = power(leak, kChunk);
+    const int shift = a.backwards ? 0 : 1;
+
+    // the state, in strips of 16 keys: lane has keys 4g ... 4g+3 of column `col`
+    f4 S[ST][VT], W[SLOPE ? ST : 1][SLOPE ? VT : 1];
+    {
+        const int64_t at = ((int64_t)unit * a.segments + seg) * state_size;
+        const float* first = !MAIN ? nullptr : seg > 0 ? a.starts + at : (a.first ? a.first + unit * state_size : nullptr);
+        const float* slope_first = MODE == LEAKY_SLOPE && seg > 0 ? a.slope_starts + at : nullptr;
+#pragma unroll
+        for (int s = 0; s < ST; ++s)
+#pragma unroll
+            for (int v = 0; v < VT; ++v)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int k = (s * 4 + wave) * 16 + 4 * g + r, c = v * 16 + col;
+                    const bool on = begin <= length && k < a.keys && c < vleft;
+                    const int64_t from = (int64_t)k * a.state_k + (int64_t)(v0 + c) * a.state_v;
+                    S[s][v][r] = first && on ? first[from] : 0.f;
+                    if constexpr (SLOPE) W[s][v][r] = slope_first && on ? slope_first[from] : 0.f;
+                }
+    }
+    auto share = [&](f4 x, int which, int strip, int v) {
+        T* p = state + which * P * VP * kPitch + (v * 16 + col) * kPitch + strip * 16 + 4 * g;
+        if constexpr (F32) {
+            *reinterpret_cast<f4*>(p) = x;
+        } else {
+            const b4 hi = __builtin_convertvector(x, b4);
+            *reinterpret_cast<b4*>(p) = hi;
+            *reinterpret_cast<b4*>(p + VP * kPitch) = __builtin_convertvector(x - __builtin_convertvector(hi, f4), b4);
+        }
+    };
+
+    // What the next chunk needs, on its way.  WHOLE: a thread's pieces are an offset from the chunk's first address (the offset ~0
+    // lies outside of every buffer and reads 0); otherwise they are read element by element.
+    const int count0 = stop > begin ? (stop - begin - 1) % kChunk + 1 : 0;   // tokens of the first chunk
+    int p0 = stop > begin ? begin - (kChunk - count0) : stop;                // place of the chunk's first row
+    auto place = [&](int p) { return (int64_t)(a.backwards ? length - 1 - p : p); };
+    const T* key = (const T*)a.key + n * a.key_n + h * a.key_h;
+    const T* value = (const T*)a.value + n * a.value_n + h * a.value_h + v0;
+    const T* query = MAIN ? (const T*)a.query + n * a.query_n + h * a.query_h : nullptr;
+    Vec nk[kLoads], nv[vLoads];
+    F qf[MAIN ? KP / D : 1];
+    auto fetch = [&](auto& to, const T* base, int64_t stride, int left, int from, auto pieces) {       // rows `from` ... of the pass
+        constexpr int per = decltype(pieces)::value;
+        const int64_t low = place(a.backwards ? from + kChunk - 1 : from);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base) + low * stride, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < (kChunk * per + 255) / 256; ++i) {
+            const int at = i * 256 + threadIdx.x, row = at / per, c = at % per * V;
+            const bool on = from + row >= begin && (kChunk * per % 256 == 0 || at < kChunk * per);
+            if constexpr (WHOLE) {
+                const int off = ((a.backwards ? kChunk - 1 - row : row) * (int)stride + c) * (int)sizeof(T);
+                to[i] = __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b128(r, on && c < left ? off : -1, 0, 0));
+            } else {
+                to[i] = load_vec(base + (on ? place(from + row) : 0) * stride + c, on ? left - c : 0, false);
+            }
+        }
+    };
+    auto fetch_rows = [&](int from) {
+        fetch(nk, key, a.key_t, a.keys, from, std::integral_constant<int, KV>{});
+        fetch(nv, value, a.value_t, vleft, from, std::integral_constant<int, VV>{});
+    };
+    auto fetch_query = [&](int from) {                                       // this lane's place: row 16 wave + col
+        if constexpr (MAIN) {
+            const int row = wave * 16 + col;
+            const int64_t low = place(a.backwards ? from + kChunk - 1 : from);
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(query) + low * a.query_t, 0, 0x7fffffff, 0x00020000);
+            const bool on = from + row >= begin;
+            const int off = ((a.backwards ? kChunk - 1 - row : row) * (int)a.query_t + g * V) * (int)sizeof(T);
+#pragma unroll
+            for (int d = 0; d < KP / D; ++d) {
+                const int c = d * D + g * V;
+                if constexpr (WHOLE) qf[d] = __builtin_bit_cast(F, __builtin_amdgcn_raw_buffer_load_b128(r, on && c < a.keys ? off + d * D * (int)sizeof(T) : -1, 0, 0));
+                else qf[d] = load_vec(query + (on ? place(from + row) : 0) * a.query_t + c, on ? a.keys - c : 0, false);
+            }
+        }
+    };
+    if (stop > begin) {
+        fetch_query(p0);
+        fetch_rows(p0);
+    }
+
+    // weights of the scores: key 4g + r of the strip of this lane's place (from the place on: none), and of strips in front of it,
+    // in which a factor a^(16 strips) is left out
+    float near[4], far[4], near_slope[4], far_slope[4];
+    if (MAIN) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int back = col - 4 * g - r;
+            near[r] = power_at(powers, back) * a.key_scale;
+            far[r] = powers[16 + back] * a.key_scale;
+            if (SLOPE) {
+                near_slope[r] = slope_at(powers, back);
+                far_slope[r] = slope_at(powers, 16 + back);
+            }
+        }
+    }
+    const float apart[3] = {1.f, powers[16], powers[32]}, apart_slope[3] = {0.f, 16.f * powers[15], 32.f * powers[31]};
+    float total = 0;                                                         // LEAKY_SLOPE
+
+    for (; p0 < stop; p0 += kChunk) {
+        __syncthreads();                                                     // the chunk before is done with LDS
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = i * 256 + threadIdx.x;
+            if (kChunk * KV % 256 == 0 || at < kChunk * KV) *reinterpret_cast<Vec*>(keys + at / KV * kPitch + at % KV * V) = nk[i];
+        }
+#pragma unroll
+        for (int i = 0; i < vLoads; ++i) {
+            const int at = i * 256 + threadIdx.x;
+            if (kChunk * VV % 256 == 0 || at < kChunk * VV) *reinterpret_cast<Vec*>(values + at / VV * vPitch + at % VV * V) = nv[i];
+        }
+        if constexpr (MAIN) {
+#pragma unroll
+            for (int s = 0; s < ST; ++s) {
+                if (KT % 4 != 0 && s * 4 + wave >= KT) continue;
+#pragma unroll
+                for (int v = 0; v < VT; ++v) {
+                    share(S[s][v], 0, s * 4 + wave, v);
+                    if constexpr (SLOPE) share(W[s][v], 1, s * 4 + wave, v);
+                }
+            }
+        }
+        __syncthreads();
+        const bool more = p0 + kChunk < stop;
+        if (more) fetch_rows(p0 + kChunk);
+
+        const int missing = p0 < begin ? begin - p0 : 0;
+        const double step = missing ? power(leak, kChunk - missing) : whole_leak;
+        const float step_hi = (float)step, step_lo = (float)(step - (double)step_hi);
+        const float step_slope = SLOPE ? (float)(kChunk - missing) * powers[kChunk - 1 - missing] : 0.f;
+
+        auto chunk = [&](auto which) {
+            constexpr int w = decltype(which)::value;
+            f4 acc[VT], dacc[SLOPE ? VT : 1], scores[4], dscores[SLOPE ? 4 : 1];
+            if constexpr (MAIN) {
+                // scores, transposed: lane has keys 4g ... 4g+3 of each strip for its place
+#pragma unroll
+                for (int s = 0; s < 4; ++s) scores[s] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < KP / D; ++d)
+#pragma unroll
+                    for (int s = 0; s <= w; ++s) scores[s] = mma(along(keys, kPitch, s * 16, d * D), qf[d], scores[s]);
+                // the state's part
+#pragma unroll
+                for (int v = 0; v < VT; ++v) acc[v] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < KP / D; ++d)
+#pragma unroll
+                    for (int part = 0; part < P; ++part)
+#pragma unroll
+                        for (int v = 0; v < VT; ++v) acc[v] = mma(along(state + part * VP * kPitch, kPitch, v * 16, d * D), qf[d], acc[v]);
+                const int i = w * 16 + col - missing + shift;                // places of the chunk up to this lane's
+                const float reach = power_at(powers, i);
+                if constexpr (SLOPE) {
+                    const float reach_slope = slope_at(powers, i);
+#pragma unroll
+                    for (int v = 0; v < VT; ++v) dacc[v] = f4{0, 0, 0, 0};
+#pragma unroll
+                    for (int d = 0; d < KP / D; ++d)
+#pragma unroll
+                        for (int part = 0; part < P; ++part)
+#pragma unroll
+                            for (int v = 0; v < VT; ++v)
+                                dacc[v] = mma(along(state + (P + part) * VP * kPitch, kPitch, v * 16, d * D), qf[d], dacc[v]);
+#pragma unroll
+                    for (int v = 0; v < VT; ++v) dacc[v] = dacc[v] * reach + acc[v] * reach_slope;
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            dscores[s][r] = s > w || (s == w && col <= 4 * g + r) ? 0.f
+                                            : s == w ? scores[s][r] * near_slope[r]
+                                                     : scores[s][r] * fmaf(apart_slope[w - s - 1], far[r], apart[w - s - 1] * far_slope[r]);
+                    }
+                }
+                if (more) fetch_query(p0 + kChunk);
+#pragma unroll
+                for (int v = 0; v < VT; ++v) acc[v] *= reach;
+#pragma unroll
+                for (int s = 0; s <= w; ++s)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        scores[s][r] = s == w ? (col >= 4 * g + r ? scores[s][r] * near[r] : 0.f)
+                                              : scores[s][r] * (s + 1 == w ? far[r] : far[r] * apart[w - s - 1]);
+            }
+#pragma unroll
+            for (int s = 0; s < ST; ++s)
+#pragma unroll
+                for (int v = 0; v < VT; ++v) {
+                    if constexpr (SLOPE) W[s][v] = W[s][v] * step_hi + S[s][v] * step_slope;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[s][v][r] = fmaf(S[s][v][r], step_hi, S[s][v][r] * step_lo);
+                }
+#pragma unroll
+            for (int d = 0; d < kChunk / D; ++d) {
+                F vf[VT];                                                    // values, terms across the places
+#pragma unroll
+                for (int v = 0; v < VT; ++v) vf[v] = across(values, vPitch, v * 16, d * D);
+                if constexpr (MAIN) {
+                    if (d * D <= w * 16) {
+                        auto add = [&](f4 (&to)[VT], const f4 (&from)[4]) {
+                            if constexpr (F32) {
+#pragma unroll
+                                for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], from[d], to[v]);
+                            } else {
+                                const auto x = split<2>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                                for (int part = 0; part < 2; ++part)
+#pragma unroll
+                                    for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], x.part[part], to[v]);
+                            }
+                        };
+                        add(acc, scores);
+                        if constexpr (SLOPE) add(dacc, dscores);
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < ST; ++s) {
+                    if (s * 4 + w >= KT) continue;
+                    const F kf = across(keys, kPitch, (s * 4 + w) * 16, d * D);
+                    auto add = [&](f4 (&to)[VT], const float* weights) {
+                        const f4 w0 = *reinterpret_cast<const f4*>(weights + d * D + 4 * g);
+                        if constexpr (F32) {
+                            const f4 x = kf * w0;
+#pragma unroll
+                            for (int v = 0; v < VT; ++v) to[v] = mma(x, vf[v], to[v]);
+                        } else {
+                            const f4 w1 = *reinterpret_cast<const f4*>(weights + d * D + 16 + 4 * g);
+                            const auto x = split<3>(__builtin_convertvector(kf, f8) * __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                            for (int part = 0; part < 3; ++part)
+#pragma unroll
+                                for (int v = 0; v < VT; ++v) to[v] = mma(x.part[part], vf[v], to[v]);
+                        }
+                    };
+                    add(S[s], behind[0]);
+                    if constexpr (SLOPE) add(W[s], behind[1]);
+                }
+            }
+            if constexpr (MAIN) {
+                const int p = p0 + w * 16 + col;
+                if (p >= begin) {
+                    T* o = out + place(p) * a.out_t;
+                    const T* x = SLOPE ? (const T*)a.other + n * a.other_n + h * a.other_h + v0 + place(p) * a.other_t : nullptr;
+#pragma unroll
+                    for (int v = 0; v < VT; ++v) {
+                        const int c = v * 16 + 4 * g;
+                        const f4 y = acc[v] * a.out_scale;
+                        if (a.whole_out && c + 4 <= vleft) {
+                            if constexpr (F32) *reinterpret_cast<f4*>(o + c) = y;
+                            else *reinterpret_cast<b4*>(o + c) = __builtin_convertvector(y, b4);
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (c + r < vleft) o[c + r] = (T)y[r];
+                        }
+                        if constexpr (SLOPE) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (c + r < vleft) total = fmaf((float)x[c + r], dacc[v][r], total);
+                        }
+                    }
+                }
+            }
+        };
+        if (wave == 0) chunk(std::integral_constant<int, 0>{});
+        else if (wave == 1) chunk(std::integral_constant<int, 1>{});
+        else if (wave == 2) chunk(std::integral_constant<int, 2>{});
+        else chunk(std::integral_constant<int, 3>{});
+    }
+
+    const bool last = MAIN && ((begin < length && length <= begin + a.segment) || (length == 0 && seg == 0));
+    float *to = nullptr, *slope_to = nullptr;
+    if (!MAIN) {
+        const int64_t at = ((int64_t)unit * a.segments + seg + 1) * state_size;
+        to = a.starts + at;
+        if (SLOPE) slope_to = a.slope_starts + at;
+    } else if (last && a.last) {
+        to = a.last + unit * state_size;
+    }
+    const float* grad_last = MODE == LEAKY_SLOPE && last && a.grad_last ? a.grad_last + unit * state_size : nullptr;
+    double slope = (double)total * a.out_scale;
+    if (to || grad_last) {
+#pragma unroll
+        for (int s = 0; s < ST; ++s)
+#pragma unroll
+            for (int v = 0; v < VT; ++v)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int k = (s * 4 + wave) * 16 + 4 * g + r, c = v * 16 + col;
+                    const int64_t at = (int64_t)k * a.state_k + (int64_t)(v0 + c) * a.state_v;
+                    if (k < a.keys && c < vleft) {
+                        if (to) to[at] = S[s][v][r];
+                        if constexpr (SLOPE) {
+                            if (slope_to) slope_to[at] = W[s][v][r];
+                            if (grad_last) slope += (double)W[s][v][r] * grad_last[at];
+                        }
+                    }
+                }
+    }
+    if (MODE == LEAKY_SLOPE) {
+        for (int d = 32; d > 0; d >>= 1) slope += __shfl_xor(slope, d);
+        if (lane == 0) sums[wave] = slope;
+        __syncthreads();
+        if (threadIdx.x == 0) a.slopes[((int64_t)unit * a.segments + seg) * a.slices + slice] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    }
+    // tokens behind the sample's end
+    if (MAIN) {
+        for (int64_t at = threadIdx.x; at < (int64_t)(end - max(begin, length)) * VP; at += 256) {
+            const int p = max(begin, length) + (int)(at / VP), c = (int)(at % VP);
+            if (c < vleft) out[p * a.out_t + c] = (T)0.f;
+        }
+    }
+}
+
+// values of a slice, in sixteens
+inline int slice_tiles(int64_t values) {
+    const int64_t slices = (values + 63) / 64;
+    return (int)(((values + slices - 1) / slices + 15) / 16);
+}
+
+template <typename T, int MODE>
+int launch_leaky_mode(const LeakyPass& p, dim3 grid, bool whole, hipStream_t s) {
+    const int vt = slice_tiles(p.values);
+#define LAUNCH(K, V, WHOLE) hipLaunchKernelGGL((leaky_kernel<T, K, V, MODE, WHOLE>), grid, dim3(256), 0, s, p)
+#define BY_KEYS(V, WHOLE)                           \
+    if (p.keys <= 32) LAUNCH(2, V, WHOLE);          \
+    else if (p.keys <= 64) LAUNCH(4, V, WHOLE);     \
+    else if (p.keys <= 96) LAUNCH(6, V, WHOLE);     \
+    else LAUNCH(8, V, WHOLE)
+    if (!whole) {
+        if (vt <= 2) { if (p.keys <= 64) LAUNCH(4, 2, false); else LAUNCH(8, 2, false); }
+        else { if (p.keys <= 64) LAUNCH(4, 4, false); else LAUNCH(8, 4, false); }
+    }
+    else if (vt == 1) { BY_KEYS(1, true); }
+    else if (vt == 2) { BY_KEYS(2, true); }
+    else if (vt == 3) { BY_KEYS(3, true); }
+    else { BY_KEYS(4, true); }
+#undef BY_KEYS
+#undef LAUNCH
+    return (int)hipGetLastError();
+}
+
+// Tiles of a slice as the kernel that is launched has them.
+inline int launched_tiles(int64_t values, bool whole) {
+    const int vt = slice_tiles(values);
+    return whole ? vt : vt <= 2 ? 2 : 4;
+}
+
+template <typename T> int launch_leaky(const LeakyPass& p, int mode, bool whole, hipStream_t stream);    // attention_f32.hip, attention_bf16.hip
+
+}  // namespace slayer

@@ -102,7 +102,7 @@ _SIGNATURES = {
     'slayer_recurrent_steps_bwd': (_INT, [_P] * 5 + [_F, _F, _F, _INT] + [_I64] * 3 + [_P, _I64, _P]),
     'slayer_leaky_attention_workspace': (_I64, [_AP, _INT]),
     'slayer_leaky_attention_fwd': (_INT, [_P] * 6 + [_AP, _P, _I64, _P]),
-    'slayer_leaky_attention_bwd': (_INT, [_P] * 11 + [_AP, _P, _I64, _P]),
+    'slayer_leaky_attention_bwd': (_INT, [_P] * 12 + [_AP, _P, _I64, _P]),
     'slayer_leaky_attention_step': (_INT, [_P] * 5 + [_AP, _P]),
     'slayer_group_norm_workspace': (_I64, [_INT] + [_I64] * 4 + [_INT]),
     'slayer_group_norm_fwd': (_INT, [_P] * 6 + [_INT] + [_I64] * 4 + [_F, _INT, _P, _I64, _P]),

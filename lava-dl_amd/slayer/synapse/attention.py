@@ -164,7 +164,7 @@ def _forward(query, key, value, decay, state, lengths, scale, return_state):
         workspace, floats = _workspace(args, 0, query.device)
         N.check(N.lib().slayer_leaky_attention_fwd(N.ptr(out), N.ptr(last), N.ptr(query), N.ptr(key), N.ptr(value), N.ptr(state),
                                                    ctypes.byref(args), N.ptr(workspace), floats, N.stream_handle()))
-    return out, last, query, key, value, decay, state
+    return out, last, query, key, value, decay, state, workspace
 
 
 class _LeakyAttention(torch.autograd.Function):
@@ -179,7 +179,7 @@ class _LeakyAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out, grad_last):
-        query, key, value, decay, state, lengths = ctx.saved_tensors
+        query, key, value, decay, state, starts, lengths = ctx.saved_tensors
         if grad_out is None:
             if grad_last is None:
                 return (None,) * 8
@@ -188,12 +188,12 @@ class _LeakyAttention(torch.autograd.Function):
         grad_last = None if grad_last is None else grad_last.contiguous()
         need = ctx.needs_input_grad
         new = [torch.empty(x.shape, dtype=x.dtype, device=x.device) if wanted else None
-               for x, wanted in zip((query, key, value, decay, state), (need[0], need[1], need[2] or need[4], *need[3:5]))]
+               for x, wanted in zip((query, key, value, decay, state), (need[0] or need[3], need[1], need[2] or need[4], *need[3:5]))]
         args = _call(query, key, value, decay, lengths, ctx.scale)
         args.grad_stride[:] = grad_out.stride()[:3]
         with N.device_guard(query.device):
             workspace, floats = _workspace(args, 1, query.device)
             N.check(N.lib().slayer_leaky_attention_bwd(*(N.ptr(x) for x in new), N.ptr(grad_out), N.ptr(grad_last), N.ptr(query),
-                                                       N.ptr(key), N.ptr(value), N.ptr(state), ctypes.byref(args),
-                                                       N.ptr(workspace), floats, N.stream_handle()))
-        return (*new[:2], new[2] if need[2] else None, *new[3:], None, None, None)
+                                                       N.ptr(key), N.ptr(value), N.ptr(state), N.ptr(starts),
+                                                       ctypes.byref(args), N.ptr(workspace), floats, N.stream_handle()))
+        return (*(x if wanted else None for x, wanted in zip(new, need)), None, None, None)
