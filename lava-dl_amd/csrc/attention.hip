@@ -131,6 +131,9 @@ int check_leaky(const slayer_attention* a) {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
+// A segment's workgroup adds up the states of up to so many segments itself (a launch between the two kernels is 10 us).
+constexpr int kJoin = 8;
+
 // Segments of a pass: enough workgroups for the chip (512: two a compute unit), and chunks enough in each that reading keys and
 // values a second time for the states in front of them pays.  The same for every pass of a call.
 int segment_tokens(const slayer_attention* a) {
@@ -188,6 +191,7 @@ int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3
     p.slices = slices_of(a, query, key, value, keys, values);
     p.segment = segment_tokens(a);
     p.segments = segments_of(a);
+    p.joined = p.segments > kJoin;
     p.backwards = backwards;
     p.whole_out = aligned(out, out_stride, size, 4 * size);
     p.out_scale = backwards ? 1.f : (float)a->scale;
@@ -202,6 +206,8 @@ int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3
     auto launch = [&](int mode) { return f32 ? launch_leaky<float>(p, mode, whole, stream) : launch_leaky<bf16>(p, mode, whole, stream); };
     if (p.segments > 1 && !ready) {
         if (int e = launch(slope ? LEAKY_STATE_SLOPE : LEAKY_STATE)) return e;
+    }
+    if (p.joined && !ready) {
         const int64_t blocks = (int64_t)p.units * ceil_div((int64_t)keys * values, 256);
         if (blocks > (1 << 24) - 1) return SLAYER_ERANGE;
         hipLaunchKernelGGL(leaky_join_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p);

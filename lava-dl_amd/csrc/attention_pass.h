@@ -15,7 +15,8 @@ struct LeakyPass {
     const float* decay;
     const void* lengths;
     const float* first;            // [samples][heads] states with strides first_k, first_v, or nullptr: zeros
-    float* starts;                 // states in front of the segments, [samples * heads][segments] of them
+    float* starts;                 // states in front of the segments, [samples * heads][segments] of them (not `joined`: what the
+                                   // segment before each adds)
     float* last;                   // state behind the last token, or nullptr
     float* slope_starts;           // LEAKY_SLOPE: derivatives of the states in `starts`
     const float* grad_last;        // LEAKY_SLOPE: gradient of the last state, or nullptr
@@ -24,7 +25,7 @@ struct LeakyPass {
     int64_t out_n, out_t, out_h, query_n, query_t, query_h, key_n, key_t, key_h, value_n, value_t, value_h, other_n, other_t, other_h;
     int tokens, heads, keys, values, state_k, state_v;      // the strides of a state's axes
     int units;                     // samples * heads
-    int one_decay, lengths64, segments, segment, slices, backwards;
+    int one_decay, lengths64, segments, segment, slices, backwards, joined;
     int whole_out;                 // four results are a multiple of their size apart from the tensor's start
     float out_scale, key_scale;    // of the results; of what `key` stands for, in scores and in the state
 };
@@ -121,6 +122,9 @@ __device__ __forceinline__ float slope_at(const float* powers, int n) { return n
 //       W'      = a^64 W + 64 a^63 S + sum over j of (63-j) a^(62-j) key[j] (outer) value[j]
 //     of which the workgroup returns the sum of its products with `other`.  LEAKY_STATE_SLOPE: S and W from zero.
 //   WHOLE: the rows of all tensors are made of whole, aligned 16-byte pieces.
+#ifndef LEAKY_TWO_BUFFERS
+#define LEAKY_TWO_BUFFERS 40000
+#endif
 #ifndef LEAKY_WAVES
 #define LEAKY_WAVES(T, KT, VT, MODE) 2
 #endif
@@ -130,19 +134,26 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
     typedef typename Elements<T>::Vec Vec;
     constexpr bool MAIN = MODE == LEAKY_MAIN || MODE == LEAKY_SLOPE, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
     constexpr int V = Elements<T>::kVec, D = Frag<T>::kDepth, P = F32 ? 1 : 2;       // parts of a state in LDS
-    constexpr int KP = KT * 16, VP = VT * 16, kPitch = KP + V, vPitch = VP + V;
+    constexpr int KP = KT * 16, VP = VT * 16;
+    // rows of LDS: sixteen rows of keys, read along, start in different banks; so do the eight (float32: four) rows of values that
+    // an access across them touches
+    constexpr int kPitch = KP + V, vPitch = F32 ? VP + 4 : VP + (VT % 2 ? 0 : 16);
     constexpr int KV = KP / V, VV = VP / V;                                  // 16-byte pieces of a row
     constexpr int kLoads = (kChunk * KV + 255) / 256, vLoads = (kChunk * VV + 255) / 256;
     constexpr int ST = (KT + 3) / 4;                                         // strips of the state of a wave
     constexpr int kStates = MAIN ? (SLOPE ? 2 : 1) : 0;                      // states in LDS
-    __shared__ __align__(16) T keys[kChunk * kPitch];
-    __shared__ __align__(16) T values[kChunk * vPitch];
-    __shared__ __align__(16) T state[kStates ? kStates * P * VP * kPitch : 8];       // transposed: [state][part][value][key]
+    constexpr int kTile = kChunk * kPitch, vTile = kChunk * vPitch, sTile = kStates * P * VP * kPitch;
+    // two buffers, and one barrier a chunk, where two workgroups still fit a compute unit
+    constexpr int BUFFERS = (kTile + vTile + sTile) * (int)sizeof(T) <= LEAKY_TWO_BUFFERS ? 2 : 1;
+    __shared__ __align__(16) T tiles[BUFFERS * (kTile + vTile + sTile)];     // keys, values, state: [state][part][value][key]
     __shared__ __align__(16) float powers[kChunk + 4];                       // a^i
     __shared__ __align__(16) float behind[SLOPE ? 2 : 1][kChunk];            // what key j counts behind the chunk; its derivative
     __shared__ double sums[4];
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
+    const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    // Strips of the later places cost more (float32, 64 keys and values: 10, 12, 14 and 16 sixteenths of a product of 64 x 64 x 64 / 4),
+    // and the waves of a place in the workgroup share a SIMD: the second workgroup of a compute unit has them the other way round.
+    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x & 256 ? 3 - (threadIdx.x >> 6) : threadIdx.x >> 6);
     const int segments = MAIN ? a.segments : a.segments - 1;
     // the slices of a segment, which read the same queries and keys, eight workgroups apart: on the same XCD, with one L2
     int slice, at_segment = blockIdx.x;
@@ -174,22 +185,38 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
     // the state, in strips of 16 keys: lane has keys 4g ... 4g+3 of column `col`
     f4 S[ST][VT], W[SLOPE ? ST : 1][SLOPE ? VT : 1];
     {
-        const int64_t at = ((int64_t)unit * a.segments + seg) * state_size;
-        const float* first = !MAIN ? nullptr : seg > 0 ? a.starts + at : (a.first ? a.first + unit * state_size : nullptr);
-        const float* slope_first = MODE == LEAKY_SLOPE && seg > 0 ? a.slope_starts + at : nullptr;
+        // in front of the segment: from `starts` where the states are joined, or what the segments before it have left there, added up
+        const int from = !MAIN || begin > length ? seg + 1 : a.joined && seg > 0 ? seg : 0;
+        const double past = power(leak, a.segment);
+        const float past_hi = (float)past, past_lo = (float)(past - (double)past_hi);
+        const float past_slope = SLOPE ? (float)(a.segment * power(leak, a.segment - 1)) : 0.f;
 #pragma unroll
         for (int s = 0; s < ST; ++s)
 #pragma unroll
-            for (int v = 0; v < VT; ++v)
+            for (int v = 0; v < VT; ++v) {
+                S[s][v] = f4{0, 0, 0, 0};
+                if constexpr (SLOPE) W[s][v] = f4{0, 0, 0, 0};
+            }
+        for (int j = from; j <= seg; ++j) {
+            const int64_t at = ((int64_t)unit * a.segments + j) * state_size;
+            const float* first = j > 0 ? a.starts + at : (a.first ? a.first + unit * state_size : nullptr);
+            const float* slope_first = SLOPE && j > 0 ? a.slope_starts + at : nullptr;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int k = (s * 4 + wave) * 16 + 4 * g + r, c = v * 16 + col;
-                    const bool on = begin <= length && k < a.keys && c < vleft;
-                    const int64_t from = (int64_t)k * a.state_k + (int64_t)(v0 + c) * a.state_v;
-                    S[s][v][r] = first && on ? first[from] : 0.f;
-                    if constexpr (SLOPE) W[s][v][r] = slope_first && on ? slope_first[from] : 0.f;
-                }
+            for (int s = 0; s < ST; ++s)
+#pragma unroll
+                for (int v = 0; v < VT; ++v)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int k = (s * 4 + wave) * 16 + 4 * g + r, c = v * 16 + col;
+                        const bool on = k < a.keys && c < vleft;
+                        const int64_t element = (int64_t)k * a.state_k + (int64_t)(v0 + c) * a.state_v;
+                        const float x = S[s][v][r];
+                        if constexpr (SLOPE) W[s][v][r] = fmaf(W[s][v][r], past_hi, fmaf(x, past_slope, slope_first && on ? slope_first[element] : 0.f));
+                        S[s][v][r] = fmaf(x, past_hi, fmaf(x, past_lo, first && on ? first[element] : 0.f));
+                    }
+        }
     }
+    T *keys = tiles, *values = tiles + kTile, *state = tiles + kTile + vTile;
     auto share = [&](f4 x, int which, int strip, int v) {
         T* p = state + which * P * VP * kPitch + (v * 16 + col) * kPitch + strip * 16 + 4 * g;
         if constexpr (F32) {
@@ -253,24 +280,19 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
 
     // weights of the scores: key 4g + r of the strip of this lane's place (from the place on: none), and of strips in front of it,
     // in which a factor a^(16 strips) is left out
-    float near[4], far[4], near_slope[4], far_slope[4];
+    float near[4], far[4];
     if (MAIN) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int back = col - 4 * g - r;
             near[r] = power_at(powers, back) * a.key_scale;
             far[r] = powers[16 + back] * a.key_scale;
-            if (SLOPE) {
-                near_slope[r] = slope_at(powers, back);
-                far_slope[r] = slope_at(powers, 16 + back);
-            }
         }
     }
-    const float apart[3] = {1.f, powers[16], powers[32]}, apart_slope[3] = {0.f, 16.f * powers[15], 32.f * powers[31]};
+    const float apart[3] = {1.f, powers[16], powers[32]};
     float total = 0;                                                         // LEAKY_SLOPE
 
-    for (; p0 < stop; p0 += kChunk) {
-        __syncthreads();                                                     // the chunk before is done with LDS
+    auto fill = [&]() {                                                      // LDS for the next chunk
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int at = i * 256 + threadIdx.x;
@@ -292,7 +314,17 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                 }
             }
         }
+    };
+    int turn = 0;
+    for (; p0 < stop; p0 += kChunk) {
+        if (BUFFERS == 1) __syncthreads();                                   // the chunk before is done with LDS
+        fill();
         __syncthreads();
+        const T *lk = keys, *lv = values, *ls = state;
+        if (BUFFERS == 2) {
+            turn = kTile + vTile + sTile - turn;
+            keys = tiles + turn; values = keys + kTile; state = values + vTile;
+        }
         const bool more = p0 + kChunk < stop;
         if (more) fetch_rows(p0 + kChunk);
 
@@ -303,7 +335,32 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
 
         auto chunk = [&](auto which) {
             constexpr int w = decltype(which)::value;
-            f4 acc[VT], dacc[SLOPE ? VT : 1], scores[4], dscores[SLOPE ? 4 : 1];
+            f4 scores[4];
+            // adds the products of weighted scores and values
+            auto add_values = [&](f4 (&to)[VT], const f4 (&from)[4], int d, const F (&vf)[VT]) {
+                if constexpr (F32) {
+#pragma unroll
+                    for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], from[d], to[v]);
+                } else {
+                    const auto x = split<2>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], x.part[part], to[v]);
+                }
+            };
+            // the state's part of the results
+            auto of_state = [&](f4 (&to)[VT], int which) {
+#pragma unroll
+                for (int v = 0; v < VT; ++v) to[v] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < KP / D; ++d)
+#pragma unroll
+                    for (int part = 0; part < P; ++part)
+#pragma unroll
+                        for (int v = 0; v < VT; ++v)
+                            to[v] = mma(along(ls + (which * P + part) * VP * kPitch, kPitch, v * 16, d * D), qf[d], to[v]);
+            };
             if constexpr (MAIN) {
                 // scores, transposed: lane has keys 4g ... 4g+3 of each strip for its place
 #pragma unroll
@@ -311,40 +368,49 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
 #pragma unroll
                 for (int d = 0; d < KP / D; ++d)
 #pragma unroll
-                    for (int s = 0; s <= w; ++s) scores[s] = mma(along(keys, kPitch, s * 16, d * D), qf[d], scores[s]);
-                // the state's part
-#pragma unroll
-                for (int v = 0; v < VT; ++v) acc[v] = f4{0, 0, 0, 0};
-#pragma unroll
-                for (int d = 0; d < KP / D; ++d)
-#pragma unroll
-                    for (int part = 0; part < P; ++part)
-#pragma unroll
-                        for (int v = 0; v < VT; ++v) acc[v] = mma(along(state + part * VP * kPitch, kPitch, v * 16, d * D), qf[d], acc[v]);
-                const int i = w * 16 + col - missing + shift;                // places of the chunk up to this lane's
-                const float reach = power_at(powers, i);
-                if constexpr (SLOPE) {
+                    for (int s = 0; s <= w; ++s) scores[s] = mma(along(lk, kPitch, s * 16, d * D), qf[d], scores[s]);
+            }
+            const int i = w * 16 + col - missing + shift;                    // places of the chunk up to this lane's
+            const float reach = MAIN ? power_at(powers, i) : 0.f;
+            const int p = p0 + w * 16 + col;
+            if constexpr (MODE == LEAKY_SLOPE) {
+                f4 dacc[VT], dscores[4];
+                of_state(dacc, 1);
+                {
+                    f4 acc[VT];
+                    of_state(acc, 0);
                     const float reach_slope = slope_at(powers, i);
 #pragma unroll
-                    for (int v = 0; v < VT; ++v) dacc[v] = f4{0, 0, 0, 0};
-#pragma unroll
-                    for (int d = 0; d < KP / D; ++d)
-#pragma unroll
-                        for (int part = 0; part < P; ++part)
-#pragma unroll
-                            for (int v = 0; v < VT; ++v)
-                                dacc[v] = mma(along(state + (P + part) * VP * kPitch, kPitch, v * 16, d * D), qf[d], dacc[v]);
-#pragma unroll
                     for (int v = 0; v < VT; ++v) dacc[v] = dacc[v] * reach + acc[v] * reach_slope;
+                }
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) {
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int back = (w - s) * 16 + col - 4 * g - r;
+                        dscores[s][r] = s > w || back < 1 ? 0.f : scores[s][r] * slope_at(powers, s > w ? 0 : back);
+                    }
+#pragma unroll
+                for (int d = 0; d < kChunk / D; ++d) {
+                    if (d * D > w * 16) continue;
+                    F vf[VT];
+#pragma unroll
+                    for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D);
+                    add_values(dacc, dscores, d, vf);
+                }
+                if (p >= begin) {
+                    const T* x = (const T*)a.other + n * a.other_n + h * a.other_h + v0 + place(p) * a.other_t;
+#pragma unroll
+                    for (int v = 0; v < VT; ++v)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            dscores[s][r] = s > w || (s == w && col <= 4 * g + r) ? 0.f
-                                            : s == w ? scores[s][r] * near_slope[r]
-                                                     : scores[s][r] * fmaf(apart_slope[w - s - 1], far[r], apart[w - s - 1] * far_slope[r]);
-                    }
+                            if (v * 16 + 4 * g + r < vleft) total = fmaf((float)x[v * 16 + 4 * g + r], dacc[v][r], total);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            f4 acc[VT];
+            if constexpr (MAIN) {
+                of_state(acc, 0);
                 if (more) fetch_query(p0 + kChunk);
 #pragma unroll
                 for (int v = 0; v < VT; ++v) acc[v] *= reach;
@@ -367,30 +433,15 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
             for (int d = 0; d < kChunk / D; ++d) {
                 F vf[VT];                                                    // values, terms across the places
 #pragma unroll
-                for (int v = 0; v < VT; ++v) vf[v] = across(values, vPitch, v * 16, d * D);
+                for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D);
                 if constexpr (MAIN) {
-                    if (d * D <= w * 16) {
-                        auto add = [&](f4 (&to)[VT], const f4 (&from)[4]) {
-                            if constexpr (F32) {
-#pragma unroll
-                                for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], from[d], to[v]);
-                            } else {
-                                const auto x = split<2>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                                for (int part = 0; part < 2; ++part)
-#pragma unroll
-                                    for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], x.part[part], to[v]);
-                            }
-                        };
-                        add(acc, scores);
-                        if constexpr (SLOPE) add(dacc, dscores);
-                    }
+                    if (d * D <= w * 16) add_values(acc, scores, d, vf);
                 }
 #pragma unroll
                 for (int s = 0; s < ST; ++s) {
                     if (s * 4 + w >= KT) continue;
-                    const F kf = across(keys, kPitch, (s * 4 + w) * 16, d * D);
-                    auto add = [&](f4 (&to)[VT], const float* weights) {
+                    const F kf = across(lk, kPitch, (s * 4 + w) * 16, d * D);
+                    auto add_keys = [&](f4 (&to)[VT], const float* weights) {
                         const f4 w0 = *reinterpret_cast<const f4*>(weights + d * D + 4 * g);
                         if constexpr (F32) {
                             const f4 x = kf * w0;
@@ -405,15 +456,13 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                                 for (int v = 0; v < VT; ++v) to[v] = mma(x.part[part], vf[v], to[v]);
                         }
                     };
-                    add(S[s], behind[0]);
-                    if constexpr (SLOPE) add(W[s], behind[1]);
+                    add_keys(S[s], behind[0]);
+                    if constexpr (SLOPE) add_keys(W[s], behind[1]);
                 }
             }
             if constexpr (MAIN) {
-                const int p = p0 + w * 16 + col;
                 if (p >= begin) {
                     T* o = out + place(p) * a.out_t;
-                    const T* x = SLOPE ? (const T*)a.other + n * a.other_n + h * a.other_h + v0 + place(p) * a.other_t : nullptr;
 #pragma unroll
                     for (int v = 0; v < VT; ++v) {
                         const int c = v * 16 + 4 * g;
@@ -425,11 +474,6 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
                                 if (c + r < vleft) o[c + r] = (T)y[r];
-                        }
-                        if constexpr (SLOPE) {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (c + r < vleft) total = fmaf((float)x[c + r], dacc[v][r], total);
                         }
                     }
                 }

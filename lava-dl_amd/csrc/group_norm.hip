@@ -13,16 +13,22 @@ namespace slayer {
 
 enum { ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU };
 
+// 1 / (1 + exp(-z)) with the hardware's base-two exponential and reciprocal, a unit in the last place each: together within
+// (3 + 1.5 |z|) 2^-24 of it where it matters (for negative z it is the exponential that falls).  The precise functions take three
+// times the instructions, which is what bounded the kernels of bfloat16 rows.
+__device__ __forceinline__ float logistic(float z) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+}
 template <int ACT> __device__ __forceinline__ float activate(float z) {
     if (ACT == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
-    if (ACT == ACT_SILU) return z / (1.f + expf(-z));
+    if (ACT == ACT_SILU) return z * logistic(z);
     if (ACT == ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
     return z;
 }
 template <int ACT> __device__ __forceinline__ float slope(float z) {
     if (ACT == ACT_RELU) return z > 0.f ? 1.f : 0.f;
     if (ACT == ACT_SILU) {
-        const float s = 1.f / (1.f + expf(-z));
+        const float s = logistic(z);
         return s * fmaf(z, 1.f - s, 1.f);
     }
     if (ACT == ACT_GELU) return fmaf(z, 0.39894228040143268f * expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
@@ -43,28 +49,61 @@ struct NormArgs {
     int64_t samples, pixels;
     int channels, groups, width;     // width = channels / groups
     int whole, whole_rows;           // 16-byte accesses to a channel row, to a group's row
+    int whole_params;                // ... to weight and bias
     int lanes, splits, tiles;        // lanes of a row; pieces of an image, tiles of channels
     float eps;
 };
 
-__device__ __forceinline__ void load_params(float* w, float* b, const NormArgs& a, int c, int n) {
-    constexpr int most = 8;
+// weight and bias of the first `n` of V channels
+template <int V>
+__device__ __forceinline__ void load_params(float (&w)[V], float (&b)[V], const NormArgs& a, int c, int n) {
+    const bool whole = n >= V && a.whole_params && c % 4 == 0;
 #pragma unroll
-    for (int e = 0; e < most; ++e) {
-        if (e >= n) break;
-        w[e] = a.weight ? a.weight[c + e] : 1.f;
-        b[e] = a.bias ? a.bias[c + e] : 0.f;
+    for (int e = 0; e < V; ++e) {
+        w[e] = 1.f;
+        b[e] = 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+        if (whole) {
+            if (a.weight) {
+                const f4 v = *reinterpret_cast<const f4*>(a.weight + c + e);
+                w[e] = v[0]; w[e + 1] = v[1]; w[e + 2] = v[2]; w[e + 3] = v[3];
+            }
+            if (a.bias) {
+                const f4 v = *reinterpret_cast<const f4*>(a.bias + c + e);
+                b[e] = v[0]; b[e + 1] = v[1]; b[e + 2] = v[2]; b[e + 3] = v[3];
+            }
+        } else {
+#pragma unroll
+            for (int i = e; i < e + 4; ++i) {
+                if (a.weight && i < n) w[i] = a.weight[c + i];
+                if (a.bias && i < n) b[i] = a.bias[c + i];
+            }
+        }
     }
 }
 
 // ---- rows ---------------------------------------------------------------------------------------------------------------------
+// The rows a workgroup takes at a time (`per`), or those of all workgroups together, are a multiple of the groups, so a thread stays
+// with its channels.
 template <typename T, int ACT, int IT>
-__global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
+__global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a, int per) {
     constexpr int V = Elements<T>::kVec;
-    const int lane = threadIdx.x % a.lanes;
-    const int64_t rows = a.samples * a.groups, per = 256 / a.lanes;
+    const int lane = threadIdx.x % a.lanes, sub = threadIdx.x / a.lanes;
+    const int64_t rows = a.samples * a.groups;
     const float inv = 1.f / (float)a.width;
-    for (int64_t row = blockIdx.x * per + threadIdx.x / a.lanes; row < rows; row += gridDim.x * per) {
+    const int c = (int)((blockIdx.x * (unsigned)per + sub) % (unsigned)a.groups) * a.width;
+    float w[IT][V], b[IT][V];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int at = (i * a.lanes + lane) * V, left = a.width - at;
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[i][e] = b[i][e] = 0;
+        if (left > 0) load_params(w[i], b[i], a, c + at, left < V ? left : V);
+    }
+    if (sub >= per) return;
+    for (int64_t row = (int64_t)blockIdx.x * per + sub; row < rows; row += (int64_t)gridDim.x * per) {
         const T* in = (const T*)a.in + row * a.width;
         float x[IT][V], sum = 0;
 #pragma unroll
@@ -88,22 +127,18 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
             a.mean[row] = mean;
             a.scale[row] = scale;
         }
-        const int c = (int)(row % a.groups) * a.width;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int at = (i * a.lanes + lane) * V, left = a.width - at;
             if (left <= 0) continue;
-            float w[V], b[V];
-            load_params(w, b, a, c + at, left < V ? left : V);
 #pragma unroll
-            for (int e = 0; e < V; ++e) x[i][e] = activate<ACT>(fmaf((x[i][e] - mean) * scale, w[e], b[e]));
+            for (int e = 0; e < V; ++e) x[i][e] = activate<ACT>(fmaf((x[i][e] - mean) * scale, w[i][e], b[i][e]));
             store_vec((T*)a.out + row * a.width + at, from_floats(x[i]), left, a.whole_rows);
         }
     }
 }
 
-// dx, and this workgroup's part of the sums over the rows: work[slot][2][width], slot % groups = the group.  The rows a workgroup
-// takes at a time (`per`), or those of all workgroups together, are a multiple of the groups, so a thread stays with its channels.
+// dx, and this workgroup's part of the sums over the rows: work[slot][2][width], slot % groups = the group.
 //   shared: the rows of a workgroup that have the same channels are summed in LDS first.
 template <typename T, int ACT, int IT>
 __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(NormArgs a, int per, bool shared) {
@@ -112,7 +147,7 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(NormArgs a, int per,
     const int lane = threadIdx.x % a.lanes, sub = threadIdx.x / a.lanes;
     const int64_t rows = a.samples * a.groups;
     const float inv = 1.f / (float)a.width;
-    const int group = (int)(((int64_t)blockIdx.x * per + sub) % a.groups), c = group * a.width;
+    const int c = (int)((blockIdx.x * (unsigned)per + sub) % (unsigned)a.groups) * a.width;
     float w[IT][V], b[IT][V], dw[IT][V], db[IT][V];
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
@@ -178,25 +213,29 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(NormArgs a, int per,
     }
 }
 
-// dweight and dbias: the sum over the slots of a group.  64 channels and 16 shares of the slots a workgroup.
+// dweight and dbias: the sum over the slots of a group.  Sixteen channels and 64 shares of the slots a workgroup.
 __global__ __launch_bounds__(1024) void norm_rows_sum_kernel(float* __restrict__ dweight, float* __restrict__ dbias,
                                                              const float* __restrict__ work, int64_t slots, int groups, int width) {
-    __shared__ float sums[2][16][64];
-    const int i = threadIdx.x & 63, share = threadIdx.x >> 6, c = blockIdx.x * 64 + i, channels = groups * width;
+    __shared__ float sums[64][33];
+    const int i = threadIdx.x % 16, share = threadIdx.x / 16, c = blockIdx.x * 16 + i, channels = groups * width;
     float w = 0, b = 0;
-    if (c < channels)
-        for (int64_t slot = c / width + (int64_t)share * groups; slot < slots; slot += 16 * groups) {
+    if (c < channels) {
+#pragma unroll 8
+        for (int64_t slot = c / width + (int64_t)share * groups; slot < slots; slot += 64 * groups) {
             w += work[slot * 2 * width + c % width];
             b += work[slot * 2 * width + width + c % width];
         }
-    sums[0][share][i] = w;
-    sums[1][share][i] = b;
+    }
+    sums[share][i] = w;
+    sums[share][16 + i] = b;
     __syncthreads();
-    if (share < 2 && c < channels) {
-        float sum = 0;
-        for (int s = 0; s < 16; ++s) sum += sums[share][s][i];
-        float* to = share ? dbias : dweight;
-        if (to) to[c] = sum;
+    if (threadIdx.x < 512) {                                     // 32 sums, sixteen lanes each
+        const int which = threadIdx.x / 16;
+        float sum = (sums[i][which] + sums[i + 16][which]) + (sums[i + 32][which] + sums[i + 48][which]);
+        sum = sum_lanes(sum, 16);
+        const int channel = blockIdx.x * 16 + which % 16;
+        float* to = which < 16 ? dweight : dbias;
+        if (i == 0 && channel < channels && to) to[channel] = sum;
     }
 }
 
@@ -275,33 +314,33 @@ __device__ __forceinline__ float sum_block(float v, float* shared) {            
     return (shared[0] + shared[1]) + (shared[2] + shared[3]);
 }
 
-// mean and scale of a group from the sums of its channels: the channels' means first, then squares about the group's.
+// mean and scale of a group from the sums of its channels and pieces: the mean, then the squares about it.
 template <typename T>
 __global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a) {
     __shared__ float shared[4];
-    const int64_t n = blockIdx.x / a.groups;
-    const int c0 = (int)(blockIdx.x % a.groups) * a.width;
+    const int64_t n = blockIdx.x / a.groups, per = (a.pixels + a.splits - 1) / a.splits;
+    const int c0 = (int)(blockIdx.x % a.groups) * a.width, count = a.width * a.splits;
     const T* first = (const T*)a.in + n * a.pixels * a.channels + c0;
     const float* work = a.work + (n * a.splits * a.channels + c0) * 2;
-    const float inv = 1.f / (float)a.pixels;
+    const float inv = 1.f / ((float)a.pixels * (float)a.width);
+    auto pixels_of = [&](int split) {
+        const int64_t left = a.pixels - split * per;
+        return (float)(left < per ? (left > 0 ? left : 0) : per);
+    };
     float sum = 0;
-    for (int c = threadIdx.x; c < a.width; c += 256) {
-        float s1 = 0;
-        for (int s = 0; s < a.splits; ++s) s1 += work[((int64_t)s * a.channels + c) * 2];
-        sum += (float)first[c] + s1 * inv;
+    for (int i = threadIdx.x; i < count; i += 256) {
+        const int split = i / a.width, c = i % a.width;
+        sum = fmaf(pixels_of(split), (float)first[c], sum + work[((int64_t)split * a.channels + c) * 2]);
     }
-    const float mean = sum_block(sum, shared) / (float)a.width;
+    const float mean = sum_block(sum, shared) * inv;
     float square = 0;
-    for (int c = threadIdx.x; c < a.width; c += 256) {
-        float s1 = 0, s2 = 0;
-        for (int s = 0; s < a.splits; ++s) {
-            s1 += work[((int64_t)s * a.channels + c) * 2];
-            s2 += work[((int64_t)s * a.channels + c) * 2 + 1];
-        }
-        const float m = s1 * inv, d = (float)first[c] + m - mean;
-        square += fmaxf(s2 * inv - m * m, 0.f) + d * d;
+    for (int i = threadIdx.x; i < count; i += 256) {
+        const int split = i / a.width, c = i % a.width;
+        const float* s = work + ((int64_t)split * a.channels + c) * 2;
+        const float d = mean - (float)first[c];
+        square += fmaf(d, fmaf(pixels_of(split), d, -2.f * s[0]), s[1]);
     }
-    const float var = sum_block(square, shared) / (float)a.width;
+    const float var = fmaxf(sum_block(square, shared) * inv, 0.f);
     if (threadIdx.x == 0) {
         a.mean[blockIdx.x] = mean;
         a.scale[blockIdx.x] = 1.f / sqrtf(var + a.eps);
@@ -364,7 +403,8 @@ __global__ __launch_bounds__(256) void norm_bwd_stats_kernel(NormArgs a) {
     store_sums<V>(a.work, s1, s2, a, p);
 }
 
-// Workgroups up to samples * groups: the two means of a group, into `means`.  The others: dweight and dbias of 256 channels.
+// Workgroups up to samples * groups: the two means of a group, into `means`.  The others: dweight and dbias of sixteen channels, in
+// sixteen shares of the pieces.
 __global__ __launch_bounds__(256) void norm_bwd_join_kernel(NormArgs a, float* __restrict__ means, float* __restrict__ dweight,
                                                             float* __restrict__ dbias) {
     __shared__ float shared[4];
@@ -374,12 +414,12 @@ __global__ __launch_bounds__(256) void norm_bwd_join_kernel(NormArgs a, float* _
         const int c0 = (int)(blockIdx.x % a.groups) * a.width;
         const float* work = a.work + (n * a.splits * a.channels + c0) * 2;
         float s1 = 0, s2 = 0;
-        for (int c = threadIdx.x; c < a.width; c += 256) {
+        for (int i = threadIdx.x; i < a.width * a.splits; i += 256) {
+            const int c = i % a.width;
             const float w = a.weight ? a.weight[c0 + c] : 1.f;
-            for (int s = 0; s < a.splits; ++s) {
-                s1 = fmaf(w, work[((int64_t)s * a.channels + c) * 2], s1);
-                s2 = fmaf(w, work[((int64_t)s * a.channels + c) * 2 + 1], s2);
-            }
+            const float* s = work + ((int64_t)(i / a.width) * a.channels + c) * 2;
+            s1 = fmaf(w, s[0], s1);
+            s2 = fmaf(w, s[1], s2);
         }
         const float size = (float)a.pixels * (float)a.width;
         s1 = sum_block(s1, shared) / size;
@@ -389,15 +429,25 @@ __global__ __launch_bounds__(256) void norm_bwd_join_kernel(NormArgs a, float* _
             means[2 * blockIdx.x + 1] = s2;
         }
     } else {
-        const int c = (int)(blockIdx.x - units) * 256 + threadIdx.x;
-        if (c >= a.channels) return;
+        __shared__ float sums[16][33];
+        const int c = (int)(blockIdx.x - units) * 16 + threadIdx.x % 16, share = threadIdx.x / 16;
         float b = 0, w = 0;
-        for (int64_t s = 0; s < a.samples * a.splits; ++s) {
-            b += a.work[(s * a.channels + c) * 2];
-            w += a.work[(s * a.channels + c) * 2 + 1];
+        if (c < a.channels) {
+#pragma unroll 8
+            for (int64_t s = share; s < a.samples * a.splits; s += 16) {
+                b += a.work[(s * a.channels + c) * 2];
+                w += a.work[(s * a.channels + c) * 2 + 1];
+            }
         }
-        if (dweight) dweight[c] = w;
-        if (dbias) dbias[c] = b;
+        sums[share][threadIdx.x % 16] = w;
+        sums[share][16 + threadIdx.x % 16] = b;
+        __syncthreads();
+        if (threadIdx.x < 32 && c < a.channels) {
+            float sum = 0;
+            for (int s = 0; s < 16; ++s) sum += sums[s][threadIdx.x];
+            float* to = threadIdx.x < 16 ? dweight : dbias;
+            if (to) to[c] = sum;
+        }
     }
 }
 
@@ -449,7 +499,7 @@ struct Cut {
     bool rows;
     int lanes, its;            // rows: lanes of a group and accesses of a lane
     int per;                   // rows, backwards: groups a workgroup takes at a time
-    int64_t blocks, slots;     // rows, backwards
+    int64_t fwd_blocks, blocks, slots;     // rows; backwards
     bool shared;
     int splits, tiles;         // pixels
 };
@@ -471,9 +521,9 @@ Cut cut_of(int dtype, int64_t samples, int64_t pixels, int64_t channels, int64_t
             c.per = (int)most;
             multiple = groups / gcd(groups, most);
         }
-        c.blocks = ceil_div(rows, c.per);
-        if (c.blocks > 1024) c.blocks = 1024;
-        c.blocks = ceil_div(c.blocks, multiple) * multiple;
+        const int64_t all = ceil_div(rows, c.per);
+        c.fwd_blocks = ceil_div(all < 2048 ? all : 2048, multiple) * multiple;
+        c.blocks = ceil_div(all < 1024 ? all : 1024, multiple) * multiple;
         c.shared = groups <= most && c.per * 2 * width * 4 <= 65536;
         c.slots = c.blocks * (c.shared ? groups : c.per);
     } else {
@@ -517,6 +567,7 @@ NormArgs args_of(void* out, const void* in, const void* grad, const float* weigh
     const bool base = ((uintptr_t)out | (uintptr_t)in | (uintptr_t)grad) % 16 == 0;
     a.whole = base && channels * size % 16 == 0;
     a.whole_rows = base && a.width * size % 16 == 0;
+    a.whole_params = ((uintptr_t)weight | (uintptr_t)bias) % 16 == 0;
     a.lanes = c.lanes; a.splits = c.splits; a.tiles = c.tiles;
     a.eps = eps;
     return a;
@@ -525,15 +576,16 @@ NormArgs args_of(void* out, const void* in, const void* grad, const float* weigh
 template <typename T>
 int launch_fwd(const NormArgs& a, const Cut& c, int activation, hipStream_t s) {
     if (c.rows) {
-        int64_t blocks = ceil_div(a.samples * a.groups, 256 / a.lanes);
-        if (blocks > 4096) blocks = 4096;
-#define LAUNCH(ACT)                                                                                                              \
-    if (c.its == 1) hipLaunchKernelGGL((norm_rows_kernel<T, ACT, 1>), dim3((unsigned)blocks), dim3(256), 0, s, a);                \
-    else if (c.its == 2) hipLaunchKernelGGL((norm_rows_kernel<T, ACT, 2>), dim3((unsigned)blocks), dim3(256), 0, s, a);           \
-    else if (c.its == 4) hipLaunchKernelGGL((norm_rows_kernel<T, ACT, 4>), dim3((unsigned)blocks), dim3(256), 0, s, a);           \
-    else hipLaunchKernelGGL((norm_rows_kernel<T, ACT, 8>), dim3((unsigned)blocks), dim3(256), 0, s, a)
+        if (c.fwd_blocks > (1 << 23)) return SLAYER_ERANGE;
+#define ONE(ACT, IT) hipLaunchKernelGGL((norm_rows_kernel<T, ACT, IT>), dim3((unsigned)c.fwd_blocks), dim3(256), 0, s, a, c.per)
+#define LAUNCH(ACT)                     \
+    if (c.its == 1) ONE(ACT, 1);        \
+    else if (c.its == 2) ONE(ACT, 2);   \
+    else if (c.its == 4) ONE(ACT, 4);   \
+    else ONE(ACT, 8)
         BY_ACT(LAUNCH)
 #undef LAUNCH
+#undef ONE
         return (int)hipGetLastError();
     }
     const int64_t blocks = a.samples * a.splits * a.tiles;
@@ -549,6 +601,7 @@ int launch_fwd(const NormArgs& a, const Cut& c, int activation, hipStream_t s) {
 template <typename T>
 int launch_bwd(const NormArgs& a, const Cut& c, int activation, float* dweight, float* dbias, float* means, hipStream_t s) {
     if (c.rows) {
+        if (c.blocks > (1 << 23)) return SLAYER_ERANGE;
         const size_t lds = a.work && c.shared ? (size_t)c.per * 2 * a.width * sizeof(float) : 0;
 #define ONE(ACT, IT) hipLaunchKernelGGL((norm_rows_bwd_kernel<T, ACT, IT>), dim3((unsigned)c.blocks), dim3(256), lds, s, a, c.per, c.shared)
 #define LAUNCH(ACT)                     \
@@ -561,7 +614,7 @@ int launch_bwd(const NormArgs& a, const Cut& c, int activation, float* dweight, 
 #undef ONE
         if (int e = (int)hipGetLastError()) return e;
         if (!a.work) return 0;
-        hipLaunchKernelGGL(norm_rows_sum_kernel, dim3((unsigned)ceil_div(a.channels, 64)), dim3(1024), 0, s, dweight, dbias, a.work, c.slots,
+        hipLaunchKernelGGL(norm_rows_sum_kernel, dim3((unsigned)ceil_div(a.channels, 16)), dim3(1024), 0, s, dweight, dbias, a.work, c.slots,
                            a.groups, a.width);
         return (int)hipGetLastError();
     }
@@ -570,7 +623,7 @@ int launch_bwd(const NormArgs& a, const Cut& c, int activation, float* dweight, 
 #define LAUNCH(ACT) hipLaunchKernelGGL((norm_bwd_stats_kernel<T, ACT>), dim3((unsigned)blocks), dim3(256), 0, s, a)
     BY_ACT(LAUNCH)
 #undef LAUNCH
-    hipLaunchKernelGGL(norm_bwd_join_kernel, dim3((unsigned)(units + ceil_div(a.channels, 256))), dim3(256), 0, s, a, means, dweight, dbias);
+    hipLaunchKernelGGL(norm_bwd_join_kernel, dim3((unsigned)(units + ceil_div(a.channels, 16))), dim3(256), 0, s, a, means, dweight, dbias);
 #define LAUNCH(ACT) hipLaunchKernelGGL((norm_bwd_apply_kernel<T, ACT>), dim3((unsigned)blocks), dim3(256), 0, s, a, means)
     BY_ACT(LAUNCH)
 #undef LAUNCH
