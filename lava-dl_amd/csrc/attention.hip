@@ -193,9 +193,10 @@ int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3
     p.segments = segments_of(a);
     p.joined = p.segments > kJoin;
     p.backwards = backwards;
-    p.whole_out = aligned(out, out_stride, size, 4 * size);
-    p.out_scale = backwards ? 1.f : (float)a->scale;
-    p.key_scale = backwards ? (float)a->scale : 1.f;      // the state it starts from is not scaled
+    p.whole_out = values % 4 == 0 && aligned(out, out_stride, size, 4 * size) && out_stride[1] < ((int64_t)1 << 31) / (kChunk * size) - 256;
+    p.score_scale = (float)a->scale;
+    p.state_scale = backwards ? 1.f : (float)a->scale;    // backwards the state it starts from is not scaled, but what is added to it
+    p.key_scale = backwards ? (float)a->scale : 1.f;
     if (slope) {
         p.slope_starts = slope->starts;
         p.grad_last = slope->grad_last;
@@ -213,7 +214,7 @@ int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3
         hipLaunchKernelGGL(leaky_join_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p);
         if (int e = (int)hipGetLastError()) return e;
     }
-    return launch(slope ? LEAKY_SLOPE : LEAKY_MAIN);
+    return launch(slope ? LEAKY_SLOPE : last ? LEAKY_LAST : LEAKY_MAIN);
 }
 
 // Floats of the states in front of the segments.

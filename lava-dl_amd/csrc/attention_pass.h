@@ -26,8 +26,8 @@ struct LeakyPass {
     int tokens, heads, keys, values, state_k, state_v;      // the strides of a state's axes
     int units;                     // samples * heads
     int one_decay, lengths64, segments, segment, slices, backwards, joined;
-    int whole_out;                 // four results are a multiple of their size apart from the tensor's start
-    float out_scale, key_scale;    // of the results; of what `key` stands for, in scores and in the state
+    int whole_out;                 // values come in fours that can be written at once, within the reach of a 32-bit offset
+    float score_scale, state_scale, key_scale;      // of scores, of the state in results, of keys in the state
 };
 
 // ---- fragments of the matrix instructions.  A fragment holds kDepth terms of a product for 16 rows (or columns): lane l has
@@ -54,21 +54,21 @@ __device__ __forceinline__ f4 mma(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mf
 
 // terms along the row of `tile`
 template <typename T>
-__device__ __forceinline__ typename Frag<T>::Type along(const T* tile, int pitch, int row, int term) {
-    const int lane = threadIdx.x & 63;
+__device__ __forceinline__ typename Frag<T>::Type along(const T* tile, int pitch, int row, int term, int lane) {
     return *reinterpret_cast<const typename Frag<T>::Type*>(tile + (row + (lane & 15)) * pitch + term + (lane >> 4) * Elements<T>::kVec);
 }
 // terms across the rows of `tile`, the sixteen columns from `column` on
-__device__ __forceinline__ f4 across(const float* tile, int pitch, int column, int term) {
-    const int lane = threadIdx.x & 63;
+__device__ __forceinline__ f4 across(const float* tile, int pitch, int column, int term, int lane) {
     const float* p = tile + (term + (lane >> 4) * 4) * pitch + column + (lane & 15);
     return f4{p[0], p[pitch], p[2 * pitch], p[3 * pitch]};
 }
 typedef __attribute__((address_space(3))) short LdsShort;
 typedef short s4 __attribute__((ext_vector_type(4)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
 // ds_read_b64_tr_b16: the sixteen lanes of a group read four rows of sixteen columns, lane i gets column i of the four
-__device__ __forceinline__ b8 across(const bf16* tile, int pitch, int column, int term) {
-    const int lane = threadIdx.x & 63, i = lane & 15;
+__device__ __forceinline__ b8 across(const bf16* tile, int pitch, int column, int term, int lane) {
+    const int i = lane & 15;
     const bf16* p = tile + (term + (lane >> 4) * 4 + (i >> 2)) * pitch + column + (i & 3) * 4;
     const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(LdsShort*)p);
     const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)(LdsShort*)(p + 16 * pitch));
@@ -77,8 +77,8 @@ __device__ __forceinline__ b8 across(const bf16* tile, int pitch, int column, in
 }
 
 // A float32 operand: in float32, or as bfloat16 numbers that sum to it, so that what the kernel makes itself is not rounded to
-// the type of the tensors on the way: two for scores and states, which end in a result of that type (within 2^-17, a hundredth of
-// what rounding the result costs), three for the leaked keys, which end in a float32 state (within 2^-25).
+// the type of the tensors on the way: two for what ends in a result of that type (within 2^-17, a hundredth of what
+// rounding the result costs), three for leaked keys that end in a float32 state (within 2^-25).
 template <int PARTS> struct Split { b8 part[PARTS]; };
 template <int PARTS>
 __device__ __forceinline__ Split<PARTS> split(f8 v) {
@@ -107,7 +107,28 @@ __device__ __forceinline__ int sample_length(const LeakyPass& a, int n) {
 }
 
 
-enum { LEAKY_STATE, LEAKY_MAIN, LEAKY_STATE_SLOPE, LEAKY_SLOPE };
+enum { LEAKY_STATE, LEAKY_MAIN, LEAKY_LAST, LEAKY_STATE_SLOPE, LEAKY_SLOPE };
+
+// Values that are not finite.  A score that the mask leaves out is 0, and 0 times such a value is not: a strip with masked scores takes
+// the products without these values and says which results they belong to.
+__device__ __forceinline__ bool any_not_finite(f4 v) {
+    const u4 x = __builtin_bit_cast(u4, v) & 0x7fffffffu;
+    return max(max(x[0], x[1]), max(x[2], x[3])) >= 0x7f800000u;
+}
+__device__ __forceinline__ bool any_not_finite(b8 v) {
+    const u4 x = (__builtin_bit_cast(u4, v) & 0x7f807f80u) + 0x00800080u;     // an exponent of all ones carries into the sign
+    return ((x[0] | x[1]) | (x[2] | x[3])) & 0x80008000u;
+}
+template <typename F> __device__ __forceinline__ F where_not_finite(F v, F yes, F no) {
+    constexpr int count = sizeof(F) == 16 && sizeof(v[0]) == 4 ? 4 : 8;
+    F r;
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+        const float x = (float)v[i];
+        r[i] = x - x == 0.f ? no[i] : yes[i];
+    }
+    return r;
+}
 
 // a^n and its derivative n a^(n-1); both 0 for n < 0
 __device__ __forceinline__ float power_at(const float* powers, int n) { return n >= 0 ? powers[n] : 0.f; }
@@ -117,6 +138,7 @@ __device__ __forceinline__ float slope_at(const float* powers, int n) { return n
 // Wave w makes the outputs of places 16w ... 16w+15 (transposed: lane = place) and the rows of the state w, w+4, ... (16 each).
 // The first chunk is the one that is not full, with its tokens at the end, so that weights behind a token are the same in all.
 //   LEAKY_STATE: only the state, from zero, into `starts` behind the segment's place (for the segments but the last).
+//   LEAKY_LAST:  results and the last state, which is held more exactly than results of bfloat16 need.
 //   LEAKY_SLOPE: results, and the derivative of each with respect to a, in which the state's derivative W takes the place of S:
 //       dout[i] = a^(i+1) query[i] W + (i+1) a^i query[i] S + sum over j of (i-j) a^(i-j-1) (query[i] . key[j]) value[j]
 //       W'      = a^64 W + 64 a^63 S + sum over j of (63-j) a^(62-j) key[j] (outer) value[j]
@@ -125,6 +147,9 @@ __device__ __forceinline__ float slope_at(const float* powers, int n) { return n
 #ifndef LEAKY_TWO_BUFFERS
 #define LEAKY_TWO_BUFFERS 40000
 #endif
+#ifndef LEAKY_FENCE
+#define LEAKY_FENCE __builtin_amdgcn_sched_barrier(0)
+#endif
 #ifndef LEAKY_WAVES
 #define LEAKY_WAVES(T, KT, VT, MODE) 2
 #endif
@@ -132,7 +157,8 @@ template <typename T, int KT, int VT, int MODE, bool WHOLE>
 __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kernel(LeakyPass a) {
     typedef typename Frag<T>::Type F;
     typedef typename Elements<T>::Vec Vec;
-    constexpr bool MAIN = MODE == LEAKY_MAIN || MODE == LEAKY_SLOPE, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
+    constexpr bool MAIN = MODE == LEAKY_MAIN || MODE == LEAKY_LAST || MODE == LEAKY_SLOPE, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
+    constexpr bool FINE = F32 || MODE != LEAKY_MAIN;                         // the state to float32, not to a hundredth of bfloat16
     constexpr int V = Elements<T>::kVec, D = Frag<T>::kDepth, P = F32 ? 1 : 2;       // parts of a state in LDS
     constexpr int KP = KT * 16, VP = VT * 16;
     // rows of LDS: sixteen rows of keys, read along, start in different banks; so do the eight (float32: four) rows of values that
@@ -147,6 +173,7 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
     constexpr int BUFFERS = (kTile + vTile + sTile) * (int)sizeof(T) <= LEAKY_TWO_BUFFERS ? 2 : 1;
     __shared__ __align__(16) T tiles[BUFFERS * (kTile + vTile + sTile)];     // keys, values, state: [state][part][value][key]
     __shared__ __align__(16) float powers[kChunk + 4];                       // a^i
+    __shared__ float weights[MAIN ? 48 : 1];                                 // of scores: a^(i - 16), 0 for i < 16
     __shared__ __align__(16) float behind[SLOPE ? 2 : 1][kChunk];            // what key j counts behind the chunk; its derivative
     __shared__ double sums[4];
 
@@ -172,6 +199,74 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
     if (!MAIN && end > length) return;                                       // no segment behind it needs this one's state
     const int64_t state_size = (int64_t)a.keys * a.values;
     T* out = (T*)a.out + n * a.out_n + h * a.out_h + v0;
+    const int shift = a.backwards ? 0 : 1;
+    f4 S[ST][VT], W[SLOPE ? ST : 1][SLOPE ? VT : 1];
+    T *keys = tiles, *values = tiles + kTile, *state = tiles + kTile + vTile;
+    auto share = [&](f4 x, int which, int strip, int v, int g, int col) {
+        T* p = state + which * P * VP * kPitch + (v * 16 + col) * kPitch + strip * 16 + 4 * g;
+        if constexpr (F32) {
+            *reinterpret_cast<f4*>(p) = x;
+        } else {
+            const b4 hi = __builtin_convertvector(x, b4);
+            *reinterpret_cast<b4*>(p) = hi;
+            *reinterpret_cast<b4*>(p + VP * kPitch) = __builtin_convertvector(x - __builtin_convertvector(hi, f4), b4);
+        }
+    };
+
+    // What the next chunk needs, on its way.  WHOLE: a thread's pieces are an offset from the chunk's first address (the offset ~0
+    // lies outside of every buffer and reads 0); otherwise they are read element by element.
+    const int count0 = stop > begin ? (stop - begin - 1) % kChunk + 1 : 0;   // tokens of the first chunk
+    int p0 = stop > begin ? begin - (kChunk - count0) : stop;                // place of the chunk's first row
+    auto place = [&](int p) { return (int64_t)(a.backwards ? length - 1 - p : p); };
+    const int64_t low0 = place(a.backwards ? p0 + kChunk - 1 : p0), turn = a.backwards ? -kChunk : kChunk;
+    const T* key = (const T*)a.key + n * a.key_n + h * a.key_h + low0 * a.key_t;             // the chunk's first address
+    const T* value = (const T*)a.value + n * a.value_n + h * a.value_h + v0 + low0 * a.value_t;
+    const T* query = MAIN ? (const T*)a.query + n * a.query_n + h * a.query_h + low0 * a.query_t : nullptr;
+    Vec nk[kLoads], nv[vLoads];
+    F qf[MAIN ? KP / D : 1];
+    constexpr int kNowhere = (int)0x80000000;
+    // `missing`: rows of the chunk that are not there (the first chunk's)
+    auto fetch = [&](auto& to, const T* base, int64_t stride, int left, int missing, auto pieces, int thread) {
+        constexpr int per = decltype(pieces)::value;
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < (kChunk * per + 255) / 256; ++i) {
+            const int at = i * 256 + thread, row = at / per, c = at % per * V, from = a.backwards ? kChunk - 1 - row : row;
+            const bool on = row >= missing && (kChunk * per % 256 == 0 || at < kChunk * per);
+            if constexpr (WHOLE) {
+                const int off = (from * (int)stride + c) * (int)sizeof(T);
+                to[i] = __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b128(r, on && c < left ? off : kNowhere, 0, 0));
+            } else {
+                to[i] = load_vec(base + (on ? from * stride : 0) + c, on ? left - c : 0, false);
+            }
+        }
+    };
+    auto fetch_rows = [&](int missing, int thread) {
+        fetch(nk, key, a.key_t, a.keys, missing, std::integral_constant<int, KV>{}, thread);
+        fetch(nv, value, a.value_t, vleft, missing, std::integral_constant<int, VV>{}, thread);
+        key += turn * a.key_t;
+        value += turn * a.value_t;
+    };
+    auto fetch_query = [&](int missing, int g, int col) {                    // this lane's place: row 16 wave + col
+        if constexpr (MAIN) {
+            const int row = wave * 16 + col, from = a.backwards ? kChunk - 1 - row : row;
+            const bool on = row >= missing;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(query), 0, 0x7fffffff, 0x00020000);
+            const int off = (from * (int)a.query_t + g * V) * (int)sizeof(T);
+#pragma unroll
+            for (int d = 0; d < KP / D; ++d) {
+                const int c = d * D + g * V;
+                if constexpr (WHOLE) qf[d] = __builtin_bit_cast(F, __builtin_amdgcn_raw_buffer_load_b128(r, on && c < a.keys ? off + d * D * (int)sizeof(T) : kNowhere, 0, 0));
+                else qf[d] = load_vec(query + (on ? from * a.query_t : 0) + c, on ? a.keys - c : 0, false);
+            }
+            query += turn * a.query_t;
+        }
+    };
+    if (stop > begin) {
+        fetch_query(begin - p0, g, col);
+        fetch_rows(begin - p0, threadIdx.x);
+    }
+
     if (threadIdx.x <= kChunk) powers[threadIdx.x] = (float)power(leak, threadIdx.x);
     __syncthreads();
     if (threadIdx.x < kChunk) {
@@ -179,17 +274,16 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
         behind[0][threadIdx.x] = powers[left + (a.backwards ? 1 : 0)] * a.key_scale;
         if (SLOPE) behind[SLOPE ? 1 : 0][threadIdx.x] = slope_at(powers, left);
     }
+    if (MAIN && threadIdx.x < 48) weights[MAIN ? threadIdx.x : 0] = power_at(powers, (int)threadIdx.x - 16) * a.score_scale;
     const double whole_leak = power(leak, kChunk);
-    const int shift = a.backwards ? 0 : 1;
 
     // the state, in strips of 16 keys: lane has keys 4g ... 4g+3 of column `col`
-    f4 S[ST][VT], W[SLOPE ? ST : 1][SLOPE ? VT : 1];
     {
         // in front of the segment: from `starts` where the states are joined, or what the segments before it have left there, added up
         const int from = !MAIN || begin > length ? seg + 1 : a.joined && seg > 0 ? seg : 0;
-        const double past = power(leak, a.segment);
+        const double past = from < seg ? power(leak, a.segment) : 1;
         const float past_hi = (float)past, past_lo = (float)(past - (double)past_hi);
-        const float past_slope = SLOPE ? (float)(a.segment * power(leak, a.segment - 1)) : 0.f;
+        const float past_slope = SLOPE && from < seg ? (float)(a.segment * power(leak, a.segment - 1)) : 0.f;
 #pragma unroll
         for (int s = 0; s < ST; ++s)
 #pragma unroll
@@ -216,117 +310,55 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                     }
         }
     }
-    T *keys = tiles, *values = tiles + kTile, *state = tiles + kTile + vTile;
-    auto share = [&](f4 x, int which, int strip, int v) {
-        T* p = state + which * P * VP * kPitch + (v * 16 + col) * kPitch + strip * 16 + 4 * g;
-        if constexpr (F32) {
-            *reinterpret_cast<f4*>(p) = x;
-        } else {
-            const b4 hi = __builtin_convertvector(x, b4);
-            *reinterpret_cast<b4*>(p) = hi;
-            *reinterpret_cast<b4*>(p + VP * kPitch) = __builtin_convertvector(x - __builtin_convertvector(hi, f4), b4);
-        }
-    };
-
-    // What the next chunk needs, on its way.  WHOLE: a thread's pieces are an offset from the chunk's first address (the offset ~0
-    // lies outside of every buffer and reads 0); otherwise they are read element by element.
-    const int count0 = stop > begin ? (stop - begin - 1) % kChunk + 1 : 0;   // tokens of the first chunk
-    int p0 = stop > begin ? begin - (kChunk - count0) : stop;                // place of the chunk's first row
-    auto place = [&](int p) { return (int64_t)(a.backwards ? length - 1 - p : p); };
-    const T* key = (const T*)a.key + n * a.key_n + h * a.key_h;
-    const T* value = (const T*)a.value + n * a.value_n + h * a.value_h + v0;
-    const T* query = MAIN ? (const T*)a.query + n * a.query_n + h * a.query_h : nullptr;
-    Vec nk[kLoads], nv[vLoads];
-    F qf[MAIN ? KP / D : 1];
-    auto fetch = [&](auto& to, const T* base, int64_t stride, int left, int from, auto pieces) {       // rows `from` ... of the pass
-        constexpr int per = decltype(pieces)::value;
-        const int64_t low = place(a.backwards ? from + kChunk - 1 : from);
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base) + low * stride, 0, 0x7fffffff, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < (kChunk * per + 255) / 256; ++i) {
-            const int at = i * 256 + threadIdx.x, row = at / per, c = at % per * V;
-            const bool on = from + row >= begin && (kChunk * per % 256 == 0 || at < kChunk * per);
-            if constexpr (WHOLE) {
-                const int off = ((a.backwards ? kChunk - 1 - row : row) * (int)stride + c) * (int)sizeof(T);
-                to[i] = __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b128(r, on && c < left ? off : -1, 0, 0));
-            } else {
-                to[i] = load_vec(base + (on ? place(from + row) : 0) * stride + c, on ? left - c : 0, false);
-            }
-        }
-    };
-    auto fetch_rows = [&](int from) {
-        fetch(nk, key, a.key_t, a.keys, from, std::integral_constant<int, KV>{});
-        fetch(nv, value, a.value_t, vleft, from, std::integral_constant<int, VV>{});
-    };
-    auto fetch_query = [&](int from) {                                       // this lane's place: row 16 wave + col
-        if constexpr (MAIN) {
-            const int row = wave * 16 + col;
-            const int64_t low = place(a.backwards ? from + kChunk - 1 : from);
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(query) + low * a.query_t, 0, 0x7fffffff, 0x00020000);
-            const bool on = from + row >= begin;
-            const int off = ((a.backwards ? kChunk - 1 - row : row) * (int)a.query_t + g * V) * (int)sizeof(T);
-#pragma unroll
-            for (int d = 0; d < KP / D; ++d) {
-                const int c = d * D + g * V;
-                if constexpr (WHOLE) qf[d] = __builtin_bit_cast(F, __builtin_amdgcn_raw_buffer_load_b128(r, on && c < a.keys ? off + d * D * (int)sizeof(T) : -1, 0, 0));
-                else qf[d] = load_vec(query + (on ? place(from + row) : 0) * a.query_t + c, on ? a.keys - c : 0, false);
-            }
-        }
-    };
-    if (stop > begin) {
-        fetch_query(p0);
-        fetch_rows(p0);
-    }
-
-    // weights of the scores: key 4g + r of the strip of this lane's place (from the place on: none), and of strips in front of it,
-    // in which a factor a^(16 strips) is left out
-    float near[4], far[4];
-    if (MAIN) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int back = col - 4 * g - r;
-            near[r] = power_at(powers, back) * a.key_scale;
-            far[r] = powers[16 + back] * a.key_scale;
-        }
-    }
     const float apart[3] = {1.f, powers[16], powers[32]};
     float total = 0;                                                         // LEAKY_SLOPE
 
-    auto fill = [&]() {                                                      // LDS for the next chunk
+    __shared__ int not_finite[2];                                            // the last chunk (of every second) with such values
+    if (threadIdx.x < 2) not_finite[threadIdx.x] = p0 - 1;
+    int parity = 0;
+    auto fill = [&](int thread, int g, int col) {                            // LDS for the next chunk
+        bool bad = false;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int at = i * 256 + threadIdx.x;
+            const int at = i * 256 + thread;
             if (kChunk * KV % 256 == 0 || at < kChunk * KV) *reinterpret_cast<Vec*>(keys + at / KV * kPitch + at % KV * V) = nk[i];
         }
 #pragma unroll
         for (int i = 0; i < vLoads; ++i) {
-            const int at = i * 256 + threadIdx.x;
+            const int at = i * 256 + thread;
             if (kChunk * VV % 256 == 0 || at < kChunk * VV) *reinterpret_cast<Vec*>(values + at / VV * vPitch + at % VV * V) = nv[i];
+            if (MAIN) bad = bad || any_not_finite(nv[i]);
         }
+        if (MAIN && bad) not_finite[parity] = p0;
         if constexpr (MAIN) {
 #pragma unroll
             for (int s = 0; s < ST; ++s) {
                 if (KT % 4 != 0 && s * 4 + wave >= KT) continue;
 #pragma unroll
                 for (int v = 0; v < VT; ++v) {
-                    share(S[s][v], 0, s * 4 + wave, v);
-                    if constexpr (SLOPE) share(W[s][v], 1, s * 4 + wave, v);
+                    share(S[s][v], 0, s * 4 + wave, v, g, col);
+                    if constexpr (SLOPE) share(W[s][v], 1, s * 4 + wave, v, g, col);
                 }
             }
         }
     };
-    int turn = 0;
-    for (; p0 < stop; p0 += kChunk) {
+    int buffer = 0;
+    for (; p0 < stop; p0 += kChunk, parity ^= 1) {
+        // the thread's place, worked out anew: kept, the addresses made of it for the four strips would take 60 registers
+        int thread = threadIdx.x;
+        asm volatile("" : "+v"(thread));
+        const int lane = thread & 63, g = lane >> 4, col = lane & 15;
         if (BUFFERS == 1) __syncthreads();                                   // the chunk before is done with LDS
-        fill();
+        fill(thread, g, col);
         __syncthreads();
         const T *lk = keys, *lv = values, *ls = state;
+        const bool odd_values = MAIN && __builtin_amdgcn_readfirstlane(not_finite[parity]) == p0;
         if (BUFFERS == 2) {
-            turn = kTile + vTile + sTile - turn;
-            keys = tiles + turn; values = keys + kTile; state = values + vTile;
+            buffer = kTile + vTile + sTile - buffer;
+            keys = tiles + buffer; values = keys + kTile; state = values + vTile;
         }
         const bool more = p0 + kChunk < stop;
-        if (more) fetch_rows(p0 + kChunk);
+        if (more) fetch_rows(0, thread);
 
         const int missing = p0 < begin ? begin - p0 : 0;
         const double step = missing ? power(leak, kChunk - missing) : whole_leak;
@@ -337,7 +369,33 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
             constexpr int w = decltype(which)::value;
             f4 scores[4];
             // adds the products of weighted scores and values
+            auto weigh = [&](F v, const f4 (&from)[4], int d, f4 to) {
+                if constexpr (F32) {
+                    return mma(v, from[d], to);
+                } else {
+                    const auto x = split<2>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    return mma(v, x.part[1], mma(v, x.part[0], to));
+                }
+            };
             auto add_values = [&](f4 (&to)[VT], const f4 (&from)[4], int d, const F (&vf)[VT]) {
+                if (odd_values && (d + 1) * D > w * 16) {                    // some of these scores are masked
+                    F there, none, one;                                      // `there`: 1 for places up to this lane's
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        there[e] = (T)(d * D + (e >> 2) * 16 + 4 * g + (e & 3) <= w * 16 + col ? 1.f : 0.f);
+                        none[e] = (T)0.f;
+                        one[e] = (T)1.f;
+                    }
+#pragma unroll
+                    for (int v = 0; v < VT; ++v) {
+                        const f4 reached = mma(where_not_finite(vf[v], one, none), there, f4{0, 0, 0, 0});
+                        to[v] = weigh(where_not_finite(vf[v], none, vf[v]), from, d, to[v]);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (reached[r] > 0.f) to[v][r] = __builtin_nanf("");
+                    }
+                    return;
+                }
                 if constexpr (F32) {
 #pragma unroll
                     for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], from[d], to[v]);
@@ -359,7 +417,7 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                     for (int part = 0; part < P; ++part)
 #pragma unroll
                         for (int v = 0; v < VT; ++v)
-                            to[v] = mma(along(ls + (which * P + part) * VP * kPitch, kPitch, v * 16, d * D), qf[d], to[v]);
+                            to[v] = mma(along(ls + (which * P + part) * VP * kPitch, kPitch, v * 16, d * D, lane), qf[d], to[v]);
             };
             if constexpr (MAIN) {
                 // scores, transposed: lane has keys 4g ... 4g+3 of each strip for its place
@@ -368,18 +426,40 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
 #pragma unroll
                 for (int d = 0; d < KP / D; ++d)
 #pragma unroll
-                    for (int s = 0; s <= w; ++s) scores[s] = mma(along(lk, kPitch, s * 16, d * D), qf[d], scores[s]);
+                    for (int s = 0; s <= w; ++s) scores[s] = mma(along(lk, kPitch, s * 16, d * D, lane), qf[d], scores[s]);
             }
+            LEAKY_FENCE;
             const int i = w * 16 + col - missing + shift;                    // places of the chunk up to this lane's
-            const float reach = MAIN ? power_at(powers, i) : 0.f;
+            const float reach = MAIN ? power_at(powers, i) * a.state_scale : 0.f;
             const int p = p0 + w * 16 + col;
+            auto store = [&](const f4 (&acc)[VT]) {
+                if (a.whole_out) {                                           // four results that are all there or not at all
+                    const int row = w * 16 + col, from = a.backwards ? kChunk - 1 - row : row;
+                    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+                        out + (int64_t)(a.backwards ? length - kChunk - p0 : p0) * a.out_t, 0, 0x7fffffff, 0x00020000);
+                    const int off = (from * (int)a.out_t + 4 * g) * (int)sizeof(T);
+#pragma unroll
+                    for (int v = 0; v < VT; ++v) {
+                        const int to = p >= begin && v * 16 + 4 * g < vleft ? off + v * 16 * (int)sizeof(T) : kNowhere;
+                        if constexpr (F32) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, acc[v]), r, to, 0, 0);
+                        else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, __builtin_convertvector(acc[v], b4)), r, to, 0, 0);
+                    }
+                } else if (p >= begin) {
+                    T* o = out + place(p) * a.out_t;
+#pragma unroll
+                    for (int v = 0; v < VT; ++v)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (v * 16 + 4 * g + r < vleft) o[v * 16 + 4 * g + r] = (T)acc[v][r];
+                }
+            };
             if constexpr (MODE == LEAKY_SLOPE) {
                 f4 dacc[VT], dscores[4];
                 of_state(dacc, 1);
                 {
                     f4 acc[VT];
                     of_state(acc, 0);
-                    const float reach_slope = slope_at(powers, i);
+                    const float reach_slope = slope_at(powers, i) * a.state_scale;
 #pragma unroll
                     for (int v = 0; v < VT; ++v) dacc[v] = dacc[v] * reach + acc[v] * reach_slope;
                 }
@@ -388,14 +468,14 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int back = (w - s) * 16 + col - 4 * g - r;
-                        dscores[s][r] = s > w || back < 1 ? 0.f : scores[s][r] * slope_at(powers, s > w ? 0 : back);
+                        dscores[s][r] = s > w || back < 1 ? 0.f : scores[s][r] * (slope_at(powers, s > w ? 0 : back) * a.score_scale);
                     }
 #pragma unroll
                 for (int d = 0; d < kChunk / D; ++d) {
                     if (d * D > w * 16) continue;
                     F vf[VT];
 #pragma unroll
-                    for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D);
+                    for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
                     add_values(dacc, dscores, d, vf);
                 }
                 if (p >= begin) {
@@ -411,9 +491,18 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
             f4 acc[VT];
             if constexpr (MAIN) {
                 of_state(acc, 0);
-                if (more) fetch_query(p0 + kChunk);
+                LEAKY_FENCE;
+                if (more) fetch_query(0, g, col);
 #pragma unroll
                 for (int v = 0; v < VT; ++v) acc[v] *= reach;
+                // weights of the scores: key 4g + r of the strip of this lane's place, and of strips in front of it, in which a
+                // factor a^(16 strips) is left out
+                float near[4], far[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    near[r] = weights[16 + col - 4 * g - r];
+                    far[r] = weights[32 + col - 4 * g - r];
+                }
 #pragma unroll
                 for (int s = 0; s <= w; ++s)
 #pragma unroll
@@ -421,26 +510,40 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                         scores[s][r] = s == w ? (col >= 4 * g + r ? scores[s][r] * near[r] : 0.f)
                                               : scores[s][r] * (s + 1 == w ? far[r] : far[r] * apart[w - s - 1]);
             }
+            constexpr bool APART = F32 && MAIN;                              // values read twice rather than all sums kept at once
+            if constexpr (APART) {
+#pragma unroll
+                for (int d = 0; d < kChunk / D; ++d) {
+                    if (d * D > w * 16) continue;
+                    LEAKY_FENCE;
+                    F vf[VT];
+#pragma unroll
+                    for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
+                    add_values(acc, scores, d, vf);
+                }
+                store(acc);
+            }
 #pragma unroll
             for (int s = 0; s < ST; ++s)
 #pragma unroll
                 for (int v = 0; v < VT; ++v) {
                     if constexpr (SLOPE) W[s][v] = W[s][v] * step_hi + S[s][v] * step_slope;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) S[s][v][r] = fmaf(S[s][v][r], step_hi, S[s][v][r] * step_lo);
+                    for (int r = 0; r < 4; ++r) S[s][v][r] = FINE ? fmaf(S[s][v][r], step_hi, S[s][v][r] * step_lo) : S[s][v][r] * step_hi;
                 }
 #pragma unroll
             for (int d = 0; d < kChunk / D; ++d) {
+                LEAKY_FENCE;
                 F vf[VT];                                                    // values, terms across the places
 #pragma unroll
-                for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D);
-                if constexpr (MAIN) {
+                for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
+                if constexpr (MAIN && !APART) {
                     if (d * D <= w * 16) add_values(acc, scores, d, vf);
                 }
 #pragma unroll
                 for (int s = 0; s < ST; ++s) {
                     if (s * 4 + w >= KT) continue;
-                    const F kf = across(lk, kPitch, (s * 4 + w) * 16, d * D);
+                    const F kf = across(lk, kPitch, (s * 4 + w) * 16, d * D, lane);
                     auto add_keys = [&](f4 (&to)[VT], const float* weights) {
                         const f4 w0 = *reinterpret_cast<const f4*>(weights + d * D + 4 * g);
                         if constexpr (F32) {
@@ -449,9 +552,9 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                             for (int v = 0; v < VT; ++v) to[v] = mma(x, vf[v], to[v]);
                         } else {
                             const f4 w1 = *reinterpret_cast<const f4*>(weights + d * D + 16 + 4 * g);
-                            const auto x = split<3>(__builtin_convertvector(kf, f8) * __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7));
+                            const auto x = split<FINE ? 3 : 2>(__builtin_convertvector(kf, f8) * __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                            for (int part = 0; part < 3; ++part)
+                            for (int part = 0; part < (FINE ? 3 : 2); ++part)
 #pragma unroll
                                 for (int v = 0; v < VT; ++v) to[v] = mma(x.part[part], vf[v], to[v]);
                         }
@@ -460,24 +563,7 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                     if constexpr (SLOPE) add_keys(W[s], behind[1]);
                 }
             }
-            if constexpr (MAIN) {
-                if (p >= begin) {
-                    T* o = out + place(p) * a.out_t;
-#pragma unroll
-                    for (int v = 0; v < VT; ++v) {
-                        const int c = v * 16 + 4 * g;
-                        const f4 y = acc[v] * a.out_scale;
-                        if (a.whole_out && c + 4 <= vleft) {
-                            if constexpr (F32) *reinterpret_cast<f4*>(o + c) = y;
-                            else *reinterpret_cast<b4*>(o + c) = __builtin_convertvector(y, b4);
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (c + r < vleft) o[c + r] = (T)y[r];
-                        }
-                    }
-                }
-            }
+            if constexpr (MAIN && !APART) store(acc);
         };
         if (wave == 0) chunk(std::integral_constant<int, 0>{});
         else if (wave == 1) chunk(std::integral_constant<int, 1>{});
@@ -495,7 +581,7 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
         to = a.last + unit * state_size;
     }
     const float* grad_last = MODE == LEAKY_SLOPE && last && a.grad_last ? a.grad_last + unit * state_size : nullptr;
-    double slope = (double)total * a.out_scale;
+    double slope = total;
     if (to || grad_last) {
 #pragma unroll
         for (int s = 0; s < ST; ++s)
