@@ -280,14 +280,14 @@ extern "C" int slayer_leaky_attention_bwd(void* grad_query, void* grad_key, void
     hipStream_t s = (hipStream_t)stream;
     if (a->samples == 0) return grad_decay ? launch_zero_fill(grad_decay, a->num_decays, s) : 0;
     if (a->tokens > 0 && (!grad_out || !query || !key || !value)) return SLAYER_ENULL;
-    if (!workspace || (grad_state && !grad_value) || (grad_decay && !grad_query)) return SLAYER_ENULL;
+    if (!workspace || (a->tokens > 0 && ((grad_state && !grad_value) || (grad_decay && !grad_query)))) return SLAYER_ENULL;
     if (floats < slayer_leaky_attention_workspace(a, 1)) return SLAYER_EINVAL;
     const int K = (int)a->keys, V = (int)a->values;
     const Contiguous k(a, K), v(a, V);
     float *space = workspace + 2 * slope_count(a), *slope_starts = space + starts_floats(a);
     const Place q{query, a->query_stride}, kk{key, a->key_stride}, vv{value, a->value_stride}, g{grad_out, a->grad_stride};
     const Slope slope{(double*)workspace, grad_last, q, slope_starts};
-    if (grad_query) {
+    if (grad_query || grad_decay) {                          // (with no tokens there may be no tensors either)
         const bool ready = starts && !grad_decay;            // the states of the forward call are those of this pass
         if (int e = run_pass(a, grad_query, k.stride, g, vv, kk, V, K, true, false, state, nullptr, grad_decay ? &slope : nullptr,
                              ready ? const_cast<float*>(starts) : space, ready, s)) return e;
@@ -298,7 +298,7 @@ extern "C" int slayer_leaky_attention_bwd(void* grad_query, void* grad_key, void
             if (int e = (int)hipGetLastError()) return e;
         }
     }
-    if (grad_value)
+    if (grad_value || grad_state)
         if (int e = run_pass(a, grad_value, v.stride, kk, q, g, K, V, false, true, grad_last, grad_state, nullptr, space, false, s)) return e;
     if (grad_key) return run_pass(a, grad_key, k.stride, vv, g, q, V, K, true, true, grad_last, nullptr, nullptr, space, grad_value != nullptr, s);
     return 0;

@@ -77,8 +77,8 @@ __device__ __forceinline__ b8 across(const bf16* tile, int pitch, int column, in
 }
 
 // A float32 operand: in float32, or as bfloat16 numbers that sum to it, so that what the kernel makes itself is not rounded to
-// the type of the tensors on the way: two for what ends in a result of that type (within 2^-17, a hundredth of what
-// rounding the result costs), three for leaked keys that end in a float32 state (within 2^-25).
+// the type of the tensors on the way: two for what ends in a result of that type (within 2^-16, a 256th of what
+// rounding the result costs), three for leaked keys that end in a float32 state (within 2^-24).
 template <int PARTS> struct Split { b8 part[PARTS]; };
 template <int PARTS>
 __device__ __forceinline__ Split<PARTS> split(f8 v) {
@@ -267,6 +267,8 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
         fetch_rows(begin - p0, threadIdx.x);
     }
 
+    __shared__ int not_finite[2];                                            // the last chunk (of every second) with such values
+    if (threadIdx.x < 2) not_finite[threadIdx.x] = p0 - 1;
     if (threadIdx.x <= kChunk) powers[threadIdx.x] = (float)power(leak, threadIdx.x);
     __syncthreads();
     if (threadIdx.x < kChunk) {
@@ -313,8 +315,6 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
     const float apart[3] = {1.f, powers[16], powers[32]};
     float total = 0;                                                         // LEAKY_SLOPE
 
-    __shared__ int not_finite[2];                                            // the last chunk (of every second) with such values
-    if (threadIdx.x < 2) not_finite[threadIdx.x] = p0 - 1;
     int parity = 0;
     auto fill = [&](int thread, int g, int col) {                            // LDS for the next chunk
         bool bad = false;
