@@ -134,16 +134,31 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 // A segment's workgroup adds up the states of up to so many segments itself (a launch between the two kernels is 10 us).
 constexpr int kJoin = 8;
 
+// Sixteens of values in a slice of up to 64: wide slices, whose scores are worked out once for all of them.
+int slice_tiles(int64_t values) {
+    const int64_t slices = ceil_div(values, 64);
+    return ceil_div(ceil_div(values, slices), 16);
+}
+
 // Segments of a pass: enough workgroups for the chip (512: two a compute unit), and chunks enough in each that reading keys and
 // values a second time for the states in front of them pays.  The same for every pass of a call.
 int segment_tokens(const slayer_attention* a) {
-    const int64_t chunks = a->tokens > 0 ? ceil_div(a->tokens, kChunk) : 1, units = a->samples * a->heads;
+    const int64_t chunks = a->tokens > 0 ? ceil_div(a->tokens, kChunk) : 1;
+    const int64_t units = a->samples * a->heads * ceil_div(a->keys > a->values ? a->keys : a->values, 64);
     int64_t segments = units > 0 ? 512 / units : 1;
     if (segments > chunks / 4) segments = chunks / 4;
     if (segments < 1) segments = 1;
     return ceil_div(chunks, segments) * kChunk;
 }
 int segments_of(const slayer_attention* a) { return a->tokens > 0 ? ceil_div(a->tokens, segment_tokens(a)) : 1; }
+
+// ... and narrower slices where the workgroups leave most of the chip idle.
+int tiles_of(const slayer_attention* a, int64_t values, bool whole) {
+    int tiles = slice_tiles(values);
+    if (!whole) return tiles <= 2 ? 2 : 4;
+    while (tiles > 1 && a->samples * a->heads * segments_of(a) * ceil_div(values, 16 * tiles) <= 64) tiles /= 2;
+    return tiles;
+}
 
 // aligned: every row that starts at `p` with these strides is a multiple of `bytes`
 bool aligned(const void* p, const int64_t (&stride)[3], int size, int bytes) {
@@ -159,7 +174,7 @@ bool whole_rows(const slayer_attention* a, const Place& query, const Place& key,
            query.stride[1] + key.stride[1] + value.stride[1] < ((int64_t)1 << 31) / (kChunk * size) - 256;
 }
 int slices_of(const slayer_attention* a, const Place& query, const Place& key, const Place& value, int keys, int values) {
-    return ceil_div(values, launched_tiles(values, whole_rows(a, query, key, value, keys, values)) * 16);
+    return ceil_div(values, tiles_of(a, values, whole_rows(a, query, key, value, keys, values)) * 16);
 }
 struct Slope { double* slopes; const float* grad_last; Place other; float* starts; };
 
@@ -188,7 +203,8 @@ int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3
     p.state_v = transposed ? keys : 1;
     p.one_decay = a->num_decays == 1;
     p.lengths64 = a->lengths_bytes == 8;
-    p.slices = slices_of(a, query, key, value, keys, values);
+    p.tiles = tiles_of(a, values, whole);
+    p.slices = ceil_div(values, p.tiles * 16);
     p.segment = segment_tokens(a);
     p.segments = segments_of(a);
     p.joined = p.segments > kJoin;
@@ -203,6 +219,8 @@ int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3
         p.other = slope->other.p;
         p.other_n = slope->other.stride[0]; p.other_t = slope->other.stride[1]; p.other_h = slope->other.stride[2];
         p.slopes = slope->slopes;
+        p.whole_other = values % 4 == 0 && aligned(p.other, slope->other.stride, size, 4 * size) &&
+                        p.other_t < ((int64_t)1 << 31) / (kChunk * size) - 256;
     }
     auto launch = [&](int mode) { return f32 ? launch_leaky<float>(p, mode, whole, stream) : launch_leaky<bf16>(p, mode, whole, stream); };
     if (p.segments > 1 && !ready) {

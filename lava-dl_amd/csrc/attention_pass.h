@@ -25,7 +25,9 @@ struct LeakyPass {
     int64_t out_n, out_t, out_h, query_n, query_t, query_h, key_n, key_t, key_h, value_n, value_t, value_h, other_n, other_t, other_h;
     int tokens, heads, keys, values, state_k, state_v;      // the strides of a state's axes
     int units;                     // samples * heads
-    int one_decay, lengths64, segments, segment, slices, backwards, joined;
+    // slices of the values, `tiles` sixteens each (1 to 4; 2 or 4 where rows are not made of whole pieces)
+    int one_decay, lengths64, segments, segment, slices, tiles, backwards, joined;
+    int whole_other;               // `other` comes in fours that can be read at once
     int whole_out;                 // values come in fours that can be written at once, within the reach of a 32-bit offset
     float score_scale, state_scale, key_scale;      // of scores, of the state in results, of keys in the state
 };
@@ -154,7 +156,7 @@ __device__ __forceinline__ float slope_at(const float* powers, int n) { return n
 #define LEAKY_WAVES(T, KT, VT, MODE) 2
 #endif
 template <typename T, int KT, int VT, int MODE, bool WHOLE>
-__global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kernel(LeakyPass a) {
+__global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kernel(LeakyPass a) {
     typedef typename Frag<T>::Type F;
     typedef typename Elements<T>::Vec Vec;
     constexpr bool MAIN = MODE == LEAKY_MAIN || MODE == LEAKY_LAST || MODE == LEAKY_SLOPE, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
@@ -262,8 +264,32 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
             query += turn * a.query_t;
         }
     };
+    // LEAKY_SLOPE: what this lane's results are multiplied with
+    typedef std::conditional_t<F32, f4, b4> Quad;
+    Quad other[MODE == LEAKY_SLOPE ? VT : 1];
+    const T* others = MODE == LEAKY_SLOPE ? (const T*)a.other + n * a.other_n + h * a.other_h + v0 + low0 * a.other_t : nullptr;
+    auto fetch_other = [&](int missing, int g, int col) {
+        if constexpr (MODE == LEAKY_SLOPE) {
+            const int row = wave * 16 + col, from = a.backwards ? kChunk - 1 - row : row;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(others), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+            for (int v = 0; v < VT; ++v) {
+                const int c = v * 16 + 4 * g;
+                if (a.whole_other) {
+                    const int off = row >= missing && c < vleft ? (from * (int)a.other_t + c) * (int)sizeof(T) : kNowhere;
+                    if constexpr (F32) other[v] = __builtin_bit_cast(Quad, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+                    else other[v] = __builtin_bit_cast(Quad, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) other[v][e] = row >= missing && c + e < vleft ? others[from * a.other_t + c + e] : (T)0.f;
+                }
+            }
+            others += turn * a.other_t;
+        }
+    };
     if (stop > begin) {
         fetch_query(begin - p0, g, col);
+        fetch_other(begin - p0, g, col);
         fetch_rows(begin - p0, threadIdx.x);
     }
 
@@ -478,14 +504,11 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                     for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
                     add_values(dacc, dscores, d, vf);
                 }
-                if (p >= begin) {
-                    const T* x = (const T*)a.other + n * a.other_n + h * a.other_h + v0 + place(p) * a.other_t;
 #pragma unroll
-                    for (int v = 0; v < VT; ++v)
+                for (int v = 0; v < VT; ++v)                                 // (0 for places and values that are not there)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (v * 16 + 4 * g + r < vleft) total = fmaf((float)x[v * 16 + 4 * g + r], dacc[v][r], total);
-                }
+                    for (int r = 0; r < 4; ++r) total = fmaf((float)other[v][r], dacc[v][r], total);
+                if (more) fetch_other(0, g, col);
                 __builtin_amdgcn_sched_barrier(0);
             }
             f4 acc[VT];
@@ -510,8 +533,7 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                         scores[s][r] = s == w ? (col >= 4 * g + r ? scores[s][r] * near[r] : 0.f)
                                               : scores[s][r] * (s + 1 == w ? far[r] : far[r] * apart[w - s - 1]);
             }
-            constexpr bool APART = F32 && MAIN;                              // values read twice rather than all sums kept at once
-            if constexpr (APART) {
+            if constexpr (MAIN) {                                            // (values are read twice: fewer sums are kept at once)
 #pragma unroll
                 for (int d = 0; d < kChunk / D; ++d) {
                     if (d * D > w * 16) continue;
@@ -537,9 +559,6 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                 F vf[VT];                                                    // values, terms across the places
 #pragma unroll
                 for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
-                if constexpr (MAIN && !APART) {
-                    if (d * D <= w * 16) add_values(acc, scores, d, vf);
-                }
 #pragma unroll
                 for (int s = 0; s < ST; ++s) {
                     if (s * 4 + w >= KT) continue;
@@ -563,7 +582,6 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
                     if constexpr (SLOPE) add_keys(W[s], behind[1]);
                 }
             }
-            if constexpr (MAIN && !APART) store(acc);
         };
         if (wave == 0) chunk(std::integral_constant<int, 0>{});
         else if (wave == 1) chunk(std::integral_constant<int, 1>{});
@@ -615,15 +633,9 @@ __global__ __launch_bounds__(256, MODE == LEAKY_SLOPE && KT * VT > 16 ? 1 : LEAK
     }
 }
 
-// values of a slice, in sixteens
-inline int slice_tiles(int64_t values) {
-    const int64_t slices = (values + 63) / 64;
-    return (int)(((values + slices - 1) / slices + 15) / 16);
-}
-
 template <typename T, int MODE>
 int launch_leaky_mode(const LeakyPass& p, dim3 grid, bool whole, hipStream_t s) {
-    const int vt = slice_tiles(p.values);
+    const int vt = p.tiles;
 #define LAUNCH(K, V, WHOLE) hipLaunchKernelGGL((leaky_kernel<T, K, V, MODE, WHOLE>), grid, dim3(256), 0, s, p)
 #define BY_KEYS(V, WHOLE)                           \
     if (p.keys <= 32) LAUNCH(2, V, WHOLE);          \
@@ -631,7 +643,7 @@ int launch_leaky_mode(const LeakyPass& p, dim3 grid, bool whole, hipStream_t s) 
     else if (p.keys <= 96) LAUNCH(6, V, WHOLE);     \
     else LAUNCH(8, V, WHOLE)
     if (!whole) {
-        if (vt <= 2) { if (p.keys <= 64) LAUNCH(4, 2, false); else LAUNCH(8, 2, false); }
+        if (vt == 2) { if (p.keys <= 64) LAUNCH(4, 2, false); else LAUNCH(8, 2, false); }
         else { if (p.keys <= 64) LAUNCH(4, 4, false); else LAUNCH(8, 4, false); }
     }
     else if (vt == 1) { BY_KEYS(1, true); }
@@ -641,12 +653,6 @@ int launch_leaky_mode(const LeakyPass& p, dim3 grid, bool whole, hipStream_t s) 
 #undef BY_KEYS
 #undef LAUNCH
     return (int)hipGetLastError();
-}
-
-// Tiles of a slice as the kernel that is launched has them.
-inline int launched_tiles(int64_t values, bool whole) {
-    const int vt = slice_tiles(values);
-    return whole ? vt : vt <= 2 ? 2 : 4;
 }
 
 template <typename T> int launch_leaky(const LeakyPass& p, int mode, bool whole, hipStream_t stream);    // attention_f32.hip, attention_bf16.hip
