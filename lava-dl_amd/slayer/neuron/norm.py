@@ -154,6 +154,7 @@ def _norm_sizes(input, groups):
 
 
 def _norm_fwd(input, weight, bias, groups, eps, activation, keep):
+    """(out, statistics or None): the means and then the scales of all groups, and behind them the call's workspace."""
     dtype = N.ELEMENT_TYPES[input.dtype]
     sizes = _norm_sizes(input, groups)
     lib = N.lib()
@@ -161,45 +162,50 @@ def _norm_fwd(input, weight, bias, groups, eps, activation, keep):
     if floats < 0:
         N.check(int(floats))
     out = torch.empty_like(input)
-    mean = scale = workspace = None
+    stats = mean = scale = workspace = None
     if keep or floats:
-        stats = torch.empty(2 * sizes[0] * groups + floats, dtype=torch.float32, device=input.device)
-        mean, scale, workspace = stats.split((sizes[0] * groups, sizes[0] * groups, floats))
+        count = sizes[0] * groups
+        stats = torch.empty(2 * count + floats, dtype=torch.float32, device=input.device)
+        mean = stats.data_ptr()
+        scale, workspace = mean + 4 * count, mean + 8 * count
     with N.device_guard(input.device):
-        N.check(lib.slayer_group_norm_fwd(N.ptr(out), N.ptr(mean), N.ptr(scale), N.ptr(input), N.ptr(weight), N.ptr(bias),
-                                          dtype, *sizes, eps, activation, N.ptr(workspace), floats, N.stream_handle()))
-    return out, mean, scale
+        N.check(lib.slayer_group_norm_fwd(out.data_ptr(), mean, scale, input.data_ptr(), N.ptr(weight), N.ptr(bias), dtype, *sizes,
+                                          eps, activation, workspace, floats, N.stream_handle()))
+    return out, stats
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input, weight, bias, groups, eps, activation):
         input = input.contiguous()
-        out, mean, scale = _norm_fwd(input, weight, bias, groups, eps, activation, True)
-        ctx.save_for_backward(input, weight, bias, mean, scale)
+        out, stats = _norm_fwd(input, weight, bias, groups, eps, activation, True)
+        ctx.save_for_backward(input, weight, bias, stats)
         ctx.args = (groups, activation)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_output):
-        input, weight, bias, mean, scale = ctx.saved_tensors
+        input, weight, bias, stats = ctx.saved_tensors
         groups, activation = ctx.args
         grad_output = grad_output.contiguous()
         dtype, sizes = N.ELEMENT_TYPES[input.dtype], _norm_sizes(input, groups)
         grad = torch.empty_like(input)
-        wanted = [torch.empty_like(t) if t is not None and need else None
-                  for t, need in ((weight, ctx.needs_input_grad[1]), (bias, ctx.needs_input_grad[2]))]
+        need_weight, need_bias = weight is not None and ctx.needs_input_grad[1], bias is not None and ctx.needs_input_grad[2]
+        channels, mean = sizes[2], stats.data_ptr()
         lib = N.lib()
         floats = lib.slayer_group_norm_workspace(dtype, *sizes, 1)
         if floats < 0:
             N.check(int(floats))
+        sums = torch.empty((2, channels), dtype=torch.float32, device=input.device)
         workspace = torch.empty(floats, dtype=torch.float32, device=input.device)
+        at = sums.data_ptr()
         with N.device_guard(input.device):
-            N.check(lib.slayer_group_norm_bwd(N.ptr(grad), N.ptr(wanted[0]), N.ptr(wanted[1]), N.ptr(grad_output),
-                                              N.ptr(input), N.ptr(mean), N.ptr(scale), N.ptr(weight), N.ptr(bias), dtype,
-                                              *sizes, activation, N.ptr(workspace), floats, N.stream_handle()))
-        return grad, wanted[0], wanted[1], None, None, None
+            N.check(lib.slayer_group_norm_bwd(grad.data_ptr(), at if need_weight else None, at + 4 * channels if need_bias else None,
+                                              grad_output.data_ptr(), input.data_ptr(), mean, mean + 4 * sizes[0] * groups,
+                                              N.ptr(weight), N.ptr(bias), dtype, *sizes, activation, workspace.data_ptr(), floats,
+                                              N.stream_handle()))
+        return grad, sums[0] if need_weight else None, sums[1] if need_bias else None, None, None, None
 
 
 class GroupNorm(torch.nn.Module):
