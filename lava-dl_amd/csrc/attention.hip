@@ -140,13 +140,14 @@ int slice_tiles(int64_t values) {
     return ceil_div(ceil_div(values, slices), 16);
 }
 
-// Segments of a pass: enough workgroups for the chip (512: two a compute unit), and chunks enough in each that reading keys and
-// values a second time for the states in front of them pays.  The same for every pass of a call.
+// Segments of a pass: up to 512 workgroups, two a compute unit, from two chunks each on.  Keys and values are then read a second time
+// for the states in front of them: [8,1000,4,64] float32, forward, 42 us with segments of four chunks, 32 with two; seven chunks
+// and fewer are faster in one piece ([4,256,16,64] float32: 20 us, 23 in two).  The same for every pass of a call.
 int segment_tokens(const slayer_attention* a) {
     const int64_t chunks = a->tokens > 0 ? ceil_div(a->tokens, kChunk) : 1;
     const int64_t units = a->samples * a->heads * ceil_div(a->keys > a->values ? a->keys : a->values, 64);
-    int64_t segments = units > 0 ? 512 / units : 1;
-    if (segments > chunks / 4) segments = chunks / 4;
+    int64_t segments = units > 0 && chunks >= 8 ? 512 / units : 1;
+    if (segments > chunks / 2) segments = chunks / 2;
     if (segments < 1) segments = 1;
     return ceil_div(chunks, segments) * kChunk;
 }

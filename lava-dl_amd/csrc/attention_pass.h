@@ -80,7 +80,7 @@ __device__ __forceinline__ b8 across(const bf16* tile, int pitch, int column, in
 
 // A float32 operand: in float32, or as bfloat16 numbers that sum to it, so that what the kernel makes itself is not rounded to
 // the type of the tensors on the way: two for what ends in a result of that type (within 2^-16, a 256th of what
-// rounding the result costs), three for leaked keys that end in a float32 state (within 2^-24).
+// rounding the result costs), three for what ends in a float32 state or in the decays' gradient (within 2^-24).
 template <int PARTS> struct Split { b8 part[PARTS]; };
 template <int PARTS>
 __device__ __forceinline__ Split<PARTS> split(f8 v) {
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
     typedef typename Elements<T>::Vec Vec;
     constexpr bool MAIN = MODE == LEAKY_MAIN || MODE == LEAKY_LAST || MODE == LEAKY_SLOPE, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
     constexpr bool FINE = F32 || MODE != LEAKY_MAIN;                         // the state to float32, not to a hundredth of bfloat16
-    constexpr int V = Elements<T>::kVec, D = Frag<T>::kDepth, P = F32 ? 1 : 2;       // parts of a state in LDS
+    constexpr int V = Elements<T>::kVec, D = Frag<T>::kDepth, P = F32 ? 1 : MODE == LEAKY_SLOPE ? 3 : 2;      // parts of a state in LDS
     constexpr int KP = KT * 16, VP = VT * 16;
     // rows of LDS: sixteen rows of keys, read along, start in different banks; so do the eight (float32: four) rows of values that
     // an access across them touches
@@ -209,9 +209,12 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
         if constexpr (F32) {
             *reinterpret_cast<f4*>(p) = x;
         } else {
-            const b4 hi = __builtin_convertvector(x, b4);
-            *reinterpret_cast<b4*>(p) = hi;
-            *reinterpret_cast<b4*>(p + VP * kPitch) = __builtin_convertvector(x - __builtin_convertvector(hi, f4), b4);
+#pragma unroll
+            for (int part = 0; part < P; ++part) {
+                const b4 y = __builtin_convertvector(x, b4);
+                *reinterpret_cast<b4*>(p + part * VP * kPitch) = y;
+                x -= __builtin_convertvector(y, f4);
+            }
         }
     };
 
@@ -395,15 +398,16 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
             constexpr int w = decltype(which)::value;
             f4 scores[4];
             // adds the products of weighted scores and values
-            auto weigh = [&](F v, const f4 (&from)[4], int d, f4 to) {
+            auto weigh = [&](F v, const f4 (&from)[4], int d, f4 to, auto parts) {
                 if constexpr (F32) {
                     return mma(v, from[d], to);
                 } else {
-                    const auto x = split<2>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-                    return mma(v, x.part[1], mma(v, x.part[0], to));
+                    const auto x = split<decltype(parts)::value>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    for (int part = 0; part < decltype(parts)::value; ++part) to = mma(v, x.part[part], to);
+                    return to;
                 }
             };
-            auto add_values = [&](f4 (&to)[VT], const f4 (&from)[4], int d, const F (&vf)[VT]) {
+            auto add_values = [&](f4 (&to)[VT], const f4 (&from)[4], int d, const F (&vf)[VT], auto parts) {
                 if (odd_values && (d + 1) * D > w * 16) {                    // some of these scores are masked
                     F there, none, one;                                      // `there`: 1 for places up to this lane's
 #pragma unroll
@@ -415,7 +419,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
 #pragma unroll
                     for (int v = 0; v < VT; ++v) {
                         const f4 reached = mma(where_not_finite(vf[v], one, none), there, f4{0, 0, 0, 0});
-                        to[v] = weigh(where_not_finite(vf[v], none, vf[v]), from, d, to[v]);
+                        to[v] = weigh(where_not_finite(vf[v], none, vf[v]), from, d, to[v], parts);
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             if (reached[r] > 0.f) to[v][r] = __builtin_nanf("");
@@ -426,21 +430,21 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
 #pragma unroll
                     for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], from[d], to[v]);
                 } else {
-                    const auto x = split<2>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    const auto x = split<decltype(parts)::value>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                    for (int part = 0; part < 2; ++part)
+                    for (int part = 0; part < decltype(parts)::value; ++part)
 #pragma unroll
                         for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], x.part[part], to[v]);
                 }
             };
             // the state's part of the results
-            auto of_state = [&](f4 (&to)[VT], int which) {
+            auto of_state = [&](f4 (&to)[VT], int which, int parts) {
 #pragma unroll
                 for (int v = 0; v < VT; ++v) to[v] = f4{0, 0, 0, 0};
 #pragma unroll
                 for (int d = 0; d < KP / D; ++d)
 #pragma unroll
-                    for (int part = 0; part < P; ++part)
+                    for (int part = 0; part < (parts < P ? parts : P); ++part)
 #pragma unroll
                         for (int v = 0; v < VT; ++v)
                             to[v] = mma(along(ls + (which * P + part) * VP * kPitch, kPitch, v * 16, d * D, lane), qf[d], to[v]);
@@ -481,28 +485,29 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
             };
             if constexpr (MODE == LEAKY_SLOPE) {
                 f4 dacc[VT], dscores[4];
-                of_state(dacc, 1);
+                of_state(dacc, 1, 3);
                 {
                     f4 acc[VT];
-                    of_state(acc, 0);
+                    of_state(acc, 0, 3);
                     const float reach_slope = slope_at(powers, i) * a.state_scale;
 #pragma unroll
                     for (int v = 0; v < VT; ++v) dacc[v] = dacc[v] * reach + acc[v] * reach_slope;
                 }
 #pragma unroll
-                for (int s = 0; s < 4; ++s)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int back = (w - s) * 16 + col - 4 * g - r;
-                        dscores[s][r] = s > w || back < 1 ? 0.f : scores[s][r] * (slope_at(powers, s > w ? 0 : back) * a.score_scale);
-                    }
-#pragma unroll
                 for (int d = 0; d < kChunk / D; ++d) {
                     if (d * D > w * 16) continue;
+                    LEAKY_FENCE;
+#pragma unroll
+                    for (int s = d * D / 16; s < (d + 1) * D / 16; ++s)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int back = (w - s) * 16 + col - 4 * g - r;
+                            dscores[s][r] = s > w || back < 1 ? 0.f : scores[s][r] * (slope_at(powers, s > w ? 0 : back) * a.score_scale);
+                        }
                     F vf[VT];
 #pragma unroll
                     for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
-                    add_values(dacc, dscores, d, vf);
+                    add_values(dacc, dscores, d, vf, std::integral_constant<int, 3>{});
                 }
 #pragma unroll
                 for (int v = 0; v < VT; ++v)                                 // (0 for places and values that are not there)
@@ -513,7 +518,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
             }
             f4 acc[VT];
             if constexpr (MAIN) {
-                of_state(acc, 0);
+                of_state(acc, 0, 2);
                 LEAKY_FENCE;
                 if (more) fetch_query(0, g, col);
 #pragma unroll
@@ -541,7 +546,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
                     F vf[VT];
 #pragma unroll
                     for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
-                    add_values(acc, scores, d, vf);
+                    add_values(acc, scores, d, vf, std::integral_constant<int, 2>{});
                 }
                 store(acc);
             }

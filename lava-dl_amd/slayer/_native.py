@@ -245,7 +245,15 @@ ELEMENT_TYPES = {torch.float32: 0, torch.bfloat16: 1}
 def require_elements(*tensors):
     """``require_gpu`` for the operators that also take bfloat16: (device, number of the type all tensors share)."""
     first = tensors[0]
-    for t in tensors:
+    if torch.is_tensor(first) and first.is_cuda:
+        device, dtype = first.device, first.dtype
+        for t in tensors:
+            if not torch.is_tensor(t) or t.dtype is not dtype or t.device != device:
+                break
+        else:
+            if dtype in ELEMENT_TYPES:
+                return device, ELEMENT_TYPES[dtype]
+    for t in tensors:                             # which of them it is
         if not torch.is_tensor(t):
             raise RuntimeError(f'expected a tensor, got {type(t)}')
         if not t.is_cuda:
@@ -257,7 +265,7 @@ def require_elements(*tensors):
             raise RuntimeError(f'tensors of different types: {first.dtype} and {t.dtype}')
         if t.device != first.device:
             raise RuntimeError(f'tensors on different devices: {first.device} and {t.device}')
-    return first.device, ELEMENT_TYPES[first.dtype]
+    raise RuntimeError('tensors that do not belong together')
 
 
 def scan_tolerance(grad):

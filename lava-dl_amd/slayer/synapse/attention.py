@@ -3,8 +3,6 @@
 The state of a head is a matrix that leaks like the current of a CUBA neuron and is driven by outer products of keys and
 values instead of weighted spikes.  The bodies are slayer_leaky_attention_fwd / bwd / step of libslayer_hip.so.
 """
-import ctypes
-
 import torch
 
 from .. import _native as N
@@ -84,11 +82,12 @@ def leaky_attention_step(query, key, value, decay, state, scale=1.0):
     torch.Tensor [N, H, V] of the type of the inputs.  There is no gradient: the state it would need is overwritten.
     """
     device, dtype = N.require_elements(query, key, value)
-    if query.dim() != 3 or key.shape != query.shape or value.dim() != 3 or value.shape[:2] != query.shape[:2]:
+    shape, wide = query.shape, value.shape
+    if len(shape) != 3 or key.shape != shape or len(wide) != 3 or wide[:2] != shape[:2]:
         raise RuntimeError(f'expected query and key [N, H, K] and value [N, H, V], got {tuple(query.shape)}, '
                            f'{tuple(key.shape)} and {tuple(value.shape)}')
-    n, h, k = query.shape
-    v = value.shape[2]
+    n, h, k = shape
+    v = wide[2]
     _check_sizes(h, k, v)
     _check_decay(decay, h, device)
     _check_state(state, (n, h, k, v), device)
@@ -97,13 +96,12 @@ def leaky_attention_step(query, key, value, decay, state, scale=1.0):
     if N.wants_grad(query, key, value, decay, state):
         raise RuntimeError('leaky_attention_step has no gradient: call it under torch.no_grad(), or leaky_attention')
     query, key, value, decay = _rows(query), _rows(key), _rows(value), decay.contiguous()
-    out = torch.empty((n, h, v), dtype=query.dtype, device=device)
-    args = _arguments(n, 1, h, k, v, dtype, decay, None, scale)
-    for name, x in (('query', query), ('key', key), ('value', value)):
-        getattr(args, name + '_stride')[:] = (x.stride(0), 0, x.stride(1))
+    out = torch.empty(wide, dtype=query.dtype, device=device)
+    (qn, qh, _), (kn, kh, _), (vn, vh, _) = query.stride(), key.stride(), value.stride()
+    args = N.Attention(n, 1, h, k, v, decay.numel(), decay.data_ptr(), None, 0, dtype, scale, (qn, 0, qh), (kn, 0, kh), (vn, 0, vh))
     with N.device_guard(device):
-        N.check(N.lib().slayer_leaky_attention_step(N.ptr(out), N.ptr(state), N.ptr(query), N.ptr(key), N.ptr(value),
-                                                    ctypes.byref(args), N.stream_handle()))
+        N.check(N.lib().slayer_leaky_attention_step(out.data_ptr(), state.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(),
+                                                    args, N.stream_handle()))
     return out
 
 
@@ -114,14 +112,14 @@ def _check_sizes(heads, keys, values):
 
 
 def _check_decay(decay, heads, device):
-    if not torch.is_tensor(decay) or decay.dtype != torch.float32 or decay.shape not in ((1,), (heads,)):
+    if not torch.is_tensor(decay) or decay.dtype is not torch.float32 or decay.dim() != 1 or decay.shape[0] not in (1, heads):
         raise RuntimeError(f'decay: expected one float32 value or {heads}')
     if decay.device != device:
         raise RuntimeError(f'tensors on different devices: {device} and {decay.device}')
 
 
 def _check_state(state, shape, device):
-    if not torch.is_tensor(state) or state.dtype != torch.float32 or tuple(state.shape) != shape:
+    if not torch.is_tensor(state) or state.dtype is not torch.float32 or state.shape != shape:
         raise RuntimeError(f'state: expected a float32 tensor {list(shape)}')
     if state.device != device:
         raise RuntimeError(f'tensors on different devices: {device} and {state.device}')
@@ -132,21 +130,16 @@ def _rows(x):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def _arguments(n, t, h, k, v, dtype, decay, lengths, scale):
-    return N.Attention(n, t, h, k, v, decay.numel(), N.ptr(decay), N.ptr(lengths),
-                       0 if lengths is None else lengths.element_size(), dtype, scale)
-
-
 def _call(query, key, value, decay, lengths, scale):
     """The structure of the C calls."""
     n, t, h, k = query.shape
-    args = _arguments(n, t, h, k, value.shape[3], N.ELEMENT_TYPES[query.dtype], decay, lengths, scale)
-    args.query_stride[:], args.key_stride[:], args.value_stride[:] = query.stride()[:3], key.stride()[:3], value.stride()[:3]
-    return args
+    return N.Attention(n, t, h, k, value.shape[3], decay.numel(), decay.data_ptr(), N.ptr(lengths),
+                       0 if lengths is None else lengths.element_size(), N.ELEMENT_TYPES[query.dtype], scale, query.stride()[:3],
+                       key.stride()[:3], value.stride()[:3])
 
 
 def _workspace(args, backward, device):
-    floats = N.lib().slayer_leaky_attention_workspace(ctypes.byref(args), backward)
+    floats = N.lib().slayer_leaky_attention_workspace(args, backward)
     if floats < 0:
         N.check(int(floats))
     return torch.empty(floats, dtype=torch.float32, device=device) if floats else None, floats
@@ -163,7 +156,7 @@ def _forward(query, key, value, decay, state, lengths, scale, return_state):
     with N.device_guard(query.device):
         workspace, floats = _workspace(args, 0, query.device)
         N.check(N.lib().slayer_leaky_attention_fwd(N.ptr(out), N.ptr(last), N.ptr(query), N.ptr(key), N.ptr(value), N.ptr(state),
-                                                   ctypes.byref(args), N.ptr(workspace), floats, N.stream_handle()))
+                                                   args, N.ptr(workspace), floats, N.stream_handle()))
     return out, last, query, key, value, decay, state, workspace
 
 
@@ -195,5 +188,5 @@ class _LeakyAttention(torch.autograd.Function):
             workspace, floats = _workspace(args, 1, query.device)
             N.check(N.lib().slayer_leaky_attention_bwd(*(N.ptr(x) for x in new), N.ptr(grad_out), N.ptr(grad_last), N.ptr(query),
                                                        N.ptr(key), N.ptr(value), N.ptr(state), N.ptr(starts),
-                                                       ctypes.byref(args), N.ptr(workspace), floats, N.stream_handle()))
+                                                       args, N.ptr(workspace), floats, N.stream_handle()))
         return (*(x if wanted else None for x, wanted in zip(new, need)), None, None, None)
