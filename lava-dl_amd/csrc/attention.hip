@@ -177,12 +177,13 @@ bool whole_rows(const slayer_attention* a, const Place& query, const Place& key,
 int slices_of(const slayer_attention* a, const Place& query, const Place& key, const Place& value, int keys, int values) {
     return ceil_div(values, tiles_of(a, values, whole_rows(a, query, key, value, keys, values)) * 16);
 }
+struct Both { void* out; const int64_t (&out_stride)[3]; Place query; };
 struct Slope { double* slopes; const float* grad_last; Place other; float* starts; };
 
 // One pass with its segments: states in front of them, joined, unless they are there already (`ready`), and the main kernel.
 int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3], Place query, Place key, Place value, int keys,
-             int values, bool transposed, bool backwards, const float* first, float* last, const Slope* slope, float* starts, bool ready,
-             hipStream_t stream) {
+             int values, bool transposed, bool backwards, const float* first, float* last, const Slope* slope, const Both* both, float* starts,
+             bool ready, hipStream_t stream) {
     const bool f32 = a->dtype == SLAYER_FLOAT32;
     const int size = f32 ? 4 : 2;
     const bool whole = whole_rows(a, query, key, value, keys, values);
@@ -204,7 +205,7 @@ int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3
     p.state_v = transposed ? keys : 1;
     p.one_decay = a->num_decays == 1;
     p.lengths64 = a->lengths_bytes == 8;
-    p.tiles = tiles_of(a, values, whole);
+    p.tiles = both ? (values <= 32 ? 2 : 4) : tiles_of(a, values, whole);
     p.slices = ceil_div(values, p.tiles * 16);
     p.segment = segment_tokens(a);
     p.segments = segments_of(a);
@@ -214,6 +215,14 @@ int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3
     p.score_scale = (float)a->scale;
     p.state_scale = backwards ? 1.f : (float)a->scale;    // backwards the state it starts from is not scaled, but what is added to it
     p.key_scale = backwards ? (float)a->scale : 1.f;
+    if (both) {
+        p.out2 = both->out;
+        p.query2 = both->query.p;
+        p.query2_n = both->query.stride[0]; p.query2_t = both->query.stride[1]; p.query2_h = both->query.stride[2];
+        p.out2_n = both->out_stride[0]; p.out2_t = both->out_stride[1]; p.out2_h = both->out_stride[2];
+        p.whole_out2 = keys % 4 == 0 && aligned(both->out, both->out_stride, size, 4 * size) &&
+                       both->out_stride[1] < ((int64_t)1 << 31) / (kChunk * size) - 256;
+    }
     if (slope) {
         p.slope_starts = slope->starts;
         p.grad_last = slope->grad_last;
@@ -233,7 +242,7 @@ int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3
         hipLaunchKernelGGL(leaky_join_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p);
         if (int e = (int)hipGetLastError()) return e;
     }
-    return launch(slope ? LEAKY_SLOPE : last ? LEAKY_LAST : LEAKY_MAIN);
+    return launch(slope ? LEAKY_SLOPE : both ? (last ? LEAKY_BOTH_LAST : LEAKY_BOTH) : last ? LEAKY_LAST : LEAKY_MAIN);
 }
 
 // Floats of the states in front of the segments.
@@ -288,7 +297,7 @@ extern "C" int slayer_leaky_attention_fwd(void* out, float* last, const void* qu
     if (floats < need) return SLAYER_EINVAL;
     const Contiguous o(a, a->values);
     return run_pass(a, out, o.stride, {query, a->query_stride}, {key, a->key_stride}, {value, a->value_stride}, (int)a->keys, (int)a->values,
-                    false, false, state, last, nullptr, workspace, false, (hipStream_t)stream);
+                    false, false, state, last, nullptr, nullptr, workspace, false, (hipStream_t)stream);
 }
 
 extern "C" int slayer_leaky_attention_bwd(void* grad_query, void* grad_key, void* grad_value, float* grad_decay, float* grad_state,
@@ -308,7 +317,7 @@ extern "C" int slayer_leaky_attention_bwd(void* grad_query, void* grad_key, void
     const Slope slope{(double*)workspace, grad_last, q, slope_starts};
     if (grad_query || grad_decay) {                          // (with no tokens there may be no tensors either)
         const bool ready = starts && !grad_decay;            // the states of the forward call are those of this pass
-        if (int e = run_pass(a, grad_query, k.stride, g, vv, kk, V, K, true, false, state, nullptr, grad_decay ? &slope : nullptr,
+        if (int e = run_pass(a, grad_query, k.stride, g, vv, kk, V, K, true, false, state, nullptr, grad_decay ? &slope : nullptr, nullptr,
                              ready ? const_cast<float*>(starts) : space, ready, s)) return e;
         if (grad_decay) {
             const int parts = segments_of(a) * slices_of(a, g, vv, kk, V, K);
@@ -317,9 +326,16 @@ extern "C" int slayer_leaky_attention_bwd(void* grad_query, void* grad_key, void
             if (int e = (int)hipGetLastError()) return e;
         }
     }
+    // value's and key's gradients in one pass where its workgroups hold a whole head of 64 keys and values; in narrow slices, whose
+    // chunks take less time, where there are few of them
+    if (grad_value && grad_key && K <= 64 && V <= 64 && whole_rows(a, kk, q, g, K, V) && whole_rows(a, vv, g, q, V, K) &&
+        a->samples * a->heads * segments_of(a) > 64) {
+        const Both both{grad_key, k.stride, vv};
+        return run_pass(a, grad_value, v.stride, kk, q, g, K, V, false, true, grad_last, grad_state, nullptr, &both, space, false, s);
+    }
     if (grad_value || grad_state)
-        if (int e = run_pass(a, grad_value, v.stride, kk, q, g, K, V, false, true, grad_last, grad_state, nullptr, space, false, s)) return e;
-    if (grad_key) return run_pass(a, grad_key, k.stride, vv, g, q, V, K, true, true, grad_last, nullptr, nullptr, space, grad_value != nullptr, s);
+        if (int e = run_pass(a, grad_value, v.stride, kk, q, g, K, V, false, true, grad_last, grad_state, nullptr, nullptr, space, false, s)) return e;
+    if (grad_key) return run_pass(a, grad_key, k.stride, vv, g, q, V, K, true, true, grad_last, nullptr, nullptr, nullptr, space, grad_value != nullptr, s);
     return 0;
 }
 

@@ -20,14 +20,18 @@ struct LeakyPass {
     float* last;                   // state behind the last token, or nullptr
     float* slope_starts;           // LEAKY_SLOPE: derivatives of the states in `starts`
     const float* grad_last;        // LEAKY_SLOPE: gradient of the last state, or nullptr
+    const void* query2;            // LEAKY_BOTH
+    void* out2;
     const void* other;             // LEAKY_SLOPE: what the derivative of the results is multiplied with, laid out as they are
     double* slopes;                // LEAKY_SLOPE: [samples][heads][segments][slices]
     int64_t out_n, out_t, out_h, query_n, query_t, query_h, key_n, key_t, key_h, value_n, value_t, value_h, other_n, other_t, other_h;
+    int64_t query2_n, query2_t, query2_h, out2_n, out2_t, out2_h;
     int tokens, heads, keys, values, state_k, state_v;      // the strides of a state's axes
     int units;                     // samples * heads
     // slices of the values, `tiles` sixteens each (1 to 4; 2 or 4 where rows are not made of whole pieces)
     int one_decay, lengths64, segments, segment, slices, tiles, backwards, joined;
     int whole_other;               // `other` comes in fours that can be read at once
+    int whole_out2;
     int whole_out;                 // values come in fours that can be written at once, within the reach of a 32-bit offset
     float score_scale, state_scale, key_scale;      // of scores, of the state in results, of keys in the state
 };
@@ -58,6 +62,12 @@ __device__ __forceinline__ f4 mma(b8 a, b8 b, f4 c) { return __builtin_amdgcn_mf
 template <typename T>
 __device__ __forceinline__ typename Frag<T>::Type along(const T* tile, int pitch, int row, int term, int lane) {
     return *reinterpret_cast<const typename Frag<T>::Type*>(tile + (row + (lane & 15)) * pitch + term + (lane >> 4) * Elements<T>::kVec);
+}
+// ... in halves (float32: the same)
+__device__ __forceinline__ f4 along_halves(const float* tile, int pitch, int row, int term, int lane) { return along(tile, pitch, row, term, lane); }
+__device__ __forceinline__ b8 along_halves(const bf16* tile, int pitch, int row, int term, int lane) {
+    const bf16* p = tile + (row + (lane & 15)) * pitch + term + (lane >> 4) * 4;
+    return __builtin_shufflevector(*reinterpret_cast<const b4*>(p), *reinterpret_cast<const b4*>(p + 16), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 // terms across the rows of `tile`, the sixteen columns from `column` on
 __device__ __forceinline__ f4 across(const float* tile, int pitch, int column, int term, int lane) {
@@ -109,7 +119,7 @@ __device__ __forceinline__ int sample_length(const LeakyPass& a, int n) {
 }
 
 
-enum { LEAKY_STATE, LEAKY_MAIN, LEAKY_LAST, LEAKY_STATE_SLOPE, LEAKY_SLOPE };
+enum { LEAKY_STATE, LEAKY_MAIN, LEAKY_LAST, LEAKY_BOTH, LEAKY_BOTH_LAST, LEAKY_STATE_SLOPE, LEAKY_SLOPE };
 
 // Values that are not finite.  A score that the mask leaves out is 0, and 0 times such a value is not: a strip with masked scores takes
 // the products without these values and says which results they belong to.
@@ -141,6 +151,9 @@ __device__ __forceinline__ float slope_at(const float* powers, int n) { return n
 // The first chunk is the one that is not full, with its tokens at the end, so that weights behind a token are the same in all.
 //   LEAKY_STATE: only the state, from zero, into `starts` behind the segment's place (for the segments but the last).
 //   LEAKY_LAST:  results and the last state, which is held more exactly than results of bfloat16 need.
+//   LEAKY_BOTH:  the gradients of value and key together: beside out[i], from query and key, also out2[i], from query2 and value,
+//       out2[i] = a^i query2[i] S^T + sum over j <= i of a^(i-j) (query2[i] . value[j]) key[j],
+//     for which the state and the chunk's keys and values (queries and gradients) are there already.  One slice.  LEAKY_BOTH_LAST.
 //   LEAKY_SLOPE: results, and the derivative of each with respect to a, in which the state's derivative W takes the place of S:
 //       dout[i] = a^(i+1) query[i] W + (i+1) a^i query[i] S + sum over j of (i-j) a^(i-j-1) (query[i] . key[j]) value[j]
 //       W'      = a^64 W + 64 a^63 S + sum over j of (63-j) a^(62-j) key[j] (outer) value[j]
@@ -159,8 +172,9 @@ template <typename T, int KT, int VT, int MODE, bool WHOLE>
 __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kernel(LeakyPass a) {
     typedef typename Frag<T>::Type F;
     typedef typename Elements<T>::Vec Vec;
-    constexpr bool MAIN = MODE == LEAKY_MAIN || MODE == LEAKY_LAST || MODE == LEAKY_SLOPE, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
-    constexpr bool FINE = F32 || MODE != LEAKY_MAIN;                         // the state to float32, not to a hundredth of bfloat16
+    constexpr bool BOTH = MODE == LEAKY_BOTH || MODE == LEAKY_BOTH_LAST, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
+    constexpr bool MAIN = MODE != LEAKY_STATE && MODE != LEAKY_STATE_SLOPE;
+    constexpr bool FINE = F32 || (MODE != LEAKY_MAIN && MODE != LEAKY_BOTH);                         // the state to float32, not to a hundredth of bfloat16
     constexpr int V = Elements<T>::kVec, D = Frag<T>::kDepth, P = F32 ? 1 : MODE == LEAKY_SLOPE ? 3 : 2;      // parts of a state in LDS
     constexpr int KP = KT * 16, VP = VT * 16;
     // rows of LDS: sixteen rows of keys, read along, start in different banks; so do the eight (float32: four) rows of values that
@@ -201,6 +215,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
     if (!MAIN && end > length) return;                                       // no segment behind it needs this one's state
     const int64_t state_size = (int64_t)a.keys * a.values;
     T* out = (T*)a.out + n * a.out_n + h * a.out_h + v0;
+    T* out2 = BOTH ? (T*)a.out2 + n * a.out2_n + h * a.out2_h : nullptr;
     const int shift = a.backwards ? 0 : 1;
     f4 S[ST][VT], W[SLOPE ? ST : 1][SLOPE ? VT : 1];
     T *keys = tiles, *values = tiles + kTile, *state = tiles + kTile + vTile;
@@ -267,6 +282,29 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
             query += turn * a.query_t;
         }
     };
+    // LEAKY_BOTH: the terms of query2 in halves, as the state is read across its rows
+    F qf2[BOTH ? VP / D : 1];
+    const T* query2 = BOTH ? (const T*)a.query2 + n * a.query2_n + h * a.query2_h + low0 * a.query2_t : nullptr;
+    auto fetch_query2 = [&](int missing, int g, int col) {
+        if constexpr (BOTH) {
+            const int row = wave * 16 + col, from = a.backwards ? kChunk - 1 - row : row;
+            const bool on = row >= missing;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(query2), 0, 0x7fffffff, 0x00020000);
+            const int off = (from * (int)a.query2_t + 4 * g) * (int)sizeof(T);
+#pragma unroll
+            for (int d = 0; d < VP / D; ++d) {
+                const int c = d * D + 4 * g;
+                if constexpr (F32) {
+                    qf2[d] = __builtin_bit_cast(F, __builtin_amdgcn_raw_buffer_load_b128(r, on && c < a.values ? off + d * D * (int)sizeof(T) : kNowhere, 0, 0));
+                } else {
+                    const b4 lo = __builtin_bit_cast(b4, __builtin_amdgcn_raw_buffer_load_b64(r, on && c < a.values ? off + d * D * (int)sizeof(T) : kNowhere, 0, 0));
+                    const b4 hi = __builtin_bit_cast(b4, __builtin_amdgcn_raw_buffer_load_b64(r, on && c + 16 < a.values ? off + (d * D + 16) * (int)sizeof(T) : kNowhere, 0, 0));
+                    qf2[d] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+            }
+            query2 += turn * a.query2_t;
+        }
+    };
     // LEAKY_SLOPE: what this lane's results are multiplied with
     typedef std::conditional_t<F32, f4, b4> Quad;
     Quad other[MODE == LEAKY_SLOPE ? VT : 1];
@@ -292,6 +330,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
     };
     if (stop > begin) {
         fetch_query(begin - p0, g, col);
+        fetch_query2(begin - p0, g, col);
         fetch_other(begin - p0, g, col);
         fetch_rows(begin - p0, threadIdx.x);
     }
@@ -351,6 +390,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
         for (int i = 0; i < kLoads; ++i) {
             const int at = i * 256 + thread;
             if (kChunk * KV % 256 == 0 || at < kChunk * KV) *reinterpret_cast<Vec*>(keys + at / KV * kPitch + at % KV * V) = nk[i];
+            if (BOTH) bad = bad || any_not_finite(nk[i]);
         }
 #pragma unroll
         for (int i = 0; i < vLoads; ++i) {
@@ -407,7 +447,8 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
                     return to;
                 }
             };
-            auto add_values = [&](f4 (&to)[VT], const f4 (&from)[4], int d, const F (&vf)[VT], auto parts) {
+            auto add_values = [&](auto& to, const f4 (&from)[4], int d, const auto& vf, auto parts) {
+                constexpr int N = sizeof(vf) / sizeof(F);
                 if (odd_values && (d + 1) * D > w * 16) {                    // some of these scores are masked
                     F there, none, one;                                      // `there`: 1 for places up to this lane's
 #pragma unroll
@@ -417,7 +458,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
                         one[e] = (T)1.f;
                     }
 #pragma unroll
-                    for (int v = 0; v < VT; ++v) {
+                    for (int v = 0; v < N; ++v) {
                         const f4 reached = mma(where_not_finite(vf[v], one, none), there, f4{0, 0, 0, 0});
                         to[v] = weigh(where_not_finite(vf[v], none, vf[v]), from, d, to[v], parts);
 #pragma unroll
@@ -428,13 +469,13 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
                 }
                 if constexpr (F32) {
 #pragma unroll
-                    for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], from[d], to[v]);
+                    for (int v = 0; v < N; ++v) to[v] = mma(vf[v], from[d], to[v]);
                 } else {
                     const auto x = split<decltype(parts)::value>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
                     for (int part = 0; part < decltype(parts)::value; ++part)
 #pragma unroll
-                        for (int v = 0; v < VT; ++v) to[v] = mma(vf[v], x.part[part], to[v]);
+                        for (int v = 0; v < N; ++v) to[v] = mma(vf[v], x.part[part], to[v]);
                 }
             };
             // the state's part of the results
@@ -462,25 +503,26 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
             const int i = w * 16 + col - missing + shift;                    // places of the chunk up to this lane's
             const float reach = MAIN ? power_at(powers, i) * a.state_scale : 0.f;
             const int p = p0 + w * 16 + col;
-            auto store = [&](const f4 (&acc)[VT]) {
-                if (a.whole_out) {                                           // four results that are all there or not at all
+            auto store = [&](const auto& acc, T* out, int64_t out_t, int left, bool whole) {
+                constexpr int N = sizeof(acc) / sizeof(f4);
+                if (whole) {                                                 // four results that are all there or not at all
                     const int row = w * 16 + col, from = a.backwards ? kChunk - 1 - row : row;
                     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-                        out + (int64_t)(a.backwards ? length - kChunk - p0 : p0) * a.out_t, 0, 0x7fffffff, 0x00020000);
-                    const int off = (from * (int)a.out_t + 4 * g) * (int)sizeof(T);
+                        out + (int64_t)(a.backwards ? length - kChunk - p0 : p0) * out_t, 0, 0x7fffffff, 0x00020000);
+                    const int off = (from * (int)out_t + 4 * g) * (int)sizeof(T);
 #pragma unroll
-                    for (int v = 0; v < VT; ++v) {
-                        const int to = p >= begin && v * 16 + 4 * g < vleft ? off + v * 16 * (int)sizeof(T) : kNowhere;
+                    for (int v = 0; v < N; ++v) {
+                        const int to = p >= begin && v * 16 + 4 * g < left ? off + v * 16 * (int)sizeof(T) : kNowhere;
                         if constexpr (F32) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, acc[v]), r, to, 0, 0);
                         else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u2, __builtin_convertvector(acc[v], b4)), r, to, 0, 0);
                     }
                 } else if (p >= begin) {
-                    T* o = out + place(p) * a.out_t;
+                    T* o = out + place(p) * out_t;
 #pragma unroll
-                    for (int v = 0; v < VT; ++v)
+                    for (int v = 0; v < N; ++v)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if (v * 16 + 4 * g + r < vleft) o[v * 16 + 4 * g + r] = (T)acc[v][r];
+                            if (v * 16 + 4 * g + r < left) o[v * 16 + 4 * g + r] = (T)acc[v][r];
                 }
             };
             if constexpr (MODE == LEAKY_SLOPE) {
@@ -516,15 +558,8 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
                 if (more) fetch_other(0, g, col);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            f4 acc[VT];
-            if constexpr (MAIN) {
-                of_state(acc, 0, 2);
-                LEAKY_FENCE;
-                if (more) fetch_query(0, g, col);
-#pragma unroll
-                for (int v = 0; v < VT; ++v) acc[v] *= reach;
-                // weights of the scores: key 4g + r of the strip of this lane's place, and of strips in front of it, in which a
-                // factor a^(16 strips) is left out
+            auto weigh_scores = [&]() {
+                // key 4g + r of the strip of this lane's place, and of strips in front of it, in which a factor a^(16 strips) is left out
                 float near[4], far[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -537,6 +572,15 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
                     for (int r = 0; r < 4; ++r)
                         scores[s][r] = s == w ? (col >= 4 * g + r ? scores[s][r] * near[r] : 0.f)
                                               : scores[s][r] * (s + 1 == w ? far[r] : far[r] * apart[w - s - 1]);
+            };
+            f4 acc[VT];
+            if constexpr (MAIN) {
+                of_state(acc, 0, 2);
+                LEAKY_FENCE;
+                if (more) fetch_query(0, g, col);
+#pragma unroll
+                for (int v = 0; v < VT; ++v) acc[v] *= reach;
+                weigh_scores();
             }
             if constexpr (MAIN) {                                            // (values are read twice: fewer sums are kept at once)
 #pragma unroll
@@ -548,7 +592,40 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
                     for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
                     add_values(acc, scores, d, vf, std::integral_constant<int, 2>{});
                 }
-                store(acc);
+                store(acc, out, a.out_t, vleft, a.whole_out);
+            }
+            if constexpr (BOTH) {
+                LEAKY_FENCE;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) scores[s] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < VP / D; ++d)
+#pragma unroll
+                    for (int s = 0; s <= w; ++s) scores[s] = mma(along_halves(lv, vPitch, s * 16, d * D, lane), qf2[d], scores[s]);
+                f4 acc2[KT];
+#pragma unroll
+                for (int k = 0; k < KT; ++k) acc2[k] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int d = 0; d < VP / D; ++d)
+#pragma unroll
+                    for (int part = 0; part < P; ++part)
+#pragma unroll
+                        for (int k = 0; k < KT; ++k) acc2[k] = mma(across(ls + part * VP * kPitch, kPitch, k * 16, d * D, lane), qf2[d], acc2[k]);
+                LEAKY_FENCE;
+                if (more) fetch_query2(0, g, col);
+#pragma unroll
+                for (int k = 0; k < KT; ++k) acc2[k] *= reach;
+                weigh_scores();
+#pragma unroll
+                for (int d = 0; d < kChunk / D; ++d) {
+                    if (d * D > w * 16) continue;
+                    LEAKY_FENCE;
+                    F kf[KT];
+#pragma unroll
+                    for (int k = 0; k < KT; ++k) kf[k] = across(lk, kPitch, k * 16, d * D, lane);
+                    add_values(acc2, scores, d, kf, std::integral_constant<int, 2>{});
+                }
+                store(acc2, out2, a.out2_t, a.keys, a.whole_out2);
             }
 #pragma unroll
             for (int s = 0; s < ST; ++s)
@@ -635,6 +712,11 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
             const int p = max(begin, length) + (int)(at / VP), c = (int)(at % VP);
             if (c < vleft) out[p * a.out_t + c] = (T)0.f;
         }
+        if constexpr (BOTH)
+            for (int64_t at = threadIdx.x; at < (int64_t)(end - max(begin, length)) * KP; at += 256) {
+                const int p = max(begin, length) + (int)(at / KP), c = (int)(at % KP);
+                if (c < a.keys) out2[p * a.out2_t + c] = (T)0.f;
+            }
     }
 }
 
@@ -656,6 +738,18 @@ int launch_leaky_mode(const LeakyPass& p, dim3 grid, bool whole, hipStream_t s) 
     else if (vt == 3) { BY_KEYS(3, true); }
     else { BY_KEYS(4, true); }
 #undef BY_KEYS
+#undef LAUNCH
+    return (int)hipGetLastError();
+}
+
+// LEAKY_BOTH: up to 64 keys and values, in whole pieces
+template <typename T, int MODE>
+int launch_leaky_both(const LeakyPass& p, dim3 grid, hipStream_t s) {
+#define LAUNCH(K, V) hipLaunchKernelGGL((leaky_kernel<T, K, V, MODE, true>), grid, dim3(256), 0, s, p)
+    if (p.keys <= 32 && p.tiles == 2) LAUNCH(2, 2);
+    else if (p.keys <= 32) LAUNCH(2, 4);
+    else if (p.tiles == 2) LAUNCH(4, 2);
+    else LAUNCH(4, 4);
 #undef LAUNCH
     return (int)hipGetLastError();
 }

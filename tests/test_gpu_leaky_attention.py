@@ -56,6 +56,9 @@ SIZES = [  # n, t, h, k, v, lengths
     (2, 1, 2, 16, 16, None), (1, 64, 3, 64, 64, None), (3, 65, 2, 20, 12, [65, 0, 1]), (2, 130, 1, 33, 7, [130, 64]),
     (2, 300, 5, 64, 64, [1, 300]), (1, 200, 2, 128, 128, None), (4, 63, 2, 1, 1, [63, 62, 0, 5]), (1, 129, 2, 48, 80, None),
     (2, 100, 2, 96, 40, [100, 37]), (1, 1300, 1, 32, 64, None), (2, 70, 2, 100, 128, None), (3, 520, 1, 8, 100, [520, 256, 255]),
+    # heads enough for the joint pass of value's and key's gradients, in one piece and in segments
+    (40, 70, 2, 64, 64, None), (23, 100, 3, 24, 40, list(range(0, 92, 4))), (9, 600, 2, 32, 64, [600, 0, 1, 64, 128, 300, 599, 512, 513]),
+    (70, 65, 1, 56, 16, None),
 ]
 
 
@@ -274,6 +277,32 @@ def test_values_that_are_not_finite_reach_no_earlier_token(t, s, bad, dtype):
             assert not torch.isfinite(y[1, s:, 0, 3]).any()
             rest = [0, 1, 2] + list(range(4, 20))
             assert torch.equal(y[1, :, 0, rest], ref[1, :, 0, rest])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n,t,s', [(2, 200, 70), (40, 200, 70), (40, 64, 31), (20, 1100, 700)])
+def test_gradients_that_are_not_finite_reach_no_later_token(n, t, s, dtype):
+    import lava_dl_amd.slayer as slayer
+    gen = torch.Generator().manual_seed(15)
+    decay = torch.tensor([100.0, 4096.0], device=DEV)
+    x = [y.to(DEV).requires_grad_() for y in inputs(gen, n, t, 2, 24, 24, dtype, False)[:3]]
+    g = torch.randn(n, t, 2, 24, generator=gen).to(DEV).to(dtype)
+    out = slayer.synapse.leaky_attention(*x, decay)
+    ref = torch.autograd.grad(out, x, g, retain_graph=True)
+    for bad in (float('nan'), float('inf')):
+        h = g.clone()
+        h[1, s, 0, 3] = bad
+        got = torch.autograd.grad(out, x, h, retain_graph=True)
+        for a, b in zip(got, ref):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[2:], b[2:]) and torch.equal(a[1, :, 1], b[1, :, 1])
+            assert torch.equal(a[1, s + 1:, 0], b[1, s + 1:, 0])
+        assert torch.equal(got[0][1, :s, 0], ref[0][1, :s, 0]) and not torch.isfinite(got[0][1, s, 0]).any()
+        assert not torch.isfinite(got[1][1, :s + 1, 0]).any() and not torch.isfinite(got[2][1, :s + 1, 0, 3]).any()
+        y = [v.detach().clone() for v in x]                                   # ... and a key that is not finite no earlier one's value
+        y[1][1, s, 0, 5] = bad
+        y = [v.requires_grad_() for v in y]
+        dv = torch.autograd.grad(slayer.synapse.leaky_attention(*y, decay), y, g)[2]
+        assert torch.equal(dv[1, :s, 0], ref[2][1, :s, 0]) and torch.equal(dv[1, s + 1:, 0], ref[2][1, s + 1:, 0])
 
 
 def test_nothing_to_do():
