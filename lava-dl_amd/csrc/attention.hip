@@ -326,12 +326,16 @@ extern "C" int slayer_leaky_attention_bwd(void* grad_query, void* grad_key, void
             if (int e = (int)hipGetLastError()) return e;
         }
     }
-    // value's and key's gradients in one pass where its workgroups hold a whole head of 64 keys and values; in narrow slices, whose
-    // chunks take less time, where there are few of them
-    if (grad_value && grad_key && K <= 64 && V <= 64 && whole_rows(a, kk, q, g, K, V) && whole_rows(a, vv, g, q, V, K) &&
-        a->samples * a->heads * segments_of(a) > 64) {
-        const Both both{grad_key, k.stride, vv};
-        return run_pass(a, grad_value, v.stride, kk, q, g, K, V, false, true, grad_last, grad_state, nullptr, &both, space, false, s);
+    // value's and key's gradients in one pass where a workgroup holds a whole head, up to 96 by 64; in narrow slices, whose chunks take
+    // less time, where there are few of them.  The narrower side is the pass's value.
+    if (grad_value && grad_key && (K < V ? K : V) <= 64 && (K < V ? V : K) <= 96 && whole_rows(a, kk, q, g, K, V) &&
+        whole_rows(a, vv, g, q, V, K) && a->samples * a->heads * segments_of(a) > 64) {
+        if (V <= 64) {
+            const Both both{grad_key, k.stride, vv};
+            return run_pass(a, grad_value, v.stride, kk, q, g, K, V, false, true, grad_last, grad_state, nullptr, &both, space, false, s);
+        }
+        const Both both{grad_value, v.stride, kk};
+        return run_pass(a, grad_key, k.stride, vv, g, q, V, K, true, true, grad_last, grad_state, nullptr, &both, space, false, s);
     }
     if (grad_value || grad_state)
         if (int e = run_pass(a, grad_value, v.stride, kk, q, g, K, V, false, true, grad_last, grad_state, nullptr, nullptr, space, false, s)) return e;

@@ -742,14 +742,15 @@ int launch_leaky_mode(const LeakyPass& p, dim3 grid, bool whole, hipStream_t s) 
     return (int)hipGetLastError();
 }
 
-// LEAKY_BOTH: up to 64 keys and values, in whole pieces
+// LEAKY_BOTH: up to 96 keys and 64 values, in whole pieces
 template <typename T, int MODE>
 int launch_leaky_both(const LeakyPass& p, dim3 grid, hipStream_t s) {
 #define LAUNCH(K, V) hipLaunchKernelGGL((leaky_kernel<T, K, V, MODE, true>), grid, dim3(256), 0, s, p)
-    if (p.keys <= 32 && p.tiles == 2) LAUNCH(2, 2);
-    else if (p.keys <= 32) LAUNCH(2, 4);
-    else if (p.tiles == 2) LAUNCH(4, 2);
-    else LAUNCH(4, 4);
+#define BY_VALUES(K) if (p.tiles == 2) LAUNCH(K, 2); else LAUNCH(K, 4)
+    if (p.keys <= 32) { BY_VALUES(2); }
+    else if (p.keys <= 64) { BY_VALUES(4); }
+    else { BY_VALUES(6); }
+#undef BY_VALUES
 #undef LAUNCH
     return (int)hipGetLastError();
 }

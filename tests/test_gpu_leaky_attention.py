@@ -58,7 +58,7 @@ SIZES = [  # n, t, h, k, v, lengths
     (2, 100, 2, 96, 40, [100, 37]), (1, 1300, 1, 32, 64, None), (2, 70, 2, 100, 128, None), (3, 520, 1, 8, 100, [520, 256, 255]),
     # heads enough for the joint pass of value's and key's gradients, in one piece and in segments
     (40, 70, 2, 64, 64, None), (23, 100, 3, 24, 40, list(range(0, 92, 4))), (9, 600, 2, 32, 64, [600, 0, 1, 64, 128, 300, 599, 512, 513]),
-    (70, 65, 1, 56, 16, None),
+    (70, 65, 1, 56, 16, None), (35, 100, 2, 80, 48, None), (35, 130, 2, 16, 96, list(range(96, 131))), (70, 66, 1, 88, 8, None),
 ]
 
 
