@@ -131,7 +131,8 @@ int check_leaky(const slayer_attention* a) {
 
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
-// A segment's workgroup adds up the states of up to so many segments itself (a launch between the two kernels is 10 us).
+// A segment's workgroup adds up the states of up to so many segments itself ([32,1500,4,64] float32, forward: 86 us, 95 with the
+// launch that joins them).
 constexpr int kJoin = 8;
 
 // Sixteens of values in a slice of up to 64: wide slices, whose scores are worked out once for all of them.

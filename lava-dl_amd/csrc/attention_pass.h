@@ -14,7 +14,7 @@ struct LeakyPass {
     const void *query, *key, *value;
     const float* decay;
     const void* lengths;
-    const float* first;            // [samples][heads] states with strides first_k, first_v, or nullptr: zeros
+    const float* first;            // states in front of the first token, [samples * heads], or nullptr: zeros
     float* starts;                 // states in front of the segments, [samples * heads][segments] of them (not `joined`: what the
                                    // segment before each adds)
     float* last;                   // state behind the last token, or nullptr
@@ -159,22 +159,27 @@ __device__ __forceinline__ float slope_at(const float* powers, int n) { return n
 //       W'      = a^64 W + 64 a^63 S + sum over j of (63-j) a^(62-j) key[j] (outer) value[j]
 //     of which the workgroup returns the sum of its products with `other`.  LEAKY_STATE_SLOPE: S and W from zero.
 //   WHOLE: the rows of all tensors are made of whole, aligned 16-byte pieces.
-#ifndef LEAKY_TWO_BUFFERS
-#define LEAKY_TWO_BUFFERS 40000
-#endif
-#ifndef LEAKY_FENCE
-#define LEAKY_FENCE __builtin_amdgcn_sched_barrier(0)
-#endif
-#ifndef LEAKY_WAVES
-#define LEAKY_WAVES(T, KT, VT, MODE) 2
-#endif
+//
+//   What bounds it (64 keys and values, two workgroups a compute unit).  float32: the matrix cores, whose 3.25 products of 64 x 64 x 64
+// a chunk take 6 656 cycles of each SIMD; [32,1500,4,64] in four segments 64 us, of which 37 are those and 39 would be a copy of the
+// same bytes.  bfloat16: a chunk of a workgroup takes 5 500 cycles alone and 6 500 beside another (filling LDS 900, scores 850, state
+// 780, the products with values and keys 1 700 to 2 100, results 430), about what the memory needs for it, 7 400 for two;
+// [64,1000,8,64] 60 us from the last-level cache and 72 from memory, 262 MB, where a kernel that only moves the tensors takes 52 and
+// 63: pieces of 128 bytes cost it a fifth.  A third workgroup a compute unit, slices of 32 values and priorities for one of the two
+// were no faster.
+//   Registers decide: above 256 of them, or with any in scratch memory (whose accesses wait for the chunk on its way), the same
+// kernels took 1.4 to 2 times as long.  So a strip is compiled for its wave, addresses are made anew in every chunk, the values are
+// read twice, and `phase_end` keeps the compiler from starting the reads of a later phase.
+__device__ __forceinline__ void phase_end() { __builtin_amdgcn_sched_barrier(0); }
+constexpr int kTwoBuffers = 40000;             // bytes of LDS tiles up to which there are two of each
+
 template <typename T, int KT, int VT, int MODE, bool WHOLE>
-__global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kernel(LeakyPass a) {
+__global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
     typedef typename Frag<T>::Type F;
     typedef typename Elements<T>::Vec Vec;
     constexpr bool BOTH = MODE == LEAKY_BOTH || MODE == LEAKY_BOTH_LAST, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
     constexpr bool MAIN = MODE != LEAKY_STATE && MODE != LEAKY_STATE_SLOPE;
-    constexpr bool FINE = F32 || (MODE != LEAKY_MAIN && MODE != LEAKY_BOTH);                         // the state to float32, not to a hundredth of bfloat16
+    constexpr bool FINE = F32 || (MODE != LEAKY_MAIN && MODE != LEAKY_BOTH);    // the state to float32, not to a 256th of bfloat16
     constexpr int V = Elements<T>::kVec, D = Frag<T>::kDepth, P = F32 ? 1 : MODE == LEAKY_SLOPE ? 3 : 2;      // parts of a state in LDS
     constexpr int KP = KT * 16, VP = VT * 16;
     // rows of LDS: sixteen rows of keys, read along, start in different banks; so do the eight (float32: four) rows of values that
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
     constexpr int kStates = MAIN ? (SLOPE ? 2 : 1) : 0;                      // states in LDS
     constexpr int kTile = kChunk * kPitch, vTile = kChunk * vPitch, sTile = kStates * P * VP * kPitch;
     // two buffers, and one barrier a chunk, where two workgroups still fit a compute unit
-    constexpr int BUFFERS = (kTile + vTile + sTile) * (int)sizeof(T) <= LEAKY_TWO_BUFFERS ? 2 : 1;
+    constexpr int BUFFERS = (kTile + vTile + sTile) * (int)sizeof(T) <= kTwoBuffers ? 2 : 1;
     __shared__ __align__(16) T tiles[BUFFERS * (kTile + vTile + sTile)];     // keys, values, state: [state][part][value][key]
     __shared__ __align__(16) float powers[kChunk + 4];                       // a^i
     __shared__ float weights[MAIN ? 48 : 1];                                 // of scores: a^(i - 16), 0 for i < 16
@@ -194,8 +199,8 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
     __shared__ double sums[4];
 
     const int lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-    // Strips of the later places cost more (float32, 64 keys and values: 10, 12, 14 and 16 sixteenths of a product of 64 x 64 x 64 / 4),
-    // and the waves of a place in the workgroup share a SIMD: the second workgroup of a compute unit has them the other way round.
+    // Strips of the later places cost more (float32, 64 keys and values: 10, 12, 14 and 16 times sixteen instructions), and waves with the
+    // same place in their workgroups share a SIMD: the second workgroup of a compute unit has them the other way round.
     const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x & 256 ? 3 - (threadIdx.x >> 6) : threadIdx.x >> 6);
     const int segments = MAIN ? a.segments : a.segments - 1;
     // the slices of a segment, which read the same queries and keys, eight workgroups apart: on the same XCD, with one L2
@@ -233,7 +238,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
         }
     };
 
-    // What the next chunk needs, on its way.  WHOLE: a thread's pieces are an offset from the chunk's first address (the offset ~0
+    // What the next chunk needs, on its way.  WHOLE: a thread's pieces are an offset from the chunk's first address (kNowhere
     // lies outside of every buffer and reads 0); otherwise they are read element by element.
     const int count0 = stop > begin ? (stop - begin - 1) % kChunk + 1 : 0;   // tokens of the first chunk
     int p0 = stop > begin ? begin - (kChunk - count0) : stop;                // place of the chunk's first row
@@ -499,7 +504,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
 #pragma unroll
                     for (int s = 0; s <= w; ++s) scores[s] = mma(along(lk, kPitch, s * 16, d * D, lane), qf[d], scores[s]);
             }
-            LEAKY_FENCE;
+            phase_end();
             const int i = w * 16 + col - missing + shift;                    // places of the chunk up to this lane's
             const float reach = MAIN ? power_at(powers, i) * a.state_scale : 0.f;
             const int p = p0 + w * 16 + col;
@@ -538,7 +543,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
 #pragma unroll
                 for (int d = 0; d < kChunk / D; ++d) {
                     if (d * D > w * 16) continue;
-                    LEAKY_FENCE;
+                    phase_end();
 #pragma unroll
                     for (int s = d * D / 16; s < (d + 1) * D / 16; ++s)
 #pragma unroll
@@ -556,7 +561,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
 #pragma unroll
                     for (int r = 0; r < 4; ++r) total = fmaf((float)other[v][r], dacc[v][r], total);
                 if (more) fetch_other(0, g, col);
-                __builtin_amdgcn_sched_barrier(0);
+                phase_end();
             }
             auto weigh_scores = [&]() {
                 // key 4g + r of the strip of this lane's place, and of strips in front of it, in which a factor a^(16 strips) is left out
@@ -576,7 +581,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
             f4 acc[VT];
             if constexpr (MAIN) {
                 of_state(acc, 0, 2);
-                LEAKY_FENCE;
+                phase_end();
                 if (more) fetch_query(0, g, col);
 #pragma unroll
                 for (int v = 0; v < VT; ++v) acc[v] *= reach;
@@ -586,7 +591,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
 #pragma unroll
                 for (int d = 0; d < kChunk / D; ++d) {
                     if (d * D > w * 16) continue;
-                    LEAKY_FENCE;
+                    phase_end();
                     F vf[VT];
 #pragma unroll
                     for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
@@ -595,7 +600,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
                 store(acc, out, a.out_t, vleft, a.whole_out);
             }
             if constexpr (BOTH) {
-                LEAKY_FENCE;
+                phase_end();
 #pragma unroll
                 for (int s = 0; s < 4; ++s) scores[s] = f4{0, 0, 0, 0};
 #pragma unroll
@@ -611,7 +616,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
                     for (int part = 0; part < P; ++part)
 #pragma unroll
                         for (int k = 0; k < KT; ++k) acc2[k] = mma(across(ls + part * VP * kPitch, kPitch, k * 16, d * D, lane), qf2[d], acc2[k]);
-                LEAKY_FENCE;
+                phase_end();
                 if (more) fetch_query2(0, g, col);
 #pragma unroll
                 for (int k = 0; k < KT; ++k) acc2[k] *= reach;
@@ -619,7 +624,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
 #pragma unroll
                 for (int d = 0; d < kChunk / D; ++d) {
                     if (d * D > w * 16) continue;
-                    LEAKY_FENCE;
+                    phase_end();
                     F kf[KT];
 #pragma unroll
                     for (int k = 0; k < KT; ++k) kf[k] = across(lk, kPitch, k * 16, d * D, lane);
@@ -637,7 +642,7 @@ __global__ __launch_bounds__(256, LEAKY_WAVES(T, KT, VT, MODE)) void leaky_kerne
                 }
 #pragma unroll
             for (int d = 0; d < kChunk / D; ++d) {
-                LEAKY_FENCE;
+                phase_end();
                 F vf[VT];                                                    // values, terms across the places
 #pragma unroll
                 for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
