@@ -165,13 +165,12 @@ __device__ __forceinline__ float slope_at(const float* powers, int n) { return n
 // same bytes.  bfloat16: a chunk of a workgroup takes 5 500 cycles alone and 6 500 beside another (filling LDS 900, scores 850, state
 // 780, the products with values and keys 1 700 to 2 100, results 430), about what the memory needs for it, 7 400 for two;
 // [64,1000,8,64] 60 us from the last-level cache and 72 from memory, 262 MB, where a kernel that only moves the tensors takes 52 and
-// 63: pieces of 128 bytes cost it a fifth.  A third workgroup a compute unit, slices of 32 values and priorities for one of the two
-// were no faster.
+// 63: pieces of 128 bytes cost it a fifth.  A third workgroup a compute unit, slices of 32 values, priorities for one of the two
+// and two sets of tiles (one barrier a chunk) were no faster.
 //   Registers decide: above 256 of them, or with any in scratch memory (whose accesses wait for the chunk on its way), the same
 // kernels took 1.4 to 2 times as long.  So a strip is compiled for its wave, addresses are made anew in every chunk, the values are
 // read twice, and `phase_end` keeps the compiler from starting the reads of a later phase.
 __device__ __forceinline__ void phase_end() { __builtin_amdgcn_sched_barrier(0); }
-constexpr int kTwoBuffers = 40000;             // bytes of LDS tiles up to which there are two of each
 
 template <typename T, int KT, int VT, int MODE, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
@@ -190,9 +189,9 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
     constexpr int ST = (KT + 3) / 4;                                         // strips of the state of a wave
     constexpr int kStates = MAIN ? (SLOPE ? 2 : 1) : 0;                      // states in LDS
     constexpr int kTile = kChunk * kPitch, vTile = kChunk * vPitch, sTile = kStates * P * VP * kPitch;
-    // two buffers, and one barrier a chunk, where two workgroups still fit a compute unit
-    constexpr int BUFFERS = (kTile + vTile + sTile) * (int)sizeof(T) <= kTwoBuffers ? 2 : 1;
-    __shared__ __align__(16) T tiles[BUFFERS * (kTile + vTile + sTile)];     // keys, values, state: [state][part][value][key]
+    __shared__ __align__(16) T keys[kTile];
+    __shared__ __align__(16) T values[vTile];
+    __shared__ __align__(16) T state[sTile > 0 ? sTile : 8];                 // [state][part][value][key]
     __shared__ __align__(16) float powers[kChunk + 4];                       // a^i
     __shared__ float weights[MAIN ? 48 : 1];                                 // of scores: a^(i - 16), 0 for i < 16
     __shared__ __align__(16) float behind[SLOPE ? 2 : 1][kChunk];            // what key j counts behind the chunk; its derivative
@@ -203,7 +202,8 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
     // same place in their workgroups share a SIMD: the second workgroup of a compute unit has them the other way round.
     const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x & 256 ? 3 - (threadIdx.x >> 6) : threadIdx.x >> 6);
     const int segments = MAIN ? a.segments : a.segments - 1;
-    // the slices of a segment, which read the same queries and keys, eight workgroups apart: on the same XCD, with one L2
+    // The slices of a segment, which read the same queries and keys, eight workgroups apart: on the same XCD, with one L2.  (Heads and
+    // samples are left spread over the XCDs: samples of different lengths then load them alike.)
     int slice, at_segment = blockIdx.x;
     if (at_segment < (a.units * segments & ~7) * a.slices) {
         slice = at_segment / 8 % a.slices;
@@ -223,7 +223,6 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
     T* out2 = BOTH ? (T*)a.out2 + n * a.out2_n + h * a.out2_h : nullptr;
     const int shift = a.backwards ? 0 : 1;
     f4 S[ST][VT], W[SLOPE ? ST : 1][SLOPE ? VT : 1];
-    T *keys = tiles, *values = tiles + kTile, *state = tiles + kTile + vTile;
     auto share = [&](f4 x, int which, int strip, int v, int g, int col) {
         T* p = state + which * P * VP * kPitch + (v * 16 + col) * kPitch + strip * 16 + 4 * g;
         if constexpr (F32) {
@@ -340,8 +339,8 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
         fetch_rows(begin - p0, threadIdx.x);
     }
 
-    __shared__ int not_finite[2];                                            // the last chunk (of every second) with such values
-    if (threadIdx.x < 2) not_finite[threadIdx.x] = p0 - 1;
+    __shared__ int not_finite;                                               // the last chunk with such values
+    if (threadIdx.x == 0) not_finite = p0 - 1;
     if (threadIdx.x <= kChunk) powers[threadIdx.x] = (float)power(leak, threadIdx.x);
     __syncthreads();
     if (threadIdx.x < kChunk) {
@@ -388,7 +387,6 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
     const float apart[3] = {1.f, powers[16], powers[32]};
     float total = 0;                                                         // LEAKY_SLOPE
 
-    int parity = 0;
     auto fill = [&](int thread, int g, int col) {                            // LDS for the next chunk
         bool bad = false;
 #pragma unroll
@@ -403,7 +401,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
             if (kChunk * VV % 256 == 0 || at < kChunk * VV) *reinterpret_cast<Vec*>(values + at / VV * vPitch + at % VV * V) = nv[i];
             if (MAIN) bad = bad || any_not_finite(nv[i]);
         }
-        if (MAIN && bad) not_finite[parity] = p0;
+        if (MAIN && bad) not_finite = p0;
         if constexpr (MAIN) {
 #pragma unroll
             for (int s = 0; s < ST; ++s) {
@@ -416,21 +414,15 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
             }
         }
     };
-    int buffer = 0;
-    for (; p0 < stop; p0 += kChunk, parity ^= 1) {
+    for (; p0 < stop; p0 += kChunk) {
         // the thread's place, worked out anew: kept, the addresses made of it for the four strips would take 60 registers
         int thread = threadIdx.x;
         asm volatile("" : "+v"(thread));
         const int lane = thread & 63, g = lane >> 4, col = lane & 15;
-        if (BUFFERS == 1) __syncthreads();                                   // the chunk before is done with LDS
+        __syncthreads();                                                     // the chunk before is done with LDS
         fill(thread, g, col);
         __syncthreads();
-        const T *lk = keys, *lv = values, *ls = state;
-        const bool odd_values = MAIN && __builtin_amdgcn_readfirstlane(not_finite[parity]) == p0;
-        if (BUFFERS == 2) {
-            buffer = kTile + vTile + sTile - buffer;
-            keys = tiles + buffer; values = keys + kTile; state = values + vTile;
-        }
+        const bool odd_values = MAIN && __builtin_amdgcn_readfirstlane(not_finite) == p0;
         const bool more = p0 + kChunk < stop;
         if (more) fetch_rows(0, thread);
 
@@ -493,7 +485,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
                     for (int part = 0; part < (parts < P ? parts : P); ++part)
 #pragma unroll
                         for (int v = 0; v < VT; ++v)
-                            to[v] = mma(along(ls + (which * P + part) * VP * kPitch, kPitch, v * 16, d * D, lane), qf[d], to[v]);
+                            to[v] = mma(along(state + (which * P + part) * VP * kPitch, kPitch, v * 16, d * D, lane), qf[d], to[v]);
             };
             if constexpr (MAIN) {
                 // scores, transposed: lane has keys 4g ... 4g+3 of each strip for its place
@@ -502,7 +494,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
 #pragma unroll
                 for (int d = 0; d < KP / D; ++d)
 #pragma unroll
-                    for (int s = 0; s <= w; ++s) scores[s] = mma(along(lk, kPitch, s * 16, d * D, lane), qf[d], scores[s]);
+                    for (int s = 0; s <= w; ++s) scores[s] = mma(along(keys, kPitch, s * 16, d * D, lane), qf[d], scores[s]);
             }
             phase_end();
             const int i = w * 16 + col - missing + shift;                    // places of the chunk up to this lane's
@@ -553,7 +545,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
                         }
                     F vf[VT];
 #pragma unroll
-                    for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
+                    for (int v = 0; v < VT; ++v) vf[v] = across(values, vPitch, v * 16, d * D, lane);
                     add_values(dacc, dscores, d, vf, std::integral_constant<int, 3>{});
                 }
 #pragma unroll
@@ -594,7 +586,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
                     phase_end();
                     F vf[VT];
 #pragma unroll
-                    for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
+                    for (int v = 0; v < VT; ++v) vf[v] = across(values, vPitch, v * 16, d * D, lane);
                     add_values(acc, scores, d, vf, std::integral_constant<int, 2>{});
                 }
                 store(acc, out, a.out_t, vleft, a.whole_out);
@@ -606,7 +598,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
 #pragma unroll
                 for (int d = 0; d < VP / D; ++d)
 #pragma unroll
-                    for (int s = 0; s <= w; ++s) scores[s] = mma(along_halves(lv, vPitch, s * 16, d * D, lane), qf2[d], scores[s]);
+                    for (int s = 0; s <= w; ++s) scores[s] = mma(along_halves(values, vPitch, s * 16, d * D, lane), qf2[d], scores[s]);
                 f4 acc2[KT];
 #pragma unroll
                 for (int k = 0; k < KT; ++k) acc2[k] = f4{0, 0, 0, 0};
@@ -615,7 +607,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
 #pragma unroll
                     for (int part = 0; part < P; ++part)
 #pragma unroll
-                        for (int k = 0; k < KT; ++k) acc2[k] = mma(across(ls + part * VP * kPitch, kPitch, k * 16, d * D, lane), qf2[d], acc2[k]);
+                        for (int k = 0; k < KT; ++k) acc2[k] = mma(across(state + part * VP * kPitch, kPitch, k * 16, d * D, lane), qf2[d], acc2[k]);
                 phase_end();
                 if (more) fetch_query2(0, g, col);
 #pragma unroll
@@ -627,7 +619,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
                     phase_end();
                     F kf[KT];
 #pragma unroll
-                    for (int k = 0; k < KT; ++k) kf[k] = across(lk, kPitch, k * 16, d * D, lane);
+                    for (int k = 0; k < KT; ++k) kf[k] = across(keys, kPitch, k * 16, d * D, lane);
                     add_values(acc2, scores, d, kf, std::integral_constant<int, 2>{});
                 }
                 store(acc2, out2, a.out2_t, a.keys, a.whole_out2);
@@ -645,11 +637,11 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
                 phase_end();
                 F vf[VT];                                                    // values, terms across the places
 #pragma unroll
-                for (int v = 0; v < VT; ++v) vf[v] = across(lv, vPitch, v * 16, d * D, lane);
+                for (int v = 0; v < VT; ++v) vf[v] = across(values, vPitch, v * 16, d * D, lane);
 #pragma unroll
                 for (int s = 0; s < ST; ++s) {
                     if (s * 4 + w >= KT) continue;
-                    const F kf = across(lk, kPitch, (s * 4 + w) * 16, d * D, lane);
+                    const F kf = across(keys, kPitch, (s * 4 + w) * 16, d * D, lane);
                     auto add_keys = [&](f4 (&to)[VT], const float* weights) {
                         const f4 w0 = *reinterpret_cast<const f4*>(weights + d * D + 4 * g);
                         if constexpr (F32) {
