@@ -2,14 +2,15 @@
  * slayer_hip.h -- C ABI of libslayer_hip.so, the MI355X (gfx950) implementation of
  * lava-dl SLAYER's neuron-dynamics and temporal-op kernels.
  *
- * Every entry point replaces one function of the reference's JIT-built CUDA
- * modules (citations are relative to src/lava/lib/dl/slayer/ in lava-nc/lava-dl);
+ * Every entry point (but those for token mixing, which the reference does not
+ * have) replaces one function of the reference's JIT-built CUDA modules (citations are relative to src/lava/lib/dl/slayer/ in lava-nc/lava-dl);
  * the arithmetic follows the reference's CPU branch, which is the semantic
  * definition (int64 states on the CPU, float32 tensors at every op boundary).
  *
  * Conventions
  *   - All tensor pointers are DEVICE pointers to contiguous float32 data laid out
- *     [M neurons][T steps], time innermost (M = numel / T).
+ *     [M neurons][T steps], time innermost (M = numel / T).  (The token-mixing entry
+ *     points say what they take themselves.)
  *   - Nothing is allocated, freed or synchronised inside; work is enqueued on
  *     `stream` (a hipStream_t passed as void*, NULL = the null stream) of the
  *     device that is current when the call is made.

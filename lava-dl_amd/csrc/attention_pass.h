@@ -164,7 +164,7 @@ __device__ __forceinline__ float slope_at(const float* powers, int n) { return n
 // a chunk take 6 656 cycles of each SIMD; [32,1500,4,64] in four segments 64 us, of which 37 are those and 39 would be a copy of the
 // same bytes.  bfloat16: a chunk of a workgroup takes 5 500 cycles alone and 6 500 beside another (filling LDS 900, scores 850, state
 // 780, the products with values and keys 1 700 to 2 100, results 430), about what the memory needs for it, 7 400 for two;
-// [64,1000,8,64] 60 us from the last-level cache and 72 from memory, 262 MB, where a kernel that only moves the tensors takes 52 and
+// [64,1000,8,64], calls in a row, 65 us from the last-level cache and 79 from memory, 262 MB, where a kernel that only moves the tensors takes 52 and
 // 63: pieces of 128 bytes cost it a fifth.  A third workgroup a compute unit, slices of 32 values, priorities for one of the two
 // and two sets of tiles (one barrier a chunk) were no faster.
 //   Registers decide: above 256 of them, or with any in scratch memory (whose accesses wait for the chunk on its way), the same
