@@ -245,7 +245,7 @@ int run_pass(const slayer_attention* a, void* out, const int64_t (&out_stride)[3
         hipLaunchKernelGGL(leaky_join_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, p);
         if (int e = (int)hipGetLastError()) return e;
     }
-    return launch(slope ? LEAKY_SLOPE : both ? (last ? LEAKY_BOTH_LAST : LEAKY_BOTH) : last ? LEAKY_LAST : LEAKY_MAIN);
+    return launch(slope ? LEAKY_SLOPE : both ? LEAKY_BOTH : LEAKY_MAIN);
 }
 
 // Floats of the states in front of the segments.

@@ -13,9 +13,7 @@ int launch_leaky<bf16>(const LeakyPass& p, int mode, bool whole, hipStream_t str
     switch (mode) {
         case LEAKY_STATE: return launch_leaky_mode<bf16, LEAKY_STATE>(p, grid, whole, stream);
         case LEAKY_MAIN: return launch_leaky_mode<bf16, LEAKY_MAIN>(p, grid, whole, stream);
-        case LEAKY_LAST: return launch_leaky_mode<bf16, LEAKY_LAST>(p, grid, whole, stream);
-        case LEAKY_BOTH: return launch_leaky_both<bf16, LEAKY_BOTH>(p, grid, stream);
-        case LEAKY_BOTH_LAST: return launch_leaky_both<bf16, LEAKY_BOTH_LAST>(p, grid, stream);
+        case LEAKY_BOTH: return launch_leaky_both<bf16>(p, grid, stream);
         case LEAKY_STATE_SLOPE: return launch_leaky_mode<bf16, LEAKY_STATE_SLOPE>(p, grid, whole, stream);
         default: return launch_leaky_mode<bf16, LEAKY_SLOPE>(p, grid, whole, stream);
     }

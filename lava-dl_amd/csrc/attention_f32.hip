@@ -12,10 +12,8 @@ int launch_leaky<float>(const LeakyPass& p, int mode, bool whole, hipStream_t st
     const dim3 grid((unsigned)blocks);
     switch (mode) {
         case LEAKY_STATE: return launch_leaky_mode<float, LEAKY_STATE>(p, grid, whole, stream);
-        case LEAKY_MAIN:                                                     // the same in float32
-        case LEAKY_LAST: return launch_leaky_mode<float, LEAKY_MAIN>(p, grid, whole, stream);
-        case LEAKY_BOTH:
-        case LEAKY_BOTH_LAST: return launch_leaky_both<float, LEAKY_BOTH>(p, grid, stream);
+        case LEAKY_MAIN: return launch_leaky_mode<float, LEAKY_MAIN>(p, grid, whole, stream);
+        case LEAKY_BOTH: return launch_leaky_both<float>(p, grid, stream);
         case LEAKY_STATE_SLOPE: return launch_leaky_mode<float, LEAKY_STATE_SLOPE>(p, grid, whole, stream);
         default: return launch_leaky_mode<float, LEAKY_SLOPE>(p, grid, whole, stream);
     }

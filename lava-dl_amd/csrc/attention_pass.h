@@ -88,17 +88,17 @@ __device__ __forceinline__ b8 across(const bf16* tile, int pitch, int column, in
     return b8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// A float32 operand: in float32, or as bfloat16 numbers that sum to it, so that what the kernel makes itself is not rounded to
-// the type of the tensors on the way: two for what ends in a result of that type (within 2^-16, a 256th of what
-// rounding the result costs), three for what ends in a float32 state or in the decays' gradient (within 2^-24).
-template <int PARTS> struct Split { b8 part[PARTS]; };
-template <int PARTS>
-__device__ __forceinline__ Split<PARTS> split(f8 v) {
-    Split<PARTS> o;
+// A float32 operand: in float32, or as three bfloat16 numbers that sum to it (within 2^-24), so that what the kernel makes itself (scores,
+// states, leaked keys) keeps float32's digits on the way.  Two would leave 2^-16 of every term, which is more than the rounding of
+// a bfloat16 result as soon as the terms cancel to a 256th of their magnitudes.
+constexpr int kParts = 3;
+struct Split { b8 part[kParts]; };
+__device__ __forceinline__ Split split(f8 v) {
+    Split o;
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) {
+    for (int i = 0; i < kParts; ++i) {
         o.part[i] = __builtin_convertvector(v, b8);
-        if (i + 1 < PARTS) v -= __builtin_convertvector(o.part[i], f8);
+        if (i + 1 < kParts) v -= __builtin_convertvector(o.part[i], f8);
     }
     return o;
 }
@@ -119,7 +119,7 @@ __device__ __forceinline__ int sample_length(const LeakyPass& a, int n) {
 }
 
 
-enum { LEAKY_STATE, LEAKY_MAIN, LEAKY_LAST, LEAKY_BOTH, LEAKY_BOTH_LAST, LEAKY_STATE_SLOPE, LEAKY_SLOPE };
+enum { LEAKY_STATE, LEAKY_MAIN, LEAKY_BOTH, LEAKY_STATE_SLOPE, LEAKY_SLOPE };
 
 // Values that are not finite.  A score that the mask leaves out is 0, and 0 times such a value is not: a strip with masked scores takes
 // the products without these values and says which results they belong to.
@@ -150,10 +150,10 @@ __device__ __forceinline__ float slope_at(const float* powers, int n) { return n
 // Wave w makes the outputs of places 16w ... 16w+15 (transposed: lane = place) and the rows of the state w, w+4, ... (16 each).
 // The first chunk is the one that is not full, with its tokens at the end, so that weights behind a token are the same in all.
 //   LEAKY_STATE: only the state, from zero, into `starts` behind the segment's place (for the segments but the last).
-//   LEAKY_LAST:  results and the last state, which is held more exactly than results of bfloat16 need.
+//   LEAKY_MAIN:  results, and the last state.
 //   LEAKY_BOTH:  the gradients of value and key together: beside out[i], from query and key, also out2[i], from query2 and value,
 //       out2[i] = a^i query2[i] S^T + sum over j <= i of a^(i-j) (query2[i] . value[j]) key[j],
-//     for which the state and the chunk's keys and values (queries and gradients) are there already.  One slice.  LEAKY_BOTH_LAST.
+//     for which the state and the chunk's keys and values (queries and gradients) are there already.  One slice.
 //   LEAKY_SLOPE: results, and the derivative of each with respect to a, in which the state's derivative W takes the place of S:
 //       dout[i] = a^(i+1) query[i] W + (i+1) a^i query[i] S + sum over j of (i-j) a^(i-j-1) (query[i] . key[j]) value[j]
 //       W'      = a^64 W + 64 a^63 S + sum over j of (63-j) a^(62-j) key[j] (outer) value[j]
@@ -176,10 +176,9 @@ template <typename T, int KT, int VT, int MODE, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
     typedef typename Frag<T>::Type F;
     typedef typename Elements<T>::Vec Vec;
-    constexpr bool BOTH = MODE == LEAKY_BOTH || MODE == LEAKY_BOTH_LAST, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
+    constexpr bool BOTH = MODE == LEAKY_BOTH, SLOPE = MODE >= LEAKY_STATE_SLOPE, F32 = sizeof(T) == 4;
     constexpr bool MAIN = MODE != LEAKY_STATE && MODE != LEAKY_STATE_SLOPE;
-    constexpr bool FINE = F32 || (MODE != LEAKY_MAIN && MODE != LEAKY_BOTH);    // the state to float32, not to a 256th of bfloat16
-    constexpr int V = Elements<T>::kVec, D = Frag<T>::kDepth, P = F32 ? 1 : MODE == LEAKY_SLOPE ? 3 : 2;      // parts of a state in LDS
+    constexpr int V = Elements<T>::kVec, D = Frag<T>::kDepth, P = F32 ? 1 : kParts;      // parts of a state in LDS
     constexpr int KP = KT * 16, VP = VT * 16;
     // rows of LDS: sixteen rows of keys, read along, start in different banks; so do the eight (float32: four) rows of values that
     // an access across them touches
@@ -435,16 +434,16 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
             constexpr int w = decltype(which)::value;
             f4 scores[4];
             // adds the products of weighted scores and values
-            auto weigh = [&](F v, const f4 (&from)[4], int d, f4 to, auto parts) {
+            auto weigh = [&](F v, const f4 (&from)[4], int d, f4 to) {
                 if constexpr (F32) {
                     return mma(v, from[d], to);
                 } else {
-                    const auto x = split<decltype(parts)::value>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
-                    for (int part = 0; part < decltype(parts)::value; ++part) to = mma(v, x.part[part], to);
+                    const Split x = split(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    for (int part = 0; part < kParts; ++part) to = mma(v, x.part[part], to);
                     return to;
                 }
             };
-            auto add_values = [&](auto& to, const f4 (&from)[4], int d, const auto& vf, auto parts) {
+            auto add_values = [&](auto& to, const f4 (&from)[4], int d, const auto& vf) {
                 constexpr int N = sizeof(vf) / sizeof(F);
                 if (odd_values && (d + 1) * D > w * 16) {                    // some of these scores are masked
                     F there, none, one;                                      // `there`: 1 for places up to this lane's
@@ -457,7 +456,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
 #pragma unroll
                     for (int v = 0; v < N; ++v) {
                         const f4 reached = mma(where_not_finite(vf[v], one, none), there, f4{0, 0, 0, 0});
-                        to[v] = weigh(where_not_finite(vf[v], none, vf[v]), from, d, to[v], parts);
+                        to[v] = weigh(where_not_finite(vf[v], none, vf[v]), from, d, to[v]);
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             if (reached[r] > 0.f) to[v][r] = __builtin_nanf("");
@@ -468,21 +467,21 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
 #pragma unroll
                     for (int v = 0; v < N; ++v) to[v] = mma(vf[v], from[d], to[v]);
                 } else {
-                    const auto x = split<decltype(parts)::value>(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    const Split x = split(__builtin_shufflevector(from[2 * d], from[2 * d + 1], 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                    for (int part = 0; part < decltype(parts)::value; ++part)
+                    for (int part = 0; part < kParts; ++part)
 #pragma unroll
                         for (int v = 0; v < N; ++v) to[v] = mma(vf[v], x.part[part], to[v]);
                 }
             };
             // the state's part of the results
-            auto of_state = [&](f4 (&to)[VT], int which, int parts) {
+            auto of_state = [&](f4 (&to)[VT], int which) {
 #pragma unroll
                 for (int v = 0; v < VT; ++v) to[v] = f4{0, 0, 0, 0};
 #pragma unroll
                 for (int d = 0; d < KP / D; ++d)
 #pragma unroll
-                    for (int part = 0; part < (parts < P ? parts : P); ++part)
+                    for (int part = 0; part < P; ++part)
 #pragma unroll
                         for (int v = 0; v < VT; ++v)
                             to[v] = mma(along(state + (which * P + part) * VP * kPitch, kPitch, v * 16, d * D, lane), qf[d], to[v]);
@@ -524,10 +523,10 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
             };
             if constexpr (MODE == LEAKY_SLOPE) {
                 f4 dacc[VT], dscores[4];
-                of_state(dacc, 1, 3);
+                of_state(dacc, 1);
                 {
                     f4 acc[VT];
-                    of_state(acc, 0, 3);
+                    of_state(acc, 0);
                     const float reach_slope = slope_at(powers, i) * a.state_scale;
 #pragma unroll
                     for (int v = 0; v < VT; ++v) dacc[v] = dacc[v] * reach + acc[v] * reach_slope;
@@ -546,7 +545,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
                     F vf[VT];
 #pragma unroll
                     for (int v = 0; v < VT; ++v) vf[v] = across(values, vPitch, v * 16, d * D, lane);
-                    add_values(dacc, dscores, d, vf, std::integral_constant<int, 3>{});
+                    add_values(dacc, dscores, d, vf);
                 }
 #pragma unroll
                 for (int v = 0; v < VT; ++v)                                 // (0 for places and values that are not there)
@@ -572,7 +571,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
             };
             f4 acc[VT];
             if constexpr (MAIN) {
-                of_state(acc, 0, 2);
+                of_state(acc, 0);
                 phase_end();
                 if (more) fetch_query(0, g, col);
 #pragma unroll
@@ -587,7 +586,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
                     F vf[VT];
 #pragma unroll
                     for (int v = 0; v < VT; ++v) vf[v] = across(values, vPitch, v * 16, d * D, lane);
-                    add_values(acc, scores, d, vf, std::integral_constant<int, 2>{});
+                    add_values(acc, scores, d, vf);
                 }
                 store(acc, out, a.out_t, vleft, a.whole_out);
             }
@@ -620,7 +619,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
                     F kf[KT];
 #pragma unroll
                     for (int k = 0; k < KT; ++k) kf[k] = across(keys, kPitch, k * 16, d * D, lane);
-                    add_values(acc2, scores, d, kf, std::integral_constant<int, 2>{});
+                    add_values(acc2, scores, d, kf);
                 }
                 store(acc2, out2, a.out2_t, a.keys, a.whole_out2);
             }
@@ -630,7 +629,7 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
                 for (int v = 0; v < VT; ++v) {
                     if constexpr (SLOPE) W[s][v] = W[s][v] * step_hi + S[s][v] * step_slope;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) S[s][v][r] = FINE ? fmaf(S[s][v][r], step_hi, S[s][v][r] * step_lo) : S[s][v][r] * step_hi;
+                    for (int r = 0; r < 4; ++r) S[s][v][r] = fmaf(S[s][v][r], step_hi, S[s][v][r] * step_lo);
                 }
 #pragma unroll
             for (int d = 0; d < kChunk / D; ++d) {
@@ -650,9 +649,9 @@ __global__ __launch_bounds__(256, 2) void leaky_kernel(LeakyPass a) {
                             for (int v = 0; v < VT; ++v) to[v] = mma(x, vf[v], to[v]);
                         } else {
                             const f4 w1 = *reinterpret_cast<const f4*>(weights + d * D + 16 + 4 * g);
-                            const auto x = split<FINE ? 3 : 2>(__builtin_convertvector(kf, f8) * __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7));
+                            const Split x = split(__builtin_convertvector(kf, f8) * __builtin_shufflevector(w0, w1, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                            for (int part = 0; part < (FINE ? 3 : 2); ++part)
+                            for (int part = 0; part < kParts; ++part)
 #pragma unroll
                                 for (int v = 0; v < VT; ++v) to[v] = mma(x.part[part], vf[v], to[v]);
                         }
@@ -740,9 +739,9 @@ int launch_leaky_mode(const LeakyPass& p, dim3 grid, bool whole, hipStream_t s) 
 }
 
 // LEAKY_BOTH: up to 96 keys and 64 values, in whole pieces
-template <typename T, int MODE>
+template <typename T>
 int launch_leaky_both(const LeakyPass& p, dim3 grid, hipStream_t s) {
-#define LAUNCH(K, V) hipLaunchKernelGGL((leaky_kernel<T, K, V, MODE, true>), grid, dim3(256), 0, s, p)
+#define LAUNCH(K, V) hipLaunchKernelGGL((leaky_kernel<T, K, V, LEAKY_BOTH, true>), grid, dim3(256), 0, s, p)
 #define BY_VALUES(K) if (p.tiles == 2) LAUNCH(K, 2); else LAUNCH(K, 4)
     if (p.keys <= 32) { BY_VALUES(2); }
     else if (p.keys <= 64) { BY_VALUES(4); }
