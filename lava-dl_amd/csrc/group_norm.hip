@@ -285,29 +285,58 @@ __device__ __forceinline__ void store_sums(float* work, const float (&s1)[V], co
     }
 }
 
-// Sums of x and its square less a pivot, the first pixel of the image in the same channel: near the values, so that a mean far from
-// zero costs the variance nothing.
+// Mean and sum of squares about it, for each channel and piece.  Every mean is that of the values so far, in a thread (Welford, Note on
+// a Method for Calculating Corrected Sums of Squares and Products, 1962), and what is joined are squares about means and squares of
+// their distances: terms that are not negative, so nothing cancels, wherever the mean lies and whatever a single pixel holds.  What the
+// distances leave when they are added up corrects a joined mean, which is rounded where it is large.
 template <typename T>
 __global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
     constexpr int V = Elements<T>::kVec;
+    __shared__ float parts[256][2 * V + 1];
     const Piece p = piece_of<V>(a);
     const T* in = (const T*)a.in + p.n * a.pixels * a.channels + p.c;
-    float pivot[V], s1[V], s2[V];
-    to_floats(pivot, load_vec(in, p.left, a.whole));
+    float mean[V], square[V], count = 0;
 #pragma unroll
-    for (int e = 0; e < V; ++e) s1[e] = s2[e] = 0;
+    for (int e = 0; e < V; ++e) mean[e] = square[e] = 0;
     if (p.left > 0)
         for (int64_t q = p.p0 + p.row; q < p.p1; q += p.rows) {
             float x[V];
             to_floats(x, load_vec(in + q * a.channels, p.left, a.whole));
+            count += 1.f;
+            const float inv = __builtin_amdgcn_rcpf(count);     // within a unit in the last place, of what the mean moves by
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float d = x[e] - pivot[e];
-                s1[e] += d;
-                s2[e] = fmaf(d, d, s2[e]);
+                const float d = x[e] - mean[e];
+                mean[e] = fmaf(d, inv, mean[e]);
+                square[e] = fmaf(d, x[e] - mean[e], square[e]);
             }
         }
-    store_sums<V>(a.work, s1, s2, a, p);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        parts[threadIdx.x][2 * e] = mean[e];
+        parts[threadIdx.x][2 * e + 1] = square[e];
+    }
+    __syncthreads();
+    const int base = p.c - (int)(threadIdx.x % a.lanes) * V;
+    const int64_t all = p.p1 > p.p0 ? p.p1 - p.p0 : 0;
+    const float inv = all > 0 ? 1.f / (float)all : 0.f;
+    const float few = (float)(all / p.rows);                    // pixels of a row of threads; the first `more` have one more
+    const int more = (int)(all % p.rows);
+    for (int c = threadIdx.x; c < a.lanes * V && base + c < a.channels; c += 256) {
+        auto pixels_of = [&](int row) { return row < more ? few + 1.f : few; };
+        auto part = [&](int row, int which) { return parts[row * a.lanes + c / V][c % V * 2 + which]; };
+        float m = 0, off = 0, sq = 0;
+        for (int r = 0; r < p.rows; ++r) m = fmaf(pixels_of(r), part(r, 0), m);
+        m *= inv;
+        for (int r = 0; r < p.rows; ++r) {
+            const float d = part(r, 0) - m;
+            off = fmaf(pixels_of(r), d, off);
+            sq += fmaf(pixels_of(r) * d, d, part(r, 1));
+        }
+        float* to = a.work + ((p.n * a.splits + p.split) * a.channels + base + c) * 2;
+        to[0] = fmaf(off, inv, m);
+        to[1] = sq;
+    }
 }
 
 __device__ __forceinline__ float sum_block(float v, float* shared) {            // of 256 threads
@@ -318,13 +347,11 @@ __device__ __forceinline__ float sum_block(float v, float* shared) {            
     return (shared[0] + shared[1]) + (shared[2] + shared[3]);
 }
 
-// mean and scale of a group from the sums of its channels and pieces: the mean, then the squares about it.
-template <typename T>
+// mean and scale of a group from those of its channels and pieces
 __global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a) {
     __shared__ float shared[4];
     const int64_t n = blockIdx.x / a.groups, per = (a.pixels + a.splits - 1) / a.splits;
     const int c0 = (int)(blockIdx.x % a.groups) * a.width, count = a.width * a.splits;
-    const T* first = (const T*)a.in + n * a.pixels * a.channels + c0;
     const float* work = a.work + (n * a.splits * a.channels + c0) * 2;
     const float inv = 1.f / ((float)a.pixels * (float)a.width);
     auto pixels_of = [&](int split) {
@@ -332,21 +359,20 @@ __global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a) {
         return (float)(left < per ? (left > 0 ? left : 0) : per);
     };
     float sum = 0;
-    for (int i = threadIdx.x; i < count; i += 256) {
-        const int split = i / a.width, c = i % a.width;
-        sum = fmaf(pixels_of(split), (float)first[c], sum + work[((int64_t)split * a.channels + c) * 2]);
-    }
+    for (int i = threadIdx.x; i < count; i += 256)
+        sum = fmaf(pixels_of(i / a.width), work[((int64_t)(i / a.width) * a.channels + i % a.width) * 2], sum);
     const float mean = sum_block(sum, shared) * inv;
-    float square = 0;
+    float off = 0, square = 0;
     for (int i = threadIdx.x; i < count; i += 256) {
-        const int split = i / a.width, c = i % a.width;
-        const float* s = work + ((int64_t)split * a.channels + c) * 2;
-        const float d = mean - (float)first[c];
-        square += fmaf(d, fmaf(pixels_of(split), d, -2.f * s[0]), s[1]);
+        const float* part = work + ((int64_t)(i / a.width) * a.channels + i % a.width) * 2;
+        const float d = part[0] - mean;
+        off = fmaf(pixels_of(i / a.width), d, off);
+        square += fmaf(pixels_of(i / a.width) * d, d, part[1]);
     }
-    const float var = fmaxf(sum_block(square, shared) * inv, 0.f);
+    off = sum_block(off, shared) * inv;
+    const float var = sum_block(square, shared) * inv;
     if (threadIdx.x == 0) {
-        a.mean[blockIdx.x] = mean;
+        a.mean[blockIdx.x] = mean + off;
         a.scale[blockIdx.x] = 1.f / sqrtf(var + a.eps);
     }
 }
@@ -595,7 +621,7 @@ int launch_fwd(const NormArgs& a, const Cut& c, int activation, hipStream_t s) {
     const int64_t blocks = a.samples * a.splits * a.tiles;
     if (blocks > (1 << 23)) return SLAYER_ERANGE;
     hipLaunchKernelGGL(norm_stats_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, a);
-    hipLaunchKernelGGL(norm_join_kernel<T>, dim3((unsigned)(a.samples * a.groups)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(a.samples * a.groups)), dim3(256), 0, s, a);
 #define LAUNCH(ACT) hipLaunchKernelGGL((norm_apply_kernel<T, ACT>), dim3((unsigned)blocks), dim3(256), 0, s, a)
     BY_ACT(LAUNCH)
 #undef LAUNCH
