@@ -313,6 +313,13 @@ def device_guard(dev):
     return _no_guard if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
+def written(t):
+    """Tells autograd that a kernel has written into ``t``: a graph that has saved it then raises instead of taking the new
+    values for the old ones.  (Tensors of inference mode are in no graph.)"""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
 def ptr(t):
     return None if t is None else t.data_ptr()
 

@@ -79,7 +79,8 @@ def leaky_attention_step(query, key, value, decay, state, scale=1.0):
 
     Returns
     -------
-    torch.Tensor [N, H, V] of the type of the inputs.  There is no gradient: the state it would need is overwritten.
+    torch.Tensor [N, H, V] of the type of the inputs.  There is no gradient: the state it would need is overwritten.  (A graph
+    that has saved the state, as ``leaky_attention`` does with the one it starts from, says so when it is run backward.)
     """
     device, dtype = N.require_elements(query, key, value)
     shape, wide = query.shape, value.shape
@@ -102,6 +103,7 @@ def leaky_attention_step(query, key, value, decay, state, scale=1.0):
     with N.device_guard(device):
         N.check(N.lib().slayer_leaky_attention_step(out.data_ptr(), state.data_ptr(), query.data_ptr(), key.data_ptr(), value.data_ptr(),
                                                     args, N.stream_handle()))
+    N.written(state)
     return out
 
 

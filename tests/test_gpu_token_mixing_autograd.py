@@ -1,0 +1,45 @@
+"""The token-mixing operators and autograd: what a graph has saved, forward-mode differentiation, recomputation."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = 'cuda:0'
+
+
+def tokens(gen, n=2, t=5, h=2, k=16, v=8):
+    return [torch.randn(n, t, h, d, generator=gen).to(DEV) for d in (k, k, v)]
+
+
+def test_a_saved_state_that_is_stepped_is_noticed():
+    import lava_dl_amd.slayer as slayer
+    gen = torch.Generator().manual_seed(1)
+    q, k, v = tokens(gen)
+    decay, state = torch.tensor([50.0], device=DEV), torch.randn(2, 2, 16, 8, generator=gen).to(DEV)
+    query = q.clone().requires_grad_()
+    out = slayer.synapse.leaky_attention(query, k, v, decay, state=state)
+    want, = torch.autograd.grad(out.sum(), query, retain_graph=True)
+    copy = state.clone()
+    slayer.synapse.leaky_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, copy)           # another tensor: nothing happens
+    assert torch.equal(torch.autograd.grad(out.sum(), query, retain_graph=True)[0], want)
+    with torch.no_grad():
+        slayer.synapse.leaky_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, state[:])    # a view of the saved one
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        out.sum().backward()
+
+
+def test_a_state_of_inference_mode_is_stepped():
+    import lava_dl_amd.slayer as slayer
+    gen = torch.Generator().manual_seed(2)
+    q, k, v = tokens(gen)
+    decay = torch.tensor([50.0], device=DEV)
+    plain = torch.zeros(2, 2, 16, 8, device=DEV)
+    ref = slayer.synapse.leaky_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, plain)
+    with torch.inference_mode():
+        state = torch.zeros(2, 2, 16, 8, device=DEV)
+        assert torch.equal(slayer.synapse.leaky_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, state), ref) and torch.equal(state, plain)
+        again = torch.zeros_like(plain)
+    plain.zero_()
+    with torch.inference_mode():                                                           # an ordinary tensor in inference mode
+        slayer.synapse.leaky_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, plain)
+    assert torch.equal(plain, state) and not again.any()
