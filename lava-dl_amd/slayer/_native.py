@@ -10,6 +10,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # SLAYER_HIP_LIB points at an alternative build of the same library (e.g. a tuning build)
@@ -297,10 +298,12 @@ def raise_on_mismatch(what, fast, check, rel=None):
 
 
 def wants_grad(*tensors):
-    """True when a backward pass could reach one of the tensors: otherwise the operators call their
-    kernels directly and skip the autograd node (a few microseconds per call, which is most of a
-    call on a tensor of one time step)."""
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+    """True when a backward pass could reach one of the tensors, or one of them carries a forward-mode tangent (which the
+    autograd node refuses, as it has no rule for it): otherwise the operators call their kernels directly and skip the
+    autograd node (a few microseconds per call, which is most of a call on a tensor of one time step)."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 _no_guard = contextlib.nullcontext()

@@ -143,7 +143,7 @@ def group_norm(input, num_groups, weight=None, bias=None, eps=1e-5, activation=N
     weight = weight if weight is None else weight.float().contiguous()
     bias = bias if bias is None else bias.float().contiguous()
     code = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, weight, bias)):
+    if N.wants_grad(*(t for t in (input, weight, bias) if t is not None)):
         return _GroupNorm.apply(input, weight, bias, num_groups, eps, code)
     return _norm_fwd(input.contiguous(), weight, bias, num_groups, eps, code, False)[0]
 

@@ -55,7 +55,7 @@ def leaky_attention(query, key, value, decay, state=None, lengths=None, scale=1.
             raise RuntimeError(f'tensors on different devices: {device} and {lengths.device}')
         lengths = lengths.contiguous()
     inputs = (query, key, value, decay, state)
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in inputs):
+    if N.wants_grad(*(x for x in inputs if x is not None)):
         out, last = _LeakyAttention.apply(*inputs, lengths, float(scale), return_state)
     else:
         out, last = _forward(*inputs, lengths, float(scale), return_state)[:2]

@@ -43,3 +43,39 @@ def test_a_state_of_inference_mode_is_stepped():
     with torch.inference_mode():                                                           # an ordinary tensor in inference mode
         slayer.synapse.leaky_attention_step(q[:, 0], k[:, 0], v[:, 0], decay, plain)
     assert torch.equal(plain, state) and not again.any()
+
+
+@pytest.mark.parametrize('grad', [True, False])
+def test_forward_mode_tangents_are_refused(grad):
+    """There is no rule for them: an error, not a result without its tangent."""
+    import lava_dl_amd.slayer as slayer
+    from torch.autograd import forward_ad
+    gen = torch.Generator().manual_seed(3)
+    q, k, v = tokens(gen)
+    decay, state = torch.tensor([50.0, 7.0], device=DEV), torch.zeros(2, 2, 16, 8, device=DEV)
+    w = torch.randn(8, generator=gen).to(DEV)
+    calls = [(lambda *x: slayer.synapse.leaky_attention(*x[:4], state=x[4]), [q, k, v, decay, state]),
+             (lambda *x: slayer.synapse.leaky_attention_step(*x), [q[:, 0], k[:, 0], v[:, 0], decay, state.clone()]),
+             (lambda *x: slayer.neuron.norm.group_norm(x[0], 2, x[1], x[2], activation='silu'), [v.flatten(0, 2), w, w.clone()]),
+             (lambda *x: slayer.neuron.norm.group_norm(x[0], 2, x[1], x[2], activation='silu'), [v.flatten(1, 2), w, w.clone()]),
+             (lambda x: slayer.neuron.counter_dropout(x, 0.5, 1), [v])]
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        for call, inputs in calls:
+            ref = call(*(x.clone() for x in inputs))                                       # no tangent: as ever
+            for i in range(len(inputs)):
+                x = [y.clone() for y in inputs]
+                x[i] = forward_ad.make_dual(x[i], torch.ones_like(x[i]))
+                with pytest.raises((RuntimeError, NotImplementedError)):
+                    call(*x)
+            assert torch.equal(call(*(x.clone() for x in inputs)), ref)
+
+
+def test_neuron_dynamics_refuse_forward_mode_tangents():
+    import lava_dl_amd.slayer as slayer
+    from torch.autograd import forward_ad
+    x, decay, state = torch.randn(2, 3, 20, device=DEV), torch.tensor([400.0], device=DEV), torch.tensor([0.0], device=DEV)
+    li = slayer.neuron.dynamics.leaky_integrator.dynamics
+    with forward_ad.dual_level():
+        li(x, decay, state, 64)
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            li(forward_ad.make_dual(x, torch.ones_like(x)), decay, state, 64)
