@@ -29,7 +29,7 @@ class LeakyAttention(torch.nn.Module):
         of the dropout.
 
     The projections take the type of the tokens (``.to(torch.bfloat16)`` makes them bfloat16); decays, the norm's
-    weights and the state are float32 all the same.
+    weights and the state are float32 all the same (a bfloat16 decay of 4095 would be one of 4096, which remembers nothing).
     """
 
     def __init__(self, features, heads, head_features=64, decay=None, train_decay=False, dropout=0.0, activation='silu', seed=0):
@@ -50,6 +50,17 @@ class LeakyAttention(torch.nn.Module):
         else:
             self.register_buffer('decay', decay)
 
+    def _apply(self, fn, recurse=True):
+        """As torch's, but what is float32 stays float32 where ``fn`` changes types."""
+        def keep(t):
+            changed = fn(t)
+            return changed if changed.dtype == t.dtype else t.to(changed.device)
+
+        if recurse:
+            for child in self.children():
+                child._apply(keep if child is self.norm else fn)
+        return super()._apply(keep, recurse=False)
+
     def _heads(self, x):
         """query, key and value, views of one tensor [..., heads, head_features]."""
         return self.project(x).unflatten(-1, (3, self.heads, self.head_features)).unbind(-3)
@@ -59,7 +70,7 @@ class LeakyAttention(torch.nn.Module):
 
     def forward(self, x, state=None, lengths=None, return_state=False):
         """``x``: [N, T, C]; ``state``, ``lengths`` and ``return_state`` as for ``slayer.synapse.leaky_attention``."""
-        y, state = leaky_attention(*self._heads(x), self.decay.float(), state, lengths, self.scale, return_state=True)
+        y, state = leaky_attention(*self._heads(x), self.decay, state, lengths, self.scale, return_state=True)
         y = self._finish(y)
         return (y, state) if return_state else y
 
@@ -70,4 +81,4 @@ class LeakyAttention(torch.nn.Module):
     @torch.no_grad()
     def step(self, x, state):
         """One token of each sample in generation: ``x`` [N, C] to [N, C], ``state`` is updated in place."""
-        return self._finish(leaky_attention_step(*self._heads(x), self.decay.float(), state, self.scale))
+        return self._finish(leaky_attention_step(*self._heads(x), self.decay, state, self.scale))
