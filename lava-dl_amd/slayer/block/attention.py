@@ -2,6 +2,7 @@
 activation, dropout from a counter, between two dense projections."""
 import torch
 
+from ..neuron.base import P_SCALE
 from ..neuron.dropout import CounterDropout
 from ..neuron.norm import GroupNorm
 from ..synapse.attention import leaky_attention, leaky_attention_step
@@ -21,7 +22,8 @@ class LeakyAttention(torch.nn.Module):
         12-bit decays of the heads, 0 to 4096; None: from 512 (a memory of eight tokens) to 4 (of a thousand), each the
         same factor from the next.
     train_decay : bool
-        the decays are trained parameters.
+        the decays are trained parameters; those that training has moved out of 0 to 4096 are set to the nearer end where they
+        are used next, as the neurons' are.
     dropout : float
         probability; per element.
     activation : as for ``slayer.neuron.norm.group_norm``.
@@ -38,6 +40,8 @@ class LeakyAttention(torch.nn.Module):
             decay = [512 / 128 ** (i / max(heads - 1, 1)) for i in range(heads)]
         if len(decay) != heads:
             raise ValueError(f'expected {heads} decays, got {len(decay)}')
+        if not all(0 <= d <= P_SCALE for d in decay):
+            raise ValueError(f'decays have to be between 0 and {P_SCALE}, got {list(decay)}')
         self.heads, self.head_features = heads, head_features
         self.scale = head_features ** -0.5
         self.project = torch.nn.Linear(features, 3 * heads * head_features, bias=False)
@@ -61,6 +65,11 @@ class LeakyAttention(torch.nn.Module):
                 child._apply(keep if child is self.norm else fn)
         return super()._apply(keep, recurse=False)
 
+    def _decay(self):
+        if isinstance(self.decay, torch.nn.Parameter):
+            self.decay.data.clamp_(0, P_SCALE)
+        return self.decay
+
     def _heads(self, x):
         """query, key and value, views of one tensor [..., heads, head_features]."""
         return self.project(x).unflatten(-1, (3, self.heads, self.head_features)).unbind(-3)
@@ -70,7 +79,7 @@ class LeakyAttention(torch.nn.Module):
 
     def forward(self, x, state=None, lengths=None, return_state=False):
         """``x``: [N, T, C]; ``state``, ``lengths`` and ``return_state`` as for ``slayer.synapse.leaky_attention``."""
-        y, state = leaky_attention(*self._heads(x), self.decay, state, lengths, self.scale, return_state=True)
+        y, state = leaky_attention(*self._heads(x), self._decay(), state, lengths, self.scale, return_state=True)
         y = self._finish(y)
         return (y, state) if return_state else y
 
@@ -81,4 +90,4 @@ class LeakyAttention(torch.nn.Module):
     @torch.no_grad()
     def step(self, x, state):
         """One token of each sample in generation: ``x`` [N, C] to [N, C], ``state`` is updated in place."""
-        return self._finish(leaky_attention_step(*self._heads(x), self.decay, state, self.scale))
+        return self._finish(leaky_attention_step(*self._heads(x), self._decay(), state, self.scale))

@@ -22,3 +22,27 @@ def test_bfloat16_is_that_of_the_projections():
     assert y.dtype == torch.bfloat16 and state.dtype == torch.float32
     assert torch.equal(y, ref) and torch.equal(state, last)
     assert torch.equal(block.step(x[:, 0], state), by_hand.step(x[:, 0], last)) and torch.equal(state, last)
+
+
+@pytest.mark.parametrize('step', [False, True])
+def test_trained_decays_stay_in_their_range(step):
+    """A decay below 0 would be a state that grows without end, one above 4096 a state whose sign alternates."""
+    import lava_dl_amd.slayer as slayer
+    torch.manual_seed(2)
+    block = slayer.block.LeakyAttention(16, 3, 16, decay=[0.0, 30.0, 4096.0], train_decay=True).to(DEV)
+    x = torch.randn(2, 50, 16, device=DEV)
+    with torch.no_grad():
+        ref, last = block(x, return_state=True)
+        state = block.initial_state(2)
+        first = block.step(x[:, 0], state)
+        block.decay.add_(torch.tensor([-400.0, 0.0, 900.0], device=DEV))      # what an optimizer may do
+    if step:
+        moved = block.initial_state(2)
+        assert torch.equal(block.step(x[:, 0], moved), first) and torch.equal(moved, state)
+    else:
+        y, end = block(x, return_state=True)
+        assert torch.equal(y, ref) and torch.equal(end, last)
+        again = block(x)                                                      # two calls, then the gradients of both
+        grads = torch.autograd.grad(y.sum() + again.sum(), block.decay)[0]
+        assert torch.isfinite(grads).all()
+    assert block.decay.tolist() == [0.0, 30.0, 4096.0]

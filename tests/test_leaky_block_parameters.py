@@ -36,3 +36,12 @@ def test_other_changes_reach_all_of_it():
     assert all(p.dtype == torch.float32 for p in block.parameters()) and block.decay.dtype == torch.float32
     both = slayer.block.LeakyAttention(32, 4, 16).to('meta', torch.bfloat16)
     assert both.decay.is_meta and both.decay.dtype == torch.float32 and both.back.weight.dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize('decay', [[1.0, -0.5], [4096.5, 1.0], [float('nan'), 1.0]])
+def test_decays_out_of_range_are_refused(decay):
+    import lava_dl_amd.slayer as slayer
+    with pytest.raises(ValueError, match='between 0 and 4096'):
+        slayer.block.LeakyAttention(16, 2, 16, decay=decay)
+    slayer.block.LeakyAttention(16, 2, 16, decay=[0.0, 4096.0])
+    slayer.block.LeakyAttention(16, 2, 16, decay=torch.tensor([0.0, 4096.0]))
