@@ -75,7 +75,8 @@ class LeakyAttention(torch.nn.Module):
         return self.project(x).unflatten(-1, (3, self.heads, self.head_features)).unbind(-3)
 
     def _finish(self, y):
-        return self.back(self.dropout(self.norm(y.flatten(-2).flatten(0, -2))).view(*y.shape[:-2], -1))
+        rows = y.reshape(y.shape[:-2].numel(), self.heads * self.head_features)
+        return self.back(self.dropout(self.norm(rows)).view(*y.shape[:-2], rows.shape[1]))
 
     def forward(self, x, state=None, lengths=None, return_state=False):
         """``x``: [N, T, C]; ``state``, ``lengths`` and ``return_state`` as for ``slayer.synapse.leaky_attention``."""

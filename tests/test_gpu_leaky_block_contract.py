@@ -46,3 +46,18 @@ def test_trained_decays_stay_in_their_range(step):
         grads = torch.autograd.grad(y.sum() + again.sum(), block.decay)[0]
         assert torch.isfinite(grads).all()
     assert block.decay.tolist() == [0.0, 30.0, 4096.0]
+
+
+@pytest.mark.parametrize('n,t', [(0, 5), (2, 0), (0, 0)])
+def test_no_samples_or_no_tokens(n, t):
+    import lava_dl_amd.slayer as slayer
+    torch.manual_seed(3)
+    block = slayer.block.LeakyAttention(24, 3, 8, dropout=0.5, train_decay=True).to(DEV)
+    x = torch.zeros(n, t, 24, device=DEV, requires_grad=True)
+    state = torch.randn(n, 3, 8, 8, device=DEV)
+    y, last = block(x, state=state, return_state=True)
+    assert y.shape == x.shape and torch.equal(last, state)
+    y.sum().backward()
+    assert x.grad.shape == x.shape and not any(p.grad.any() for p in block.parameters())
+    if n == 0:
+        assert block.step(x.detach().new_zeros(0, 24), state).shape == (0, 24)
