@@ -80,9 +80,8 @@ class LeakyAttention(torch.nn.Module):
 
     def forward(self, x, state=None, lengths=None, return_state=False):
         """``x``: [N, T, C]; ``state``, ``lengths`` and ``return_state`` as for ``slayer.synapse.leaky_attention``."""
-        y, state = leaky_attention(*self._heads(x), self._decay(), state, lengths, self.scale, return_state=True)
-        y = self._finish(y)
-        return (y, state) if return_state else y
+        mixed = leaky_attention(*self._heads(x), self._decay(), state, lengths, self.scale, return_state)
+        return (self._finish(mixed[0]), mixed[1]) if return_state else self._finish(mixed)
 
     def initial_state(self, samples):
         """The state in front of a first token: zeros, float32."""

@@ -61,3 +61,20 @@ def test_no_samples_or_no_tokens(n, t):
     assert x.grad.shape == x.shape and not any(p.grad.any() for p in block.parameters())
     if n == 0:
         assert block.step(x.detach().new_zeros(0, 24), state).shape == (0, 24)
+
+
+def test_the_last_state_is_made_where_it_is_asked_for(monkeypatch):
+    import lava_dl_amd.slayer as slayer
+    import lava_dl_amd.slayer.block.attention as module
+    torch.manual_seed(4)
+    block = slayer.block.LeakyAttention(24, 3, 8).to(DEV)
+    x, asked, call = torch.randn(2, 70, 24, device=DEV), [], module.leaky_attention
+
+    def watched(*args, **names):
+        result = call(*args, **names)
+        asked.append(isinstance(result, tuple))
+        return result
+    monkeypatch.setattr(module, 'leaky_attention', watched)
+    y = block(x)
+    other, state = block(x, return_state=True)
+    assert asked == [False, True] and torch.equal(y, other) and state.shape == (2, 3, 8, 8)
