@@ -154,7 +154,7 @@ def _norm_sizes(input, groups):
 
 
 def _norm_fwd(input, weight, bias, groups, eps, activation, keep):
-    """(out, statistics or None): the means and then the scales of all groups, and behind them the call's workspace."""
+    """(out, statistics or None): the means and then the scales of all groups."""
     dtype = N.ELEMENT_TYPES[input.dtype]
     sizes = _norm_sizes(input, groups)
     lib = N.lib()
@@ -162,15 +162,16 @@ def _norm_fwd(input, weight, bias, groups, eps, activation, keep):
     if floats < 0:
         N.check(int(floats))
     out = torch.empty_like(input)
-    stats = mean = scale = workspace = None
+    stats = mean = scale = None
     if keep or floats:
         count = sizes[0] * groups
-        stats = torch.empty(2 * count + floats, dtype=torch.float32, device=input.device)
+        stats = torch.empty(2 * count, dtype=torch.float32, device=input.device)
         mean = stats.data_ptr()
-        scale, workspace = mean + 4 * count, mean + 8 * count
+        scale = mean + 4 * count
+    workspace = torch.empty(floats, dtype=torch.float32, device=input.device) if floats else None
     with N.device_guard(input.device):
         N.check(lib.slayer_group_norm_fwd(out.data_ptr(), mean, scale, input.data_ptr(), N.ptr(weight), N.ptr(bias), dtype, *sizes,
-                                          eps, activation, workspace, floats, N.stream_handle()))
+                                          eps, activation, N.ptr(workspace), floats, N.stream_handle()))
     return out, stats
 
 

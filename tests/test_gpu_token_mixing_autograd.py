@@ -79,3 +79,14 @@ def test_neuron_dynamics_refuse_forward_mode_tangents():
         li(x, decay, state, 64)
         with pytest.raises((RuntimeError, NotImplementedError)):
             li(forward_ad.make_dual(x, torch.ones_like(x)), decay, state, 64)
+
+
+@pytest.mark.parametrize('shape,groups', [((300, 64), 4), ((3, 500, 64), 4), ((2, 9000), 1)])
+def test_a_norm_keeps_its_statistics_and_no_workspace(shape, groups):
+    import lava_dl_amd.slayer as slayer
+    x, w, b = (torch.randn(s, device=DEV, requires_grad=True) for s in (shape, shape[-1:], shape[-1:]))
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append((t.data_ptr(), t.untyped_storage().nbytes())) or t, lambda t: t):
+        slayer.neuron.norm.group_norm(x, groups, w, b)
+    given = {t.data_ptr() for t in (x, w, b)}
+    assert [size for at, size in kept if at not in given] == [2 * shape[0] * groups * 4]
