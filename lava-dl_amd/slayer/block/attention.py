@@ -74,14 +74,15 @@ class LeakyAttention(torch.nn.Module):
         """query, key and value, views of one tensor [..., heads, head_features]."""
         return self.project(x).unflatten(-1, (3, self.heads, self.head_features)).unbind(-3)
 
-    def _finish(self, y):
+    def _finish(self, y, offset=None):
         rows = y.reshape(y.shape[:-2].numel(), self.heads * self.head_features)
-        return self.back(self.dropout(self.norm(rows)).view(*y.shape[:-2], rows.shape[1]))
+        return self.back(self.dropout(self.norm(rows), offset).view(*y.shape[:-2], rows.shape[1]))
 
-    def forward(self, x, state=None, lengths=None, return_state=False):
-        """``x``: [N, T, C]; ``state``, ``lengths`` and ``return_state`` as for ``slayer.synapse.leaky_attention``."""
+    def forward(self, x, state=None, lengths=None, return_state=False, offset=None):
+        """``x``: [N, T, C]; ``state``, ``lengths`` and ``return_state`` as for ``slayer.synapse.leaky_attention``, ``offset`` as
+        for ``slayer.neuron.CounterDropout``."""
         mixed = leaky_attention(*self._heads(x), self._decay(), state, lengths, self.scale, return_state)
-        return (self._finish(mixed[0]), mixed[1]) if return_state else self._finish(mixed)
+        return (self._finish(mixed[0], offset), mixed[1]) if return_state else self._finish(mixed, offset)
 
     def initial_state(self, samples):
         """The state in front of a first token: zeros, float32."""

@@ -75,7 +75,10 @@ class _CounterDropout(torch.autograd.Function):
 
 class CounterDropout(torch.nn.Module):
     """:func:`counter_dropout` while training, the identity otherwise.  ``offset`` counts the calls made while training;
-    set it (and ``seed``) to repeat them."""
+    set it (and ``seed``) to repeat them.
+
+    A call inside a backward pass is one that was made before, as activation checkpointing makes it: counting on would give it
+    another mask than the result it belongs to, so it is refused.  Give ``forward`` the offset of the call then."""
 
     def __init__(self, p=0.5, seed=0, per_neuron=False):
         super().__init__()
@@ -83,11 +86,17 @@ class CounterDropout(torch.nn.Module):
             raise ValueError(f'dropout probability has to be between 0 and 1, got {p}')
         self.p, self.seed, self.per_neuron, self.offset = p, seed, per_neuron, 0
 
-    def forward(self, input):
+    def forward(self, input, offset=None):
+        """``offset``: as for :func:`counter_dropout`; None: counted up."""
         if not self.training or self.p == 0:
             return input
-        self.offset += 1
-        return counter_dropout(input, self.p, self.seed, self.offset - 1, self.per_neuron)
+        if offset is None:
+            if torch._C._current_graph_task_id() != -1:
+                raise RuntimeError('CounterDropout: a call inside a backward pass (activation checkpointing?) would count on and '
+                                   'take another mask than the call it repeats: pass that call\'s offset')
+            offset = self.offset
+            self.offset += 1
+        return counter_dropout(input, self.p, self.seed, offset, self.per_neuron)
 
     def extra_repr(self):
         return f'p={self.p}, seed={self.seed}, per_neuron={self.per_neuron}'

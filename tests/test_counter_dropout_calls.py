@@ -1,0 +1,52 @@
+"""Which numbers the dropout module takes for a call, without a GPU: the generator in numpy stands in for the kernel."""
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+from .util_philox import keep
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """(seed, offset) of each call."""
+    import lava_dl_amd.slayer.neuron.dropout as module
+    made = []
+
+    def plain(input, p, seed, offset=0, per_neuron=False):
+        made.append((seed, offset))
+        limit = round(p * 65536)
+        mask = torch.from_numpy(keep(input.numel(), seed, offset, limit)).reshape(input.shape)
+        return torch.where(mask, input * (65536 / (65536 - limit)), 0)
+    monkeypatch.setattr(module, 'counter_dropout', plain)
+    return made
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_a_call_inside_a_backward_pass_is_refused_without_its_offset(calls, reentrant):
+    import lava_dl_amd.slayer as slayer
+    drop = slayer.neuron.CounterDropout(0.5, seed=3)
+    x = torch.randn(64, requires_grad=True)
+    y = checkpoint(lambda t: drop(t) ** 2, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match='offset'):
+        y.sum().backward()
+    drop.offset = 7                                                          # with its offset it is the same call again
+    for call in range(2):
+        want, = torch.autograd.grad((drop(x, offset=call) ** 2).sum(), x)
+        y = checkpoint(lambda t: drop(t, offset=call) ** 2, x, use_reentrant=reentrant)
+        x.grad = None
+        y.sum().backward()
+        assert torch.equal(x.grad, want)
+    assert drop.offset == 7
+    drop.eval()
+    x.grad = None
+    checkpoint(lambda t: drop(t) ** 2, x, use_reentrant=reentrant).sum().backward()
+    assert torch.equal(x.grad, 2 * x.detach())
+
+
+def test_calls_count_up(calls):
+    import lava_dl_amd.slayer as slayer
+    drop, x = slayer.neuron.CounterDropout(0.5, seed=3), torch.randn(8, requires_grad=True)
+    for _ in range(3):
+        drop(x).sum().backward()
+    drop(x, offset=9)
+    assert calls == [(3, 0), (3, 1), (3, 2), (3, 9)] and drop.offset == 3

@@ -78,3 +78,21 @@ def test_the_last_state_is_made_where_it_is_asked_for(monkeypatch):
     y = block(x)
     other, state = block(x, return_state=True)
     assert asked == [False, True] and torch.equal(y, other) and state.shape == (2, 3, 8, 8)
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_recomputed_activations(reentrant):
+    """Activation checkpointing gives the gradients of the result that it belongs to."""
+    import lava_dl_amd.slayer as slayer
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(5)
+    block = slayer.block.LeakyAttention(24, 3, 8, dropout=0.5, seed=11).to(DEV)
+    x = torch.randn(2, 70, 24, device=DEV, requires_grad=True)
+    y = block(x, offset=4)
+    want = torch.autograd.grad(y.square().sum(), [x, *block.parameters()])
+    again = checkpoint(lambda t: block(t, offset=4), x, use_reentrant=reentrant)
+    assert torch.equal(again, y)
+    again.square().sum().backward()
+    assert all(torch.equal(a, b.grad) for a, b in zip(want, [x, *block.parameters()]))
+    with pytest.raises(RuntimeError, match='offset'):
+        checkpoint(block, x, use_reentrant=reentrant).sum().backward()
