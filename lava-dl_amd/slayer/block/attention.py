@@ -27,14 +27,14 @@ class LeakyAttention(torch.nn.Module):
     dropout : float
         probability; per element.
     activation : as for ``slayer.neuron.norm.group_norm``.
-    seed : int
-        of the dropout.
+    seed : int or None
+        of the dropout, as for ``slayer.neuron.CounterDropout``.
 
     The projections take the type of the tokens (``.to(torch.bfloat16)`` makes them bfloat16); decays, the norm's
     weights and the state are float32 all the same (a bfloat16 decay of 4095 would be one of 4096, which remembers nothing).
     """
 
-    def __init__(self, features, heads, head_features=64, decay=None, train_decay=False, dropout=0.0, activation='silu', seed=0):
+    def __init__(self, features, heads, head_features=64, decay=None, train_decay=False, dropout=0.0, activation='silu', seed=None):
         super().__init__()
         if decay is None:
             decay = [512 / 128 ** (i / max(heads - 1, 1)) for i in range(heads)]

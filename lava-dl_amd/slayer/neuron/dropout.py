@@ -74,26 +74,35 @@ class _CounterDropout(torch.autograd.Function):
 
 
 class CounterDropout(torch.nn.Module):
-    """:func:`counter_dropout` while training, the identity otherwise.  ``offset`` counts the calls made while training;
-    set it (and ``seed``) to repeat them.
+    """:func:`counter_dropout` while training, the identity otherwise.
 
-    A call inside a backward pass is one that was made before, as activation checkpointing makes it: counting on would give it
-    another mask than the result it belongs to, so it is refused.  Give ``forward`` the offset of the call then."""
+    ``seed`` None: every call draws a seed of its own from torch's host generator, so layers (and processes that are seeded
+    differently) have masks of their own, ``torch.manual_seed`` repeats them, and activation checkpointing, which restores the
+    generator, repeats that of the call it makes again.
 
-    def __init__(self, p=0.5, seed=0, per_neuron=False):
+    An integer ``seed``: ``offset`` counts the calls made while training; set it (and ``seed``) to repeat them.  Layers of equal
+    shape and seed have equal masks.  A call inside a backward pass is one that was made before, as activation checkpointing makes
+    it: counting on would give it another mask than the result it belongs to, so it is refused.  Give ``forward`` the offset of
+    the call then."""
+
+    def __init__(self, p=0.5, seed=None, per_neuron=False):
         super().__init__()
         if not 0 <= p <= 1:
             raise ValueError(f'dropout probability has to be between 0 and 1, got {p}')
         self.p, self.seed, self.per_neuron, self.offset = p, seed, per_neuron, 0
 
     def forward(self, input, offset=None):
-        """``offset``: as for :func:`counter_dropout`; None: counted up."""
+        """``offset``: as for :func:`counter_dropout`; None: counted up (0 where every call has a seed of its own)."""
         if not self.training or self.p == 0:
             return input
+        if self.seed is None:
+            seed = int(torch.empty((), dtype=torch.int64, device='cpu').random_())
+            return counter_dropout(input, self.p, seed, offset or 0, self.per_neuron)
         if offset is None:
             if torch._C._current_graph_task_id() != -1:
                 raise RuntimeError('CounterDropout: a call inside a backward pass (activation checkpointing?) would count on and '
-                                   'take another mask than the call it repeats: pass that call\'s offset')
+                                   'take another mask than the call it repeats: pass that call\'s offset, or leave the seed to '
+                                   'torch\'s generator (seed=None)')
             offset = self.offset
             self.offset += 1
         return counter_dropout(input, self.p, self.seed, offset, self.per_neuron)

@@ -50,3 +50,33 @@ def test_calls_count_up(calls):
         drop(x).sum().backward()
     drop(x, offset=9)
     assert calls == [(3, 0), (3, 1), (3, 2), (3, 9)] and drop.offset == 3
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_checkpointing_repeats_the_call_of_the_generator(calls, reentrant):
+    import lava_dl_amd.slayer as slayer
+    drop = slayer.neuron.CounterDropout(0.5)
+    x = torch.randn(64, requires_grad=True)
+    for _ in range(3):
+        x.grad = None
+        parts = [checkpoint(lambda t: drop(t) ** 2, x, use_reentrant=reentrant) for _ in range(2)]      # two, then back through both
+        masks = [(y.detach() != 0) for y in parts]
+        (parts[0].sum() + parts[1].sum()).backward()
+        assert not torch.equal(*masks)
+        assert torch.allclose(x.grad, sum(2 * 4 * x.detach() * m for m in masks))
+    assert len(set(calls)) == 6 and len(calls) == 12
+
+
+def test_every_layer_and_every_call_has_a_mask_of_its_own(calls):
+    import lava_dl_amd.slayer as slayer
+    x = torch.randn(64)
+    layers = [slayer.neuron.CounterDropout(0.5) for _ in range(3)] + [slayer.block.LeakyAttention(8, 2, 4, dropout=0.5).dropout for _ in range(2)]
+    torch.manual_seed(1)
+    first = [layer(x) for _ in range(2) for layer in layers]
+    assert len(set(calls)) == 10 and len({tuple(y.tolist()) for y in first}) == 10
+    torch.manual_seed(1)
+    assert all(torch.equal(a, b) for a, b in zip(first, [layer(x) for _ in range(2) for layer in layers]))
+    for seed, offset in calls:
+        assert 0 <= seed < 1 << 64 and offset == 0
+    with torch.device('meta'):                                               # another default device has nothing to do with it
+        layers[0](x)

@@ -96,3 +96,28 @@ def test_recomputed_activations(reentrant):
     assert all(torch.equal(a, b.grad) for a, b in zip(want, [x, *block.parameters()]))
     with pytest.raises(RuntimeError, match='offset'):
         checkpoint(block, x, use_reentrant=reentrant).sum().backward()
+
+
+@pytest.mark.parametrize('reentrant', [False, True])
+def test_layers_have_masks_of_their_own_and_checkpointing_repeats_them(reentrant):
+    import lava_dl_amd.slayer as slayer
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(6)
+    layers = [slayer.block.LeakyAttention(24, 3, 8, dropout=0.5).to(DEV) for _ in range(2)]
+    wrt = [p for layer in layers for p in layer.parameters()]
+    x = torch.randn(2, 70, 24, device=DEV, requires_grad=True)
+    ones = torch.ones(140, 24, device=DEV)
+    assert not torch.equal(layers[0].dropout(ones), layers[1].dropout(ones))
+
+    def run(call):
+        torch.manual_seed(7)
+        y = x
+        for layer in layers:
+            y = call(layer, y)
+        return y, torch.autograd.grad(y.square().sum(), [x, *wrt]) if call is not again else y.square().sum().backward()
+
+    def again(layer, y):
+        return checkpoint(layer, y, use_reentrant=reentrant)
+    y, want = run(lambda layer, y: layer(y))
+    other, _ = run(again)
+    assert torch.equal(y, other) and all(torch.equal(a, b.grad) for a, b in zip(want, [x, *wrt]))
