@@ -80,8 +80,8 @@ class CounterDropout(torch.nn.Module):
     differently) have masks of their own, ``torch.manual_seed`` repeats them, and activation checkpointing, which restores the
     generator, repeats that of the call it makes again.
 
-    An integer ``seed``: ``offset`` counts the calls made while training; set it (and ``seed``) to repeat them.  Layers of equal
-    shape and seed have equal masks.  A call inside a backward pass is one that was made before, as activation checkpointing makes
+    An integer ``seed``: ``offset`` counts the calls made while training; set it (and ``seed``) to repeat them.  It is part of the
+    ``state_dict``, so that a run that is taken up again goes on with it.  Layers of equal shape and seed have equal masks.  A call inside a backward pass is one that was made before, as activation checkpointing makes
     it: counting on would give it another mask than the result it belongs to, so it is refused.  Give ``forward`` the offset of
     the call then."""
 
@@ -106,6 +106,19 @@ class CounterDropout(torch.nn.Module):
             offset = self.offset
             self.offset += 1
         return counter_dropout(input, self.p, self.seed, offset, self.per_neuron)
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        if self.seed is not None:                           # its 64 bits in a signed number
+            destination[prefix + 'offset'] = torch.tensor(self.offset - (self.offset >> 63 << 64), device='cpu')
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        key = prefix + 'offset'
+        if key in state_dict:                               # (one from a module without a seed has none)
+            self.offset = int(state_dict[key]) % (1 << 64)
+            if key in unexpected_keys:
+                unexpected_keys.remove(key)
 
     def extra_repr(self):
         return f'p={self.p}, seed={self.seed}, per_neuron={self.per_neuron}'

@@ -80,3 +80,37 @@ def test_every_layer_and_every_call_has_a_mask_of_its_own(calls):
         assert 0 <= seed < 1 << 64 and offset == 0
     with torch.device('meta'):                                               # another default device has nothing to do with it
         layers[0](x)
+
+
+def test_the_count_is_saved_and_loaded(calls, tmp_path):
+    import lava_dl_amd.slayer as slayer
+    x = torch.randn(8)
+
+    def make(seed=3):
+        return torch.nn.Sequential(torch.nn.Linear(8, 8), slayer.neuron.CounterDropout(0.5, seed=seed))
+    model = make()
+    for _ in range(5):
+        model(x)
+    torch.save(model.state_dict(), tmp_path / 'model')
+    after = [model(x) for _ in range(2)]
+    taken_up = make()
+    taken_up.load_state_dict(torch.load(tmp_path / 'model', weights_only=True))
+    assert taken_up[1].offset == 5 and all(torch.equal(taken_up(x), y) for y in after)
+    for offset in (0, (1 << 63) - 1, 1 << 63, (1 << 64) - 1):
+        model[1].offset = offset
+        taken_up.load_state_dict(model.state_dict())
+        assert taken_up[1].offset == offset
+    old = {name: value for name, value in model.state_dict().items() if 'offset' not in name}
+    taken_up.load_state_dict(old)                                            # a state without a count leaves it as it is
+    assert taken_up[1].offset == offset
+    free = make(seed=None)
+    assert set(free.state_dict()) == set(old)
+    free.load_state_dict(model.state_dict())
+    taken_up.load_state_dict(free.state_dict())
+    with pytest.raises(RuntimeError, match='other'):
+        taken_up.load_state_dict({**old, '1.other': x})
+    block = slayer.block.LeakyAttention(8, 2, 4, dropout=0.5, seed=1)
+    block.dropout.offset = 6
+    other = slayer.block.LeakyAttention(8, 2, 4, dropout=0.5, seed=1)
+    other.load_state_dict(block.state_dict())
+    assert other.dropout.offset == 6

@@ -44,4 +44,3 @@ def test_decays_out_of_range_are_refused(decay):
     with pytest.raises(ValueError, match='between 0 and 4096'):
         slayer.block.LeakyAttention(16, 2, 16, decay=decay)
     slayer.block.LeakyAttention(16, 2, 16, decay=[0.0, 4096.0])
-    slayer.block.LeakyAttention(16, 2, 16, decay=torch.tensor([0.0, 4096.0]))
