@@ -19,7 +19,7 @@ def leaky_attention(query, key, value, decay, state=None, lengths=None, scale=1.
         float32 or bfloat16 GPU tensors [N, T, H, K], K at most 128.
     value : torch.Tensor
         [N, T, H, V] of the same type, V at most 128.  Any strides: what has neighbouring elements along the last axis is
-        read where it lies.
+        read where it lies, what has not (the time-innermost tensors of the neurons, turned) is copied first.
     decay : torch.Tensor
         float32, one value or one for each head: 12-bit decays as the neurons have them, 0 keeps everything, 4096 nothing.
         Need not be whole; may be trained.
@@ -165,8 +165,10 @@ def _forward(query, key, value, decay, state, lengths, scale, return_state):
 class _LeakyAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, query, key, value, decay, state, lengths, scale, return_state):
-        out, last, *saved = _forward(query, key, value, decay, state, lengths, scale, return_state)
-        ctx.save_for_backward(*saved, lengths)
+        out, last, *saved, starts = _forward(query, key, value, decay, state, lengths, scale, return_state)
+        if not ctx.needs_input_grad[0] or ctx.needs_input_grad[3]:           # who else has no use for the states of the segments
+            starts = None
+        ctx.save_for_backward(*saved, starts, lengths)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return out, last

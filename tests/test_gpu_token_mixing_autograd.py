@@ -90,3 +90,21 @@ def test_a_norm_keeps_its_statistics_and_no_workspace(shape, groups):
         slayer.neuron.norm.group_norm(x, groups, w, b)
     given = {t.data_ptr() for t in (x, w, b)}
     assert [size for at, size in kept if at not in given] == [2 * shape[0] * groups * 4]
+
+
+@pytest.mark.parametrize('wrt,kept_states', [(('q', 'k', 'v'), True), (('q',), True), (('k', 'v'), False), (('q', 'k', 'v', 'decay'), False)])
+def test_attention_keeps_the_states_of_its_segments_for_the_query_alone(wrt, kept_states):
+    """... whose pass takes them; with the decays' gradient it makes them again, beside their derivatives."""
+    import lava_dl_amd.slayer as slayer
+    gen = torch.Generator().manual_seed(4)
+    q, k, v = tokens(gen, t=1500)
+    x = dict(q=q, k=k, v=v, decay=torch.tensor([50.0, 3.0], device=DEV))
+    leaves = [x[name].requires_grad_() for name in wrt]
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t.data_ptr()) or t, lambda t: t):
+        out = slayer.synapse.leaky_attention(*x.values())
+    assert (len(set(kept) - {t.data_ptr() for t in x.values()}) == 1) == kept_states
+    for once in range(2):                                                    # the graph may be run twice
+        grads = torch.autograd.grad(out.square().sum(), leaves, retain_graph=True)
+        assert once == 0 or all(torch.equal(a, b) for a, b in zip(grads, first))
+        first = grads
