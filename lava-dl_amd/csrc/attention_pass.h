@@ -88,9 +88,10 @@ __device__ __forceinline__ b8 across(const bf16* tile, int pitch, int column, in
     return b8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
-// A float32 operand: in float32, or as three bfloat16 numbers that sum to it (within 2^-24), so that what the kernel makes itself (scores,
-// states, leaked keys) keeps float32's digits on the way.  Two would leave 2^-16 of every term, which is more than the rounding of
-// a bfloat16 result as soon as the terms cancel to a 256th of their magnitudes.
+// A float32 operand: in float32, or as three bfloat16 numbers that sum to it, so that what the kernel makes itself (scores, states, leaked
+// keys) keeps float32's digits on the way.  Two would leave 2^-16 of every term, which is more than the rounding of a bfloat16
+// result as soon as the terms cancel to a 256th of their magnitudes; [64,1000,8,64], forward, calls in a row: 65 us with two, 82 with
+// three.  A value that is not finite, or beyond the largest bfloat16, leaves a NaN.
 constexpr int kParts = 3;
 struct Split { b8 part[kParts]; };
 __device__ __forceinline__ Split split(f8 v) {
@@ -162,14 +163,16 @@ __device__ __forceinline__ float slope_at(const float* powers, int n) { return n
 //
 //   What bounds it (64 keys and values, two workgroups a compute unit).  float32: the matrix cores, whose 3.25 products of 64 x 64 x 64
 // a chunk take 6 656 cycles of each SIMD; [32,1500,4,64] in four segments 64 us, of which 37 are those and 39 would be a copy of the
-// same bytes.  bfloat16: a chunk of a workgroup takes 5 500 cycles alone and 6 500 beside another (filling LDS 900, scores 850, state
-// 780, the products with values and keys 1 700 to 2 100, results 430), about what the memory needs for it, 7 400 for two;
-// [64,1000,8,64], calls in a row, 65 us from the last-level cache and 79 from memory, 262 MB, where a kernel that only moves the tensors takes 52 and
-// 63: pieces of 128 bytes cost it a fifth.  A third workgroup a compute unit, slices of 32 values, priorities for one of the two
-// and two sets of tiles (one barrier a chunk) were no faster.
-//   Registers decide: above 256 of them, or with any in scratch memory (whose accesses wait for the chunk on its way), the same
-// kernels took 1.4 to 2 times as long.  So a strip is compiled for its wave, addresses are made anew in every chunk, the values are
-// read twice, and `phase_end` keeps the compiler from starting the reads of a later phase.
+// same bytes.  bfloat16: vector instructions, 55 % of a compute unit's busy cycles (about half of them, counted in the
+// code, split scores, states and keys into parts), LDS 38 %, the matrix cores 23 %; [64,1000,8,64], calls in a row, 82 us from the last-level cache and 91 from memory,
+// 262 MB, where a kernel that only moves the tensors takes 52 and 63: pieces of 128 bytes cost it a fifth.  A third workgroup a compute
+// unit, slices of 32 values, priorities for one of the two and two sets of tiles (one barrier a chunk) were no faster.
+//   Registers decide: versions of the forward and joint kernels with more than 256 of them, or with many in scratch memory (whose
+// accesses wait for the chunk on its way), took 1.4 to 2 times as long.  So a strip is compiled for its wave, addresses are made anew in
+// every chunk, the values are read twice, and `phase_end` keeps the compiler from starting the reads of a later phase.  What does
+// not fit all the same: float32 LEAKY_SLOPE spills at KT, VT = 4, 4 (9 registers), 6, 3 (64) and 8, 2 (10), float32 LEAKY_BOTH at 6, 4 (26; 219 us,
+// 236 as two passes, [32,1500,4] with 96 keys and 64 values), bfloat16 LEAKY_SLOPE at 6, 3 (2); LEAKY_SLOPE with VT = 4 and KT = 6 or 8, or
+// 8, 3, and float32 LEAKY_MAIN at 8, 4 leave room for one workgroup a compute unit.
 __device__ __forceinline__ void phase_end() { __builtin_amdgcn_sched_barrier(0); }
 
 template <typename T, int KT, int VT, int MODE, bool WHOLE>

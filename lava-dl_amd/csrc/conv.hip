@@ -319,10 +319,10 @@ __global__ __launch_bounds__(kWave) void conv_mfma_kernel(float* __restrict__ ou
 
 // The same kernel for more than 32 taps, where the float instruction (one pass of the matrix pipe per 4 window
 // samples) is what bounds it: every tap and every sample is split into three bfloat16 parts that add up to it
-// to within 2^-27 (each part the rounding to nearest of what the parts before it leave), and the products of the
+// (each part the rounding to nearest of what the parts before it leave), and the products of the
 // parts are taken with the bfloat16 instruction (one pass per 32 window samples: two window groups at a time) --
 // part i of the taps with part j of the samples for i + j <= 2, six products, each exact, summed in float32.  What
-// is left out (i + j >= 3 and the remainders) is below 2^-25 of a product: less than the rounding of a float sum.
+// is left out (i + j >= 3) is 2^-24 of a product at most: the rounding of one float sum.
 // The parts are made once per sample on the way into the ring (three planes of four bfloat16 per quad).
 // A part that is zero in every lane of a tile and its neighbour (wave-uniform: spikes, small
 // integers, anything of at most 8 significant bits has no second and third part) is left out together with its

@@ -8,8 +8,9 @@
 // come first, for each channel and piece of the image, are joined, and a second kernel applies them.
 //   Rows, 48000 tokens of 256 channels in 4 groups, bfloat16: forward 14 to 15 us (3.2 to 3.5 TB/s), backward 20 (3.8 TB/s), 5 for the sums of the
 // weights' gradients.  The first form, whose threads looked up their channels anew for each row and whose activations divided in full
-// precision, took 51, 29 and 21.  Pixels, [32,1024,512] float32: statistics 14 us, joining 5, applying 23 (5.9 TB/s); backward 25, 5 and 33 (6.1 TB/s): the
-// second reading comes partly from the last-level cache.
+// precision, took 51, 29 and 21.  Pixels, [32,1024,512] float32: statistics 15 us, joining 5, applying 23 (5.7 TB/s); backward 26, 5 and 33 (6.1 TB/s): the
+// second reading comes partly from the last-level cache.  Rows of more than 2048 bfloat16 channels a group take up to 512 registers backwards,
+// with ReLU some scratch memory.
 #include "common.h"
 #include "elements.h"
 

@@ -1,7 +1,7 @@
 // A float32 as the sum of three bfloat16 numbers, the operands of v_mfma_f32_16x16x32_bf16: each part is the rounding
-// to nearest of what the parts before it leave (|second| <= 2^-9, |third| <= 2^-18 of the value, what the three leave
-// out <= 2^-27).  The products of parts are exact in float32; of two split factors the products part i x part j with
-// i + j <= 2 are taken, what is left out is below 2^-26 of the product.
+// to nearest of what the parts before it leave (|second| <= 2^-8, |third| <= 2^-17 of the value's power of two, and the
+// three leave nothing of its 24 bits).  The products of parts are exact in float32; of two split factors the products part
+// i x part j with i + j <= 2 are taken, what is left out is 2^-24 of the product at most.
 //   A value that is not finite leaves a NaN (so does a finite one beyond the largest bfloat16, 3.3895e38): callers
 // either treat it (conv.hip) or recognise a result that is not finite and compute it again in float32 (synapse_walk.hip,
 // synapse_wgrad_walk.hip).

@@ -114,7 +114,7 @@ def group_norm(input, num_groups, weight=None, bias=None, eps=1e-5, activation=N
     input : torch.Tensor
         float32 or bfloat16 GPU tensor [N, ..., C].
     num_groups : int
-        divides C.
+        divides C; N * num_groups at most 2**23 where a group reaches over more than one position.
     weight, bias : torch.Tensor or None
         C floating-point values each; None: 1 and 0.
     eps : float

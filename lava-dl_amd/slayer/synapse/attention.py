@@ -37,7 +37,8 @@ def leaky_attention(query, key, value, decay, state=None, lengths=None, scale=1.
     torch.Tensor [N, T, H, V], contiguous, of the type of the inputs; with ``return_state`` a pair of it and the state.
 
     The states and all sums are float32; gradients are those of query, key, value, decay (the derivative with respect to
-    the decay itself) and state.
+    the decay itself) and state.  A value that is not finite leaves values that are not finite (an infinity may leave a NaN) in
+    the results that it reaches, and in no others.
     """
     device, dtype = N.require_elements(query, key, value)
     if query.dim() != 4 or key.shape != query.shape or value.dim() != 4 or value.shape[:3] != query.shape[:3]:
