@@ -634,7 +634,7 @@ int slayer_rf_limit(float *sin_decay, float *cos_decay, float gain_max, int64_t 
 int slayer_quantize_bwd(float *grad_in, const float *grad_out, const unsigned char *inside, float scale, int64_t n,
                         void *stream);
 
-/* ---- token mixing: leaky attention, group norm, dropout ---------------------------------------- */
+/* ---- token mixing: leaky attention, gated leak, rotary positions, norms, dropout ---------------- */
 /* Not in the reference.  Tensors of float32 or bfloat16 (`dtype`), statistics and states float32. */
 
 #define SLAYER_FLOAT32  0
@@ -694,6 +694,75 @@ int slayer_group_norm_bwd(void *grad_in, float *grad_weight, float *grad_bias, c
  * gradient is the same call on grad_out. */
 int slayer_dropout(void *out, const void *in, int dtype, int64_t n, int64_t steps, int limit, float scale, uint64_t seed,
                    uint64_t offset, void *stream);
+
+/* Gated leak: the leaky integrator whose leak a token's gate opens, for every sample and channel
+ *     leak[t] = decay / 4096 * sigmoid(gate[t]),   h[t] = (1 - leak[t]) h[t-1] + drive(leak[t]) * input[t],   h[-1] = state,
+ * drive 0: 1, 1: leak, 2: sqrt(leak (2 - leak)).  input and gate are [samples][tokens][channels] with strides (in elements) of their first
+ * two axes and neighbouring elements on the last; out and the gradients are contiguous.  Lengths as for leaky attention. */
+typedef struct slayer_gated_leak {
+    int64_t samples, tokens, channels;
+    int64_t num_decays;                             /* 1 or channels */
+    const float *decay;                             /* between 0 and 4096 */
+    const void *lengths;                            /* samples integers on the device, or NULL: all of `tokens` */
+    int lengths_bytes;                              /* 4 or 8 */
+    int dtype, drive;
+    int64_t input_stride[2], gate_stride[2], grad_stride[2];   /* sample, token; grad_stride: of grad_out */
+} slayer_gated_leak;
+
+/* Floats of the states that the forward call keeps for the backward call, and of workspace; or a negative SLAYER_E*. */
+int64_t slayer_gated_leak_starts(const slayer_gated_leak *a);
+int64_t slayer_gated_leak_workspace(const slayer_gated_leak *a, int backward);
+/* state, last: [samples][channels] floats or NULL (zeros; not wanted); starts: for the backward call, or NULL */
+int slayer_gated_leak_fwd(void *out, float *last, float *starts, const void *input, const void *gate, const float *state,
+                          const slayer_gated_leak *a, float *workspace, int64_t workspace_floats, void *stream);
+/* Gradients from those of out and of last (NULL: 0).  grad_decay (num_decays floats, the derivative with respect to the decay itself)
+ * and grad_state may be NULL. */
+int slayer_gated_leak_bwd(void *grad_input, void *grad_gate, float *grad_decay, float *grad_state, const void *grad_out,
+                          const float *grad_last, const void *input, const void *gate, const float *starts,
+                          const slayer_gated_leak *a, float *workspace, int64_t workspace_floats, void *stream);
+/* One token a sample (tokens, lengths and the token strides are not looked at): state is updated in place. */
+int slayer_gated_leak_step(void *out, float *state, const void *input, const void *gate, const slayer_gated_leak *a, void *stream);
+
+/* Rotary positions: pairs of a head's first `turned` features turned by position * frequency[i], i < turned / 2, and scaled by
+ * magnitude; the features behind them are copied.  query and key are [samples][tokens][heads][features] with strides (in elements) of
+ * their first three axes and neighbouring elements on the last; the outputs are contiguous.  inverse: the angles' sign is changed, which
+ * is the gradient's call. */
+#define SLAYER_ROTARY_HALVES 0                      /* pairs (i, i + turned / 2) */
+#define SLAYER_ROTARY_PAIRS  1                      /* pairs (2 i, 2 i + 1) */
+typedef struct slayer_rotary_call {
+    int64_t samples, tokens, query_heads, key_heads, features, turned;   /* either number of heads may be 0 */
+    const double *frequency;                        /* radians a token, on the device */
+    const void *position;                           /* integers on the device, or NULL: 0, 1, ... for each sample */
+    int position_bytes;                             /* 4 or 8 */
+    int position_each;                              /* 0: samples of them, of the first token; 1: samples * tokens */
+    int layout, dtype;
+    float magnitude;
+    int64_t query_stride[3], key_stride[3];         /* sample, token, head */
+} slayer_rotary_call;
+int slayer_rotary(void *out_query, void *out_key, const void *query, const void *key, const slayer_rotary_call *r, int inverse,
+                  void *stream);
+
+/* A norm behind a block and one in front of the next with the block's gate and residual scale, on rows of `channels` (up to 16384):
+ *     total = residual + factor * scale * act(gate) * inner * input / rms(input),   out = outer * total / rms(total),
+ * rms(v) = sqrt(mean(v^2) + eps).  A parameter that is NULL: no scale; no norm of input (inner); no out (outer; out has to be NULL).
+ * residual NULL: 0.  Rows have strides (in elements) and neighbouring elements; the outputs are contiguous. */
+typedef struct slayer_residual_norm {
+    int64_t rows, channels;
+    const float *inner, *outer, *scale;             /* channels floats or NULL */
+    int dtype, residual_dtype;                      /* of input, gate, out; of residual and total: dtype or SLAYER_FLOAT32 */
+    int activation;                                 /* of the gate: 0 no gate, 1 the gate itself, 2 sigmoid, 3 silu */
+    float eps, factor;
+    int64_t input_stride, residual_stride, gate_stride, grad_out_stride, grad_total_stride;
+} slayer_residual_norm;
+int64_t slayer_residual_norm_workspace(const slayer_residual_norm *p);
+/* total may be NULL where out is not; stats: 2 * rows floats for the backward call, or NULL */
+int slayer_residual_norm_fwd(void *out, void *total, float *stats, const void *input, const void *residual, const void *gate,
+                             const slayer_residual_norm *p, void *stream);
+/* Any result may be NULL; grad_out, grad_total: NULL is 0.  The workspace is for grad_inner, grad_outer and grad_scale. */
+int slayer_residual_norm_bwd(void *grad_input, void *grad_residual, void *grad_gate, float *grad_inner, float *grad_outer,
+                             float *grad_scale, const void *grad_out, const void *grad_total, const float *stats, const void *input,
+                             const void *residual, const void *gate, const slayer_residual_norm *p, float *workspace,
+                             int64_t workspace_floats, void *stream);
 
 /* ---- cross-check implementations (debug mode) ------------------------------------------------ */
 

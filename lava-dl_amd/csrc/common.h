@@ -66,6 +66,16 @@ int launch_nan_check(unsigned* found, const NanCheck& tensors, hipStream_t strea
 int launch_reduce_param_grad(float* grad, const float* partial, float* scratch, int64_t M, int64_t npb,
                              int64_t num_params, hipStream_t stream);
 int launch_zero_fill(float* p, int64_t n, hipStream_t stream);
+
+// out[k][c] = factor * sum over the rows of parts[k][row * pitch + c], for up to four k, in one fixed order.  (column_sums.hip)
+struct ColumnSums {
+    float* out[4];
+    const float* parts[4];
+    int64_t rows, columns, pitch;
+    float factor;
+};
+int launch_column_sums(const ColumnSums& sums, int count, hipStream_t stream);
+
 inline int finish_delay_gradient(const slayer_delays* d, const float* grad_spikes, bool in_scan, int64_t M, int64_t npb,
                                  int64_t T, hipStream_t stream) {
     if (!d || !d->grad_out_delay) return 0;

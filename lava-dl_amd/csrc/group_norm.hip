@@ -18,21 +18,6 @@ namespace slayer {
 
 enum { ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU };
 
-// 1 / (1 + exp(-z)) from the hardware's base-two exponential and reciprocal, a unit in the last place each.  For bfloat16 tensors as they
-// are: the argument's rounding makes it (3 + 1.5 |z|) 2^-24 where it matters (for negative z it is the exponential that falls), far below
-// the rounding of the result.  For float32 tensors what the argument's rounding leaves goes into the exponential, 2^x (1 + r ln 2), and the
-// reciprocal takes a step of Newton's: 6 2^-24.  Rows of [480000,256] in 4 groups, forward, as they are / with the two / with the precise
-// functions: bfloat16 114 / 139 / 177 us, float32 193 / 216 / 250 us.
-template <typename T> __device__ __forceinline__ float logistic(float z) {
-    constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
-    constexpr float hi = (float)-kLog2e, lo = (float)(-kLog2e - (double)hi);
-    const float x = z * hi;
-    float e = __builtin_amdgcn_exp2f(x);
-    if constexpr (sizeof(T) != 4) return __builtin_amdgcn_rcpf(1.f + e);
-    e = fmaf(e, fmaf(z, lo, fmaf(z, hi, -x)) * (float)kLn2, e);
-    const float r = __builtin_amdgcn_rcpf(1.f + e);
-    return x < 126.f ? fmaf(fmaf(-(1.f + e), r, 1.f), r, r) : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x));
-}
 template <typename T, int ACT> __device__ __forceinline__ float activate(float z) {
     if (ACT == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
     if (ACT == ACT_SILU) return z * logistic<T>(z);
@@ -47,11 +32,6 @@ template <typename T, int ACT> __device__ __forceinline__ float slope(float z) {
     }
     if (ACT == ACT_GELU) return fmaf(z, 0.39894228040143268f * expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
     return 1.f;
-}
-
-__device__ __forceinline__ float sum_lanes(float v, int lanes) {
-    for (int d = lanes >> 1; d > 0; d >>= 1) v += __shfl_xor(v, d);
-    return v;
 }
 
 struct NormArgs {

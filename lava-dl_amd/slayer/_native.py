@@ -47,6 +47,32 @@ class Attention(ctypes.Structure):
 
 
 _AP = ctypes.POINTER(Attention)
+
+
+class GatedLeak(ctypes.Structure):
+    """struct slayer_gated_leak of include/slayer_hip.h (device pointers as integers)."""
+    _fields_ = [('samples', _I64), ('tokens', _I64), ('channels', _I64), ('num_decays', _I64), ('decay', _P), ('lengths', _P),
+                ('lengths_bytes', _INT), ('dtype', _INT), ('drive', _INT), ('input_stride', _I64 * 2), ('gate_stride', _I64 * 2),
+                ('grad_stride', _I64 * 2)]
+
+
+class Rotary(ctypes.Structure):
+    """struct slayer_rotary_call of include/slayer_hip.h (device pointers as integers)."""
+    _fields_ = [('samples', _I64), ('tokens', _I64), ('query_heads', _I64), ('key_heads', _I64), ('features', _I64),
+                ('turned', _I64), ('frequency', _P), ('position', _P), ('position_bytes', _INT), ('position_each', _INT),
+                ('layout', _INT), ('dtype', _INT), ('magnitude', _F), ('query_stride', _I64 * 3), ('key_stride', _I64 * 3)]
+
+
+class ResidualNorm(ctypes.Structure):
+    """struct slayer_residual_norm of include/slayer_hip.h (device pointers as integers)."""
+    _fields_ = [('rows', _I64), ('channels', _I64), ('inner', _P), ('outer', _P), ('scale', _P), ('dtype', _INT),
+                ('residual_dtype', _INT), ('activation', _INT), ('eps', _F), ('factor', _F), ('input_stride', _I64), ('residual_stride', _I64),
+                ('gate_stride', _I64), ('grad_out_stride', _I64), ('grad_total_stride', _I64)]
+
+
+_GP = ctypes.POINTER(GatedLeak)
+_RP = ctypes.POINTER(Rotary)
+_NP = ctypes.POINTER(ResidualNorm)
 _U64 = ctypes.c_uint64
 
 _SIGNATURES = {
@@ -109,6 +135,15 @@ _SIGNATURES = {
     'slayer_group_norm_fwd': (_INT, [_P] * 6 + [_INT] + [_I64] * 4 + [_F, _INT, _P, _I64, _P]),
     'slayer_group_norm_bwd': (_INT, [_P] * 9 + [_INT] + [_I64] * 4 + [_INT, _P, _I64, _P]),
     'slayer_dropout': (_INT, [_P, _P, _INT, _I64, _I64, _INT, _F, _U64, _U64, _P]),
+    'slayer_gated_leak_starts': (_I64, [_GP]),
+    'slayer_gated_leak_workspace': (_I64, [_GP, _INT]),
+    'slayer_gated_leak_fwd': (_INT, [_P] * 6 + [_GP, _P, _I64, _P]),
+    'slayer_gated_leak_bwd': (_INT, [_P] * 9 + [_GP, _P, _I64, _P]),
+    'slayer_gated_leak_step': (_INT, [_P] * 4 + [_GP, _P]),
+    'slayer_rotary': (_INT, [_P] * 4 + [_RP, _INT, _P]),
+    'slayer_residual_norm_workspace': (_I64, [_NP]),
+    'slayer_residual_norm_fwd': (_INT, [_P] * 6 + [_NP, _P]),
+    'slayer_residual_norm_bwd': (_INT, [_P] * 12 + [_NP, _P, _I64, _P]),
     'slayer_li_fwd_naive': (_INT, [_P, _P, _P, _P, _D, _INT, _I64, _I64, _I64, _I64, _I64, _P]),
     'slayer_li_bwd_naive': (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _P]),
     'slayer_ath_fwd_naive': (_INT, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _INT,

@@ -4,6 +4,7 @@ can be given."""
 from . import dynamics, cuba, alif, rf, rf_iz, adrf, adrf_iz, sigma_delta
 from . import norm
 from .dropout import Dropout, CounterDropout, counter_dropout
+from .gated import gated_leak, gated_leak_step
 
 __all__ = ['dynamics', 'cuba', 'alif', 'rf', 'rf_iz', 'adrf', 'adrf_iz', 'sigma_delta', 'norm', 'Dropout',
-           'CounterDropout', 'counter_dropout']
+           'CounterDropout', 'counter_dropout', 'gated_leak', 'gated_leak_step']

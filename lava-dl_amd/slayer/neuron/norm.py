@@ -6,7 +6,8 @@ of the time-sequential kernels.  A neuron that is given one of them hooks its we
 ``pre_hook_fx`` (neuron/base.py:127-141 in the reference).
 
 ``group_norm`` and ``GroupNorm`` are for tensors with the channels last (tokens, images) and run in slayer_group_norm_fwd / bwd
-of libslayer_hip.so."""
+of libslayer_hip.so; ``residual_norm`` and ``ResidualNorm``, the norms behind a block and in front of the next one, in
+slayer_residual_norm_fwd / bwd."""
 import torch
 
 from .. import _native as N
@@ -227,3 +228,167 @@ class GroupNorm(torch.nn.Module):
 
     def extra_repr(self):
         return f'{self.num_groups}, {self.num_channels}, eps={self.eps}, activation={self.activation}'
+
+
+GATES = {None: 1, 'none': 1, 'sigmoid': 2, 'silu': 3}
+
+
+def residual_norm(input, residual, weight=None, inner=None, gate=None, scale=None, activation='sigmoid', eps=1e-5, return_sum=True):
+    """What stands between two blocks, in one operator: the norm of a block's result, its gate and scale, the residual stream, and the
+    norm in front of the next block,
+
+        total = residual + scale * act(gate) * inner * input / rms(input),    out = weight * total / rms(total),
+
+    with rms(x) = sqrt(mean(x ** 2) + eps) over the last axis.
+
+    Parameters
+    ----------
+    input : torch.Tensor
+        float32 or bfloat16 GPU tensor [..., C], C at most 16384.  Rows that lie a fixed distance from each other (a part of a
+        projection) are read where they lie, others are copied first; so for residual and gate.
+    residual : torch.Tensor or None
+        of the same shape and type, or float32 (a stream that is kept in float32 between bfloat16 blocks); None: 0.
+    weight : torch.Tensor or None
+        C floating-point values of the norm in front of the next block; None: there is none, and no ``out``.
+    inner : torch.Tensor or None
+        C floating-point values of the norm behind the block; None: there is none.
+    gate : torch.Tensor or None
+        of the shape and type of input.
+    scale : torch.Tensor, float or None
+        C floating-point values, or one number.
+    activation : 'sigmoid', 'silu', None or 'none'
+        of the gate.
+    eps : float
+    return_sum : bool
+        whether ``total`` is wanted (always without a ``weight``).
+
+    Returns
+    -------
+    (out, total), contiguous, of the types of input and residual (of input without one); ``out`` alone without ``return_sum``, ``total``
+    alone without a ``weight``.  ``out`` is that of the sum before it is rounded to the type of ``total``.  Statistics, weights and their
+    gradients are float32.
+    """
+    if activation not in GATES:
+        raise ValueError(f'unknown activation {activation!r}: one of {list(GATES)}')
+    if not eps >= 0:
+        raise ValueError(f'eps has to be at least 0, got {eps}')
+    device, _ = N.require_elements(input) if gate is None else N.require_elements(input, gate)
+    if input.dim() < 1 or not 1 <= input.shape[-1] <= 16384:
+        raise RuntimeError(f'expected a tensor [..., C] with C up to 16384, got {tuple(input.shape)}')
+    if gate is not None and gate.shape != input.shape:
+        raise RuntimeError(f'gate: expected the shape {tuple(input.shape)}, got {tuple(gate.shape)}')
+    if residual is not None:
+        if not torch.is_tensor(residual) or residual.shape != input.shape or residual.dtype not in (input.dtype, torch.float32):
+            raise RuntimeError(f'residual: expected a tensor {list(input.shape)} of {input.dtype} or torch.float32')
+        if residual.device != device:
+            raise RuntimeError(f'tensors on different devices: {device} and {residual.device}')
+    factor = 1.0
+    if scale is not None and not torch.is_tensor(scale):
+        factor, scale = float(scale), None
+    channels = input.shape[-1]
+    parameters = []
+    for name, t in (('weight', weight), ('inner', inner), ('scale', scale)):
+        if t is not None:
+            if not torch.is_tensor(t) or t.shape != (channels,) or not t.is_floating_point():
+                raise RuntimeError(f'{name}: expected {channels} floating-point values')
+            if t.device != device:
+                raise RuntimeError(f'tensors on different devices: {device} and {t.device}')
+            t = t.float().contiguous()
+        parameters.append(t)
+    tensors = (input, residual, gate, *parameters)
+    args = (0 if gate is None else GATES[activation], float(eps), factor, return_sum or weight is None)
+    if N.wants_grad(*(t for t in tensors if t is not None)):
+        out, total = _ResidualNorm.apply(*tensors, *args)
+    else:
+        out, total = _residual_fwd(*tensors, *args, False)[:2]
+    if weight is None:
+        return total
+    return (out, total) if return_sum else out
+
+
+def _flat(x):
+    """``x`` as rows of neighbouring elements, a view where it can be one."""
+    if x is None:
+        return None
+    channels = x.shape[-1]
+    x = x.reshape(x.numel() // channels, channels)
+    return x if channels == 1 or x.stride(1) == 1 else x.contiguous()
+
+
+def _residual_call(input, residual, gate, weight, inner, scale, activation, eps, factor):
+    kind = N.ELEMENT_TYPES
+    return N.ResidualNorm(*input.shape, N.ptr(inner), N.ptr(weight), N.ptr(scale), kind[input.dtype],
+                          kind[(input if residual is None else residual).dtype], activation, eps, factor, input.stride(0),
+                          0 if residual is None else residual.stride(0), 0 if gate is None else gate.stride(0))
+
+
+def _residual_fwd(input, residual, gate, weight, inner, scale, activation, eps, factor, want_total, keep):
+    shape, device = input.shape, input.device
+    stream = (input if residual is None else residual).dtype
+    input, residual, gate = _flat(input), _flat(residual), _flat(gate)
+    out = None if weight is None else torch.empty(shape, dtype=input.dtype, device=device)
+    total = torch.empty(shape, dtype=stream, device=device) if want_total else None
+    stats = torch.empty((input.shape[0], 2), dtype=torch.float32, device=device) if keep else None
+    call = _residual_call(input, residual, gate, weight, inner, scale, activation, eps, factor)
+    with N.device_guard(device):
+        N.check(N.lib().slayer_residual_norm_fwd(N.ptr(out), N.ptr(total), N.ptr(stats), N.ptr(input), N.ptr(residual), N.ptr(gate), call,
+                                                 N.stream_handle()))
+    return out, total, input, residual, gate, stats
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, input, residual, gate, weight, inner, scale, activation, eps, factor, want_total):
+        ctx.shape, ctx.args = input.shape, (activation, eps, factor)
+        out, total, *saved = _residual_fwd(input, residual, gate, weight, inner, scale, activation, eps, factor, want_total, True)
+        ctx.save_for_backward(*saved, weight, inner, scale)
+        ctx.set_materialize_grads(False)
+        return out, total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out, grad_total):
+        if grad_out is None and grad_total is None:
+            return (None,) * 10
+        input, residual, gate, stats, weight, inner, scale = ctx.saved_tensors
+        device = input.device
+        grad_out, grad_total = _flat(grad_out), _flat(grad_total)
+        need = ctx.needs_input_grad
+        grads = [torch.empty(ctx.shape, dtype=t.dtype, device=device) if wanted else None
+                 for t, wanted in zip((input, residual, gate), need)]
+        sums = [torch.empty(t.shape, dtype=torch.float32, device=device) if wanted else None
+                for t, wanted in zip((weight, inner, scale), need[3:])]
+        call = _residual_call(input, residual, gate, weight, inner, scale, *ctx.args)
+        call.grad_out_stride = 0 if grad_out is None else grad_out.stride(0)
+        call.grad_total_stride = 0 if grad_total is None else grad_total.stride(0)
+        lib = N.lib()
+        with N.device_guard(device):
+            floats = lib.slayer_residual_norm_workspace(call) if any(need[3:]) else 0
+            if floats < 0:
+                N.check(int(floats))
+            workspace = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
+            N.check(lib.slayer_residual_norm_bwd(*(N.ptr(g) for g in grads), N.ptr(sums[1]), N.ptr(sums[0]), N.ptr(sums[2]),
+                                                 N.ptr(grad_out), N.ptr(grad_total), N.ptr(stats), N.ptr(input), N.ptr(residual),
+                                                 N.ptr(gate), call, N.ptr(workspace), floats, N.stream_handle()))
+        return (*grads, *sums, None, None, None, None)
+
+
+class ResidualNorm(torch.nn.Module):
+    """:func:`residual_norm` with trained weights: ``inner`` and ``outer`` say which of the two norms there are, ``scale`` is the residual
+    scale that every channel starts with (None: there is none), ``activation`` that of the gate, where ``forward`` is given one."""
+
+    def __init__(self, num_channels, inner=True, outer=True, scale=None, activation='sigmoid', eps=1e-5):
+        super().__init__()
+        if activation not in GATES:
+            raise ValueError(f'unknown activation {activation!r}: one of {list(GATES)}')
+        self.num_channels, self.activation, self.eps = num_channels, activation, eps
+        self.weight = torch.nn.Parameter(torch.ones(num_channels)) if outer else None
+        self.inner = torch.nn.Parameter(torch.ones(num_channels)) if inner else None
+        self.scale = None if scale is None else torch.nn.Parameter(torch.full((num_channels,), float(scale)))
+
+    def forward(self, input, residual=None, gate=None, return_sum=True):
+        return residual_norm(input, residual, self.weight, self.inner, gate, self.scale, self.activation, self.eps, return_sum)
+
+    def extra_repr(self):
+        return (f'{self.num_channels}, inner={self.inner is not None}, outer={self.weight is not None}, '
+                f'scale={self.scale is not None}, activation={self.activation}, eps={self.eps}')
