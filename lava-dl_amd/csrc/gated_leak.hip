@@ -62,31 +62,115 @@ __device__ __forceinline__ f4 decays_of(const LeakArgs& a, int c, int left) {
     return d;
 }
 
+// ---- tiles of a chain -----------------------------------------------------------------------------------------------------------
+// A chain is one strip of one sample, from tile to tile in the order of the pass.  Either a workgroup walks all tiles of a chain and
+// carries the state in LDS, or there is a workgroup for each tile, and states go through memory:
+//   Workgroups take their tiles by a ticket, the first tiles of all chains before the second ones, so a workgroup only ever waits for
+// workgroups with lower tickets, which are running or done and wait for lower ones themselves; the lowest waits for nobody, so every wait
+// ends.  Tiles form windows.  A tile leaves its pair, then reads those of the tiles before it in its window, and the state in front of
+// the window; the last tile of a window leaves the state behind it.  Which values are joined, and in which order, depends on the sizes alone
+// and not on who comes first, so that a call computed again has the same bits.
+//   What is left is a word of 64 bits that says itself that it is there (the workspace is zeroed before), read and written with relaxed
+// atomics of the whole device: no other memory hangs on it, so no fences are needed.
+typedef unsigned long long Word;
+constexpr int kWindow = 32;                    // largest window
+
+struct Chains {
+    unsigned* ticket;
+    Word *pairs, *states;                      // [tile][chain][strip], [window][chain][strip]
+    int chains, window;
+};
+
+__device__ __forceinline__ Word pair_word(float A, float H) {      // A is no NaN of the bits that would make the upper half 0
+    const unsigned a = A != A ? 0x7fc00000u : __float_as_uint(A);
+    return (Word)~a << 32 | __float_as_uint(H);
+}
+__device__ __forceinline__ Word state_word(float h) { return (Word)1 << 32 | __float_as_uint(h); }
+__device__ __forceinline__ void leave(Word* p, Word w) { __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ Word look(const Word* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+struct Pair { float a, h; };
+__device__ __forceinline__ Pair then(Pair first, Pair second) { return {first.a * second.a, fmaf(second.a, first.h, second.h)}; }
+
+// The state in front of tile `index` of `chain` (counted in the order of the pass), for the strip's 64 channels, into LDS: called by all
+// threads of the workgroup, which has left the tile's own pair before.  `initial` is the state in front of the first tile.
+template <int THREADS>
+__device__ __forceinline__ void state_before(float* to, Pair (*parts)[kStrip], const Chains& k, int64_t index, int chain, float initial) {
+    constexpr int kShares = THREADS / kStrip, kMost = kWindow / kShares;
+    const int channel = threadIdx.x % kStrip, share = threadIdx.x / kStrip;
+    const int64_t window = index / k.window, first = window * k.window;
+    const int count = (int)(index - first);                        // tiles before this one in its window, less than kWindow
+    const int per = (count + kShares - 1) / kShares, from = share * per, to_read = from + per < count ? per : count - from;
+    const Word* pairs = k.pairs + ((first + from) * k.chains + chain) * kStrip + channel;
+    Word words[kMost];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) words[i] = i < to_read ? 0 : pair_word(1.f, 0.f);
+    for (bool all = false; !all;) {
+        all = true;
+#pragma unroll
+        for (int i = 0; i < kMost; ++i)
+            if (!(words[i] >> 32)) words[i] = look(pairs + (int64_t)i * k.chains * kStrip);
+#pragma unroll
+        for (int i = 0; i < kMost; ++i) all = all && words[i] >> 32;
+        if (!all) __builtin_amdgcn_s_sleep(1);
+    }
+    Pair p = {1.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+        if (i < to_read) p = then(p, {__uint_as_float(~(unsigned)(words[i] >> 32)), __uint_as_float((unsigned)words[i])});
+    parts[share][channel] = p;
+    float h = initial;
+    if (share == 0 && window > 0) {
+        const Word* state = k.states + (window * k.chains + chain) * kStrip + channel;
+        Word w = look(state);
+        while (!(w >> 32)) {
+            __builtin_amdgcn_s_sleep(1);
+            w = look(state);
+        }
+        h = __uint_as_float((unsigned)w);
+    }
+    __syncthreads();
+    if (share == 0) {
+        for (int i = 1; i < kShares; ++i) p = then(p, parts[i][channel]);
+        to[channel] = count > 0 ? fmaf(p.a, h, p.h) : h;
+    }
+    __syncthreads();
+}
+
 // ---- forward --------------------------------------------------------------------------------------------------------------------
-// A workgroup takes one strip of one sample and walks its tiles.
-template <typename T, int DRIVE, int S, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a) {
+template <typename T, int DRIVE, int S, int WAVES, bool LOOK>
+__global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a, Chains k) {
     static_assert(4 * WAVES * S == kTile, "a tile is four lanes a wave");
     __shared__ f4 total[2][WAVES][2][16];                           // A, H of each wave and channel
     __shared__ f4 carry[2][16];
+    __shared__ Pair parts[WAVES][kStrip];
+    __shared__ unsigned ticket;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, lc = lane % 16, lt = lane / 16;
-    const int strip = blockIdx.x % a.strips;
-    const int64_t n = blockIdx.x / a.strips;
+    unsigned chain = blockIdx.x;
+    int64_t first = 0, end = a.tiles;
+    if (LOOK) {
+        if (threadIdx.x == 0) ticket = atomicAdd(k.ticket, 1u);
+        __syncthreads();
+        first = ticket / (unsigned)k.chains;
+        chain = ticket - (unsigned)first * k.chains;
+        end = first + 1;
+    }
+    const int strip = chain % (unsigned)a.strips;
+    const int64_t n = chain / (unsigned)a.strips;
     const int c = strip * kStrip + lc * 4, left = a.channels - c;
     const int64_t length = length_of(a, n);
     const f4 d = decays_of(a, c, left);
     const T* in = (const T*)a.in + n * a.in_stride[0] + c;
     const T* gate = (const T*)a.gate + n * a.gate_stride[0] + c;
     T* out = (T*)a.out + n * a.tokens * a.channels + c;
-    if (threadIdx.x < 16) {
-        f4 h = {};
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-            if (a.state && v < left) h[v] = a.state[n * a.channels + c + v];
-        carry[0][lc] = h;
+    float initial = 0;                                              // of channel threadIdx.x of the strip
+    if (threadIdx.x < kStrip) {
+        const int channel = strip * kStrip + threadIdx.x;
+        if (a.state && channel < a.channels) initial = a.state[n * a.channels + channel];
+        if (!LOOK) ((float*)carry[0])[threadIdx.x] = initial;
     }
-    for (int64_t tile = 0; tile < a.tiles; ++tile) {
-        const int turn = tile % 2;
+    for (int64_t tile = first; tile < end; ++tile) {
+        const int turn = LOOK ? 0 : tile % 2;
         const int64_t t0 = tile * kTile + (wave * 4 + lt) * S;
         float keep[S][4], add[S][4];
         typename Four<T>::Vec x[S], z[S];
@@ -135,6 +219,15 @@ __global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a) {
             total[turn][wave][1][lc] = H;
         }
         __syncthreads();
+        if (LOOK) {
+            if (k.window > 1 && threadIdx.x < kStrip && (tile + 1) % k.window != 0 && tile + 1 < a.tiles) {
+                Pair p = {1.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) p = then(p, {((float*)total[0][w][0])[threadIdx.x], ((float*)total[0][w][1])[threadIdx.x]});
+                leave(k.pairs + (tile * k.chains + chain) * kStrip + threadIdx.x, pair_word(p.a, p.h));
+            }
+            state_before<64 * WAVES>((float*)carry[0], parts, k, tile, chain, initial);
+        }
         // the state in front of the wave, and behind the tile
         f4 h = carry[turn][lc];
         if (a.starts && wave == 0 && lt == 0 && left > 0) store_four(a.starts + (n * a.tiles + tile) * a.channels + c, h, left);
@@ -149,8 +242,13 @@ __global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a) {
             }
         }
         if (wave == 0 && lt == 0) {
-            carry[turn ^ 1][lc] = h;
+            if (!LOOK) carry[turn ^ 1][lc] = h;
             if (a.last && tile == a.tiles - 1 && left > 0) store_four(a.last + n * a.channels + c, h, left);
+            if (LOOK && (tile + 1) % k.window == 0 && tile + 1 < a.tiles) {
+                Word* to = k.states + ((tile + 1) / k.window * k.chains + chain) * kStrip + lc * 4;
+#pragma unroll
+                for (int v = 0; v < 4; ++v) leave(to + v, state_word(h[v]));
+            }
         }
 #pragma unroll
         for (int v = 0; v < 4; ++v) h[v] = fmaf(before_a[v], mine[v], before_h[v]);
@@ -168,15 +266,29 @@ __global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a) {
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------
-// The same strip, its tiles from the last to the first.  Inside a tile the states go forwards, from the kept one, and G backwards.
-template <typename T, int DRIVE, int S, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a) {
+// The same chains, their tiles from the last to the first.  Inside a tile the states go forwards, from the kept one, and G backwards.
+template <typename T, int DRIVE, int S, int WAVES, bool LOOK>
+__global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a, Chains k) {
     static_assert(4 * WAVES * S == kTile, "a tile is four lanes a wave");
     __shared__ f4 total[2][WAVES][3][16];                           // A, H, G of each wave and channel
     __shared__ f4 carry[2][16];
+    __shared__ union {
+        Pair parts[WAVES][kStrip];
+        f4 sums[WAVES * 4][16];
+    } u;
+    __shared__ unsigned ticket;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, lc = lane % 16, lt = lane / 16;
-    const int strip = blockIdx.x % a.strips;
-    const int64_t n = blockIdx.x / a.strips;
+    unsigned chain = blockIdx.x;
+    int64_t first = 0, end = a.tiles;                               // counted from the last tile
+    if (LOOK) {
+        if (threadIdx.x == 0) ticket = atomicAdd(k.ticket, 1u);
+        __syncthreads();
+        first = ticket / (unsigned)k.chains;
+        chain = ticket - (unsigned)first * k.chains;
+        end = first + 1;
+    }
+    const int strip = chain % (unsigned)a.strips;
+    const int64_t n = chain / (unsigned)a.strips;
     const int c = strip * kStrip + lc * 4, left = a.channels - c;
     const int64_t length = length_of(a, n);
     const f4 d = decays_of(a, c, left);
@@ -186,36 +298,38 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a) {
     T* grad_in = (T*)a.grad_in + n * a.tokens * a.channels + c;
     T* grad_gate = (T*)a.grad_gate + n * a.tokens * a.channels + c;
     f4 slopes = {};                                                 // sum of dleak * open
-    if (threadIdx.x < 16) {
-        f4 g = {};
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-            if (a.grad_last && v < left) g[v] = a.grad_last[n * a.channels + c + v];
-        carry[0][lc] = g;
+    float initial = 0;                                              // of channel threadIdx.x of the strip
+    if (threadIdx.x < kStrip) {
+        const int channel = strip * kStrip + threadIdx.x;
+        if (a.grad_last && channel < a.channels) initial = a.grad_last[n * a.channels + channel];
+        if (!LOOK) ((float*)carry[0])[threadIdx.x] = initial;
     }
-    for (int64_t tile = a.tiles - 1; tile >= 0; --tile) {
-        const int turn = (a.tiles - 1 - tile) % 2;
+    for (int64_t index = first; index < end; ++index) {
+        const int64_t tile = a.tiles - 1 - index;
+        const int turn = LOOK ? 0 : index % 2;
         const int64_t t0 = tile * kTile + (wave * 4 + lt) * S;
-        typename Four<T>::Vec x[S], z[S], dy[S];
+        typename Four<T>::Vec x[S], dy[S];
+        float open[S][4];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            x[s] = z[s] = dy[s] = {};
-            if (t0 + s < length && left > 0) {
+            typename Four<T>::Vec z = {};
+            x[s] = dy[s] = {};
+            const bool on = t0 + s < length;
+            if (on && left > 0) {
                 x[s] = load_four(in + (t0 + s) * a.in_stride[1], left);
-                z[s] = load_four(gate + (t0 + s) * a.gate_stride[1], left);
+                z = load_four(gate + (t0 + s) * a.gate_stride[1], left);
                 dy[s] = load_four(grad + (t0 + s) * a.grad_stride[1], left);
             }
+#pragma unroll
+            for (int v = 0; v < 4; ++v) open[s][v] = on ? open_gate<T>((float)z[v]) : 0.f;   // what is not there leaks nothing, x and dy are 0
         }
         f4 start = {};
         if (left > 0) start = load_four(a.starts + (n * a.tiles + tile) * a.channels + c, left);
-        float open[S][4], before[S][4];
         f4 A = {1.f, 1.f, 1.f, 1.f}, H = {}, G = {};
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const bool on = t0 + s < length;
-                open[s][v] = on ? open_gate<T>((float)z[s][v]) : 0.f;      // what is not there leaks nothing, and x and dy are 0
                 const float leak = d[v] * open[s][v], keep = 1.f - leak;
                 A[v] *= keep;
                 H[v] = fmaf(keep, H[v], drive_of<DRIVE>(leak, keep).value * (float)x[s][v]);
@@ -257,6 +371,16 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a) {
         }
         if (lt == 0) total[turn][wave][2][lc] = G;
         __syncthreads();
+        if (LOOK) {
+            if (k.window > 1 && threadIdx.x < kStrip && (index + 1) % k.window != 0 && index + 1 < a.tiles) {
+                Pair p = {1.f, 0.f};
+#pragma unroll
+                for (int w = WAVES - 1; w >= 0; --w)
+                    p = then(p, {((float*)total[0][w][0])[threadIdx.x], ((float*)total[0][w][2])[threadIdx.x]});
+                leave(k.pairs + (index * k.chains + chain) * kStrip + threadIdx.x, pair_word(p.a, p.h));
+            }
+            state_before<64 * WAVES>((float*)carry[0], u.parts, k, index, chain, initial);
+        }
         f4 h = start, g = carry[turn][lc], mine = g;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
@@ -274,22 +398,26 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a) {
             }
         }
         if (wave == 0 && lt == 0) {
-            carry[turn ^ 1][lc] = g;
+            if (!LOOK) carry[turn ^ 1][lc] = g;
             if (a.grad_state && tile == 0 && left > 0) store_four(a.grad_state + n * a.channels + c, g, left);
+            if (LOOK && (index + 1) % k.window == 0 && index + 1 < a.tiles) {
+                Word* to = k.states + ((index + 1) / k.window * k.chains + chain) * kStrip + lc * 4;
+#pragma unroll
+                for (int v = 0; v < 4; ++v) leave(to + v, state_word(g[v]));
+            }
         }
+        float before[S][4];
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
             h[v] = fmaf(before_a[v], h[v], before_h[v]);
             g[v] = fmaf(behind_a[v], mine[v], behind_g[v]);
-        }
 #pragma unroll
-        for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
+            for (int s = 0; s < S; ++s) {
                 before[s][v] = h[v];
                 const float leak = d[v] * open[s][v], keep = 1.f - leak;
                 h[v] = fmaf(keep, h[v], drive_of<DRIVE>(leak, keep).value * (float)x[s][v]);
             }
+        }
 #pragma unroll
         for (int s = S - 1; s >= 0; --s) {
             const bool on = t0 + s < length;
@@ -313,20 +441,25 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a) {
         }
     }
     if (!a.parts) return;
-    __shared__ f4 sums[WAVES * 4][16];
-    sums[wave * 4 + lt][lc] = slopes;
+    // the decays' gradient of this workgroup's tiles: a row of `parts` for each workgroup of a strip, or one number a workgroup
+    __syncthreads();                                                // (the pairs' part of the union has been read)
+    u.sums[wave * 4 + lt][lc] = slopes;
     __syncthreads();
-    if (threadIdx.x >= 64) return;
-    const int i = threadIdx.x;
+    if (threadIdx.x >= kStrip) return;
     float sum = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES * 4; ++w) sum += sums[w][i / 4][i % 4];
+    for (int w = 0; w < WAVES * 4; ++w) sum += ((float*)u.sums[w])[threadIdx.x];
+    const int channel = strip * kStrip + threadIdx.x;
     if (a.decays > 1) {
-        if (strip * kStrip + i < a.channels) a.parts[n * a.channels + strip * kStrip + i] = sum;
+        if (channel < a.channels) a.parts[(first * a.samples + n) * a.channels + channel] = sum;
     } else {
         sum = sum_lanes(sum, 64);                                   // (channels that are not there have 0)
-        if (i == 0) a.parts[blockIdx.x] = sum;
+        if (threadIdx.x == 0) a.parts[first * k.chains + chain] = sum;
     }
+}
+
+__global__ __launch_bounds__(256) void zero_words_kernel(Word* words, int64_t count) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) words[i] = 0;
 }
 
 // ---- one token a sample ---------------------------------------------------------------------------------------------------------
@@ -381,6 +514,37 @@ LeakArgs args_of(const slayer_gated_leak* s) {
     return a;
 }
 
+// How the tiles are cut up among workgroups, and the workspace of that: the words, the ticket, the rows of the decays' gradient.
+struct Plan {
+    bool look;
+    int64_t chains, blocks, window, words, rows;        // rows: of partial sums of the decays' gradient
+};
+Plan plan_of(const slayer_gated_leak* s) {
+    Plan p = {};
+    const int64_t tiles = tiles_of(s->tokens);
+    p.chains = s->samples * strips_of(s->channels);
+    p.look = tiles > 2 && p.chains < 2048 && tiles * p.chains < (1 << 23);
+    p.blocks = p.look ? tiles * p.chains : p.chains;
+    p.window = p.look ? 2048 / p.chains : 1;
+    if (p.window > kWindow) p.window = kWindow;
+    if (p.window > tiles) p.window = tiles;
+    if (p.look) p.words = ((p.window > 1 ? tiles : 0) + (tiles + p.window - 1) / p.window) * p.chains * kStrip + 1;
+    p.rows = (p.look ? tiles : 1) * (s->num_decays == 1 ? p.chains : s->samples);
+    return p;
+}
+// The zeroed words at the front of the workspace.
+int chains_of(Chains* k, const Plan& p, const slayer_gated_leak* s, float* workspace, hipStream_t stream) {
+    if (!p.look) return 0;
+    k->chains = (int)p.chains;
+    k->window = (int)p.window;
+    k->ticket = (unsigned*)workspace;
+    k->pairs = (Word*)workspace + 1;
+    k->states = k->pairs + (p.window > 1 ? tiles_of(s->tokens) : 0) * p.chains * kStrip;
+    const int64_t blocks = (p.words + 1023) / 1024;
+    hipLaunchKernelGGL(zero_words_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, stream, (Word*)workspace, p.words);
+    return (int)hipGetLastError();
+}
+
 #define BY_DRIVE(T, LAUNCH)                                 \
     switch (s->drive) {                                     \
         case DRIVE_NONE: LAUNCH(T, DRIVE_NONE); break;      \
@@ -403,7 +567,8 @@ extern "C" int64_t slayer_gated_leak_starts(const slayer_gated_leak* s) {
 
 extern "C" int64_t slayer_gated_leak_workspace(const slayer_gated_leak* s, int backward) {
     if (int e = check_leak(s)) return e;
-    return backward ? s->samples * (s->num_decays == 1 ? strips_of(s->channels) : s->channels) : 0;
+    const Plan p = plan_of(s);
+    return 2 * p.words + (backward ? p.rows * s->num_decays : 0);
 }
 
 extern "C" int slayer_gated_leak_fwd(void* out, float* last, float* starts, const void* input, const void* gate, const float* state,
@@ -411,12 +576,21 @@ extern "C" int slayer_gated_leak_fwd(void* out, float* last, float* starts, cons
     if (int e = check_leak(s)) return e;
     if (s->samples == 0) return 0;
     if (s->tokens > 0 && (!out || !input || !gate)) return SLAYER_ENULL;
+    const Plan p = plan_of(s);
+    if (p.words > 0 && !workspace) return SLAYER_ENULL;
+    if (floats < 2 * p.words || (uintptr_t)workspace % 8 != 0) return SLAYER_EINVAL;
     LeakArgs a = args_of(s);
     a.out = out; a.last = last; a.starts = starts; a.in = input; a.gate = gate; a.state = state;
-#define LAUNCH(T, DRIVE) \
-    hipLaunchKernelGGL((leak_fwd_kernel<T, DRIVE, 8, 4>), dim3((unsigned)(a.samples * a.strips)), dim3(256), 0, (hipStream_t)stream, a)
+    Chains k = {};
+    if (int e = chains_of(&k, p, s, workspace, (hipStream_t)stream)) return e;
+#define ONE(T, DRIVE, LOOK) \
+    hipLaunchKernelGGL((leak_fwd_kernel<T, DRIVE, 8, 4, LOOK>), dim3((unsigned)p.blocks), dim3(256), 0, (hipStream_t)stream, a, k)
+#define LAUNCH(T, DRIVE)                    \
+    if (p.look) ONE(T, DRIVE, true);        \
+    else ONE(T, DRIVE, false)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
+#undef ONE
     return (int)hipGetLastError();
 }
 
@@ -426,23 +600,30 @@ extern "C" int slayer_gated_leak_bwd(void* grad_input, void* grad_gate, float* g
     if (int e = check_leak(s)) return e;
     if (s->samples == 0) return grad_decay ? launch_zero_fill(grad_decay, s->num_decays, (hipStream_t)stream) : 0;
     if (!starts || (s->tokens > 0 && (!grad_input || !grad_gate || !grad_out || !input || !gate))) return SLAYER_ENULL;
-    const int64_t need = grad_decay ? slayer_gated_leak_workspace(s, 1) : 0;
+    const Plan p = plan_of(s);
+    const int64_t need = 2 * p.words + (grad_decay ? p.rows * s->num_decays : 0);
     if (need > 0 && !workspace) return SLAYER_ENULL;
-    if (floats < need) return SLAYER_EINVAL;
+    if (floats < need || (uintptr_t)workspace % 8 != 0) return SLAYER_EINVAL;
     LeakArgs a = args_of(s);
     a.grad_in = grad_input; a.grad_gate = grad_gate; a.grad_state = grad_state; a.grad = grad_out; a.grad_last = grad_last;
     a.in = input; a.gate = gate; a.starts = (float*)starts;
-    a.parts = grad_decay ? workspace : nullptr;
-#define LAUNCH(T, DRIVE) \
-    hipLaunchKernelGGL((leak_bwd_kernel<T, DRIVE, 4, 8>), dim3((unsigned)(a.samples * a.strips)), dim3(512), 0, (hipStream_t)stream, a)
+    a.parts = grad_decay ? workspace + 2 * p.words : nullptr;
+    Chains k = {};
+    if (int e = chains_of(&k, p, s, workspace, (hipStream_t)stream)) return e;
+#define ONE(T, DRIVE, LOOK) \
+    hipLaunchKernelGGL((leak_bwd_kernel<T, DRIVE, 4, 8, LOOK>), dim3((unsigned)p.blocks), dim3(512), 0, (hipStream_t)stream, a, k)
+#define LAUNCH(T, DRIVE)                    \
+    if (p.look) ONE(T, DRIVE, true);        \
+    else ONE(T, DRIVE, false)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
+#undef ONE
     if (int e = (int)hipGetLastError()) return e;
     if (!grad_decay) return 0;
     ColumnSums sums = {};
-    sums.out[0] = grad_decay; sums.parts[0] = workspace; sums.factor = 1.f / 4096.f;
+    sums.out[0] = grad_decay; sums.parts[0] = a.parts; sums.factor = 1.f / 4096.f;
     sums.columns = sums.pitch = s->num_decays;
-    sums.rows = need / s->num_decays;
+    sums.rows = p.rows;
     return launch_column_sums(sums, 1, (hipStream_t)stream);
 }
 
