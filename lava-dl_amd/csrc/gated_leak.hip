@@ -18,22 +18,22 @@ namespace {
 
 enum { DRIVE_NONE, DRIVE_GAIN, DRIVE_VARIANCE };
 
-constexpr int kStrip = 64;                     // channels of a workgroup: sixteen lanes, four each
-constexpr int kTile = 128;                     // tokens that it holds at a time
+constexpr int kKept = 64;                      // tokens from one state that is kept for the backward pass to the next
 
 struct LeakArgs {
     void *out, *grad_in, *grad_gate;
     const void *in, *gate, *grad, *lengths;
     const float *decay, *state, *grad_last;
     float *last, *starts, *grad_state, *parts;
-    int64_t samples, tokens, tiles;
+    int64_t samples, tokens, tiles, kept;
     int64_t in_stride[2], gate_stride[2], grad_stride[2];
     int channels, strips, lengths_bytes, decays;
 };
 
-// A gate of +infinity is open, as one of 100 is (the precise form of logistic would make it NaN).
-template <typename T> __device__ __forceinline__ float open_gate(float z) {
-    return logistic<T>(sizeof(T) == 4 && z > 100.f ? 100.f : z);
+// sigmoid from the hardware's exponential and reciprocal, a unit in the last place each, for either type: (3 + 1.5 |z|) 2^-24, which is most
+// where the gate is as good as closed and the leak next to nothing.  Infinite gates are open and closed.
+__device__ __forceinline__ float open_gate(float z) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
 }
 
 // drive and its derivative from the leak and what it keeps, 1 - leak.  sqrt(leak (2 - leak)) counts as 0 with derivative 0 where its square
@@ -48,18 +48,36 @@ template <int DRIVE> __device__ __forceinline__ Drive drive_of(float leak, float
     return {square * r, keep * r};
 }
 
+// What a lane reads and writes of a row: one float32 or bfloat16, or two bfloat16 at any address that suits one of them.
+template <typename T, int V> struct Piece;
+template <> struct Piece<float, 1> { typedef float Raw; };
+template <> struct Piece<bf16, 1> { typedef unsigned short Raw; };
+template <> struct Piece<bf16, 2> { typedef unsigned Raw; };
+typedef unsigned unsigned_any __attribute__((aligned(2)));
+__device__ __forceinline__ float load_piece(const float* p) { return *p; }
+template <int V> __device__ __forceinline__ typename Piece<bf16, V>::Raw load_piece(const bf16* p) {
+    if constexpr (V == 1) return *reinterpret_cast<const unsigned short*>(p);
+    else return *reinterpret_cast<const unsigned_any*>(p);
+}
+template <int V> __device__ __forceinline__ float load_piece(const float* p) { return *p; }
+__device__ __forceinline__ float value_of(float raw, int) { return raw; }
+__device__ __forceinline__ float value_of(unsigned short raw, int) { return __uint_as_float((unsigned)raw << 16); }
+__device__ __forceinline__ float value_of(unsigned raw, int v) { return __uint_as_float(v ? raw & 0xffff0000u : raw << 16); }
+__device__ __forceinline__ void store_piece(float* p, const float (&x)[1]) { *p = x[0]; }
+__device__ __forceinline__ void store_piece(bf16* p, const float (&x)[1]) { *p = (bf16)x[0]; }
+typedef bf16 b2 __attribute__((ext_vector_type(2)));
+typedef b2 b2_any __attribute__((aligned(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void store_piece(bf16* p, const float (&x)[2]) {
+    *reinterpret_cast<b2_any*>(p) = __builtin_convertvector(f2{x[0], x[1]}, b2);
+}
+// Keeps the compiler from holding on to what it has made of x: that is made again instead of taking up registers.
+__device__ __forceinline__ void forget(float& x) { asm volatile("" : "+v"(x)); }
+
 __device__ __forceinline__ int64_t length_of(const LeakArgs& a, int64_t n) {
     if (!a.lengths) return a.tokens;
     const int64_t length = a.lengths_bytes == 4 ? ((const int*)a.lengths)[n] : ((const int64_t*)a.lengths)[n];
     return length < 0 ? 0 : length < a.tokens ? length : a.tokens;
-}
-
-__device__ __forceinline__ f4 decays_of(const LeakArgs& a, int c, int left) {
-    f4 d = {};
-#pragma unroll
-    for (int v = 0; v < 4; ++v)
-        if (v < left) d[v] = a.decay[a.decays == 1 ? 0 : c + v] * (1.f / 4096.f);
-    return d;
 }
 
 // ---- tiles of a chain -----------------------------------------------------------------------------------------------------------
@@ -92,370 +110,334 @@ __device__ __forceinline__ Word look(const Word* p) { return __hip_atomic_load(p
 struct Pair { float a, h; };
 __device__ __forceinline__ Pair then(Pair first, Pair second) { return {first.a * second.a, fmaf(second.a, first.h, second.h)}; }
 
-// The state in front of tile `index` of `chain` (counted in the order of the pass), for the strip's 64 channels, into LDS: called by all
-// threads of the workgroup, which has left the tile's own pair before.  `initial` is the state in front of the first tile.
-template <int THREADS>
-__device__ __forceinline__ void state_before(float* to, Pair (*parts)[kStrip], const Chains& k, int64_t index, int chain, float initial) {
-    constexpr int kShares = THREADS / kStrip, kMost = kWindow / kShares;
-    const int channel = threadIdx.x % kStrip, share = threadIdx.x / kStrip;
+// The pair of all tiles before tile `index` (counted in the order of the pass) in its window, and the state in front of the window
+// (`initial` in front of the first one), for channel threadIdx.x % CH: for the first CH threads.  All threads of the workgroup call it.
+struct Before { Pair pair; float state; };
+template <int THREADS, int CH>
+__device__ __forceinline__ Before look_back(Pair (*parts)[CH], const Chains& k, int64_t index, unsigned chain, float initial) {
+    constexpr int kShares = THREADS / CH, kMost = kWindow / kShares;
+    const int channel = threadIdx.x % CH, share = threadIdx.x / CH;
     const int64_t window = index / k.window, first = window * k.window;
-    const int count = (int)(index - first);                        // tiles before this one in its window, less than kWindow
-    const int per = (count + kShares - 1) / kShares, from = share * per, to_read = from + per < count ? per : count - from;
-    const Word* pairs = k.pairs + ((first + from) * k.chains + chain) * kStrip + channel;
-    Word words[kMost];
+    const int count = (int)(index - first);                        // less than kWindow
+    const int per = (count + kShares - 1) / kShares, from = share * per, mine = count - from < per ? count - from : per;
+    Before b = {{1.f, 0.f}, initial};
+    if (count > 0) {
+        const Word* pairs = k.pairs + ((first + from) * k.chains + chain) * CH + channel;
+        Word words[kMost];
 #pragma unroll
-    for (int i = 0; i < kMost; ++i) words[i] = i < to_read ? 0 : pair_word(1.f, 0.f);
-    for (bool all = false; !all;) {
-        all = true;
+        for (int i = 0; i < kMost; ++i) words[i] = i < mine ? 0 : pair_word(1.f, 0.f);
+        for (bool all = false; !all;) {
+            all = true;
+#pragma unroll
+            for (int i = 0; i < kMost; ++i)
+                if (!(words[i] >> 32)) words[i] = look(pairs + (int64_t)i * k.chains * CH);
+#pragma unroll
+            for (int i = 0; i < kMost; ++i) all = all && words[i] >> 32;
+            if (!all) __builtin_amdgcn_s_sleep(1);
+        }
 #pragma unroll
         for (int i = 0; i < kMost; ++i)
-            if (!(words[i] >> 32)) words[i] = look(pairs + (int64_t)i * k.chains * kStrip);
-#pragma unroll
-        for (int i = 0; i < kMost; ++i) all = all && words[i] >> 32;
-        if (!all) __builtin_amdgcn_s_sleep(1);
+            if (i < mine) b.pair = then(b.pair, {__uint_as_float(~(unsigned)(words[i] >> 32)), __uint_as_float((unsigned)words[i])});
+        parts[share][channel] = b.pair;
+        __syncthreads();
     }
-    Pair p = {1.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < kMost; ++i)
-        if (i < to_read) p = then(p, {__uint_as_float(~(unsigned)(words[i] >> 32)), __uint_as_float((unsigned)words[i])});
-    parts[share][channel] = p;
-    float h = initial;
-    if (share == 0 && window > 0) {
-        const Word* state = k.states + (window * k.chains + chain) * kStrip + channel;
+    if (share > 0) return b;
+    for (int i = 1; i < kShares && count > 0; ++i) b.pair = then(b.pair, parts[i][channel]);
+    if (window > 0) {
+        const Word* state = k.states + (window * k.chains + chain) * CH + channel;
         Word w = look(state);
         while (!(w >> 32)) {
             __builtin_amdgcn_s_sleep(1);
             w = look(state);
         }
-        h = __uint_as_float((unsigned)w);
+        b.state = __uint_as_float((unsigned)w);
     }
+    return b;
+}
+
+// Which chain a workgroup is in, and which of its tiles it takes.
+struct Span { unsigned chain; int64_t first, end; };
+template <bool LOOK> __device__ __forceinline__ Span span_of(const LeakArgs& a, const Chains& k) {
+    if (!LOOK) return {blockIdx.x, 0, a.tiles};
+    __shared__ unsigned ticket;
+    if (threadIdx.x == 0) ticket = atomicAdd(k.ticket, 1u);
     __syncthreads();
-    if (share == 0) {
-        for (int i = 1; i < kShares; ++i) p = then(p, parts[i][channel]);
-        to[channel] = count > 0 ? fmaf(p.a, h, p.h) : h;
-    }
-    __syncthreads();
+    const unsigned mine = __builtin_amdgcn_readfirstlane(ticket), first = mine / (unsigned)k.chains;
+    return {mine - first * k.chains, first, first + 1};
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
-template <typename T, int DRIVE, int S, int WAVES, bool LOOK>
+// S tokens a wave, V channels a lane.
+template <typename T, int V, int DRIVE, int S, int WAVES, bool LOOK>
 __global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a, Chains k) {
-    static_assert(4 * WAVES * S == kTile, "a tile is four lanes a wave");
-    __shared__ f4 total[2][WAVES][2][16];                           // A, H of each wave and channel
-    __shared__ f4 carry[2][16];
-    __shared__ Pair parts[WAVES][kStrip];
-    __shared__ unsigned ticket;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, lc = lane % 16, lt = lane / 16;
-    unsigned chain = blockIdx.x;
-    int64_t first = 0, end = a.tiles;
-    if (LOOK) {
-        if (threadIdx.x == 0) ticket = atomicAdd(k.ticket, 1u);
-        __syncthreads();
-        first = ticket / (unsigned)k.chains;
-        chain = ticket - (unsigned)first * k.chains;
-        end = first + 1;
-    }
-    const int strip = chain % (unsigned)a.strips;
-    const int64_t n = chain / (unsigned)a.strips;
-    const int c = strip * kStrip + lc * 4, left = a.channels - c;
-    const int64_t length = length_of(a, n);
-    const f4 d = decays_of(a, c, left);
-    const T* in = (const T*)a.in + n * a.in_stride[0] + c;
-    const T* gate = (const T*)a.gate + n * a.gate_stride[0] + c;
-    T* out = (T*)a.out + n * a.tokens * a.channels + c;
-    float initial = 0;                                              // of channel threadIdx.x of the strip
-    if (threadIdx.x < kStrip) {
-        const int channel = strip * kStrip + threadIdx.x;
-        if (a.state && channel < a.channels) initial = a.state[n * a.channels + channel];
-        if (!LOOK) ((float*)carry[0])[threadIdx.x] = initial;
-    }
-    for (int64_t tile = first; tile < end; ++tile) {
-        const int turn = LOOK ? 0 : tile % 2;
-        const int64_t t0 = tile * kTile + (wave * 4 + lt) * S;
-        float keep[S][4], add[S][4];
-        typename Four<T>::Vec x[S], z[S];
+    constexpr int CH = 64 * V, kTile = S * WAVES;
+    static_assert(kKept % S == 0 && kTile % kKept == 0, "a wave begins where a state is kept");
+    __shared__ Pair total[WAVES][CH];
+    __shared__ float front[WAVES][CH];                              // the state in front of each wave
+    __shared__ Pair parts[LOOK ? 64 * WAVES / CH : 1][CH];
+    const Span span = span_of<LOOK>(a, k);
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int strip = span.chain % (unsigned)a.strips;
+    const int64_t n = span.chain / (unsigned)a.strips, length = length_of(a, n);
+    const int c = strip * CH + lane * V, from = c < a.channels ? c : a.channels - V;       // lanes without channels read the last ones
+    float d[V];
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const bool on = t0 + s < length;
-            x[s] = z[s] = {};
-            if (on && left > 0) {
-                x[s] = load_four(in + (t0 + s) * a.in_stride[1], left);
-                z[s] = load_four(gate + (t0 + s) * a.gate_stride[1], left);
+    for (int v = 0; v < V; ++v) d[v] = a.decay[a.decays == 1 ? 0 : from + v] * (1.f / 4096.f);
+    const T* in = (const T*)a.in + n * a.in_stride[0];
+    const T* gate = (const T*)a.gate + n * a.gate_stride[0];
+    T* out = (T*)a.out + n * a.tokens * a.channels;
+    const int channel = strip * CH + threadIdx.x;                  // of the first CH threads
+    const bool keeps = threadIdx.x < CH && channel < a.channels;
+    float carry = keeps && a.state ? a.state[n * a.channels + channel] : 0.f;
+    for (int64_t tile = span.first; tile < span.end; ++tile) {
+        const int64_t t0 = tile * kTile + wave * S;
+        const int count = length - t0 < S ? (length > t0 ? (int)(length - t0) : 0) : S;
+        float keep[S][V], add[S][V];
+        Pair p[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) p[v] = {1.f, 0.f};
+        if (count > 0) {
+            typename Piece<T, V>::Raw x[S], z[S];
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const int64_t t = t0 + (s < count ? s : count - 1);
+                x[s] = load_piece<V>(in + t * a.in_stride[1] + from);
+                z[s] = load_piece<V>(gate + t * a.gate_stride[1] + from);
             }
-        }
-        f4 A = {1.f, 1.f, 1.f, 1.f}, H = {};
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const bool on = t0 + s < length;
+            for (int s = 0; s < S; ++s)
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const float leak = d[v] * open_gate<T>((float)z[s][v]);
-                keep[s][v] = on ? 1.f - leak : 1.f;
-                add[s][v] = on ? drive_of<DRIVE>(leak, keep[s][v]).value * (float)x[s][v] : 0.f;
-                A[v] *= keep[s][v];
-                H[v] = fmaf(keep[s][v], H[v], add[s][v]);
-            }
-        }
-        // the pairs of the lanes in front of this one, and of the wave
-        f4 before_a = {1.f, 1.f, 1.f, 1.f}, before_h = {};
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-#pragma unroll
-            for (int by = 16; by < 64; by *= 2) {
-                const float oa = __shfl_up(A[v], by), oh = __shfl_up(H[v], by);
-                if (lane >= by) {
-                    H[v] = fmaf(A[v], oh, H[v]);
-                    A[v] *= oa;
+                for (int v = 0; v < V; ++v) {
+                    const float leak = d[v] * open_gate(value_of(z[s], v));
+                    keep[s][v] = 1.f - leak;
+                    add[s][v] = drive_of<DRIVE>(leak, keep[s][v]).value * value_of(x[s], v);
                 }
+            if (count < S) {
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+#pragma unroll
+                    for (int v = 0; v < V; ++v)
+                        if (s >= count) {
+                            keep[s][v] = 1.f;
+                            add[s][v] = 0.f;
+                        }
             }
-            const float oa = __shfl_up(A[v], 16), oh = __shfl_up(H[v], 16);
-            if (lane >= 16) {
-                before_a[v] = oa;
-                before_h[v] = oh;
-            }
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int v = 0; v < V; ++v) p[v] = then(p[v], {keep[s][v], add[s][v]});
         }
-        if (lt == 3) {
-            total[turn][wave][0][lc] = A;
-            total[turn][wave][1][lc] = H;
-        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) total[wave][lane * V + v] = p[v];
         __syncthreads();
         if (LOOK) {
-            if (k.window > 1 && threadIdx.x < kStrip && (tile + 1) % k.window != 0 && tile + 1 < a.tiles) {
-                Pair p = {1.f, 0.f};
+            if (k.window > 1 && threadIdx.x < CH && (tile + 1) % k.window != 0 && tile + 1 < a.tiles) {
+                Pair all = {1.f, 0.f};
 #pragma unroll
-                for (int w = 0; w < WAVES; ++w) p = then(p, {((float*)total[0][w][0])[threadIdx.x], ((float*)total[0][w][1])[threadIdx.x]});
-                leave(k.pairs + (tile * k.chains + chain) * kStrip + threadIdx.x, pair_word(p.a, p.h));
+                for (int w = 0; w < WAVES; ++w) all = then(all, total[w][threadIdx.x]);
+                leave(k.pairs + (tile * k.chains + span.chain) * CH + threadIdx.x, pair_word(all.a, all.h));
             }
-            state_before<64 * WAVES>((float*)carry[0], parts, k, tile, chain, initial);
+            const Before b = look_back<64 * WAVES, CH>(parts, k, tile, span.chain, carry);
+            carry = tile % k.window == 0 ? b.state : fmaf(b.pair.a, b.state, b.pair.h);
         }
-        // the state in front of the wave, and behind the tile
-        f4 h = carry[turn][lc];
-        if (a.starts && wave == 0 && lt == 0 && left > 0) store_four(a.starts + (n * a.tiles + tile) * a.channels + c, h, left);
-        f4 mine = h;
+        if (threadIdx.x < CH) {
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            const f4 wa = total[turn][w][0][lc], wh = total[turn][w][1][lc];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                if (w == wave) mine[v] = h[v];
-                h[v] = fmaf(wa[v], h[v], wh[v]);
+            for (int w = 0; w < WAVES; ++w) {
+                front[w][threadIdx.x] = carry;
+                const int64_t start = tile * (kTile / kKept) + w * S / kKept;
+                if (w * S % kKept == 0 && a.starts && keeps && start < a.kept) a.starts[(n * a.kept + start) * a.channels + channel] = carry;
+                carry = fmaf(total[w][threadIdx.x].a, carry, total[w][threadIdx.x].h);
             }
+            if (a.last && keeps && tile == a.tiles - 1) a.last[n * a.channels + channel] = carry;
+            if (LOOK && (tile + 1) % k.window == 0 && tile + 1 < a.tiles)
+                leave(k.states + ((tile + 1) / k.window * k.chains + span.chain) * CH + threadIdx.x, state_word(carry));
         }
-        if (wave == 0 && lt == 0) {
-            if (!LOOK) carry[turn ^ 1][lc] = h;
-            if (a.last && tile == a.tiles - 1 && left > 0) store_four(a.last + n * a.channels + c, h, left);
-            if (LOOK && (tile + 1) % k.window == 0 && tile + 1 < a.tiles) {
-                Word* to = k.states + ((tile + 1) / k.window * k.chains + chain) * kStrip + lc * 4;
+        __syncthreads();
+        if (c >= a.channels) continue;
+        float h[V];
 #pragma unroll
-                for (int v = 0; v < 4; ++v) leave(to + v, state_word(h[v]));
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < 4; ++v) h[v] = fmaf(before_a[v], mine[v], before_h[v]);
+        for (int v = 0; v < V; ++v) h[v] = front[wave][lane * V + v];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            f4 y;
+            if (s < count) {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                h[v] = fmaf(keep[s][v], h[v], add[s][v]);
-                y[v] = t0 + s < length ? h[v] : 0.f;
+                for (int v = 0; v < V; ++v) h[v] = fmaf(keep[s][v], h[v], add[s][v]);
+                store_piece(out + (t0 + s) * a.channels + c, h);
+            } else if (t0 + s < a.tokens) {
+                const float none[V] = {};
+                store_piece(out + (t0 + s) * a.channels + c, none);
             }
-            if (t0 + s < a.tokens && left > 0) store_four(out + (t0 + s) * a.channels, y, left);
         }
     }
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------
 // The same chains, their tiles from the last to the first.  Inside a tile the states go forwards, from the kept one, and G backwards.
-template <typename T, int DRIVE, int S, int WAVES, bool LOOK>
+template <typename T, int V, int DRIVE, int S, int WAVES, bool LOOK>
 __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a, Chains k) {
-    static_assert(4 * WAVES * S == kTile, "a tile is four lanes a wave");
-    __shared__ f4 total[2][WAVES][3][16];                           // A, H, G of each wave and channel
-    __shared__ f4 carry[2][16];
-    __shared__ union {
-        Pair parts[WAVES][kStrip];
-        f4 sums[WAVES * 4][16];
-    } u;
-    __shared__ unsigned ticket;
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, lc = lane % 16, lt = lane / 16;
-    unsigned chain = blockIdx.x;
-    int64_t first = 0, end = a.tiles;                               // counted from the last tile
-    if (LOOK) {
-        if (threadIdx.x == 0) ticket = atomicAdd(k.ticket, 1u);
-        __syncthreads();
-        first = ticket / (unsigned)k.chains;
-        chain = ticket - (unsigned)first * k.chains;
-        end = first + 1;
-    }
-    const int strip = chain % (unsigned)a.strips;
-    const int64_t n = chain / (unsigned)a.strips;
-    const int c = strip * kStrip + lc * 4, left = a.channels - c;
-    const int64_t length = length_of(a, n);
-    const f4 d = decays_of(a, c, left);
-    const T* in = (const T*)a.in + n * a.in_stride[0] + c;
-    const T* gate = (const T*)a.gate + n * a.gate_stride[0] + c;
-    const T* grad = (const T*)a.grad + n * a.grad_stride[0] + c;
-    T* grad_in = (T*)a.grad_in + n * a.tokens * a.channels + c;
-    T* grad_gate = (T*)a.grad_gate + n * a.tokens * a.channels + c;
-    f4 slopes = {};                                                 // sum of dleak * open
-    float initial = 0;                                              // of channel threadIdx.x of the strip
-    if (threadIdx.x < kStrip) {
-        const int channel = strip * kStrip + threadIdx.x;
-        if (a.grad_last && channel < a.channels) initial = a.grad_last[n * a.channels + channel];
-        if (!LOOK) ((float*)carry[0])[threadIdx.x] = initial;
-    }
-    for (int64_t index = first; index < end; ++index) {
-        const int64_t tile = a.tiles - 1 - index;
-        const int turn = LOOK ? 0 : index % 2;
-        const int64_t t0 = tile * kTile + (wave * 4 + lt) * S;
-        typename Four<T>::Vec x[S], dy[S];
-        float open[S][4];
+    constexpr int CH = 64 * V, kTile = S * WAVES;
+    static_assert(kTile % kKept == 0, "a tile begins where a state is kept");
+    __shared__ Pair total[WAVES][CH];
+    __shared__ float total_g[WAVES][CH];
+    __shared__ float front[WAVES][CH], behind[WAVES][CH];           // the state in front of each wave, G behind it
+    __shared__ Pair parts[LOOK ? 64 * WAVES / CH : 1][CH];
+    const Span span = span_of<LOOK>(a, k);
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int strip = span.chain % (unsigned)a.strips;
+    const int64_t n = span.chain / (unsigned)a.strips, length = length_of(a, n);
+    const int c = strip * CH + lane * V, from = c < a.channels ? c : a.channels - V;       // lanes without channels read the last ones
+    float d[V], slopes[V];                                          // slopes: sum of dleak * open
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            typename Four<T>::Vec z = {};
-            x[s] = dy[s] = {};
-            const bool on = t0 + s < length;
-            if (on && left > 0) {
-                x[s] = load_four(in + (t0 + s) * a.in_stride[1], left);
-                z = load_four(gate + (t0 + s) * a.gate_stride[1], left);
-                dy[s] = load_four(grad + (t0 + s) * a.grad_stride[1], left);
-            }
+    for (int v = 0; v < V; ++v) {
+        d[v] = a.decay[a.decays == 1 ? 0 : from + v] * (1.f / 4096.f);
+        slopes[v] = 0;
+    }
+    const T* in = (const T*)a.in + n * a.in_stride[0];
+    const T* gate = (const T*)a.gate + n * a.gate_stride[0];
+    const T* grad = (const T*)a.grad + n * a.grad_stride[0];
+    T* grad_in = (T*)a.grad_in + n * a.tokens * a.channels;
+    T* grad_gate = (T*)a.grad_gate + n * a.tokens * a.channels;
+    const int channel = strip * CH + threadIdx.x;                  // of the first CH threads
+    const bool keeps = threadIdx.x < CH && channel < a.channels;
+    float carry = keeps && a.grad_last ? a.grad_last[n * a.channels + channel] : 0.f;
+    for (int64_t index = span.first; index < span.end; ++index) {   // counted from the last tile
+        const int64_t tile = a.tiles - 1 - index, t0 = tile * kTile + wave * S;
+        const int count = length - t0 < S ? (length > t0 ? (int)(length - t0) : 0) : S;
+        float start = 0;
+        if (keeps) start = a.starts[(n * a.kept + tile * (kTile / kKept)) * a.channels + channel];
+        float open[S][V];
+        typename Piece<T, V>::Raw x[S], dy[S];
+        Pair p[V];
+        float g[V];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) open[s][v] = on ? open_gate<T>((float)z[v]) : 0.f;   // what is not there leaks nothing, x and dy are 0
+        for (int v = 0; v < V; ++v) {
+            p[v] = {1.f, 0.f};
+            g[v] = 0;
         }
-        f4 start = {};
-        if (left > 0) start = load_four(a.starts + (n * a.tiles + tile) * a.channels + c, left);
-        f4 A = {1.f, 1.f, 1.f, 1.f}, H = {}, G = {};
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
+        if (count > 0) {
+            typename Piece<T, V>::Raw z[S];
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const float leak = d[v] * open[s][v], keep = 1.f - leak;
-                A[v] *= keep;
-                H[v] = fmaf(keep, H[v], drive_of<DRIVE>(leak, keep).value * (float)x[s][v]);
+                const int64_t t = t0 + (s < count ? s : count - 1);
+                z[s] = load_piece<V>(gate + t * a.gate_stride[1] + from);
+                x[s] = load_piece<V>(in + t * a.in_stride[1] + from);
+                dy[s] = load_piece<V>(grad + t * a.grad_stride[1] + from);
             }
 #pragma unroll
-            for (int s = S - 1; s >= 0; --s) G[v] = (1.f - d[v] * open[s][v]) * ((float)dy[s][v] + G[v]);
-        }
-        // the pairs of the lanes in front of this one and behind it, and of the wave
-        f4 before_a = {1.f, 1.f, 1.f, 1.f}, before_h = {}, behind_a = {1.f, 1.f, 1.f, 1.f}, behind_g = {}, B = A;
+            for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
+                for (int v = 0; v < V; ++v) open[s][v] = open_gate(value_of(z[s], v));
+            if (count < S) {                                       // what is not there leaks nothing
 #pragma unroll
-            for (int by = 16; by < 64; by *= 2) {
-                const float oa = __shfl_up(A[v], by), oh = __shfl_up(H[v], by);
-                const float ob = __shfl_down(B[v], by), og = __shfl_down(G[v], by);
-                if (lane >= by) {
-                    H[v] = fmaf(A[v], oh, H[v]);
-                    A[v] *= oa;
+                for (int s = 0; s < S; ++s)
+                    if (s >= count) {
+                        x[s] = dy[s] = 0;
+#pragma unroll
+                        for (int v = 0; v < V; ++v) open[s][v] = 0;
+                    }
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+#pragma unroll
+                for (int s = 0; s < S; ++s) {
+                    const float leak = d[v] * open[s][v], keep = 1.f - leak;
+                    p[v] = then(p[v], {keep, drive_of<DRIVE>(leak, keep).value * value_of(x[s], v)});
                 }
-                if (lane < 64 - by) {
-                    G[v] = fmaf(B[v], og, G[v]);
-                    B[v] *= ob;
-                }
-            }
-            const float oa = __shfl_up(A[v], 16), oh = __shfl_up(H[v], 16);
-            const float ob = __shfl_down(B[v], 16), og = __shfl_down(G[v], 16);
-            if (lane >= 16) {
-                before_a[v] = oa;
-                before_h[v] = oh;
-            }
-            if (lane < 48) {
-                behind_a[v] = ob;
-                behind_g[v] = og;
+#pragma unroll
+                for (int s = S - 1; s >= 0; --s) g[v] = fmaf(-d[v], open[s][v], 1.f) * (value_of(dy[s], v) + g[v]);
             }
         }
-        if (lt == 3) {
-            total[turn][wave][0][lc] = A;
-            total[turn][wave][1][lc] = H;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            total[wave][lane * V + v] = p[v];
+            total_g[wave][lane * V + v] = g[v];
         }
-        if (lt == 0) total[turn][wave][2][lc] = G;
         __syncthreads();
         if (LOOK) {
-            if (k.window > 1 && threadIdx.x < kStrip && (index + 1) % k.window != 0 && index + 1 < a.tiles) {
-                Pair p = {1.f, 0.f};
+            if (k.window > 1 && threadIdx.x < CH && (index + 1) % k.window != 0 && index + 1 < a.tiles) {
+                Pair all = {1.f, 0.f};
 #pragma unroll
-                for (int w = WAVES - 1; w >= 0; --w)
-                    p = then(p, {((float*)total[0][w][0])[threadIdx.x], ((float*)total[0][w][2])[threadIdx.x]});
-                leave(k.pairs + (index * k.chains + chain) * kStrip + threadIdx.x, pair_word(p.a, p.h));
+                for (int w = WAVES - 1; w >= 0; --w) all = then(all, {total[w][threadIdx.x].a, total_g[w][threadIdx.x]});
+                leave(k.pairs + (index * k.chains + span.chain) * CH + threadIdx.x, pair_word(all.a, all.h));
             }
-            state_before<64 * WAVES>((float*)carry[0], u.parts, k, index, chain, initial);
+            const Before b = look_back<64 * WAVES, CH>(parts, k, index, span.chain, carry);
+            carry = index % k.window == 0 ? b.state : fmaf(b.pair.a, b.state, b.pair.h);
         }
-        f4 h = start, g = carry[turn][lc], mine = g;
+        if (threadIdx.x < CH) {
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            const f4 wa = total[turn][w][0][lc], wh = total[turn][w][1][lc];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) h[v] = w < wave ? fmaf(wa[v], h[v], wh[v]) : h[v];
-        }
-#pragma unroll
-        for (int w = WAVES - 1; w >= 0; --w) {
-            const f4 wa = total[turn][w][0][lc], wg = total[turn][w][2][lc];
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                if (w == wave) mine[v] = g[v];
-                g[v] = fmaf(wa[v], g[v], wg[v]);
+            for (int w = WAVES - 1; w >= 0; --w) {
+                behind[w][threadIdx.x] = carry;
+                carry = fmaf(total[w][threadIdx.x].a, carry, total_g[w][threadIdx.x]);
             }
-        }
-        if (wave == 0 && lt == 0) {
-            if (!LOOK) carry[turn ^ 1][lc] = g;
-            if (a.grad_state && tile == 0 && left > 0) store_four(a.grad_state + n * a.channels + c, g, left);
-            if (LOOK && (index + 1) % k.window == 0 && index + 1 < a.tiles) {
-                Word* to = k.states + ((index + 1) / k.window * k.chains + chain) * kStrip + lc * 4;
+            if (a.grad_state && keeps && tile == 0) a.grad_state[n * a.channels + channel] = carry;
+            if (LOOK && (index + 1) % k.window == 0 && index + 1 < a.tiles)
+                leave(k.states + ((index + 1) / k.window * k.chains + span.chain) * CH + threadIdx.x, state_word(carry));
 #pragma unroll
-                for (int v = 0; v < 4; ++v) leave(to + v, state_word(g[v]));
+            for (int w = 0; w < WAVES; ++w) {
+                front[w][threadIdx.x] = start;
+                start = fmaf(total[w][threadIdx.x].a, start, total[w][threadIdx.x].h);
             }
         }
-        float before[S][4];
+        __syncthreads();
+        if (c >= a.channels) continue;
+        if (count > 0) {
+            float before[S][V];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            h[v] = fmaf(before_a[v], h[v], before_h[v]);
-            g[v] = fmaf(behind_a[v], mine[v], behind_g[v]);
+            for (int v = 0; v < V; ++v) {
+                float h = front[wave][lane * V + v];
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                before[s][v] = h[v];
-                const float leak = d[v] * open[s][v], keep = 1.f - leak;
-                h[v] = fmaf(keep, h[v], drive_of<DRIVE>(leak, keep).value * (float)x[s][v]);
+                for (int s = 0; s < S; ++s) {
+                    forget(open[s][v]);
+                    before[s][v] = h;
+                    const float leak = d[v] * open[s][v], keep = 1.f - leak;
+                    h = fmaf(keep, h, drive_of<DRIVE>(leak, keep).value * value_of(x[s], v));
+                }
+                g[v] = behind[wave][lane * V + v];
+            }
+#pragma unroll
+            for (int s = S - 1; s >= 0; --s) {
+                if (s >= count) continue;
+                float dx[V], dz[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    forget(open[s][v]);
+                    const float leak = d[v] * open[s][v], keep = 1.f - leak;
+                    const Drive drive = drive_of<DRIVE>(leak, keep);
+                    const float D = value_of(dy[s], v) + g[v];
+                    const float dleak = D * fmaf(drive.slope, value_of(x[s], v), -before[s][v]);
+                    dx[v] = drive.value * D;
+                    dz[v] = dleak * leak * (1.f - open[s][v]);
+                    slopes[v] = fmaf(dleak, open[s][v], slopes[v]);
+                    g[v] = keep * D;
+                }
+                store_piece(grad_in + (t0 + s) * a.channels + c, dx);
+                store_piece(grad_gate + (t0 + s) * a.channels + c, dz);
             }
         }
 #pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
-            const bool on = t0 + s < length;
-            f4 dx, dz;
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                const float leak = d[v] * open[s][v], keep = 1.f - leak;
-                const Drive drive = drive_of<DRIVE>(leak, keep);
-                const float D = (float)dy[s][v] + g[v];
-                float dleak = D * fmaf(drive.slope, (float)x[s][v], -before[s][v]);
-                dleak = on ? dleak : 0.f;
-                dx[v] = on ? drive.value * D : 0.f;
-                dz[v] = dleak * leak * (1.f - open[s][v]);
-                slopes[v] = fmaf(dleak, open[s][v], slopes[v]);
-                g[v] = keep * D;
+        for (int s = 0; s < S; ++s)
+            if (s >= count && t0 + s < a.tokens) {
+                const float none[V] = {};
+                store_piece(grad_in + (t0 + s) * a.channels + c, none);
+                store_piece(grad_gate + (t0 + s) * a.channels + c, none);
             }
-            if (t0 + s < a.tokens && left > 0) {
-                store_four(grad_in + (t0 + s) * a.channels, dx, left);
-                store_four(grad_gate + (t0 + s) * a.channels, dz, left);
-            }
-        }
     }
     if (!a.parts) return;
-    // the decays' gradient of this workgroup's tiles: a row of `parts` for each workgroup of a strip, or one number a workgroup
-    __syncthreads();                                                // (the pairs' part of the union has been read)
-    u.sums[wave * 4 + lt][lc] = slopes;
+    // the decays' gradient of this workgroup's tiles: a row of `parts` for all workgroups of a sample's strips, or one number a workgroup
+    __syncthreads();                                                // (front has been read)
+#pragma unroll
+    for (int v = 0; v < V; ++v) front[wave][lane * V + v] = c < a.channels ? slopes[v] : 0.f;
     __syncthreads();
-    if (threadIdx.x >= kStrip) return;
+    if (threadIdx.x >= CH) return;
     float sum = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES * 4; ++w) sum += ((float*)u.sums[w])[threadIdx.x];
-    const int channel = strip * kStrip + threadIdx.x;
+    for (int w = 0; w < WAVES; ++w) sum += front[w][threadIdx.x];
     if (a.decays > 1) {
-        if (channel < a.channels) a.parts[(first * a.samples + n) * a.channels + channel] = sum;
-    } else {
-        sum = sum_lanes(sum, 64);                                   // (channels that are not there have 0)
-        if (threadIdx.x == 0) a.parts[first * k.chains + chain] = sum;
+        if (channel < a.channels) a.parts[(span.first * a.samples + n) * a.channels + channel] = sum;
+        return;
     }
+    sum = sum_lanes(sum, 64);
+    if (lane == 0) a.parts[(span.first * a.samples * a.strips + span.chain) * V + wave] = sum;
 }
 
 __global__ __launch_bounds__(256) void zero_words_kernel(Word* words, int64_t count) {
@@ -469,13 +451,16 @@ __global__ __launch_bounds__(256) void leak_step_kernel(LeakArgs a, int quads) {
     const int64_t n = at / quads;
     if (n >= a.samples) return;
     const int c = (int)(at % quads) * 4, left = a.channels - c;
-    const f4 d = decays_of(a, c, left);
+    f4 d = {};
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+        if (v < left) d[v] = a.decay[a.decays == 1 ? 0 : c + v] * (1.f / 4096.f);
     const typename Four<T>::Vec x = load_four((const T*)a.in + n * a.in_stride[0] + c, left);
     const typename Four<T>::Vec z = load_four((const T*)a.gate + n * a.gate_stride[0] + c, left);
     f4 h = load_four(a.last + n * a.channels + c, left);
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-        const float leak = d[v] * open_gate<T>((float)z[v]), keep = 1.f - leak;
+        const float leak = d[v] * open_gate((float)z[v]), keep = 1.f - leak;
         h[v] = fmaf(keep, h[v], drive_of<DRIVE>(leak, keep).value * (float)x[v]);
     }
     store_four(a.last + n * a.channels + c, h, left);
@@ -483,8 +468,12 @@ __global__ __launch_bounds__(256) void leak_step_kernel(LeakArgs a, int quads) {
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------
-int64_t tiles_of(int64_t tokens) { return tokens > 0 ? (tokens + kTile - 1) / kTile : 1; }
-int64_t strips_of(int64_t channels) { return (channels + kStrip - 1) / kStrip; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Channels of a lane: two bfloat16 where they come in pairs, so that a wave reads 256 bytes of a row.
+int lane_of(const slayer_gated_leak* s) { return s->dtype == SLAYER_BFLOAT16 && s->channels % 2 == 0 ? 2 : 1; }
+// Tokens of a tile.
+constexpr int kForward = 128, kBackward = 128;
 
 int check_leak(const slayer_gated_leak* a) {
     if (!a) return SLAYER_ENULL;
@@ -496,16 +485,56 @@ int check_leak(const slayer_gated_leak* a) {
     if (!a->decay) return SLAYER_ENULL;
     if (a->tokens > kMaxT || a->channels > (1 << 24) || a->samples > ((int64_t)1 << 32)) return SLAYER_ERANGE;
     if (a->samples * a->channels > kMaxNumel / (a->tokens > 0 ? a->tokens : 1)) return SLAYER_ERANGE;
-    if (a->samples * strips_of(a->channels) > (1 << 23)) return SLAYER_ERANGE;          // a workgroup each
+    if (a->samples * ceil_div(a->channels, 64 * lane_of(a)) > (1 << 23)) return SLAYER_ERANGE;          // a workgroup each
     return 0;
 }
 
-LeakArgs args_of(const slayer_gated_leak* s) {
+// How the tiles are cut up among workgroups, and the workspace of that: the words, the ticket, the rows of the decays' gradient.
+struct Plan {
+    bool look;
+    int64_t tiles, strips, chains, blocks, window, pairs, words, rows, columns;   // rows, columns: of partial sums of the decays' gradient
+};
+Plan plan_of(const slayer_gated_leak* s, bool backward) {
+    Plan p = {};
+    const int lane = lane_of(s), tile = backward ? kBackward : kForward;
+    p.tiles = s->tokens > 0 ? ceil_div(s->tokens, tile) : 1;
+    p.strips = ceil_div(s->channels, 64 * lane);
+    p.chains = s->samples * p.strips;
+    p.look = p.tiles > 2 && p.chains < 2048 && p.tiles * p.chains < (1 << 23);
+    p.blocks = p.look ? p.tiles * p.chains : p.chains;
+    p.window = p.look ? 2048 / p.chains : 1;
+    if (p.window > kWindow) p.window = kWindow;
+    if (p.window > p.tiles) p.window = p.tiles;
+    if (p.look) {
+        p.pairs = p.window > 1 ? p.tiles * p.chains * 64 * lane : 0;
+        p.words = 1 + p.pairs + ceil_div(p.tiles, p.window) * p.chains * 64 * lane;
+    }
+    p.columns = s->num_decays;
+    p.rows = (p.look ? p.tiles : 1) * (s->num_decays == 1 ? p.chains * lane : s->samples);
+    return p;
+}
+int64_t floats_of(const Plan& p, bool sums) { return 2 * p.words + (sums ? p.rows * p.columns : 0); }
+
+// The zeroed words at the front of the workspace.
+int chains_of(Chains* k, const Plan& p, float* workspace, hipStream_t stream) {
+    if (!p.look) return 0;
+    k->chains = (int)p.chains;
+    k->window = (int)p.window;
+    k->ticket = (unsigned*)workspace;
+    k->pairs = (Word*)workspace + 1;
+    k->states = k->pairs + p.pairs;
+    const int64_t blocks = ceil_div(p.words, 1024);
+    hipLaunchKernelGGL(zero_words_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, stream, (Word*)workspace, p.words);
+    return (int)hipGetLastError();
+}
+
+LeakArgs args_of(const slayer_gated_leak* s, const Plan& p) {
     LeakArgs a = {};
     a.lengths = s->lengths; a.lengths_bytes = s->lengths_bytes;
     a.decay = s->decay; a.decays = (int)s->num_decays;
-    a.samples = s->samples; a.tokens = s->tokens; a.tiles = tiles_of(s->tokens);
-    a.channels = (int)s->channels; a.strips = (int)strips_of(s->channels);
+    a.samples = s->samples; a.tokens = s->tokens; a.tiles = p.tiles;
+    a.kept = s->tokens > 0 ? ceil_div(s->tokens, kKept) : 1;
+    a.channels = (int)s->channels; a.strips = (int)p.strips;
     for (int i = 0; i < 2; ++i) {
         a.in_stride[i] = s->input_stride[i];
         a.gate_stride[i] = s->gate_stride[i];
@@ -514,46 +543,16 @@ LeakArgs args_of(const slayer_gated_leak* s) {
     return a;
 }
 
-// How the tiles are cut up among workgroups, and the workspace of that: the words, the ticket, the rows of the decays' gradient.
-struct Plan {
-    bool look;
-    int64_t chains, blocks, window, words, rows;        // rows: of partial sums of the decays' gradient
-};
-Plan plan_of(const slayer_gated_leak* s) {
-    Plan p = {};
-    const int64_t tiles = tiles_of(s->tokens);
-    p.chains = s->samples * strips_of(s->channels);
-    p.look = tiles > 2 && p.chains < 2048 && tiles * p.chains < (1 << 23);
-    p.blocks = p.look ? tiles * p.chains : p.chains;
-    p.window = p.look ? 2048 / p.chains : 1;
-    if (p.window > kWindow) p.window = kWindow;
-    if (p.window > tiles) p.window = tiles;
-    if (p.look) p.words = ((p.window > 1 ? tiles : 0) + (tiles + p.window - 1) / p.window) * p.chains * kStrip + 1;
-    p.rows = (p.look ? tiles : 1) * (s->num_decays == 1 ? p.chains : s->samples);
-    return p;
-}
-// The zeroed words at the front of the workspace.
-int chains_of(Chains* k, const Plan& p, const slayer_gated_leak* s, float* workspace, hipStream_t stream) {
-    if (!p.look) return 0;
-    k->chains = (int)p.chains;
-    k->window = (int)p.window;
-    k->ticket = (unsigned*)workspace;
-    k->pairs = (Word*)workspace + 1;
-    k->states = k->pairs + (p.window > 1 ? tiles_of(s->tokens) : 0) * p.chains * kStrip;
-    const int64_t blocks = (p.words + 1023) / 1024;
-    hipLaunchKernelGGL(zero_words_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, stream, (Word*)workspace, p.words);
-    return (int)hipGetLastError();
-}
-
-#define BY_DRIVE(T, LAUNCH)                                 \
-    switch (s->drive) {                                     \
-        case DRIVE_NONE: LAUNCH(T, DRIVE_NONE); break;      \
-        case DRIVE_GAIN: LAUNCH(T, DRIVE_GAIN); break;      \
-        default: LAUNCH(T, DRIVE_VARIANCE); break;          \
+#define BY_DRIVE(LAUNCH, ...)                                           \
+    switch (s->drive) {                                                 \
+        case DRIVE_NONE: LAUNCH(DRIVE_NONE, __VA_ARGS__); break;        \
+        case DRIVE_GAIN: LAUNCH(DRIVE_GAIN, __VA_ARGS__); break;        \
+        default: LAUNCH(DRIVE_VARIANCE, __VA_ARGS__); break;            \
     }
-#define BY_TYPE(LAUNCH)                                     \
-    if (s->dtype == SLAYER_FLOAT32) BY_DRIVE(float, LAUNCH) \
-    else BY_DRIVE(bf16, LAUNCH)
+#define BY_TYPE(LAUNCH)                                                 \
+    if (s->dtype == SLAYER_FLOAT32) BY_DRIVE(LAUNCH, float, 1)          \
+    else if (lane_of(s) == 2) BY_DRIVE(LAUNCH, bf16, 2)                 \
+    else BY_DRIVE(LAUNCH, bf16, 1)
 
 }  // namespace
 }  // namespace slayer
@@ -562,13 +561,12 @@ using namespace slayer;
 
 extern "C" int64_t slayer_gated_leak_starts(const slayer_gated_leak* s) {
     if (int e = check_leak(s)) return e;
-    return s->samples * tiles_of(s->tokens) * s->channels;
+    return s->samples * (s->tokens > 0 ? ceil_div(s->tokens, kKept) : 1) * s->channels;
 }
 
 extern "C" int64_t slayer_gated_leak_workspace(const slayer_gated_leak* s, int backward) {
     if (int e = check_leak(s)) return e;
-    const Plan p = plan_of(s);
-    return 2 * p.words + (backward ? p.rows * s->num_decays : 0);
+    return floats_of(plan_of(s, backward), backward);
 }
 
 extern "C" int slayer_gated_leak_fwd(void* out, float* last, float* starts, const void* input, const void* gate, const float* state,
@@ -576,18 +574,19 @@ extern "C" int slayer_gated_leak_fwd(void* out, float* last, float* starts, cons
     if (int e = check_leak(s)) return e;
     if (s->samples == 0) return 0;
     if (s->tokens > 0 && (!out || !input || !gate)) return SLAYER_ENULL;
-    const Plan p = plan_of(s);
-    if (p.words > 0 && !workspace) return SLAYER_ENULL;
-    if (floats < 2 * p.words || (uintptr_t)workspace % 8 != 0) return SLAYER_EINVAL;
-    LeakArgs a = args_of(s);
+    const Plan p = plan_of(s, false);
+    const int64_t need = floats_of(p, false);
+    if (need > 0 && !workspace) return SLAYER_ENULL;
+    if (floats < need || (uintptr_t)workspace % 8 != 0) return SLAYER_EINVAL;
+    LeakArgs a = args_of(s, p);
     a.out = out; a.last = last; a.starts = starts; a.in = input; a.gate = gate; a.state = state;
     Chains k = {};
-    if (int e = chains_of(&k, p, s, workspace, (hipStream_t)stream)) return e;
-#define ONE(T, DRIVE, LOOK) \
-    hipLaunchKernelGGL((leak_fwd_kernel<T, DRIVE, 8, 4, LOOK>), dim3((unsigned)p.blocks), dim3(256), 0, (hipStream_t)stream, a, k)
-#define LAUNCH(T, DRIVE)                    \
-    if (p.look) ONE(T, DRIVE, true);        \
-    else ONE(T, DRIVE, false)
+    if (int e = chains_of(&k, p, workspace, (hipStream_t)stream)) return e;
+#define ONE(DRIVE, T, V, LOOK) \
+    hipLaunchKernelGGL((leak_fwd_kernel<T, V, DRIVE, 16, kForward / 16, LOOK>), dim3((unsigned)p.blocks), dim3(4 * kForward), 0, (hipStream_t)stream, a, k)
+#define LAUNCH(DRIVE, T, V)                    \
+    if (p.look) ONE(DRIVE, T, V, true);        \
+    else ONE(DRIVE, T, V, false)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
 #undef ONE
@@ -600,21 +599,21 @@ extern "C" int slayer_gated_leak_bwd(void* grad_input, void* grad_gate, float* g
     if (int e = check_leak(s)) return e;
     if (s->samples == 0) return grad_decay ? launch_zero_fill(grad_decay, s->num_decays, (hipStream_t)stream) : 0;
     if (!starts || (s->tokens > 0 && (!grad_input || !grad_gate || !grad_out || !input || !gate))) return SLAYER_ENULL;
-    const Plan p = plan_of(s);
-    const int64_t need = 2 * p.words + (grad_decay ? p.rows * s->num_decays : 0);
+    const Plan p = plan_of(s, true);
+    const int64_t need = floats_of(p, grad_decay);
     if (need > 0 && !workspace) return SLAYER_ENULL;
     if (floats < need || (uintptr_t)workspace % 8 != 0) return SLAYER_EINVAL;
-    LeakArgs a = args_of(s);
+    LeakArgs a = args_of(s, p);
     a.grad_in = grad_input; a.grad_gate = grad_gate; a.grad_state = grad_state; a.grad = grad_out; a.grad_last = grad_last;
     a.in = input; a.gate = gate; a.starts = (float*)starts;
     a.parts = grad_decay ? workspace + 2 * p.words : nullptr;
     Chains k = {};
-    if (int e = chains_of(&k, p, s, workspace, (hipStream_t)stream)) return e;
-#define ONE(T, DRIVE, LOOK) \
-    hipLaunchKernelGGL((leak_bwd_kernel<T, DRIVE, 4, 8, LOOK>), dim3((unsigned)p.blocks), dim3(512), 0, (hipStream_t)stream, a, k)
-#define LAUNCH(T, DRIVE)                    \
-    if (p.look) ONE(T, DRIVE, true);        \
-    else ONE(T, DRIVE, false)
+    if (int e = chains_of(&k, p, workspace, (hipStream_t)stream)) return e;
+#define ONE(DRIVE, T, V, LOOK) \
+    hipLaunchKernelGGL((leak_bwd_kernel<T, V, DRIVE, 16, kBackward / 16, LOOK>), dim3((unsigned)p.blocks), dim3(4 * kBackward), 0, (hipStream_t)stream, a, k)
+#define LAUNCH(DRIVE, T, V)                    \
+    if (p.look) ONE(DRIVE, T, V, true);        \
+    else ONE(DRIVE, T, V, false)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
 #undef ONE
@@ -622,7 +621,7 @@ extern "C" int slayer_gated_leak_bwd(void* grad_input, void* grad_gate, float* g
     if (!grad_decay) return 0;
     ColumnSums sums = {};
     sums.out[0] = grad_decay; sums.parts[0] = a.parts; sums.factor = 1.f / 4096.f;
-    sums.columns = sums.pitch = s->num_decays;
+    sums.columns = sums.pitch = p.columns;
     sums.rows = p.rows;
     return launch_column_sums(sums, 1, (hipStream_t)stream);
 }
@@ -632,12 +631,12 @@ extern "C" int slayer_gated_leak_step(void* out, float* state, const void* input
     if (int e = check_leak(s)) return e;
     if (s->samples == 0) return 0;
     if (!out || !state || !input || !gate) return SLAYER_ENULL;
-    LeakArgs a = args_of(s);
+    LeakArgs a = args_of(s, plan_of(s, false));
     a.out = out; a.last = state; a.in = input; a.gate = gate;
     const int quads = (a.channels + 3) / 4;
     const int64_t blocks = (a.samples * quads + 255) / 256;
     if (blocks > (1 << 23)) return SLAYER_ERANGE;
-#define LAUNCH(T, DRIVE) \
+#define LAUNCH(DRIVE, T, V) \
     hipLaunchKernelGGL((leak_step_kernel<T, DRIVE>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, quads)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
