@@ -83,9 +83,9 @@ __device__ __forceinline__ int64_t length_of(const LeakArgs& a, int64_t n) {
 // ---- tiles of a chain -----------------------------------------------------------------------------------------------------------
 // A chain is one strip of one sample, from tile to tile in the order of the pass.  Either a workgroup walks all tiles of a chain and
 // carries the state in LDS, or there is a workgroup for each tile, and states go through memory:
-//   Workgroups take their tiles by a ticket, the first tiles of all chains before the second ones, so a workgroup only ever waits for
-// workgroups with lower tickets, which are running or done and wait for lower ones themselves; the lowest waits for nobody, so every wait
-// ends.  Tiles form windows.  A tile leaves its pair, then reads those of the tiles before it in its window, and the state in front of
+//   A workgroup takes the next tile of its chain by a ticket, so it only ever waits for workgroups of the same chain with lower tickets,
+// which are running or done and wait for lower ones themselves; the lowest waits for nobody, so every wait ends.  (One ticket for all
+// chains would be taken at 12 ns each, whoever asks: 25 us for the 2048 tiles of a prompt.)  Tiles form windows.  A tile leaves its pair, then reads those of the tiles before it in its window, and the state in front of
 // the window; the last tile of a window leaves the state behind it.  Which values are joined, and in which order, depends on the sizes alone
 // and not on who comes first, so that a call computed again has the same bits.
 //   What is left is a word of 64 bits that says itself that it is there (the workspace is zeroed before), read and written with relaxed
@@ -93,9 +93,10 @@ __device__ __forceinline__ int64_t length_of(const LeakArgs& a, int64_t n) {
 typedef unsigned long long Word;
 constexpr int kWindow = 32;                    // largest window
 
+constexpr int kApart = 16;                     // words from one chain's ticket to the next: a cache line each
+
 struct Chains {
-    unsigned* ticket;
-    Word *pairs, *states;                      // [tile][chain][strip], [window][chain][strip]
+    Word *tickets, *pairs, *states;            // [chain], [tile][chain][strip], [window][chain][strip]
     int chains, window;
 };
 
@@ -160,10 +161,11 @@ struct Span { unsigned chain; int64_t first, end; };
 template <bool LOOK> __device__ __forceinline__ Span span_of(const LeakArgs& a, const Chains& k) {
     if (!LOOK) return {blockIdx.x, 0, a.tiles};
     __shared__ unsigned ticket;
-    if (threadIdx.x == 0) ticket = atomicAdd(k.ticket, 1u);
+    const unsigned chain = blockIdx.x % (unsigned)k.chains;
+    if (threadIdx.x == 0) ticket = (unsigned)atomicAdd(k.tickets + chain * kApart, 1ull);
     __syncthreads();
-    const unsigned mine = __builtin_amdgcn_readfirstlane(ticket), first = mine / (unsigned)k.chains;
-    return {mine - first * k.chains, first, first + 1};
+    const unsigned tile = __builtin_amdgcn_readfirstlane(ticket);
+    return {chain, tile, (int64_t)tile + 1};
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
@@ -507,7 +509,7 @@ Plan plan_of(const slayer_gated_leak* s, bool backward) {
     if (p.window > p.tiles) p.window = p.tiles;
     if (p.look) {
         p.pairs = p.window > 1 ? p.tiles * p.chains * 64 * lane : 0;
-        p.words = 1 + p.pairs + ceil_div(p.tiles, p.window) * p.chains * 64 * lane;
+        p.words = p.chains * kApart + p.pairs + ceil_div(p.tiles, p.window) * p.chains * 64 * lane;
     }
     p.columns = s->num_decays;
     p.rows = (p.look ? p.tiles : 1) * (s->num_decays == 1 ? p.chains * lane : s->samples);
@@ -520,8 +522,8 @@ int chains_of(Chains* k, const Plan& p, float* workspace, hipStream_t stream) {
     if (!p.look) return 0;
     k->chains = (int)p.chains;
     k->window = (int)p.window;
-    k->ticket = (unsigned*)workspace;
-    k->pairs = (Word*)workspace + 1;
+    k->tickets = (Word*)workspace;
+    k->pairs = k->tickets + p.chains * kApart;
     k->states = k->pairs + p.pairs;
     const int64_t blocks = ceil_div(p.words, 1024);
     hipLaunchKernelGGL(zero_words_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, stream, (Word*)workspace, p.words);
