@@ -71,6 +71,25 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void store_piece(bf16* p, const float (&x)[2]) {
     *reinterpret_cast<b2_any*>(p) = __builtin_convertvector(f2{x[0], x[1]}, b2);
 }
+// The channels of a lane.  A last channel without a neighbour (V is 2 and the channels are odd) is read with the one in front of it: `odd`
+// lanes have their own channel in value 1, and value 0 goes where a channel behind the last one would be.  Lanes without channels read the
+// last ones.
+template <int V> struct Lane {
+    int c, from, odd, slot;                    // first channel, first channel read, slot of value 0 in the strip
+    bool on;
+    __device__ __forceinline__ Lane(int strip, int lane, int channels) {
+        c = (strip * 64 + lane) * V;
+        on = c < channels;
+        odd = V == 2 && c + 1 == channels;
+        from = on ? c - odd : channels - V;
+        slot = lane * V;
+    }
+    __device__ __forceinline__ int at(int v) const { return slot + (v ^ odd); }
+    template <typename T> __device__ __forceinline__ void store(T* row, const float (&x)[V]) const {
+        if (!odd) store_piece(row + c, x);
+        else row[c] = (T)x[V - 1];
+    }
+};
 // Keeps the compiler from holding on to what it has made of x: that is made again instead of taking up registers.
 __device__ __forceinline__ void forget(float& x) { asm volatile("" : "+v"(x)); }
 
@@ -181,10 +200,10 @@ __global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a, Chains
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int strip = span.chain % (unsigned)a.strips;
     const int64_t n = span.chain / (unsigned)a.strips, length = length_of(a, n);
-    const int c = strip * CH + lane * V, from = c < a.channels ? c : a.channels - V;       // lanes without channels read the last ones
+    const Lane<V> own(strip, lane, a.channels);
     float d[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) d[v] = a.decay[a.decays == 1 ? 0 : from + v] * (1.f / 4096.f);
+    for (int v = 0; v < V; ++v) d[v] = a.decay[a.decays == 1 ? 0 : own.from + v] * (1.f / 4096.f);
     const T* in = (const T*)a.in + n * a.in_stride[0];
     const T* gate = (const T*)a.gate + n * a.gate_stride[0];
     T* out = (T*)a.out + n * a.tokens * a.channels;
@@ -203,8 +222,8 @@ __global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a, Chains
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 const int64_t t = t0 + (s < count ? s : count - 1);
-                x[s] = load_piece<V>(in + t * a.in_stride[1] + from);
-                z[s] = load_piece<V>(gate + t * a.gate_stride[1] + from);
+                x[s] = load_piece<V>(in + t * a.in_stride[1] + own.from);
+                z[s] = load_piece<V>(gate + t * a.gate_stride[1] + own.from);
             }
 #pragma unroll
             for (int s = 0; s < S; ++s)
@@ -230,7 +249,7 @@ __global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a, Chains
                 for (int v = 0; v < V; ++v) p[v] = then(p[v], {keep[s][v], add[s][v]});
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) total[wave][lane * V + v] = p[v];
+        for (int v = 0; v < V; ++v) total[wave][own.at(v)] = p[v];
         __syncthreads();
         if (LOOK) {
             if (k.window > 1 && threadIdx.x < CH && (tile + 1) % k.window != 0 && tile + 1 < a.tiles) {
@@ -255,19 +274,19 @@ __global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a, Chains
                 leave(k.states + ((tile + 1) / k.window * k.chains + span.chain) * CH + threadIdx.x, state_word(carry));
         }
         __syncthreads();
-        if (c >= a.channels) continue;
+        if (!own.on) continue;
         float h[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = front[wave][lane * V + v];
+        for (int v = 0; v < V; ++v) h[v] = front[wave][own.at(v)];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
             if (s < count) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) h[v] = fmaf(keep[s][v], h[v], add[s][v]);
-                store_piece(out + (t0 + s) * a.channels + c, h);
+                own.store(out + (t0 + s) * a.channels, h);
             } else if (t0 + s < a.tokens) {
                 const float none[V] = {};
-                store_piece(out + (t0 + s) * a.channels + c, none);
+                own.store(out + (t0 + s) * a.channels, none);
             }
         }
     }
@@ -287,11 +306,11 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a, Chains
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int strip = span.chain % (unsigned)a.strips;
     const int64_t n = span.chain / (unsigned)a.strips, length = length_of(a, n);
-    const int c = strip * CH + lane * V, from = c < a.channels ? c : a.channels - V;       // lanes without channels read the last ones
+    const Lane<V> own(strip, lane, a.channels);
     float d[V], slopes[V];                                          // slopes: sum of dleak * open
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        d[v] = a.decay[a.decays == 1 ? 0 : from + v] * (1.f / 4096.f);
+        d[v] = a.decay[a.decays == 1 ? 0 : own.from + v] * (1.f / 4096.f);
         slopes[v] = 0;
     }
     const T* in = (const T*)a.in + n * a.in_stride[0];
@@ -321,9 +340,9 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a, Chains
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 const int64_t t = t0 + (s < count ? s : count - 1);
-                z[s] = load_piece<V>(gate + t * a.gate_stride[1] + from);
-                x[s] = load_piece<V>(in + t * a.in_stride[1] + from);
-                dy[s] = load_piece<V>(grad + t * a.grad_stride[1] + from);
+                z[s] = load_piece<V>(gate + t * a.gate_stride[1] + own.from);
+                x[s] = load_piece<V>(in + t * a.in_stride[1] + own.from);
+                dy[s] = load_piece<V>(grad + t * a.grad_stride[1] + own.from);
             }
 #pragma unroll
             for (int s = 0; s < S; ++s)
@@ -351,8 +370,8 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a, Chains
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            total[wave][lane * V + v] = p[v];
-            total_g[wave][lane * V + v] = g[v];
+            total[wave][own.at(v)] = p[v];
+            total_g[wave][own.at(v)] = g[v];
         }
         __syncthreads();
         if (LOOK) {
@@ -381,12 +400,12 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a, Chains
             }
         }
         __syncthreads();
-        if (c >= a.channels) continue;
+        if (!own.on) continue;
         if (count > 0) {
             float before[S][V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                float h = front[wave][lane * V + v];
+                float h = front[wave][own.at(v)];
 #pragma unroll
                 for (int s = 0; s < S; ++s) {
                     forget(open[s][v]);
@@ -394,7 +413,7 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a, Chains
                     const float leak = d[v] * open[s][v], keep = 1.f - leak;
                     h = fmaf(keep, h, drive_of<DRIVE>(leak, keep).value * value_of(x[s], v));
                 }
-                g[v] = behind[wave][lane * V + v];
+                g[v] = behind[wave][own.at(v)];
             }
 #pragma unroll
             for (int s = S - 1; s >= 0; --s) {
@@ -412,23 +431,23 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a, Chains
                     slopes[v] = fmaf(dleak, open[s][v], slopes[v]);
                     g[v] = keep * D;
                 }
-                store_piece(grad_in + (t0 + s) * a.channels + c, dx);
-                store_piece(grad_gate + (t0 + s) * a.channels + c, dz);
+                own.store(grad_in + (t0 + s) * a.channels, dx);
+                own.store(grad_gate + (t0 + s) * a.channels, dz);
             }
         }
 #pragma unroll
         for (int s = 0; s < S; ++s)
             if (s >= count && t0 + s < a.tokens) {
                 const float none[V] = {};
-                store_piece(grad_in + (t0 + s) * a.channels + c, none);
-                store_piece(grad_gate + (t0 + s) * a.channels + c, none);
+                own.store(grad_in + (t0 + s) * a.channels, none);
+                own.store(grad_gate + (t0 + s) * a.channels, none);
             }
     }
     if (!a.parts) return;
     // the decays' gradient of this workgroup's tiles: a row of `parts` for all workgroups of a sample's strips, or one number a workgroup
     __syncthreads();                                                // (front has been read)
 #pragma unroll
-    for (int v = 0; v < V; ++v) front[wave][lane * V + v] = c < a.channels ? slopes[v] : 0.f;
+    for (int v = 0; v < V; ++v) front[wave][own.at(v)] = slopes[v];
     __syncthreads();
     if (threadIdx.x >= CH) return;
     float sum = 0;
@@ -438,7 +457,7 @@ __global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a, Chains
         if (channel < a.channels) a.parts[(span.first * a.samples + n) * a.channels + channel] = sum;
         return;
     }
-    sum = sum_lanes(sum, 64);
+    sum = sum_lanes(channel < a.channels ? sum : 0.f, 64);
     if (lane == 0) a.parts[(span.first * a.samples * a.strips + span.chain) * V + wave] = sum;
 }
 
@@ -472,8 +491,8 @@ __global__ __launch_bounds__(256) void leak_step_kernel(LeakArgs a, int quads) {
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Channels of a lane: two bfloat16 where they come in pairs, so that a wave reads 256 bytes of a row.
-int lane_of(const slayer_gated_leak* s) { return s->dtype == SLAYER_BFLOAT16 && s->channels % 2 == 0 ? 2 : 1; }
+// Channels of a lane: two bfloat16 where there are two, so that a wave reads 256 bytes of a row.
+int lane_of(const slayer_gated_leak* s) { return s->dtype == SLAYER_BFLOAT16 && s->channels > 1 ? 2 : 1; }
 // Tokens of a tile.
 constexpr int kForward = 128, kBackward = 128;
 
