@@ -190,7 +190,7 @@ template <bool LOOK> __device__ __forceinline__ Span span_of(const LeakArgs& a, 
 // ---- forward --------------------------------------------------------------------------------------------------------------------
 // S tokens a wave, V channels a lane.
 template <typename T, int V, int DRIVE, int S, int WAVES, bool LOOK>
-__global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a, Chains k) {
+__global__ __launch_bounds__(64 * WAVES, 4) void leak_fwd_kernel(LeakArgs a, Chains k) {
     constexpr int CH = 64 * V, kTile = S * WAVES;
     static_assert(kKept % S == 0 && kTile % kKept == 0, "a wave begins where a state is kept");
     __shared__ Pair total[WAVES][CH];
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(64 * WAVES) void leak_fwd_kernel(LeakArgs a, Chains
 // ---- backward -------------------------------------------------------------------------------------------------------------------
 // The same chains, their tiles from the last to the first.  Inside a tile the states go forwards, from the kept one, and G backwards.
 template <typename T, int V, int DRIVE, int S, int WAVES, bool LOOK>
-__global__ __launch_bounds__(64 * WAVES) void leak_bwd_kernel(LeakArgs a, Chains k) {
+__global__ __launch_bounds__(64 * WAVES, 4) void leak_bwd_kernel(LeakArgs a, Chains k) {
     constexpr int CH = 64 * V, kTile = S * WAVES;
     static_assert(kTile % kKept == 0, "a tile begins where a state is kept");
     __shared__ Pair total[WAVES][CH];
@@ -493,8 +493,9 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Channels of a lane: two bfloat16 where there are two, so that a wave reads 256 bytes of a row.
 int lane_of(const slayer_gated_leak* s) { return s->dtype == SLAYER_BFLOAT16 && s->channels > 1 ? 2 : 1; }
-// Tokens of a tile.
-constexpr int kForward = 128, kBackward = 128;
+// Tokens of a wave, of the eight waves of a workgroup.
+constexpr int tokens_of(int lane, bool backward) { return lane == 2 && backward ? 8 : 16; }
+constexpr int kWaves = 8;
 
 int check_leak(const slayer_gated_leak* a) {
     if (!a) return SLAYER_ENULL;
@@ -517,7 +518,7 @@ struct Plan {
 };
 Plan plan_of(const slayer_gated_leak* s, bool backward) {
     Plan p = {};
-    const int lane = lane_of(s), tile = backward ? kBackward : kForward;
+    const int lane = lane_of(s), tile = kWaves * tokens_of(lane, backward);
     p.tiles = s->tokens > 0 ? ceil_div(s->tokens, tile) : 1;
     p.strips = ceil_div(s->channels, 64 * lane);
     p.chains = s->samples * p.strips;
@@ -604,7 +605,7 @@ extern "C" int slayer_gated_leak_fwd(void* out, float* last, float* starts, cons
     Chains k = {};
     if (int e = chains_of(&k, p, workspace, (hipStream_t)stream)) return e;
 #define ONE(DRIVE, T, V, LOOK) \
-    hipLaunchKernelGGL((leak_fwd_kernel<T, V, DRIVE, 16, kForward / 16, LOOK>), dim3((unsigned)p.blocks), dim3(4 * kForward), 0, (hipStream_t)stream, a, k)
+    hipLaunchKernelGGL((leak_fwd_kernel<T, V, DRIVE, tokens_of(V, false), kWaves, LOOK>), dim3((unsigned)p.blocks), dim3(64 * kWaves), 0, (hipStream_t)stream, a, k)
 #define LAUNCH(DRIVE, T, V)                    \
     if (p.look) ONE(DRIVE, T, V, true);        \
     else ONE(DRIVE, T, V, false)
@@ -631,7 +632,7 @@ extern "C" int slayer_gated_leak_bwd(void* grad_input, void* grad_gate, float* g
     Chains k = {};
     if (int e = chains_of(&k, p, workspace, (hipStream_t)stream)) return e;
 #define ONE(DRIVE, T, V, LOOK) \
-    hipLaunchKernelGGL((leak_bwd_kernel<T, V, DRIVE, 16, kBackward / 16, LOOK>), dim3((unsigned)p.blocks), dim3(4 * kBackward), 0, (hipStream_t)stream, a, k)
+    hipLaunchKernelGGL((leak_bwd_kernel<T, V, DRIVE, tokens_of(V, true), kWaves, LOOK>), dim3((unsigned)p.blocks), dim3(64 * kWaves), 0, (hipStream_t)stream, a, k)
 #define LAUNCH(DRIVE, T, V)                    \
     if (p.look) ONE(DRIVE, T, V, true);        \
     else ONE(DRIVE, T, V, false)
