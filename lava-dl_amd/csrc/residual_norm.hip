@@ -37,78 +37,147 @@ template <typename T> __device__ __forceinline__ Gate gate_of(int activation, fl
     return {z * p, p * fmaf(z, 1.f - p, 1.f)};
 }
 
-// Sum over the LANES threads of a row (a workgroup of one row, or one to four waves with a row each).
+// Sum over LANES neighbouring lanes, in all of them, without LDS: each step adds the other half of 2, 4, 8, 16, 32, 64 lanes.
+template <int CTRL> __device__ __forceinline__ float add_moved(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int LANES> __device__ __forceinline__ float sum_wave(float v) {
+    v = add_moved<0xb1>(v);                                        // quads: the neighbour
+    v = add_moved<0x4e>(v);                                        // quads: the other pair
+    if (LANES >= 8) v = add_moved<0x141>(v);                       // eight lanes mirrored
+    if (LANES >= 16) v = add_moved<0x140>(v);                      // sixteen lanes mirrored
+    if (LANES >= 32) {
+        const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    }
+    if (LANES >= 64) {
+        const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    }
+    return v;
+}
+// Sum over the LANES threads of a row: a part of a wave, or a whole workgroup.
 template <int LANES> __device__ __forceinline__ float sum_row(float v, float* shared) {
-    v = sum_lanes(v, LANES < 64 ? LANES : 64);
+    v = sum_wave<LANES < 64 ? LANES : 64>(v);
     if (LANES <= 64) return v;
     __syncthreads();                                               // who reads the sum before
     if (threadIdx.x % 64 == 0) shared[threadIdx.x / 64] = v;
     __syncthreads();
-    float sum = shared[0];
-#pragma unroll
-    for (int w = 1; w < LANES / 64; ++w) sum += shared[w];
-    return sum;
+    v = shared[threadIdx.x % (LANES / 64)];
+    return sum_wave<LANES / 64 < 4 ? 4 : LANES / 64>(LANES == 128 && threadIdx.x % 4 >= 2 ? 0.f : v);
 }
 
-__device__ __forceinline__ f4 parameters(const float* p, int c, int left) {
-    f4 v = {1.f, 1.f, 1.f, 1.f};
-    if (p)
+// The channels of a thread's access of W: from + lo ... from + hi - 1.  An access at the end of a row that is no multiple of W begins
+// earlier than its own channels, so that it is one access all the same; what is not its own reads as 0 and is not written.
+struct Own { int from, lo, hi; };
+template <int W> __device__ __forceinline__ Own own_of(int c, int channels) {
+    if (c >= channels) return {0, 0, 0};
+    const int from = c + W <= channels ? c : channels > W ? channels - W : 0;
+    return {from, c - from, channels - from < W ? channels - from : W};
+}
+typedef f8 f8_any __attribute__((aligned(4)));
+typedef b8 b8_any __attribute__((aligned(2)));
+__device__ __forceinline__ void read_all(float (&x)[4], const float* p) { to_floats(x, *reinterpret_cast<const f4_any*>(p)); }
+__device__ __forceinline__ void read_all(float (&x)[8], const bf16* p) { to_floats(x, *reinterpret_cast<const b8_any*>(p)); }
+__device__ __forceinline__ void read_all(float (&x)[8], const float* p) {
+    const f8 v = *reinterpret_cast<const f8_any*>(p);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < left) v[e] = p[c + e];
-    return v;
+    for (int e = 0; e < 8; ++e) x[e] = v[e];
+}
+__device__ __forceinline__ void write_all(float* p, const float (&x)[4]) { *reinterpret_cast<f4_any*>(p) = from_floats(x); }
+__device__ __forceinline__ void write_all(bf16* p, const float (&x)[8]) { *reinterpret_cast<b8_any*>(p) = from_floats(x); }
+__device__ __forceinline__ void write_all(float* p, const float (&x)[8]) {
+    *reinterpret_cast<f8_any*>(p) = f8{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+}
+template <typename T, int W> __device__ __forceinline__ void read(float (&x)[W], const T* row, const Own& own) {
+    if (own.hi == W) {
+        read_all(x, row + own.from);
+        if (own.lo > 0)
+#pragma unroll
+            for (int e = 0; e < W; ++e) x[e] = e < own.lo ? 0.f : x[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) x[e] = e < own.hi ? (float)row[own.from + e] : 0.f;
+    }
+}
+template <typename T, int W> __device__ __forceinline__ void write(T* row, const float (&x)[W], const Own& own) {
+    if (own.lo == 0 && own.hi == W) {
+        write_all(row + own.from, x);
+    } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+            if (e >= own.lo && e < own.hi) row[own.from + e] = (T)x[e];
+    }
+}
+template <int W> __device__ __forceinline__ void parameters(float (&x)[W], const float* p, const Own& own) {
+    if (p) {
+        read(x, p, own);
+    } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) x[e] = 1.f;
+    }
 }
 
-// T: x, gate and y.  R: the residual stream.  LANES threads a row, IT times four channels each; the loop over the rows is the same for all
-// threads of a workgroup.
+// T: x, gate and y.  R: the residual stream.  LANES threads a row, IT accesses of 16 bytes of x each.  The loop over the rows is the same for
+// all threads of a workgroup.
+template <int LANES> constexpr int rows_of() { return LANES <= 64 ? 256 / LANES : 1; }
 template <typename T, typename R, int LANES, int IT>
-__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void residual_fwd_kernel(ResidualArgs a) {
-    constexpr int kThreads = LANES < 256 ? 256 : LANES, kRows = kThreads / LANES;
+__global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_fwd_kernel(ResidualArgs a) {
+    constexpr int W = Elements<T>::kVec, kRows = rows_of<LANES>();
     __shared__ float shared[16];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const float inv = 1.f / (float)a.channels;
+    Own own[IT];
+    float inner[IT][W], outer[IT][W], scale[IT][W];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        own[i] = own_of<W>((i * LANES + lane) * W, a.channels);
+        parameters(inner[i], a.inner, own[i]);
+        parameters(outer[i], a.outer, own[i]);
+        parameters(scale[i], a.scale, own[i]);
+#pragma unroll
+        for (int e = 0; e < W; ++e) scale[i][e] *= a.factor;
+    }
     for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
         const int64_t row = base + sub;
         const bool on = row < a.rows;
-        f4 b[IT], g[IT];
-        float sum = 0;
+        float b[IT][W], r[IT][W], z[IT][W], sum = 0;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int c = (i * LANES + lane) * 4, left = on ? a.channels - c : 0;
-            b[i] = g[i] = f4{};
-            if (left > 0) {
-                b[i] = __builtin_convertvector(load_four((const T*)a.in + row * a.in_stride + c, left), f4);
-                if (a.residual) g[i] = __builtin_convertvector(load_four((const R*)a.residual + row * a.residual_stride + c, left), f4);
-            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum = fmaf(b[i][e], b[i][e], sum);
+            for (int e = 0; e < W; ++e) b[i][e] = r[i][e] = z[i][e] = 0;
+            if (on && own[i].hi > 0) {
+                read(b[i], (const T*)a.in + row * a.in_stride, own[i]);
+                if (a.activation != GATE_NONE) read(z[i], (const T*)a.gate + row * a.gate_stride, own[i]);
+                if (a.residual) read(r[i], (const R*)a.residual + row * a.residual_stride, own[i]);
+            }
         }
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int e = 0; e < W; ++e) sum = fmaf(b[i][e], b[i][e], sum);
         float r1 = 1.f;
         if (a.inner) r1 = 1.f / sqrtf(sum_row<LANES>(sum, shared) * inv + a.eps);
         sum = 0;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int c = (i * LANES + lane) * 4, left = on ? a.channels - c : 0;
-            if (left <= 0) continue;
-            const f4 inner = parameters(a.inner, c, left), scale = parameters(a.scale, c, left) * a.factor;
-            typename Four<T>::Vec z = {};
-            if (a.activation != GATE_NONE) z = load_four((const T*)a.gate + row * a.gate_stride + c, left);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float v = b[i][e] * r1 * inner[e];
-                if (a.activation != GATE_NONE) v *= gate_of<T>(a.activation, (float)z[e]).value;
-                b[i][e] = fmaf(scale[e], v, g[i][e]);
+            for (int e = 0; e < W; ++e) {
+                float v = b[i][e] * r1 * inner[i][e];
+                if (a.activation != GATE_NONE) v *= gate_of<T>(a.activation, z[i][e]).value;
+                b[i][e] = fmaf(scale[i][e], v, r[i][e]);
                 sum = fmaf(b[i][e], b[i][e], sum);
             }
-            if (a.total) store_four((R*)a.total + row * a.channels + c, b[i], left);
+            if (a.total && on && own[i].hi > 0) write((R*)a.total + row * a.channels, b[i], own[i]);
         }
         float r2 = 1.f;
         if (a.outer) {
             r2 = 1.f / sqrtf(sum_row<LANES>(sum, shared) * inv + a.eps);
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
-                const int c = (i * LANES + lane) * 4, left = on ? a.channels - c : 0;
-                if (left > 0) store_four((T*)a.out + row * a.channels + c, b[i] * r2 * parameters(a.outer, c, left), left);
+#pragma unroll
+                for (int e = 0; e < W; ++e) b[i][e] = b[i][e] * r2 * outer[i][e];
+                if (on && own[i].hi > 0) write((T*)a.out + row * a.channels, b[i], own[i]);
             }
         }
         if (a.stats && lane == 0 && on) {
@@ -118,111 +187,155 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void residual_fwd_kernel
     }
 }
 
+// One workgroup's part of a parameter's gradient: the sums of its rows' threads, into parts[workgroup][channels].
+template <int LANES, int IT, int W>
+__device__ __forceinline__ void write_part(float* part, const float (&x)[IT][W], const Own (&own)[IT], int channels, float* shared) {
+    if (!part) return;
+    part += (int64_t)blockIdx.x * channels;
+    if (rows_of<LANES>() == 1) {
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+            if (own[i].hi > 0) write(part, x[i], own[i]);
+        return;
+    }
+    constexpr int kRows = rows_of<LANES>(), kWidth = LANES * IT * W;
+    const int sub = threadIdx.x / LANES;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+            if (e >= own[i].lo && e < own[i].hi) shared[sub * kWidth + own[i].from + e] = x[i][e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < channels; c += 256) {
+        float sum = 0;
+        for (int s = 0; s < kRows; ++s) sum += shared[s * kWidth + c];
+        part[c] = sum;
+    }
+}
+
 template <typename T, typename R, int LANES, int IT>
-__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void residual_bwd_kernel(ResidualArgs a) {
-    constexpr int kThreads = LANES < 256 ? 256 : LANES, kRows = kThreads / LANES;
-    __shared__ float shared[16];
+__global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel(ResidualArgs a) {
+    constexpr int W = Elements<T>::kVec, kRows = rows_of<LANES>();
+    __shared__ float shared[kRows > 1 ? 256 * IT * W : 16];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const float inv = 1.f / (float)a.channels;
-    f4 dinner[IT], douter[IT], dscale[IT];
+    const bool outwards = a.outer && a.grad_out;
+    Own own[IT];
+    float inner[IT][W], outer[IT][W], scale[IT][W], dinner[IT][W], douter[IT][W], dscale[IT][W];
 #pragma unroll
-    for (int i = 0; i < IT; ++i) dinner[i] = douter[i] = dscale[i] = f4{};
+    for (int i = 0; i < IT; ++i) {
+        own[i] = own_of<W>((i * LANES + lane) * W, a.channels);
+        parameters(inner[i], a.inner, own[i]);
+        parameters(outer[i], a.outer, own[i]);
+        parameters(scale[i], a.scale, own[i]);
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+            scale[i][e] *= a.factor;
+            dinner[i][e] = douter[i][e] = dscale[i][e] = 0;
+        }
+    }
     for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
         const int64_t row = base + sub;
         const bool on = row < a.rows;
-        const float r1 = on ? a.stats[2 * row] : 0.f, r2 = on ? a.stats[2 * row + 1] : 0.f;
-        f4 u[IT], hat[IT], dt[IT];
-        typename Four<T>::Vec z[IT];
-        float sum = 0;
+        float u[IT][W], z[IT][W], hat[IT][W], dt[IT][W], dy[IT][W], r1 = 0, r2 = 0, sum = 0;
+        if (on) {
+            r1 = a.stats[2 * row];
+            r2 = a.stats[2 * row + 1];
+        }
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int c = (i * LANES + lane) * 4, left = on ? a.channels - c : 0;
-            u[i] = hat[i] = dt[i] = f4{};
-            z[i] = {};
-            if (left <= 0) continue;
-            u[i] = __builtin_convertvector(load_four((const T*)a.in + row * a.in_stride + c, left), f4) * r1;
-            if (a.activation != GATE_NONE) z[i] = load_four((const T*)a.gate + row * a.gate_stride + c, left);
-            if (a.grad_total) dt[i] = __builtin_convertvector(load_four((const R*)a.grad_total + row * a.grad_total_stride + c, left), f4);
-            if (a.outer && a.grad_out) {
-                f4 total = {};
-                if (a.residual) total = __builtin_convertvector(load_four((const R*)a.residual + row * a.residual_stride + c, left), f4);
-                const f4 dy = __builtin_convertvector(load_four((const T*)a.grad_out + row * a.grad_out_stride + c, left), f4);
-                const f4 inner = parameters(a.inner, c, left), scale = parameters(a.scale, c, left) * a.factor, outer = parameters(a.outer, c, left);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = u[i][e] * inner[e];
-                    if (a.activation != GATE_NONE) v *= gate_of<T>(a.activation, (float)z[i][e]).value;
-                    hat[i][e] = fmaf(scale[e], v, total[e]) * r2;
-                    douter[i][e] = fmaf(dy[e], hat[i][e], douter[i][e]);
-                    const float d = dy[e] * outer[e];
-                    sum = fmaf(d, hat[i][e], sum);
-                    dt[i][e] = fmaf(r2, d, dt[i][e]);
+            for (int e = 0; e < W; ++e) u[i][e] = z[i][e] = hat[i][e] = dt[i][e] = dy[i][e] = 0;
+            if (on && own[i].hi > 0) {
+                read(u[i], (const T*)a.in + row * a.in_stride, own[i]);
+                if (a.activation != GATE_NONE) read(z[i], (const T*)a.gate + row * a.gate_stride, own[i]);
+                if (a.grad_total) read(dt[i], (const R*)a.grad_total + row * a.grad_total_stride, own[i]);
+                if (outwards) {
+                    if (a.residual) read(hat[i], (const R*)a.residual + row * a.residual_stride, own[i]);
+                    read(dy[i], (const T*)a.grad_out + row * a.grad_out_stride, own[i]);
                 }
             }
         }
-        if (a.outer && a.grad_out) {
+        Gate gate[IT][W];
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                u[i][e] *= r1;
+                gate[i][e] = {1.f, 0.f};
+                if (a.activation != GATE_NONE) gate[i][e] = gate_of<T>(a.activation, z[i][e]);
+            }
+        if (outwards) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i)
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    hat[i][e] = fmaf(scale[i][e], u[i][e] * inner[i][e] * gate[i][e].value, hat[i][e]) * r2;
+                    douter[i][e] = fmaf(dy[i][e], hat[i][e], douter[i][e]);
+                    const float d = dy[i][e] * outer[i][e];
+                    sum = fmaf(d, hat[i][e], sum);
+                    dt[i][e] = fmaf(r2, d, dt[i][e]);
+                }
             const float m = sum_row<LANES>(sum, shared) * inv * r2;
 #pragma unroll
             for (int i = 0; i < IT; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) dt[i][e] = fmaf(-m, hat[i][e], dt[i][e]);
+                for (int e = 0; e < W; ++e) dt[i][e] = fmaf(-m, hat[i][e], dt[i][e]);
         }
         sum = 0;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int c = (i * LANES + lane) * 4, left = on ? a.channels - c : 0;
-            if (left <= 0) continue;
-            if (a.grad_residual) store_four((R*)a.grad_residual + row * a.channels + c, dt[i], left);
-            const f4 inner = parameters(a.inner, c, left), scale = parameters(a.scale, c, left) * a.factor;
-            f4 dz;
+            const bool here = on && own[i].hi > 0;
+            if (a.grad_residual && here) write((R*)a.grad_residual + row * a.channels, dt[i], own[i]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float n = u[i][e] * inner[e];
-                Gate gate = {1.f, 0.f};
-                if (a.activation != GATE_NONE) gate = gate_of<T>(a.activation, (float)z[i][e]);
-                dscale[i][e] = fmaf(dt[i][e], gate.value * n, dscale[i][e]);      // (times the factor, in the end)
-                const float db = dt[i][e] * scale[e];
-                dz[e] = db * n * gate.slope;
-                const float d = db * gate.value;
+            for (int e = 0; e < W; ++e) {
+                const float n = u[i][e] * inner[i][e], db = dt[i][e] * scale[i][e], d = db * gate[i][e].value;
+                dscale[i][e] = fmaf(dt[i][e], gate[i][e].value * n, dscale[i][e]);          // (times the factor, in the end)
                 dinner[i][e] = fmaf(d, u[i][e], dinner[i][e]);
-                dt[i][e] = d * inner[e];
+                z[i][e] = db * n * gate[i][e].slope;
+                dt[i][e] = d * inner[i][e];
                 sum = fmaf(dt[i][e], u[i][e], sum);
             }
-            if (a.grad_gate) store_four((T*)a.grad_gate + row * a.channels + c, dz, left);
+            if (a.grad_gate && here) write((T*)a.grad_gate + row * a.channels, z[i], own[i]);
         }
         float m = 0;
         if (a.inner) m = sum_row<LANES>(sum, shared) * inv;
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
-            const int c = (i * LANES + lane) * 4, left = on ? a.channels - c : 0;
-            if (left > 0 && a.grad_in) store_four((T*)a.grad_in + row * a.channels + c, (dt[i] - u[i] * m) * r1, left);
+#pragma unroll
+            for (int e = 0; e < W; ++e) dt[i][e] = (dt[i][e] - u[i][e] * m) * r1;
+            if (a.grad_in && on && own[i].hi > 0) write((T*)a.grad_in + row * a.channels, dt[i], own[i]);
         }
     }
-    // this workgroup's rows: [slot][channels]
-    const int64_t slot = (int64_t)blockIdx.x * kRows + sub;
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-        const int c = (i * LANES + lane) * 4, left = a.channels - c;
-        if (left <= 0) continue;
-        if (a.part_inner) store_four(a.part_inner + slot * a.channels + c, dinner[i], left);
-        if (a.part_outer) store_four(a.part_outer + slot * a.channels + c, douter[i], left);
-        if (a.part_scale) store_four(a.part_scale + slot * a.channels + c, dscale[i] * a.factor, left);
-    }
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int e = 0; e < W; ++e) dscale[i][e] *= a.factor;
+    write_part<LANES>(a.part_inner, dinner, own, a.channels, shared);
+    write_part<LANES>(a.part_outer, douter, own, a.channels, shared);
+    write_part<LANES>(a.part_scale, dscale, own, a.channels, shared);
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 constexpr int64_t kMostChannels = 16384;
 
+// Threads of a row and accesses of a thread: eight channels a thread as long as a workgroup has threads for that (sixteen beyond; four of
+// short float32 rows, which leaves fewer threads without channels).
 struct Shape { int lanes, its, rows; int64_t fwd_blocks, bwd_blocks; };     // rows: of a workgroup at a time
-Shape shape_of(int64_t rows, int64_t channels) {
-    const int64_t quads = (channels + 3) / 4;
+Shape shape_of(int64_t rows, int64_t channels, int dtype) {
+    const int w = dtype == SLAYER_FLOAT32 ? 4 : 8;
+    const int64_t all = (channels + w - 1) / w;
     Shape s;
-    s.lanes = quads <= 8 ? 8 : quads <= 16 ? 16 : quads <= 32 ? 32 : quads <= 256 ? 64 : quads <= 1024 ? 256 : 1024;
-    s.its = quads <= s.lanes ? 1 : quads <= 2 * s.lanes ? 2 : 4;
-    s.rows = s.lanes < 256 ? 256 / s.lanes : 1;
-    const int64_t all = (rows + s.rows - 1) / s.rows;
-    s.fwd_blocks = all < 4096 ? all : 4096;
-    s.bwd_blocks = all < 512 ? all : 512;
+    s.its = all <= 64 || w == 8 ? 1 : 2;
+    s.lanes = 8;
+    while (s.lanes < 1024 && s.lanes * s.its < all) s.lanes *= 2;
+    if (s.lanes * s.its < all) s.its *= 2;
+    s.rows = s.lanes <= 64 ? 256 / s.lanes : 1;
+    const int64_t groups = (rows + s.rows - 1) / s.rows;
+    const int64_t fwd = s.lanes <= 64 ? 2048 : 524288 / s.lanes, bwd = s.lanes <= 64 ? 1024 : 262144 / s.lanes;
+    s.fwd_blocks = groups < fwd ? groups : fwd;
+    s.bwd_blocks = groups < bwd ? groups : bwd;
     return s;
 }
 
@@ -245,28 +358,30 @@ ResidualArgs args_of(const slayer_residual_norm* p) {
     return a;
 }
 
-#define BY_SHAPE(T, R, LAUNCH)                                       \
-    switch (s.lanes) {                                               \
-        case 8: LAUNCH(T, R, 8, 1); break;                           \
-        case 16: LAUNCH(T, R, 16, 1); break;                         \
-        case 32: LAUNCH(T, R, 32, 1); break;                         \
-        case 64:                                                     \
-            if (s.its == 1) LAUNCH(T, R, 64, 1);                     \
-            else if (s.its == 2) LAUNCH(T, R, 64, 2);                \
-            else LAUNCH(T, R, 64, 4);                                \
-            break;                                                   \
-        case 256:                                                    \
-            if (s.its == 2) LAUNCH(T, R, 256, 2);                    \
-            else LAUNCH(T, R, 256, 4);                               \
-            break;                                                   \
-        default:                                                     \
-            if (s.its == 2) LAUNCH(T, R, 1024, 2);                   \
-            else LAUNCH(T, R, 1024, 4);                              \
+// The shapes there are: eight to 64 threads with one access, then with eight channels a thread, then with sixteen.
+#define SHORT(T, R, LAUNCH)                          \
+    if (s.lanes == 8) LAUNCH(T, R, 8, 1);            \
+    else if (s.lanes == 16) LAUNCH(T, R, 16, 1);     \
+    else if (s.lanes == 32) LAUNCH(T, R, 32, 1);     \
+    else LAUNCH(T, R, 64, 1)
+#define LONG(T, R, IT, LAUNCH)                       \
+    if (s.lanes == 64) LAUNCH(T, R, 64, IT);         \
+    else if (s.lanes == 128) LAUNCH(T, R, 128, IT);  \
+    else if (s.lanes == 256) LAUNCH(T, R, 256, IT);  \
+    else if (s.lanes == 512) LAUNCH(T, R, 512, IT);  \
+    else if (s.its == IT) LAUNCH(T, R, 1024, IT);    \
+    else LAUNCH(T, R, 1024, 2 * IT)
+#define BY_TYPE(LAUNCH)                                                          \
+    if (p->dtype == SLAYER_FLOAT32) {                                            \
+        if (s.its == 1) { SHORT(float, float, LAUNCH); }                         \
+        else { LONG(float, float, 2, LAUNCH); }                                  \
+    } else if (p->residual_dtype == SLAYER_FLOAT32) {                            \
+        if (s.lanes <= 64) { SHORT(bf16, float, LAUNCH); }                       \
+        else { LONG(bf16, float, 1, LAUNCH); }                                   \
+    } else {                                                                     \
+        if (s.lanes <= 64) { SHORT(bf16, bf16, LAUNCH); }                        \
+        else { LONG(bf16, bf16, 1, LAUNCH); }                                    \
     }
-#define BY_TYPE(LAUNCH)                                              \
-    if (p->dtype == SLAYER_FLOAT32) BY_SHAPE(float, float, LAUNCH)   \
-    else if (p->residual_dtype == SLAYER_FLOAT32) BY_SHAPE(bf16, float, LAUNCH) \
-    else BY_SHAPE(bf16, bf16, LAUNCH)
 
 }  // namespace
 }  // namespace slayer
@@ -275,8 +390,8 @@ using namespace slayer;
 
 extern "C" int64_t slayer_residual_norm_workspace(const slayer_residual_norm* p) {
     if (int e = check_residual(p)) return e;
-    const Shape s = shape_of(p->rows, p->channels);
-    return 3 * s.bwd_blocks * s.rows * p->channels;
+    const Shape s = shape_of(p->rows, p->channels, p->dtype);
+    return 3 * s.bwd_blocks * p->channels;
 }
 
 extern "C" int slayer_residual_norm_fwd(void* out, void* total, float* stats, const void* input, const void* residual, const void* gate,
@@ -287,9 +402,9 @@ extern "C" int slayer_residual_norm_fwd(void* out, void* total, float* stats, co
         return SLAYER_ENULL;
     ResidualArgs a = args_of(p);
     a.out = out; a.total = total; a.stats = stats; a.in = input; a.residual = residual; a.gate = gate;
-    const Shape s = shape_of(p->rows, p->channels);
+    const Shape s = shape_of(p->rows, p->channels, p->dtype);
 #define LAUNCH(T, R, LANES, IT) \
-    hipLaunchKernelGGL((residual_fwd_kernel<T, R, LANES, IT>), dim3((unsigned)s.fwd_blocks), dim3(LANES < 256 ? 256 : LANES), 0, \
+    hipLaunchKernelGGL((residual_fwd_kernel<T, R, LANES, IT>), dim3((unsigned)s.fwd_blocks), dim3(LANES <= 64 ? 256 : LANES), 0, \
                        (hipStream_t)stream, a)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
@@ -319,13 +434,13 @@ extern "C" int slayer_residual_norm_bwd(void* grad_input, void* grad_residual, v
     ResidualArgs a = args_of(p);
     a.grad_in = grad_input; a.grad_residual = grad_residual; a.grad_gate = grad_gate; a.grad_out = grad_out; a.grad_total = grad_total;
     a.stats = (float*)stats; a.in = input; a.residual = residual; a.gate = gate;
-    const Shape s = shape_of(p->rows, p->channels);
-    const int64_t slots = s.bwd_blocks * s.rows, size = slots * p->channels;
+    const Shape s = shape_of(p->rows, p->channels, p->dtype);
+    const int64_t size = s.bwd_blocks * p->channels;
     a.part_inner = grad_inner ? workspace : nullptr;
     a.part_outer = grad_outer ? workspace + size : nullptr;
     a.part_scale = grad_scale ? workspace + 2 * size : nullptr;
 #define LAUNCH(T, R, LANES, IT) \
-    hipLaunchKernelGGL((residual_bwd_kernel<T, R, LANES, IT>), dim3((unsigned)s.bwd_blocks), dim3(LANES < 256 ? 256 : LANES), 0, \
+    hipLaunchKernelGGL((residual_bwd_kernel<T, R, LANES, IT>), dim3((unsigned)s.bwd_blocks), dim3(LANES <= 64 ? 256 : LANES), 0, \
                        (hipStream_t)stream, a)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
@@ -337,6 +452,6 @@ extern "C" int slayer_residual_norm_bwd(void* grad_input, void* grad_residual, v
             c.out[count] = wanted[i];
             c.parts[count++] = workspace + i * size;
         }
-    c.rows = slots; c.columns = c.pitch = p->channels; c.factor = 1.f;
+    c.rows = s.bwd_blocks; c.columns = c.pitch = p->channels; c.factor = 1.f;
     return launch_column_sums(c, count, (hipStream_t)stream);
 }
