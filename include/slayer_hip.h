@@ -742,7 +742,7 @@ typedef struct slayer_rotary_call {
 int slayer_rotary(void *out_query, void *out_key, const void *query, const void *key, const slayer_rotary_call *r, int inverse,
                   void *stream);
 
-/* A norm behind a block and one in front of the next with the block's gate and residual scale, on rows of `channels` (up to 16384):
+/* A norm behind a block and one in front of the next with the block's gate and residual scale, on rows of `channels` (up to 8192):
  *     total = residual + factor * scale * act(gate) * inner * input / rms(input),   out = outer * total / rms(total),
  * rms(v) = sqrt(mean(v^2) + eps).  A parameter that is NULL: no scale; no norm of input (inner); no out (outer; out has to be NULL).
  * residual NULL: 0.  Rows have strides (in elements) and neighbouring elements; the outputs are contiguous. */

@@ -109,13 +109,10 @@ template <typename T, int W> __device__ __forceinline__ void write(T* row, const
             if (e >= own.lo && e < own.hi) row[own.from + e] = (T)x[e];
     }
 }
-template <int W> __device__ __forceinline__ void parameters(float (&x)[W], const float* p, const Own& own) {
-    if (p) {
-        read(x, p, own);
-    } else {
+template <int W> __device__ __forceinline__ void parameters(float (&x)[W], const float* p, const Own& own, float factor = 1.f) {
+    if (p) read(x, p, own);
 #pragma unroll
-        for (int e = 0; e < W; ++e) x[e] = 1.f;
-    }
+    for (int e = 0; e < W; ++e) x[e] = p ? x[e] * factor : factor;
 }
 
 // T: x, gate and y.  R: the residual stream.  LANES threads a row, IT accesses of 16 bytes of x each.  The loop over the rows is the same for
@@ -134,9 +131,7 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_fwd_kernel
         own[i] = own_of<W>((i * LANES + lane) * W, a.channels);
         parameters(inner[i], a.inner, own[i]);
         parameters(outer[i], a.outer, own[i]);
-        parameters(scale[i], a.scale, own[i]);
-#pragma unroll
-        for (int e = 0; e < W; ++e) scale[i][e] *= a.factor;
+        parameters(scale[i], a.scale, own[i], a.factor);
     }
     for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
         const int64_t row = base + sub;
@@ -217,6 +212,7 @@ __device__ __forceinline__ void write_part(float* part, const float (&x)[IT][W],
 template <typename T, typename R, int LANES, int IT>
 __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel(ResidualArgs a) {
     constexpr int W = Elements<T>::kVec, kRows = rows_of<LANES>();
+    constexpr bool kAgain = LANES == 1024;     // parameters are read for every row: of 128 registers there are none to keep them in
     __shared__ float shared[kRows > 1 ? 256 * IT * W : 16];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const float inv = 1.f / (float)a.channels;
@@ -226,14 +222,13 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         own[i] = own_of<W>((i * LANES + lane) * W, a.channels);
-        parameters(inner[i], a.inner, own[i]);
-        parameters(outer[i], a.outer, own[i]);
-        parameters(scale[i], a.scale, own[i]);
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-            scale[i][e] *= a.factor;
-            dinner[i][e] = douter[i][e] = dscale[i][e] = 0;
+        if (!kAgain) {
+            parameters(inner[i], a.inner, own[i]);
+            parameters(outer[i], a.outer, own[i]);
+            parameters(scale[i], a.scale, own[i], a.factor);
         }
+#pragma unroll
+        for (int e = 0; e < W; ++e) dinner[i][e] = douter[i][e] = dscale[i][e] = 0;
     }
     for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.rows; base += (int64_t)gridDim.x * kRows) {
         const int64_t row = base + sub;
@@ -268,7 +263,12 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel
             }
         if (outwards) {
 #pragma unroll
-            for (int i = 0; i < IT; ++i)
+            for (int i = 0; i < IT; ++i) {
+                if (kAgain) {
+                    parameters(inner[i], a.inner, own[i]);
+                    parameters(outer[i], a.outer, own[i]);
+                    parameters(scale[i], a.scale, own[i], a.factor);
+                }
 #pragma unroll
                 for (int e = 0; e < W; ++e) {
                     hat[i][e] = fmaf(scale[i][e], u[i][e] * inner[i][e] * gate[i][e].value, hat[i][e]) * r2;
@@ -277,6 +277,7 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel
                     sum = fmaf(d, hat[i][e], sum);
                     dt[i][e] = fmaf(r2, d, dt[i][e]);
                 }
+            }
             const float m = sum_row<LANES>(sum, shared) * inv * r2;
 #pragma unroll
             for (int i = 0; i < IT; ++i)
@@ -288,6 +289,10 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel
         for (int i = 0; i < IT; ++i) {
             const bool here = on && own[i].hi > 0;
             if (a.grad_residual && here) write((R*)a.grad_residual + row * a.channels, dt[i], own[i]);
+            if (kAgain) {
+                parameters(inner[i], a.inner, own[i]);
+                parameters(scale[i], a.scale, own[i], a.factor);
+            }
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 const float n = u[i][e] * inner[i][e], db = dt[i][e] * scale[i][e], d = db * gate[i][e].value;
@@ -318,10 +323,9 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------
-constexpr int64_t kMostChannels = 16384;
+constexpr int64_t kMostChannels = 8192;
 
-// Threads of a row and accesses of a thread: eight channels a thread as long as a workgroup has threads for that (sixteen beyond; four of
-// short float32 rows, which leaves fewer threads without channels).
+// Threads of a row and accesses of a thread: eight channels a thread, four of short float32 rows, which leaves fewer threads idle.
 struct Shape { int lanes, its, rows; int64_t fwd_blocks, bwd_blocks; };     // rows: of a workgroup at a time
 Shape shape_of(int64_t rows, int64_t channels, int dtype) {
     const int w = dtype == SLAYER_FLOAT32 ? 4 : 8;
@@ -330,10 +334,11 @@ Shape shape_of(int64_t rows, int64_t channels, int dtype) {
     s.its = all <= 64 || w == 8 ? 1 : 2;
     s.lanes = 8;
     while (s.lanes < 1024 && s.lanes * s.its < all) s.lanes *= 2;
-    if (s.lanes * s.its < all) s.its *= 2;
     s.rows = s.lanes <= 64 ? 256 / s.lanes : 1;
     const int64_t groups = (rows + s.rows - 1) / s.rows;
-    const int64_t fwd = s.lanes <= 64 ? 2048 : 524288 / s.lanes, bwd = s.lanes <= 64 ? 1024 : 262144 / s.lanes;
+    // as many workgroups as run at a time; of the backward kernel, which leaves a part of each sum for every one of them, twelve waves a
+    // compute unit
+    const int64_t fwd = s.lanes <= 64 ? 2048 : 524288 / s.lanes, bwd = s.lanes <= 64 ? 768 : s.lanes < 512 ? 196608 / s.lanes : 256;
     s.fwd_blocks = groups < fwd ? groups : fwd;
     s.bwd_blocks = groups < bwd ? groups : bwd;
     return s;
@@ -358,7 +363,7 @@ ResidualArgs args_of(const slayer_residual_norm* p) {
     return a;
 }
 
-// The shapes there are: eight to 64 threads with one access, then with eight channels a thread, then with sixteen.
+// The shapes there are: eight to 64 threads with one access, then with eight channels a thread.
 #define SHORT(T, R, LAUNCH)                          \
     if (s.lanes == 8) LAUNCH(T, R, 8, 1);            \
     else if (s.lanes == 16) LAUNCH(T, R, 16, 1);     \
@@ -369,8 +374,7 @@ ResidualArgs args_of(const slayer_residual_norm* p) {
     else if (s.lanes == 128) LAUNCH(T, R, 128, IT);  \
     else if (s.lanes == 256) LAUNCH(T, R, 256, IT);  \
     else if (s.lanes == 512) LAUNCH(T, R, 512, IT);  \
-    else if (s.its == IT) LAUNCH(T, R, 1024, IT);    \
-    else LAUNCH(T, R, 1024, 2 * IT)
+    else LAUNCH(T, R, 1024, IT)
 #define BY_TYPE(LAUNCH)                                                          \
     if (p->dtype == SLAYER_FLOAT32) {                                            \
         if (s.its == 1) { SHORT(float, float, LAUNCH); }                         \

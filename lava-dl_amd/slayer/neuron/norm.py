@@ -244,7 +244,7 @@ def residual_norm(input, residual, weight=None, inner=None, gate=None, scale=Non
     Parameters
     ----------
     input : torch.Tensor
-        float32 or bfloat16 GPU tensor [..., C], C at most 16384.  Rows that lie a fixed distance from each other (a part of a
+        float32 or bfloat16 GPU tensor [..., C], C at most 8192.  Rows that lie a fixed distance from each other (a part of a
         projection) are read where they lie, others are copied first; so for residual and gate.
     residual : torch.Tensor or None
         of the same shape and type, or float32 (a stream that is kept in float32 between bfloat16 blocks); None: 0.
@@ -273,8 +273,8 @@ def residual_norm(input, residual, weight=None, inner=None, gate=None, scale=Non
     if not eps >= 0:
         raise ValueError(f'eps has to be at least 0, got {eps}')
     device, _ = N.require_elements(input) if gate is None else N.require_elements(input, gate)
-    if input.dim() < 1 or not 1 <= input.shape[-1] <= 16384:
-        raise RuntimeError(f'expected a tensor [..., C] with C up to 16384, got {tuple(input.shape)}')
+    if input.dim() < 1 or not 1 <= input.shape[-1] <= 8192:
+        raise RuntimeError(f'expected a tensor [..., C] with C up to 8192, got {tuple(input.shape)}')
     if gate is not None and gate.shape != input.shape:
         raise RuntimeError(f'gate: expected the shape {tuple(input.shape)}, got {tuple(gate.shape)}')
     if residual is not None:
