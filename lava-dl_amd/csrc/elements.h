@@ -63,11 +63,15 @@ __device__ __forceinline__ void store_vec(T* p, typename Elements<T>::Vec v, int
     }
 }
 
-// Four neighbouring elements at any address that suits one of them: the hardware takes wide accesses that are not aligned.
+// Neighbouring elements at any address that suits one of them: the hardware takes wide accesses that are not aligned.
 // `n`: how many of them exist (the others read as 0 and are not written).
 typedef f4 f4_any __attribute__((aligned(4)));
 typedef b4 b4_any __attribute__((aligned(2)));
 template <typename T> struct Four;
+template <typename T> struct Wide;             // as many as 16 bytes hold
+typedef b8 b8_any __attribute__((aligned(2)));
+template <> struct Wide<float> { typedef f4_any Any; };
+template <> struct Wide<bf16> { typedef b8_any Any; };
 template <> struct Four<float> { typedef f4 Vec; typedef f4_any Any; };
 template <> struct Four<bf16> { typedef b4 Vec; typedef b4_any Any; };
 template <typename T> __device__ __forceinline__ typename Four<T>::Vec load_four(const T* p, int n) {

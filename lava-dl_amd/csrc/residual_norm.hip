@@ -76,7 +76,6 @@ template <int W> __device__ __forceinline__ Own own_of(int c, int channels) {
     return {from, c - from, channels - from < W ? channels - from : W};
 }
 typedef f8 f8_any __attribute__((aligned(4)));
-typedef b8 b8_any __attribute__((aligned(2)));
 __device__ __forceinline__ void read_all(float (&x)[4], const float* p) { to_floats(x, *reinterpret_cast<const f4_any*>(p)); }
 __device__ __forceinline__ void read_all(float (&x)[8], const bf16* p) { to_floats(x, *reinterpret_cast<const b8_any*>(p)); }
 __device__ __forceinline__ void read_all(float (&x)[8], const float* p) {

@@ -12,6 +12,7 @@ namespace slayer {
 namespace {
 
 constexpr int kAngles = 2048;                  // pairs of all tokens of a workgroup: 16 KB of LDS
+constexpr int kSpan = 16;                      // most tokens of a workgroup
 constexpr int kMostFeatures = 4096;            // of a head
 
 struct RotaryArgs {
@@ -24,7 +25,8 @@ struct RotaryArgs {
     int64_t in_stride[2][3];
     int heads[2];
     int features, pairs, position_bytes, each, span;          // span: tokens of a workgroup
-    int units, rest;                           // accesses of a head: four pairs each, then four of the features that are copied
+    int units, rest;                           // accesses of a head: of W pairs each, then of W of the features that are copied
+    int step_unit, step_head, step_token;      // 256 accesses on
     float magnitude, sign;
 };
 
@@ -35,60 +37,133 @@ __device__ __forceinline__ int64_t position_of(const RotaryArgs& a, int64_t n, i
     return a.each ? p : p + t;
 }
 
+// Where an access lies: the head's features, the first pair (-1: features that are copied), the first feature of either half.
+template <typename T> struct Place {
+    const T* in;
+    T* out;
+    int pair, at[2];
+    bool wide;                                 // W of them; otherwise all there are, one by one
+};
+template <typename T, bool HALVES>
+__device__ __forceinline__ Place<T> place_of(const RotaryArgs& a, const int64_t (*in_at)[kSpan], const int64_t (*out_at)[kSpan], int token,
+                                             int head, int unit) {
+    constexpr int W = Elements<T>::kVec;
+    const bool key = head >= a.heads[0];
+    const int h = key ? head - a.heads[0] : head;
+    Place<T> p;
+    p.in = (const T*)(key ? a.in[1] : a.in[0]) + in_at[key][token] + h * (key ? a.in_stride[1][2] : a.in_stride[0][2]);
+    p.out = (T*)(key ? a.out[1] : a.out[0]) + out_at[key][token] + (int64_t)h * a.features;
+    if (unit < a.units) {
+        p.wide = a.pairs >= W;
+        p.pair = !p.wide ? 0 : unit * W < a.pairs - W ? unit * W : a.pairs - W;
+        p.at[0] = HALVES ? p.pair : 2 * p.pair;
+        p.at[1] = HALVES ? a.pairs + p.pair : 2 * p.pair + W;
+    } else {
+        const int at = 2 * a.pairs + (unit - a.units) * W;
+        p.wide = a.features - 2 * a.pairs >= W;
+        p.pair = -1;
+        p.at[0] = at < a.features - W ? at : a.features - W;
+        p.at[1] = 0;
+    }
+    return p;
+}
+
+// Angles of a workgroup's tokens, then its accesses: for each token and head the pairs, W at a time, and what is copied.  The last access of
+// either, where there are W, ends with the last feature and so may do some of the one before it again, with the same values: no access is
+// cut.  The angles are being made while the first features are on their way.
 template <typename T, bool HALVES>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
-    __shared__ float cosines[kAngles], sines[kAngles];
+    constexpr int W = Elements<T>::kVec;
+    typedef typename Wide<T>::Any Any;
+    typedef typename Elements<T>::Vec Vec;
+    __shared__ __align__(16) float cosines[kAngles + W], sines[kAngles + W];
+    __shared__ double positions[kSpan];
+    __shared__ int64_t in_at[2][kSpan], out_at[2][kSpan];
     const int64_t first = (int64_t)blockIdx.x * a.span;
     const int count = a.all - first < a.span ? (int)(a.all - first) : a.span;
+    if (threadIdx.x < count) {
+        const int64_t at = first + threadIdx.x, n = at / a.tokens, t = at - n * a.tokens;
+        positions[threadIdx.x] = (double)position_of(a, n, t);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            in_at[w][threadIdx.x] = n * a.in_stride[w][0] + t * a.in_stride[w][1];
+            out_at[w][threadIdx.x] = at * a.heads[w] * a.features;
+        }
+    }
+    __syncthreads();
+    const int heads = a.heads[0] + a.heads[1], per = a.units + a.rest;
+    int unit = threadIdx.x % per, head = threadIdx.x / per % heads, token = threadIdx.x / (per * heads);
+    Place<T> place = {};
+    Vec x = {}, y = {};
+    if (token < count) {
+        place = place_of<T, HALVES>(a, in_at, out_at, token, head, unit);
+        if (place.wide) {
+            x = *reinterpret_cast<const Any*>(place.in + place.at[0]);
+            if (place.pair >= 0) y = *reinterpret_cast<const Any*>(place.in + place.at[1]);
+        }
+    }
     for (int i = threadIdx.x; i < count * a.pairs; i += 256) {
-        const int64_t token = first + i / a.pairs, n = token / a.tokens;
-        const double p = (double)position_of(a, n, token - n * a.tokens), f = a.frequency[i % a.pairs] * 0.15915494309189533577;
-        const double turns = p * f, rest = (turns - rint(turns)) + fma(p, f, -turns);
+        const int t = i / a.pairs;
+        const double f = a.frequency[i - t * a.pairs] * 0.15915494309189533577;
+        const double turns = positions[t] * f, rest = (turns - rint(turns)) + fma(positions[t], f, -turns);
         float s, c;
         sincospif(2.f * (float)rest, &s, &c);
         cosines[i] = a.magnitude * c;
         sines[i] = a.sign * a.magnitude * s;
     }
     __syncthreads();
-    const int heads = a.heads[0] + a.heads[1], per = a.units + a.rest, items = count * heads * per;
-    for (int item = threadIdx.x; item < items; item += 256) {
-        const int unit = item % per, row = item / per, token = row / heads;
-        int head = row % heads;
-        const int which = head >= a.heads[0];
-        head -= which ? a.heads[0] : 0;
-        const int64_t at = first + token, n = at / a.tokens;
-        const T* in = (const T*)a.in[which] + n * a.in_stride[which][0] + (at - n * a.tokens) * a.in_stride[which][1] +
-                      head * a.in_stride[which][2];
-        T* out = (T*)a.out[which] + (at * a.heads[which] + head) * a.features;
-        if (unit >= a.units) {
-            const int i = 2 * a.pairs + (unit - a.units) * 4, left = a.features - i;
-            store_four(out + i, __builtin_convertvector(load_four(in + i, left), f4), left);
-            continue;
-        }
-        const int i = unit * 4, left = a.pairs - i;
-        const float *c = cosines + token * a.pairs + i, *s = sines + token * a.pairs + i;
-        f4 x, y, u = {}, w = {};
-        if (HALVES) {
-            x = __builtin_convertvector(load_four(in + i, left), f4);
-            y = __builtin_convertvector(load_four(in + a.pairs + i, left), f4);
-        } else {
-            const f4 p = __builtin_convertvector(load_four(in + 2 * i, 2 * left), f4);
-            const f4 q = __builtin_convertvector(load_four(in + 2 * i + 4, 2 * left - 4), f4);
-            x = f4{p[0], p[2], q[0], q[2]};
-            y = f4{p[1], p[3], q[1], q[3]};
-        }
+    while (token < count) {
+        if (place.wide) {
+            if (place.pair >= 0) {
+                const float *c = cosines + token * a.pairs + place.pair, *s = sines + token * a.pairs + place.pair;
+                float u[W], v[W], p[W], q[W];
+                to_floats(u, x);
+                to_floats(v, y);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (e < left) {
-                u[e] = fmaf(c[e], x[e], -(s[e] * y[e]));
-                w[e] = fmaf(c[e], y[e], s[e] * x[e]);
+                for (int e = 0; e < W; ++e) {
+                    const float left = HALVES ? u[e] : e < W / 2 ? u[2 * e % W] : v[2 * e % W];
+                    const float right = HALVES ? v[e] : e < W / 2 ? u[2 * e % W + 1] : v[2 * e % W + 1];
+                    const float l = fmaf(c[e], left, -(s[e] * right)), r = fmaf(c[e], right, s[e] * left);
+                    if (HALVES) {
+                        p[e] = l;
+                        q[e] = r;
+                    } else {
+                        (e < W / 2 ? p : q)[2 * e % W] = l;
+                        (e < W / 2 ? p : q)[2 * e % W + 1] = r;
+                    }
+                }
+                x = from_floats(p);
+                y = from_floats(q);
+                *reinterpret_cast<Any*>(place.out + place.at[1]) = y;
             }
-        if (HALVES) {
-            store_four(out + i, u, left);
-            store_four(out + a.pairs + i, w, left);
+            *reinterpret_cast<Any*>(place.out + place.at[0]) = x;
+        } else if (place.pair >= 0) {                              // fewer pairs than W
+            const float *c = cosines + token * a.pairs, *s = sines + token * a.pairs;
+            for (int e = 0; e < a.pairs; ++e) {
+                const int i = HALVES ? e : 2 * e, j = HALVES ? a.pairs + e : 2 * e + 1;
+                const float left = (float)place.in[i], right = (float)place.in[j];
+                place.out[i] = (T)fmaf(c[e], left, -(s[e] * right));
+                place.out[j] = (T)fmaf(c[e], right, s[e] * left);
+            }
         } else {
-            store_four(out + 2 * i, f4{u[0], w[0], u[1], w[1]}, 2 * left);
-            store_four(out + 2 * i + 4, f4{u[2], w[2], u[3], w[3]}, 2 * left - 4);
+            for (int i = 2 * a.pairs; i < a.features; ++i) place.out[i] = place.in[i];
+        }
+        unit += a.step_unit;
+        head += a.step_head;
+        token += a.step_token;
+        if (unit >= per) {
+            unit -= per;
+            ++head;
+        }
+        if (head >= heads) {
+            head -= heads;
+            ++token;
+        }
+        if (token >= count) break;
+        place = place_of<T, HALVES>(a, in_at, out_at, token, head, unit);
+        if (place.wide) {
+            x = *reinterpret_cast<const Any*>(place.in + place.at[0]);
+            if (place.pair >= 0) y = *reinterpret_cast<const Any*>(place.in + place.at[1]);
         }
     }
 }
@@ -122,12 +197,17 @@ extern "C" int slayer_rotary(void* out_query, void* out_key, const void* query, 
     }
     a.heads[0] = (int)r->query_heads; a.heads[1] = (int)r->key_heads;
     a.features = (int)r->features; a.pairs = (int)r->turned / 2;
-    a.units = (a.pairs + 3) / 4;
-    a.rest = (a.features - 2 * a.pairs + 3) / 4;
+    const int w = r->dtype == SLAYER_FLOAT32 ? 4 : 8;
+    a.units = (a.pairs + w - 1) / w;
+    a.rest = (a.features - 2 * a.pairs + w - 1) / w;
+    const int per = a.units + a.rest;
+    a.step_unit = 256 % per;
+    a.step_head = 256 / per % (int)heads;
+    a.step_token = 256 / per / (int)heads;
     a.magnitude = r->magnitude; a.sign = inverse ? -1.f : 1.f;
     // tokens of a workgroup: up to sixteen, as the angles fit, fewer where that leaves compute units idle
-    int span = a.pairs > 0 ? kAngles / a.pairs : 16;
-    if (span > 16) span = 16;
+    int span = a.pairs > 0 ? kAngles / a.pairs : kSpan;
+    if (span > kSpan) span = kSpan;
     while (span > 1 && (all + span - 1) / span < 512) span /= 2;
     a.span = span;
     const int64_t blocks = (all + span - 1) / span;
