@@ -2,7 +2,7 @@
 // launch.  With c = magnitude cos(position * frequency[i]) and s = magnitude sin(position * frequency[i]) a pair (x, y) becomes
 // (c x - s y, c y + s x); the pairs are (i, i + turned / 2) or (2i, 2i + 1), features behind the first `turned` are copied.  The gradient is
 // the same call with the angle's sign changed.
-//   Angles: the whole turns are taken off in float64, with what the product's rounding leaves, so that a position of 2^31 costs no
+//   Angles: the whole turns are taken off in float64, with what the roundings of the products leave, so that a far position costs no
 // digits; sine and cosine of the rest are float32.  All heads of a token share them: a workgroup makes those of its tokens once, in LDS.
 //   Bound: memory, each tensor read and written once.
 #include "common.h"
@@ -104,8 +104,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     }
     for (int i = threadIdx.x; i < count * a.pairs; i += 256) {
         const int t = i / a.pairs;
-        const double f = a.frequency[i - t * a.pairs] * 0.15915494309189533577;
-        const double turns = positions[t] * f, rest = (turns - rint(turns)) + fma(positions[t], f, -turns);
+        constexpr double kHigh = 0x1.45f306dc9c883p-3, kLow = -0x1.6b01ec5417056p-57;           // 1 / (2 pi)
+        const double radians = a.frequency[i - t * a.pairs], f = radians * kHigh, turns = positions[t] * f;
+        const double rest = (turns - rint(turns)) + (fma(positions[t], f, -turns) + positions[t] * fma(radians, kLow, fma(radians, kHigh, -f)));
         float s, c;
         sincospif(2.f * (float)rest, &s, &c);
         cosines[i] = a.magnitude * c;
@@ -179,6 +180,7 @@ extern "C" int slayer_rotary(void* out_query, void* out_key, const void* query, 
     if (r->samples < 0 || r->tokens < 0 || r->query_heads < 0 || r->key_heads < 0 || r->features < 1) return SLAYER_EINVAL;
     if (r->turned < 0 || r->turned % 2 != 0 || r->turned > r->features) return SLAYER_EINVAL;
     if (r->dtype != SLAYER_FLOAT32 && r->dtype != SLAYER_BFLOAT16) return SLAYER_EINVAL;
+    if (r->layout != SLAYER_ROTARY_HALVES && r->layout != SLAYER_ROTARY_PAIRS) return SLAYER_EINVAL;
     if (r->position && r->position_bytes != 4 && r->position_bytes != 8) return SLAYER_EINVAL;
     if (r->features > kMostFeatures || r->query_heads > 65536 || r->key_heads > 65536) return SLAYER_ERANGE;
     if (r->tokens > kMaxT || r->samples > ((int64_t)1 << 32) || (r->tokens > 0 && r->samples > ((int64_t)1 << 32) / r->tokens)) return SLAYER_ERANGE;

@@ -1,14 +1,16 @@
-"""A token-mixing layer of the operators that belong together: leaky attention, group norm of each head's result with an
-activation, dropout from a counter, between two dense projections."""
+"""A token-mixing layer of the operators that belong together: leaky attention, of queries and keys that may be turned with their
+position, group norm of each head's result with an activation, dropout from a counter, between two dense projections."""
 import torch
 
+from .types import KeepsTypes
 from ..neuron.base import P_SCALE
 from ..neuron.dropout import CounterDropout
 from ..neuron.norm import GroupNorm
 from ..synapse.attention import leaky_attention, leaky_attention_step
+from ..synapse.rotary import rotary
 
 
-class LeakyAttention(torch.nn.Module):
+class LeakyAttention(KeepsTypes):
     """Tokens [N, T, C] to tokens [N, T, C]: query, key and value of each head from one projection, leaky attention with
     a decay for each head, the heads' results normalised, activated and thinned out, and a projection back.
 
@@ -29,12 +31,20 @@ class LeakyAttention(torch.nn.Module):
     activation : as for ``slayer.neuron.norm.group_norm``.
     seed : int or None
         of the dropout, as for ``slayer.neuron.CounterDropout``.
+    frequency : torch.Tensor or None
+        angles, in radians a token, that queries and keys are turned by (``slayer.synapse.rotary_frequencies``); None: they are not
+        turned.
+    layout, magnitude : as for ``slayer.synapse.rotary``.
 
     The projections take the type of the tokens (``.to(torch.bfloat16)`` makes them bfloat16); decays, the norm's
-    weights and the state are float32 all the same (a bfloat16 decay of 4095 would be one of 4096, which remembers nothing).
+    weights and the state are float32 all the same (a bfloat16 decay of 4095 would be one of 4096, which remembers nothing), the angles
+    float64.
     """
 
-    def __init__(self, features, heads, head_features=64, decay=None, train_decay=False, dropout=0.0, activation='silu', seed=None):
+    kept = ('norm',)
+
+    def __init__(self, features, heads, head_features=64, decay=None, train_decay=False, dropout=0.0, activation='silu', seed=None,
+                 frequency=None, layout='halves', magnitude=1.0):
         super().__init__()
         if decay is None:
             decay = [512 / 128 ** (i / max(heads - 1, 1)) for i in range(heads)]
@@ -54,34 +64,35 @@ class LeakyAttention(torch.nn.Module):
         else:
             self.register_buffer('decay', decay)
 
-    def _apply(self, fn, recurse=True):
-        """As torch's, but what is float32 stays float32 where ``fn`` changes types."""
-        def keep(t):
-            changed = fn(t)
-            return changed if changed.dtype == t.dtype else t.to(changed.device)
-
-        if recurse:
-            for child in self.children():
-                child._apply(keep if child is self.norm else fn)
-        return super()._apply(keep, recurse=False)
+        if frequency is not None and 2 * frequency.numel() > head_features:
+            raise ValueError(f'{frequency.numel()} angles do not fit heads of {head_features} features')
+        self.register_buffer('frequency', None if frequency is None else frequency.double(), persistent=False)
+        self.layout, self.magnitude = layout, magnitude
 
     def _decay(self):
         if isinstance(self.decay, torch.nn.Parameter):
             self.decay.data.clamp_(0, P_SCALE)
         return self.decay
 
-    def _heads(self, x):
-        """query, key and value, views of one tensor [..., heads, head_features]."""
-        return self.project(x).unflatten(-1, (3, self.heads, self.head_features)).unbind(-3)
+    def _heads(self, x, position):
+        """query, key and value, views of one tensor [..., heads, head_features]; queries and keys turned, if they are."""
+        if position is not None and self.frequency is None:
+            raise ValueError('positions are given, but queries and keys are not turned (frequency=None)')
+        query, key, value = self.project(x).unflatten(-1, (3, self.heads, self.head_features)).unbind(-3)
+        if self.frequency is not None:
+            query, key = rotary(query, key, self.frequency, position, self.layout, self.magnitude)
+        return query, key, value
 
     def _finish(self, y, offset=None):
         rows = y.reshape(y.shape[:-2].numel(), self.heads * self.head_features)
         return self.back(self.dropout(self.norm(rows), offset).view(*y.shape[:-2], rows.shape[1]))
 
-    def forward(self, x, state=None, lengths=None, return_state=False, offset=None):
+    def forward(self, x, state=None, lengths=None, return_state=False, offset=None, position=None):
         """``x``: [N, T, C]; ``state``, ``lengths`` and ``return_state`` as for ``slayer.synapse.leaky_attention``, ``offset`` as
-        for ``slayer.neuron.CounterDropout``."""
-        mixed = leaky_attention(*self._heads(x), self._decay(), state, lengths, self.scale, return_state)
+        for ``slayer.neuron.CounterDropout``, ``position`` as for ``slayer.synapse.rotary`` (where queries and keys are turned; with a ``state`` it has to be given)."""
+        if self.frequency is not None and state is not None and position is None:
+            raise ValueError('queries and keys are turned: a part of a sample needs the position it begins at')
+        mixed = leaky_attention(*self._heads(x, position), self._decay(), state, lengths, self.scale, return_state)
         return (self._finish(mixed[0], offset), mixed[1]) if return_state else self._finish(mixed, offset)
 
     def initial_state(self, samples):
@@ -89,6 +100,9 @@ class LeakyAttention(torch.nn.Module):
         return torch.zeros(samples, self.heads, self.head_features, self.head_features, device=self.decay.device)
 
     @torch.no_grad()
-    def step(self, x, state):
-        """One token of each sample in generation: ``x`` [N, C] to [N, C], ``state`` is updated in place."""
-        return self._finish(leaky_attention_step(*self._heads(x), self._decay(), state, self.scale))
+    def step(self, x, state, position=None):
+        """One token of each sample in generation: ``x`` [N, C] to [N, C], ``state`` is updated in place.  ``position``: the tokens'
+        positions, int32 or int64 [N], where queries and keys are turned."""
+        if self.frequency is not None and position is None:
+            raise ValueError('queries and keys are turned: a step needs the positions of its tokens')
+        return self._finish(leaky_attention_step(*self._heads(x, position), self._decay(), state, self.scale))
