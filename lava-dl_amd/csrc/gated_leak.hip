@@ -110,7 +110,7 @@ __device__ __forceinline__ int64_t length_of(const LeakArgs& a, int64_t n) {
 //   What is left is a word of 64 bits that says itself that it is there (the workspace is zeroed before), read and written with relaxed
 // atomics of the whole device: no other memory hangs on it, so no fences are needed.
 typedef unsigned long long Word;
-constexpr int kWindow = 32;                    // largest window
+constexpr int kWindow = 16;                    // largest window
 
 constexpr int kApart = 16;                     // words from one chain's ticket to the next: a cache line each
 
@@ -522,7 +522,11 @@ Plan plan_of(const slayer_gated_leak* s, bool backward) {
     p.tiles = s->tokens > 0 ? ceil_div(s->tokens, tile) : 1;
     p.strips = ceil_div(s->channels, 64 * lane);
     p.chains = s->samples * p.strips;
-    p.look = p.tiles > 2 && p.chains < 2048 && p.tiles * p.chains < (1 << 23);
+    // A workgroup for each tile where chains are fewer than compute units; with more, walking saves the words and the launch that zeroes
+    // them.  Forward / backward, us, a workgroup for each tile and a walk: [32,512,512] bfloat16, 128 chains, 15 / 29 and 19 / 34; [48,512,512], 192
+    // chains, 22 / 37 and 20 / 36; [64,512,512], 256 chains, 25 / 43 and 24 / 39; float32, 256 chains, 20 / 33 and 20 / 35; ragged samples alike.
+    // Two tiles, [4,200,128] float32: 8.2 / 11.6 and 7.7 / 13.5.
+    p.look = p.tiles > 2 && p.chains < 192;
     p.blocks = p.look ? p.tiles * p.chains : p.chains;
     p.window = p.look ? 2048 / p.chains : 1;
     if (p.window > kWindow) p.window = kWindow;
