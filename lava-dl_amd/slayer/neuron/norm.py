@@ -273,29 +273,21 @@ def residual_norm(input, residual, weight=None, inner=None, gate=None, scale=Non
     if not eps >= 0:
         raise ValueError(f'eps has to be at least 0, got {eps}')
     device, _ = N.require_elements(input) if gate is None else N.require_elements(input, gate)
-    if input.dim() < 1 or not 1 <= input.shape[-1] <= 8192:
-        raise RuntimeError(f'expected a tensor [..., C] with C up to 8192, got {tuple(input.shape)}')
-    if gate is not None and gate.shape != input.shape:
-        raise RuntimeError(f'gate: expected the shape {tuple(input.shape)}, got {tuple(gate.shape)}')
+    shape = input.shape
+    if len(shape) < 1 or not 1 <= shape[-1] <= 8192:
+        raise RuntimeError(f'expected a tensor [..., C] with C up to 8192, got {tuple(shape)}')
+    if gate is not None and gate.shape != shape:
+        raise RuntimeError(f'gate: expected the shape {tuple(shape)}, got {tuple(gate.shape)}')
     if residual is not None:
-        if not torch.is_tensor(residual) or residual.shape != input.shape or residual.dtype not in (input.dtype, torch.float32):
-            raise RuntimeError(f'residual: expected a tensor {list(input.shape)} of {input.dtype} or torch.float32')
+        if not torch.is_tensor(residual) or residual.shape != shape or residual.dtype not in (input.dtype, torch.float32):
+            raise RuntimeError(f'residual: expected a tensor {list(shape)} of {input.dtype} or torch.float32')
         if residual.device != device:
             raise RuntimeError(f'tensors on different devices: {device} and {residual.device}')
     factor = 1.0
     if scale is not None and not torch.is_tensor(scale):
         factor, scale = float(scale), None
-    channels = input.shape[-1]
-    parameters = []
-    for name, t in (('weight', weight), ('inner', inner), ('scale', scale)):
-        if t is not None:
-            if not torch.is_tensor(t) or t.shape != (channels,) or not t.is_floating_point():
-                raise RuntimeError(f'{name}: expected {channels} floating-point values')
-            if t.device != device:
-                raise RuntimeError(f'tensors on different devices: {device} and {t.device}')
-            t = t.float().contiguous()
-        parameters.append(t)
-    tensors = (input, residual, gate, *parameters)
+    weight, inner, scale = (_parameter(name, t, shape[-1], device) for name, t in (('weight', weight), ('inner', inner), ('scale', scale)))
+    tensors = (input, residual, gate, weight, inner, scale)
     args = (0 if gate is None else GATES[activation], float(eps), factor, return_sum or weight is None)
     if N.wants_grad(*(t for t in tensors if t is not None)):
         out, total = _ResidualNorm.apply(*tensors, *args)
@@ -306,33 +298,49 @@ def residual_norm(input, residual, weight=None, inner=None, gate=None, scale=Non
     return (out, total) if return_sum else out
 
 
-def _flat(x):
-    """``x`` as rows of neighbouring elements, a view where it can be one."""
-    if x is None:
+def _parameter(name, t, channels, device):
+    """``t`` as float32 and contiguous, or None."""
+    if t is None:
         return None
+    if not torch.is_tensor(t) or t.shape != (channels,) or not t.is_floating_point():
+        raise RuntimeError(f'{name}: expected {channels} floating-point values')
+    if t.device != device:
+        raise RuntimeError(f'tensors on different devices: {device} and {t.device}')
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
+def _rows(x):
+    """``x`` as rows of neighbouring elements (a view where it can be one), and how far they are apart."""
+    if x is None:
+        return None, 0
     channels = x.shape[-1]
-    x = x.reshape(x.numel() // channels, channels)
-    return x if channels == 1 or x.stride(1) == 1 else x.contiguous()
+    if not x.is_contiguous():
+        x = x.reshape(x.numel() // channels, channels)
+        if channels == 1 or x.stride(1) == 1:
+            return x, x.stride(0)
+        x = x.contiguous()
+    return x, channels
 
 
-def _residual_call(input, residual, gate, weight, inner, scale, activation, eps, factor):
-    kind = N.ELEMENT_TYPES
-    return N.ResidualNorm(*input.shape, N.ptr(inner), N.ptr(weight), N.ptr(scale), kind[input.dtype],
-                          kind[(input if residual is None else residual).dtype], activation, eps, factor, input.stride(0),
-                          0 if residual is None else residual.stride(0), 0 if gate is None else gate.stride(0))
+def _residual_call(shape, input, residual, gate, weight, inner, scale, activation, eps, factor):
+    """The structure of the C calls, and the tensors it describes."""
+    kind, channels = N.ELEMENT_TYPES, shape[-1]
+    (input, a), (residual, b), (gate, c) = _rows(input), _rows(residual), _rows(gate)
+    dtype = kind[input.dtype]
+    call = N.ResidualNorm(input.numel() // channels, channels, N.ptr(inner), N.ptr(weight), N.ptr(scale), dtype,
+                          dtype if residual is None else kind[residual.dtype], activation, eps, factor, a, b, c)
+    return call, input, residual, gate
 
 
 def _residual_fwd(input, residual, gate, weight, inner, scale, activation, eps, factor, want_total, keep):
-    shape, device = input.shape, input.device
-    stream = (input if residual is None else residual).dtype
-    input, residual, gate = _flat(input), _flat(residual), _flat(gate)
-    out = None if weight is None else torch.empty(shape, dtype=input.dtype, device=device)
-    total = torch.empty(shape, dtype=stream, device=device) if want_total else None
-    stats = torch.empty((input.shape[0], 2), dtype=torch.float32, device=device) if keep else None
-    call = _residual_call(input, residual, gate, weight, inner, scale, activation, eps, factor)
+    shape, device, dtype = input.shape, input.device, input.dtype
+    call, input, residual, gate = _residual_call(shape, input, residual, gate, weight, inner, scale, activation, eps, factor)
+    out = None if weight is None else torch.empty(shape, dtype=dtype, device=device)
+    total = torch.empty(shape, dtype=dtype if residual is None else residual.dtype, device=device) if want_total else None
+    stats = torch.empty((call.rows, 2), dtype=torch.float32, device=device) if keep else None
     with N.device_guard(device):
-        N.check(N.lib().slayer_residual_norm_fwd(N.ptr(out), N.ptr(total), N.ptr(stats), N.ptr(input), N.ptr(residual), N.ptr(gate), call,
-                                                 N.stream_handle()))
+        N.check(N.lib().slayer_residual_norm_fwd(N.ptr(out), N.ptr(total), N.ptr(stats), input.data_ptr(), N.ptr(residual), N.ptr(gate),
+                                                 call, N.stream_handle()))
     return out, total, input, residual, gate, stats
 
 
@@ -351,24 +359,23 @@ class _ResidualNorm(torch.autograd.Function):
         if grad_out is None and grad_total is None:
             return (None,) * 10
         input, residual, gate, stats, weight, inner, scale = ctx.saved_tensors
-        device = input.device
-        grad_out, grad_total = _flat(grad_out), _flat(grad_total)
-        need = ctx.needs_input_grad
-        grads = [torch.empty(ctx.shape, dtype=t.dtype, device=device) if wanted else None
+        device, shape, need = input.device, ctx.shape, ctx.needs_input_grad
+        call = _residual_call(shape, input, residual, gate, weight, inner, scale, *ctx.args)[0]
+        grad_out, call.grad_out_stride = _rows(grad_out)
+        grad_total, call.grad_total_stride = _rows(grad_total)
+        grads = [torch.empty(shape, dtype=t.dtype, device=device) if wanted else None
                  for t, wanted in zip((input, residual, gate), need)]
-        sums = [torch.empty(t.shape, dtype=torch.float32, device=device) if wanted else None
-                for t, wanted in zip((weight, inner, scale), need[3:])]
-        call = _residual_call(input, residual, gate, weight, inner, scale, *ctx.args)
-        call.grad_out_stride = 0 if grad_out is None else grad_out.stride(0)
-        call.grad_total_stride = 0 if grad_total is None else grad_total.stride(0)
-        lib = N.lib()
-        with N.device_guard(device):
-            floats = lib.slayer_residual_norm_workspace(call) if any(need[3:]) else 0
+        lib, sums, workspace, floats = N.lib(), (None, None, None), None, 0
+        if any(need[3:6]):
+            sums = torch.empty((3, shape[-1]), dtype=torch.float32, device=device).unbind(0)
+            sums = [t if wanted else None for t, wanted in zip(sums, need[3:])]
+            floats = lib.slayer_residual_norm_workspace(call)
             if floats < 0:
                 N.check(int(floats))
-            workspace = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
+            workspace = torch.empty(floats, dtype=torch.float32, device=device)
+        with N.device_guard(device):
             N.check(lib.slayer_residual_norm_bwd(*(N.ptr(g) for g in grads), N.ptr(sums[1]), N.ptr(sums[0]), N.ptr(sums[2]),
-                                                 N.ptr(grad_out), N.ptr(grad_total), N.ptr(stats), N.ptr(input), N.ptr(residual),
+                                                 N.ptr(grad_out), N.ptr(grad_total), stats.data_ptr(), input.data_ptr(), N.ptr(residual),
                                                  N.ptr(gate), call, N.ptr(workspace), floats, N.stream_handle()))
         return (*grads, *sums, None, None, None, None)
 

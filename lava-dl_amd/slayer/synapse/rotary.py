@@ -78,21 +78,21 @@ def rotary(query, key, frequency, position=None, layout='halves', magnitude=1.0)
     """
     if layout not in LAYOUTS:
         raise ValueError(f'unknown layout {layout!r}: one of {list(LAYOUTS)}')
-    given = (query,) if key is None else (query, key)
-    device, _ = N.require_elements(*given)
-    if query.dim() not in (3, 4) or query.shape[-1] < 1 or query.shape[-1] > 4096 or \
-            (key is not None and (key.dim() != query.dim() or key.shape[:-2] != query.shape[:-2] or key.shape[-1] != query.shape[-1])):
-        raise RuntimeError(f'expected query and key [N, T, H, D] or [N, H, D] with D up to 4096, got '
-                           f'{" and ".join(str(tuple(x.shape)) for x in given)}')
+    device, _ = N.require_elements(query) if key is None else N.require_elements(query, key)
+    shape, other = query.shape, None if key is None else key.shape
+    if len(shape) not in (3, 4) or not 1 <= shape[-1] <= 4096 or \
+            (other is not None and (len(other) != len(shape) or other[:-2] != shape[:-2] or other[-1] != shape[-1])):
+        raise RuntimeError(f'expected query and key [N, T, H, D] or [N, H, D] with D up to 4096, got {tuple(shape)}'
+                           + ('' if other is None else f' and {tuple(other)}'))
     if not torch.is_tensor(frequency) or frequency.dtype is not torch.float64 or frequency.dim() != 1 or \
-            2 * frequency.shape[0] > query.shape[-1]:
-        raise RuntimeError(f'frequency: expected up to {query.shape[-1] // 2} float64 values')
+            2 * frequency.shape[0] > shape[-1]:
+        raise RuntimeError(f'frequency: expected up to {shape[-1] // 2} float64 values')
     if frequency.device != device:
         raise RuntimeError(f'tensors on different devices: {device} and {frequency.device}')
     if position is not None:
-        n, shapes = query.shape[0], [query.shape[:1]] + [query.shape[:2]] * (query.dim() == 4)
-        if not torch.is_tensor(position) or position.dtype not in (torch.int32, torch.int64) or position.shape not in shapes:
-            raise RuntimeError(f'position: expected int32 or int64 values {" or ".join(str(list(s)) for s in shapes)}')
+        if not torch.is_tensor(position) or position.dtype not in (torch.int64, torch.int32) or \
+                not (position.shape == shape[:1] or len(shape) == 4 and position.shape == shape[:2]):
+            raise RuntimeError(f'position: expected int32 or int64 values {[shape[0]]}' + (f' or {list(shape[:2])}' if len(shape) == 4 else ''))
         if position.device != device:
             raise RuntimeError(f'tensors on different devices: {device} and {position.device}')
         position = position.contiguous()
@@ -109,23 +109,27 @@ def _rows(x):
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
+def _place(x):
+    """``x`` as the kernel reads it, the strides of its samples, tokens and heads, and room for the result."""
+    if x is None:
+        return None, (0, 0, 0), None
+    x = _rows(x)
+    stride = x.stride()
+    return x, stride[:3] if len(stride) == 4 else (stride[0], 0, stride[1]), torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _run(query, key, frequency, position, layout, magnitude, inverse):
     given = query if query is not None else key
-    tokens = given.shape[1] if given.dim() == 4 else 1
-    heads, strides, x, out = [0, 0], [(0, 0, 0), (0, 0, 0)], [None, None], [None, None]
-    for i, t in enumerate((query, key)):
-        if t is None:
-            continue
-        x[i] = t = _rows(t)
-        heads[i] = t.shape[-2]
-        strides[i] = t.stride()[:3] if t.dim() == 4 else (t.stride(0), 0, t.stride(1))
-        out[i] = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-    call = N.Rotary(given.shape[0], tokens, *heads, given.shape[-1], 2 * frequency.shape[0], N.ptr(frequency), N.ptr(position),
+    shape = given.shape
+    query, query_stride, out_query = _place(query)
+    key, key_stride, out_key = _place(key)
+    call = N.Rotary(shape[0], shape[1] if len(shape) == 4 else 1, 0 if query is None else query.shape[-2], 0 if key is None else key.shape[-2],
+                    shape[-1], 2 * frequency.shape[0], frequency.data_ptr(), N.ptr(position),
                     0 if position is None else position.element_size(), position is not None and position.dim() == 2, layout,
-                    N.ELEMENT_TYPES[given.dtype], magnitude, *strides)
+                    N.ELEMENT_TYPES[given.dtype], magnitude, query_stride, key_stride)
     with N.device_guard(given.device):
-        N.check(N.lib().slayer_rotary(N.ptr(out[0]), N.ptr(out[1]), N.ptr(x[0]), N.ptr(x[1]), call, inverse, N.stream_handle()))
-    return tuple(out)
+        N.check(N.lib().slayer_rotary(N.ptr(out_query), N.ptr(out_key), N.ptr(query), N.ptr(key), call, inverse, N.stream_handle()))
+    return out_query, out_key
 
 
 class _Rotary(torch.autograd.Function):

@@ -154,7 +154,7 @@ def test_lengths_outside_are_the_nearest_inside(lengths):
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize('n,t,c', [(1, 9000, 64), (1, 20000, 3), (40, 1500, 130), (2048, 300, 4), (700, 400, 70)])
 def test_long_samples_and_many(n, t, c, dtype):
-    """Windows of 32 tiles and what lies between windows; chains so many that a workgroup walks one; both directions.  Channels apart, so
+    """Windows of tiles and what lies between windows; chains so many that a workgroup walks one; both directions.  Channels apart, so
     that a slice of them in float64 is the whole answer for it."""
     gen = torch.Generator().manual_seed(t)
     d = make(gen, n, t, c, dtype, state=True)
