@@ -184,7 +184,7 @@ def check(code):
     if code != 0:
         msg = lib().slayer_error_string(code).decode()
         raise RuntimeError(f'libslayer_hip call failed ({code}): {msg}')
-    if (_range_word or _find_range_word()).value:
+    if (_find_range_word() if _range_word is None else _range_word).value:
         _range_raised()
 
 
@@ -236,7 +236,7 @@ def range_policy(mode=None):
 
 def range_flag():
     """True when a launch that has completed raised the range flag since it was last cleared."""
-    return bool((_range_word or _find_range_word()).value)
+    return bool((_find_range_word() if _range_word is None else _range_word).value)
 
 
 def clear_range_flag():
