@@ -709,7 +709,8 @@ typedef struct slayer_gated_leak {
     int64_t input_stride[2], gate_stride[2], grad_stride[2];   /* sample, token; grad_stride: of grad_out */
 } slayer_gated_leak;
 
-/* Floats of the states that the forward call keeps for the backward call, and of workspace; or a negative SLAYER_E*. */
+/* Floats of the states that the forward call keeps for the backward call, and of workspace (at an address that is a multiple of 8, and
+ * not shared by calls that overlap); or a negative SLAYER_E*. */
 int64_t slayer_gated_leak_starts(const slayer_gated_leak *a);
 int64_t slayer_gated_leak_workspace(const slayer_gated_leak *a, int backward);
 /* state, last: [samples][channels] floats or NULL (zeros; not wanted); starts: for the backward call, or NULL */

@@ -4,12 +4,15 @@
 // respect to the state in front of it,
 //     D[t] = dy[t] + G[t+1],  G[t] = (1 - leak) D[t],  dx = drive D,  dleak = D (drive' x - h[t-1]),
 //     dgate = dleak leak (1 - open),  ddecay = sum of dleak open / 4096.
-// Both are linear recurrences s <- A s + H in one number a channel, and spans of tokens join as pairs (A, H): a thread takes a few
-// tokens of four channels in its registers, sixteen lanes the channels next to each other, the other lanes and waves the tokens that
-// follow; pairs are joined across lanes, then across waves in LDS, and with the state in front of the tile each thread walks its tokens
-// again.  The backward pass makes the states of a tile again from the one in front of it, which the forward pass has kept, so that
-// it reads neither the results nor anything rounded.
-//   Bound: memory, three tensors forward and five backward.
+// Both are linear recurrences s <- A s + H in one number a channel, and spans of tokens join as pairs (A, H).  A wave takes eight or sixteen
+// tokens of 64 or 128 neighbouring channels, a lane one float32 or two bfloat16 of each token: rows are read and written 256 bytes at a time
+// at addresses that are the same for the wave, channels need no joining, and which tokens there are is a scalar question.  Eight waves, one
+// behind the other, make a tile; their pairs meet in LDS, where one thread a channel runs through them, and with the state in front of it each
+// wave walks its tokens again in its registers.  The backward pass makes the states of a tile again from the one in front of it, which the
+// forward pass has kept (one in 64 tokens), so that it reads neither the results nor anything rounded.
+//   Bound: memory, three tensors forward and five backward, at 4.2 to 5.5 TB/s (a copy reaches 5.1).  [32,1500,256] float32: forward 27 us, backward 48;
+// [16,1450,1021] bfloat16, ragged: 30 and 46 to 52; one sample of 32768 tokens of 1024 channels, bfloat16: 45.  The forms before: lanes of four channels
+// with tokens across the lanes, 43 and 74, 53 and 122, 69 (joining across lanes takes as many instructions as the recurrence).
 #include "common.h"
 #include "elements.h"
 
@@ -31,7 +34,8 @@ struct LeakArgs {
 };
 
 // sigmoid from the hardware's exponential and reciprocal, a unit in the last place each, for either type: (3 + 1.5 |z|) 2^-24, which is most
-// where the gate is as good as closed and the leak next to nothing.  Infinite gates are open and closed.
+// where the gate is as good as closed and the leak next to nothing.  (With the precise form, eleven instructions more, the errors of
+// float32 results were the same.)  Infinite gates are open and closed.
 __device__ __forceinline__ float open_gate(float z) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
 }
@@ -54,7 +58,6 @@ template <> struct Piece<float, 1> { typedef float Raw; };
 template <> struct Piece<bf16, 1> { typedef unsigned short Raw; };
 template <> struct Piece<bf16, 2> { typedef unsigned Raw; };
 typedef unsigned unsigned_any __attribute__((aligned(2)));
-__device__ __forceinline__ float load_piece(const float* p) { return *p; }
 template <int V> __device__ __forceinline__ typename Piece<bf16, V>::Raw load_piece(const bf16* p) {
     if constexpr (V == 1) return *reinterpret_cast<const unsigned short*>(p);
     else return *reinterpret_cast<const unsigned_any*>(p);
@@ -101,22 +104,24 @@ __device__ __forceinline__ int64_t length_of(const LeakArgs& a, int64_t n) {
 
 // ---- tiles of a chain -----------------------------------------------------------------------------------------------------------
 // A chain is one strip of one sample, from tile to tile in the order of the pass.  Either a workgroup walks all tiles of a chain and
-// carries the state in LDS, or there is a workgroup for each tile, and states go through memory:
+// carries the state in registers, or there is a workgroup for each tile, and states go through memory:
 //   A workgroup takes the next tile of its chain by a ticket, so it only ever waits for workgroups of the same chain with lower tickets,
 // which are running or done and wait for lower ones themselves; the lowest waits for nobody, so every wait ends.  (One ticket for all
-// chains would be taken at 12 ns each, whoever asks: 25 us for the 2048 tiles of a prompt.)  Tiles form windows.  A tile leaves its pair, then reads those of the tiles before it in its window, and the state in front of
-// the window; the last tile of a window leaves the state behind it.  Which values are joined, and in which order, depends on the sizes alone
-// and not on who comes first, so that a call computed again has the same bits.
+// chains would be taken at 12 ns each, whoever asks: 25 us for the 2048 tiles of a prompt.)  Tiles form windows.  A tile leaves its pair, then
+// reads those of the tiles before it in its window, and the state in front of the window; the last tile of a window leaves the state
+// behind it.  Which values are joined, and in which order, depends on the sizes alone and not on who comes first, so that a call computed
+// again has the same bits.
 //   What is left is a word of 64 bits that says itself that it is there (the workspace is zeroed before), read and written with relaxed
 // atomics of the whole device: no other memory hangs on it, so no fences are needed.
+//   Windows of sixteen: of 32 tiles the words a thread waits for take the registers of a workgroup (backward, [16,1450,1021]: 53 us, and 46), of
+// eight the states have too far to go (one sample of 65536 tokens of 256 channels: forward 67 us, and 43).
 typedef unsigned long long Word;
-constexpr int kWindow = 16;                    // largest window
-
+constexpr int kWindow = 16;                    // tiles of a window
 constexpr int kApart = 16;                     // words from one chain's ticket to the next: a cache line each
 
 struct Chains {
     Word *tickets, *pairs, *states;            // [chain], [tile][chain][strip], [window][chain][strip]
-    int chains, window;
+    int chains;
 };
 
 __device__ __forceinline__ Word pair_word(float A, float H) {      // A is no NaN of the bits that would make the upper half 0
@@ -137,7 +142,7 @@ template <int THREADS, int CH>
 __device__ __forceinline__ Before look_back(Pair (*parts)[CH], const Chains& k, int64_t index, unsigned chain, float initial) {
     constexpr int kShares = THREADS / CH, kMost = kWindow / kShares;
     const int channel = threadIdx.x % CH, share = threadIdx.x / CH;
-    const int64_t window = index / k.window, first = window * k.window;
+    const int64_t window = index / kWindow, first = window * kWindow;
     const int count = (int)(index - first);                        // less than kWindow
     const int per = (count + kShares - 1) / kShares, from = share * per, mine = count - from < per ? count - from : per;
     Before b = {{1.f, 0.f}, initial};
@@ -252,14 +257,14 @@ __global__ __launch_bounds__(64 * WAVES, 4) void leak_fwd_kernel(LeakArgs a, Cha
         for (int v = 0; v < V; ++v) total[wave][own.at(v)] = p[v];
         __syncthreads();
         if (LOOK) {
-            if (k.window > 1 && threadIdx.x < CH && (tile + 1) % k.window != 0 && tile + 1 < a.tiles) {
+            if (threadIdx.x < CH && (tile + 1) % kWindow != 0 && tile + 1 < a.tiles) {
                 Pair all = {1.f, 0.f};
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) all = then(all, total[w][threadIdx.x]);
                 leave(k.pairs + (tile * k.chains + span.chain) * CH + threadIdx.x, pair_word(all.a, all.h));
             }
             const Before b = look_back<64 * WAVES, CH>(parts, k, tile, span.chain, carry);
-            carry = tile % k.window == 0 ? b.state : fmaf(b.pair.a, b.state, b.pair.h);
+            carry = tile % kWindow == 0 ? b.state : fmaf(b.pair.a, b.state, b.pair.h);
         }
         if (threadIdx.x < CH) {
 #pragma unroll
@@ -270,8 +275,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void leak_fwd_kernel(LeakArgs a, Cha
                 carry = fmaf(total[w][threadIdx.x].a, carry, total[w][threadIdx.x].h);
             }
             if (a.last && keeps && tile == a.tiles - 1) a.last[n * a.channels + channel] = carry;
-            if (LOOK && (tile + 1) % k.window == 0 && tile + 1 < a.tiles)
-                leave(k.states + ((tile + 1) / k.window * k.chains + span.chain) * CH + threadIdx.x, state_word(carry));
+            if (LOOK && (tile + 1) % kWindow == 0 && tile + 1 < a.tiles)
+                leave(k.states + ((tile + 1) / kWindow * k.chains + span.chain) * CH + threadIdx.x, state_word(carry));
         }
         __syncthreads();
         if (!own.on) continue;
@@ -375,14 +380,14 @@ __global__ __launch_bounds__(64 * WAVES, 4) void leak_bwd_kernel(LeakArgs a, Cha
         }
         __syncthreads();
         if (LOOK) {
-            if (k.window > 1 && threadIdx.x < CH && (index + 1) % k.window != 0 && index + 1 < a.tiles) {
+            if (threadIdx.x < CH && (index + 1) % kWindow != 0 && index + 1 < a.tiles) {
                 Pair all = {1.f, 0.f};
 #pragma unroll
                 for (int w = WAVES - 1; w >= 0; --w) all = then(all, {total[w][threadIdx.x].a, total_g[w][threadIdx.x]});
                 leave(k.pairs + (index * k.chains + span.chain) * CH + threadIdx.x, pair_word(all.a, all.h));
             }
             const Before b = look_back<64 * WAVES, CH>(parts, k, index, span.chain, carry);
-            carry = index % k.window == 0 ? b.state : fmaf(b.pair.a, b.state, b.pair.h);
+            carry = index % kWindow == 0 ? b.state : fmaf(b.pair.a, b.state, b.pair.h);
         }
         if (threadIdx.x < CH) {
 #pragma unroll
@@ -391,8 +396,8 @@ __global__ __launch_bounds__(64 * WAVES, 4) void leak_bwd_kernel(LeakArgs a, Cha
                 carry = fmaf(total[w][threadIdx.x].a, carry, total_g[w][threadIdx.x]);
             }
             if (a.grad_state && keeps && tile == 0) a.grad_state[n * a.channels + channel] = carry;
-            if (LOOK && (index + 1) % k.window == 0 && index + 1 < a.tiles)
-                leave(k.states + ((index + 1) / k.window * k.chains + span.chain) * CH + threadIdx.x, state_word(carry));
+            if (LOOK && (index + 1) % kWindow == 0 && index + 1 < a.tiles)
+                leave(k.states + ((index + 1) / kWindow * k.chains + span.chain) * CH + threadIdx.x, state_word(carry));
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
                 front[w][threadIdx.x] = start;
@@ -493,9 +498,11 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Channels of a lane: two bfloat16 where there are two, so that a wave reads 256 bytes of a row.
 int lane_of(const slayer_gated_leak* s) { return s->dtype == SLAYER_BFLOAT16 && s->channels > 1 ? 2 : 1; }
-// Tokens of a wave, of the eight waves of a workgroup.
+// Tokens of a wave, of the eight waves of a workgroup: as many as leave registers for a second workgroup on a compute unit (backward, pairs of
+// bfloat16, sixteen tokens: 54 us where eight take 46).
 constexpr int tokens_of(int lane, bool backward) { return lane == 2 && backward ? 8 : 16; }
 constexpr int kWaves = 8;
+constexpr int64_t kMostBlocks = (int64_t)1 << 23;                  // of 512 threads: fewer than 2^32 threads in a launch
 
 int check_leak(const slayer_gated_leak* a) {
     if (!a) return SLAYER_ENULL;
@@ -507,14 +514,14 @@ int check_leak(const slayer_gated_leak* a) {
     if (!a->decay) return SLAYER_ENULL;
     if (a->tokens > kMaxT || a->channels > (1 << 24) || a->samples > ((int64_t)1 << 32)) return SLAYER_ERANGE;
     if (a->samples * a->channels > kMaxNumel / (a->tokens > 0 ? a->tokens : 1)) return SLAYER_ERANGE;
-    if (a->samples * ceil_div(a->channels, 64 * lane_of(a)) > (1 << 23)) return SLAYER_ERANGE;          // a workgroup each
+    if (a->samples * ceil_div(a->channels, 64 * lane_of(a)) >= kMostBlocks) return SLAYER_ERANGE;          // a workgroup each
     return 0;
 }
 
 // How the tiles are cut up among workgroups, and the workspace of that: the words, the ticket, the rows of the decays' gradient.
 struct Plan {
     bool look;
-    int64_t tiles, strips, chains, blocks, window, pairs, words, rows, columns;   // rows, columns: of partial sums of the decays' gradient
+    int64_t tiles, strips, chains, blocks, pairs, words, rows, columns;   // rows, columns: of partial sums of the decays' gradient
 };
 Plan plan_of(const slayer_gated_leak* s, bool backward) {
     Plan p = {};
@@ -526,14 +533,11 @@ Plan plan_of(const slayer_gated_leak* s, bool backward) {
     // them.  Forward / backward, us, a workgroup for each tile and a walk: [32,512,512] bfloat16, 128 chains, 15 / 29 and 19 / 34; [48,512,512], 192
     // chains, 22 / 37 and 20 / 36; [64,512,512], 256 chains, 25 / 43 and 24 / 39; float32, 256 chains, 20 / 33 and 20 / 35; ragged samples alike.
     // Two tiles, [4,200,128] float32: 8.2 / 11.6 and 7.7 / 13.5.
-    p.look = p.tiles > 2 && p.chains < 192;
+    p.look = p.tiles > 2 && p.chains < 192 && p.tiles * p.chains < kMostBlocks;
     p.blocks = p.look ? p.tiles * p.chains : p.chains;
-    p.window = p.look ? 2048 / p.chains : 1;
-    if (p.window > kWindow) p.window = kWindow;
-    if (p.window > p.tiles) p.window = p.tiles;
     if (p.look) {
-        p.pairs = p.window > 1 ? p.tiles * p.chains * 64 * lane : 0;
-        p.words = p.chains * kApart + p.pairs + ceil_div(p.tiles, p.window) * p.chains * 64 * lane;
+        p.pairs = p.tiles * p.chains * 64 * lane;
+        p.words = p.chains * kApart + p.pairs + ceil_div(p.tiles, kWindow) * p.chains * 64 * lane;
     }
     p.columns = s->num_decays;
     p.rows = (p.look ? p.tiles : 1) * (s->num_decays == 1 ? p.chains * lane : s->samples);
@@ -545,7 +549,6 @@ int64_t floats_of(const Plan& p, bool sums) { return 2 * p.words + (sums ? p.row
 int chains_of(Chains* k, const Plan& p, float* workspace, hipStream_t stream) {
     if (!p.look) return 0;
     k->chains = (int)p.chains;
-    k->window = (int)p.window;
     k->tickets = (Word*)workspace;
     k->pairs = k->tickets + p.chains * kApart;
     k->states = k->pairs + p.pairs;
