@@ -6,6 +6,7 @@ operator raises when handed a tensor that is not float32 on a GPU.
 """
 import contextlib
 import ctypes
+import functools
 import os
 import threading
 
@@ -50,17 +51,20 @@ _AP = ctypes.POINTER(Attention)
 
 
 class GatedLeak(ctypes.Structure):
-    """struct slayer_gated_leak of include/slayer_hip.h (device pointers as integers)."""
+    """struct slayer_gated_leak of include/slayer_hip.h (device pointers as integers; its arrays as single fields, which ctypes sets
+    in a tenth of the time)."""
     _fields_ = [('samples', _I64), ('tokens', _I64), ('channels', _I64), ('num_decays', _I64), ('decay', _P), ('lengths', _P),
-                ('lengths_bytes', _INT), ('dtype', _INT), ('drive', _INT), ('input_stride', _I64 * 2), ('gate_stride', _I64 * 2),
-                ('grad_stride', _I64 * 2)]
+                ('lengths_bytes', _INT), ('dtype', _INT), ('drive', _INT), ('input_sample', _I64), ('input_token', _I64),
+                ('gate_sample', _I64), ('gate_token', _I64), ('grad_sample', _I64), ('grad_token', _I64)]
 
 
 class Rotary(ctypes.Structure):
-    """struct slayer_rotary_call of include/slayer_hip.h (device pointers as integers)."""
+    """struct slayer_rotary_call of include/slayer_hip.h (device pointers as integers, arrays as single fields)."""
     _fields_ = [('samples', _I64), ('tokens', _I64), ('query_heads', _I64), ('key_heads', _I64), ('features', _I64),
                 ('turned', _I64), ('frequency', _P), ('position', _P), ('position_bytes', _INT), ('position_each', _INT),
-                ('layout', _INT), ('dtype', _INT), ('magnitude', _F), ('query_stride', _I64 * 3), ('key_stride', _I64 * 3)]
+                ('layout', _INT), ('dtype', _INT), ('magnitude', _F),
+                ('query_sample', _I64), ('query_token', _I64), ('query_head', _I64), ('key_sample', _I64), ('key_token', _I64),
+                ('key_head', _I64)]
 
 
 class ResidualNorm(ctypes.Structure):
@@ -333,12 +337,30 @@ def raise_on_mismatch(what, fast, check, rel=None):
 
 
 def wants_grad(*tensors):
-    """True when a backward pass could reach one of the tensors, or one of them carries a forward-mode tangent (which the
+    """True when a backward pass could reach one of the tensors (None: no tensor), or one of them carries a forward-mode tangent (which the
     autograd node refuses, as it has no rule for it): otherwise the operators call their kernels directly and skip the
     autograd node (a few microseconds per call, which is most of a call on a tensor of one time step)."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        return True
-    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def once_differentiable(backward):
+    """torch's decorator of that name where a second derivative can be asked for at all, that is, where the backward pass records a
+    graph; otherwise ``backward`` as it is (the decorator costs as much as a launch)."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def either(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return either
+
+
+def empty_as(t):
+    """A contiguous tensor of the shape, type and device of ``t``, uninitialised."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 _no_guard = contextlib.nullcontext()

@@ -55,7 +55,7 @@ def gated_leak(input, gate, decay, state=None, lengths=None, drive='gain', retur
             raise RuntimeError(f'tensors on different devices: {device} and {lengths.device}')
         lengths = lengths.contiguous()
     inputs = (input, gate, decay, state)
-    if N.wants_grad(*(x for x in inputs if x is not None)):
+    if N.wants_grad(*inputs):
         out, last = _GatedLeak.apply(*inputs, lengths, code, return_state)
     else:
         out, last = _forward(*inputs, lengths, code, return_state, False)[:2]
@@ -90,8 +90,8 @@ def gated_leak_step(input, gate, decay, state, drive='gain'):
     if N.wants_grad(input, gate, decay, state):
         raise RuntimeError('gated_leak_step has no gradient: call it under torch.no_grad(), or gated_leak')
     input, gate, decay = _rows(input), _rows(gate), decay.contiguous()
-    out = torch.empty(shape, dtype=input.dtype, device=device)
-    args = N.GatedLeak(n, 1, c, decay.numel(), decay.data_ptr(), None, 0, dtype, code, (input.stride(0), 0), (gate.stride(0), 0))
+    out = N.empty_as(input)
+    args = N.GatedLeak(n, 1, c, decay.shape[0], decay.data_ptr(), None, 0, dtype, code, input.stride(0), 0, gate.stride(0))
     with N.device_guard(device):
         N.check(N.lib().slayer_gated_leak_step(out.data_ptr(), state.data_ptr(), input.data_ptr(), gate.data_ptr(), args,
                                                N.stream_handle()))
@@ -127,8 +127,9 @@ def _rows(x):
 def _call(input, gate, decay, lengths, drive):
     """The structure of the C calls."""
     n, t, c = input.shape
-    return N.GatedLeak(n, t, c, decay.numel(), decay.data_ptr(), N.ptr(lengths), 0 if lengths is None else lengths.element_size(),
-                       N.ELEMENT_TYPES[input.dtype], drive, input.stride()[:2], gate.stride()[:2])
+    a, b = input.stride(), gate.stride()
+    return N.GatedLeak(n, t, c, decay.shape[0], decay.data_ptr(), N.ptr(lengths), 0 if lengths is None else lengths.element_size(),
+                       N.ELEMENT_TYPES[input.dtype], drive, a[0], a[1], b[0], b[1])
 
 
 def _floats(count, device):
@@ -140,9 +141,9 @@ def _floats(count, device):
 def _forward(input, gate, decay, state, lengths, drive, return_state, keep):
     input, gate, decay = _rows(input), _rows(gate), decay.contiguous()
     state = None if state is None else state.contiguous()
-    n, t, c = input.shape
+    n, _, c = input.shape
     device = input.device
-    out = torch.empty((n, t, c), dtype=input.dtype, device=device)
+    out = N.empty_as(input)
     last = torch.empty((n, c), dtype=torch.float32, device=device) if return_state else None
     args = _call(input, gate, decay, lengths, drive)
     lib = N.lib()
@@ -150,7 +151,7 @@ def _forward(input, gate, decay, state, lengths, drive, return_state, keep):
         starts = _floats(lib.slayer_gated_leak_starts(args), device) if keep else None
         floats = lib.slayer_gated_leak_workspace(args, 0)
         workspace = _floats(floats, device)
-        N.check(lib.slayer_gated_leak_fwd(N.ptr(out), N.ptr(last), N.ptr(starts), N.ptr(input), N.ptr(gate), N.ptr(state), args,
+        N.check(lib.slayer_gated_leak_fwd(out.data_ptr(), N.ptr(last), N.ptr(starts), input.data_ptr(), gate.data_ptr(), N.ptr(state), args,
                                           N.ptr(workspace), floats, N.stream_handle()))
     return out, last, input, gate, decay, starts
 
@@ -165,28 +166,24 @@ class _GatedLeak(torch.autograd.Function):
         return out, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @N.once_differentiable
     def backward(ctx, grad_out, grad_last):
+        if grad_out is None and grad_last is None:
+            return (None,) * 7
         input, gate, decay, starts, lengths = ctx.saved_tensors
-        if grad_out is None:
-            if grad_last is None:
-                return (None,) * 7
-            grad_out = input.new_zeros(input.shape)
-        grad_out = _rows(grad_out)
+        grad_out = torch.zeros_like(input) if grad_out is None else _rows(grad_out)
         grad_last = None if grad_last is None else grad_last.contiguous()
-        n, t, c = input.shape
-        device, need = input.device, ctx.needs_input_grad
-        grad_input = torch.empty((n, t, c), dtype=input.dtype, device=device)
-        grad_gate = torch.empty((n, t, c), dtype=input.dtype, device=device)
-        grad_decay = torch.empty(decay.shape, dtype=torch.float32, device=device) if need[2] else None
-        grad_state = torch.empty((n, c), dtype=torch.float32, device=device) if need[3] else None
+        need = ctx.needs_input_grad
+        grad_input, grad_gate = N.empty_as(input), N.empty_as(gate)
+        grad_decay = torch.empty_like(decay) if need[2] else None
+        grad_state = torch.empty((input.shape[0], input.shape[2]), dtype=torch.float32, device=input.device) if need[3] else None
         args = _call(input, gate, decay, lengths, ctx.drive)
-        args.grad_stride[:] = grad_out.stride()[:2]
+        args.grad_sample, args.grad_token, _ = grad_out.stride()
         lib = N.lib()
-        with N.device_guard(device):
+        with N.device_guard(input.device):
             floats = lib.slayer_gated_leak_workspace(args, 1)
-            workspace = _floats(floats, device)
-            N.check(lib.slayer_gated_leak_bwd(N.ptr(grad_input), N.ptr(grad_gate), N.ptr(grad_decay), N.ptr(grad_state),
-                                              N.ptr(grad_out), N.ptr(grad_last), N.ptr(input), N.ptr(gate), N.ptr(starts), args,
-                                              N.ptr(workspace), floats, N.stream_handle()))
+            workspace = _floats(floats, input.device)
+            N.check(lib.slayer_gated_leak_bwd(grad_input.data_ptr(), grad_gate.data_ptr(), N.ptr(grad_decay), N.ptr(grad_state),
+                                              grad_out.data_ptr(), N.ptr(grad_last), input.data_ptr(), gate.data_ptr(),
+                                              N.ptr(starts), args, N.ptr(workspace), floats, N.stream_handle()))
         return grad_input if need[0] else None, grad_gate if need[1] else None, grad_decay, grad_state, None, None, None

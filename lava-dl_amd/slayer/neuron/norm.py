@@ -289,7 +289,7 @@ def residual_norm(input, residual, weight=None, inner=None, gate=None, scale=Non
     weight, inner, scale = (_parameter(name, t, shape[-1], device) for name, t in (('weight', weight), ('inner', inner), ('scale', scale)))
     tensors = (input, residual, gate, weight, inner, scale)
     args = (0 if gate is None else GATES[activation], float(eps), factor, return_sum or weight is None)
-    if N.wants_grad(*(t for t in tensors if t is not None)):
+    if N.wants_grad(*tensors):
         out, total = _ResidualNorm.apply(*tensors, *args)
     else:
         out, total = _residual_fwd(*tensors, *args, False)[:2]
@@ -333,10 +333,10 @@ def _residual_call(shape, input, residual, gate, weight, inner, scale, activatio
 
 
 def _residual_fwd(input, residual, gate, weight, inner, scale, activation, eps, factor, want_total, keep):
-    shape, device, dtype = input.shape, input.device, input.dtype
-    call, input, residual, gate = _residual_call(shape, input, residual, gate, weight, inner, scale, activation, eps, factor)
-    out = None if weight is None else torch.empty(shape, dtype=dtype, device=device)
-    total = torch.empty(shape, dtype=dtype if residual is None else residual.dtype, device=device) if want_total else None
+    device = input.device
+    out = None if weight is None else N.empty_as(input)
+    total = N.empty_as(input if residual is None else residual) if want_total else None
+    call, input, residual, gate = _residual_call(input.shape, input, residual, gate, weight, inner, scale, activation, eps, factor)
     stats = torch.empty((call.rows, 2), dtype=torch.float32, device=device) if keep else None
     with N.device_guard(device):
         N.check(N.lib().slayer_residual_norm_fwd(N.ptr(out), N.ptr(total), N.ptr(stats), input.data_ptr(), N.ptr(residual), N.ptr(gate),
@@ -354,7 +354,7 @@ class _ResidualNorm(torch.autograd.Function):
         return out, total
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @N.once_differentiable
     def backward(ctx, grad_out, grad_total):
         if grad_out is None and grad_total is None:
             return (None,) * 10
@@ -365,10 +365,9 @@ class _ResidualNorm(torch.autograd.Function):
         grad_total, call.grad_total_stride = _rows(grad_total)
         grads = [torch.empty(shape, dtype=t.dtype, device=device) if wanted else None
                  for t, wanted in zip((input, residual, gate), need)]
-        lib, sums, workspace, floats = N.lib(), (None, None, None), None, 0
+        sums = [torch.empty_like(t) if wanted else None for t, wanted in zip((weight, inner, scale), need[3:])]
+        lib, workspace, floats = N.lib(), None, 0
         if any(need[3:6]):
-            sums = torch.empty((3, shape[-1]), dtype=torch.float32, device=device).unbind(0)
-            sums = [t if wanted else None for t, wanted in zip(sums, need[3:])]
             floats = lib.slayer_residual_norm_workspace(call)
             if floats < 0:
                 N.check(int(floats))

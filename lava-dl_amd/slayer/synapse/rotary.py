@@ -100,7 +100,7 @@ def rotary(query, key, frequency, position=None, layout='halves', magnitude=1.0)
 
 
 def _turn(query, key, *args):
-    if N.wants_grad(*(x for x in (query, key) if x is not None)):
+    if N.wants_grad(query, key):
         return _Rotary.apply(query, key, *args)
     return _run(query, key, *args)
 
@@ -110,23 +110,22 @@ def _rows(x):
 
 
 def _place(x):
-    """``x`` as the kernel reads it, the strides of its samples, tokens and heads, and room for the result."""
+    """``x`` as the kernel reads it, its heads, the strides of its samples, tokens and heads, and room for the result."""
     if x is None:
-        return None, (0, 0, 0), None
+        return None, 0, 0, 0, 0, None
     x = _rows(x)
     stride = x.stride()
-    return x, stride[:3] if len(stride) == 4 else (stride[0], 0, stride[1]), torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return (x, x.shape[-2], *stride[:-1], N.empty_as(x)) if len(stride) == 4 else (x, x.shape[-2], stride[0], 0, stride[1], N.empty_as(x))
 
 
 def _run(query, key, frequency, position, layout, magnitude, inverse):
     given = query if query is not None else key
     shape = given.shape
-    query, query_stride, out_query = _place(query)
-    key, key_stride, out_key = _place(key)
-    call = N.Rotary(shape[0], shape[1] if len(shape) == 4 else 1, 0 if query is None else query.shape[-2], 0 if key is None else key.shape[-2],
-                    shape[-1], 2 * frequency.shape[0], frequency.data_ptr(), N.ptr(position),
-                    0 if position is None else position.element_size(), position is not None and position.dim() == 2, layout,
-                    N.ELEMENT_TYPES[given.dtype], magnitude, query_stride, key_stride)
+    query, query_heads, *query_stride, out_query = _place(query)
+    key, key_heads, *key_stride, out_key = _place(key)
+    call = N.Rotary(shape[0], shape[1] if len(shape) == 4 else 1, query_heads, key_heads, shape[-1], 2 * frequency.shape[0],
+                    frequency.data_ptr(), N.ptr(position), 0 if position is None else position.element_size(),
+                    position is not None and position.dim() == 2, layout, N.ELEMENT_TYPES[given.dtype], magnitude, *query_stride, *key_stride)
     with N.device_guard(given.device):
         N.check(N.lib().slayer_rotary(N.ptr(out_query), N.ptr(out_key), N.ptr(query), N.ptr(key), call, inverse, N.stream_handle()))
     return out_query, out_key
