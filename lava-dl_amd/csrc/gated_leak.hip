@@ -10,8 +10,8 @@
 // behind the other, make a tile; their pairs meet in LDS, where one thread a channel runs through them, and with the state in front of it each
 // wave walks its tokens again in its registers.  The backward pass makes the states of a tile again from the one in front of it, which the
 // forward pass has kept (one in 64 tokens), so that it reads neither the results nor anything rounded.
-//   Bound: memory, three tensors forward and five backward, at 4.2 to 5.5 TB/s (a copy reaches 5.1).  [32,1500,256] float32: forward 27 us, backward 48;
-// [16,1450,1021] bfloat16, ragged: 30 and 46 to 52; one sample of 32768 tokens of 1024 channels, bfloat16: 45.  The forms before: lanes of four channels
+//   Bound: memory, three tensors forward and five backward, at 4.2 to 5.5 TB/s (a copy reaches 5.1).  [32,1500,256] float32: forward 26 us, backward 48;
+// [16,1450,1021] bfloat16, ragged: 30 and 45 to 52; one sample of 32768 tokens of 1024 channels, bfloat16: 44.  The forms before: lanes of four channels
 // with tokens across the lanes, 43 and 74, 53 and 122, 69 (joining across lanes takes as many instructions as the recurrence).
 #include "common.h"
 #include "elements.h"
@@ -299,8 +299,9 @@ __global__ __launch_bounds__(64 * WAVES, 4) void leak_fwd_kernel(LeakArgs a, Cha
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------
 // The same chains, their tiles from the last to the first.  Inside a tile the states go forwards, from the kept one, and G backwards.
+// LOOK: 80 registers, a third workgroup on a compute unit ([32,1500,256] float32: 48 us, and 50 with 82 registers and two).
 template <typename T, int V, int DRIVE, int S, int WAVES, bool LOOK>
-__global__ __launch_bounds__(64 * WAVES, 4) void leak_bwd_kernel(LeakArgs a, Chains k) {
+__global__ __launch_bounds__(64 * WAVES, LOOK ? 6 : 4) void leak_bwd_kernel(LeakArgs a, Chains k) {
     constexpr int CH = 64 * V, kTile = S * WAVES;
     static_assert(kTile % kKept == 0, "a tile begins where a state is kept");
     __shared__ Pair total[WAVES][CH];

@@ -5,10 +5,13 @@
 // Backwards, with dt the derivative with respect to total, means over the row:
 //     dt = dtotal + (dy outer - hat mean(dy outer hat)) / rms(total),  dr = dt,  db = dt factor scale,  dz = db inner u act'(z),
 //     d = db act(z) inner,  dx = (d - u mean(d u)) / rms(x);  sums over the rows: dscale of dt factor b, dinner of db act(z) u, douter of dy hat.
-//   The norms see the sum as it is, not the one that is rounded to the stream's type.  A row lies in the registers of a wave, or of a
-// workgroup where it is longer, so that each tensor is read or written once; the backward pass makes the row again and takes the
-// reciprocals of the two rms from the forward pass.
-//   Bound: memory.
+//   The norms see the sum as it is, not the one that is rounded to the stream's type.  A row lies in the registers of a part of a wave, a wave, or
+// a workgroup where it is longer, eight channels a thread, so that each tensor is read or written once; the backward pass makes the row
+// again and takes the reciprocals of the two rms from the forward pass.  Parameters stay in registers from row to row, as do the sums of
+// their gradients; rows are summed up without LDS inside a wave.
+//   Bound: memory.  [48000,256] bfloat16, all there is: forward 23 us (5.3 TB/s), backward 39 (5.0), its sums 4.  [8192,4096] bfloat16 on a float32 stream,
+// an outer norm and a scale: 72 (5.6) and 125 (4.8), sums 5.  With four channels a thread, parameters read for every row and sums
+// through LDS the same took 44 and 93, 112 and 241.
 #include "common.h"
 #include "elements.h"
 
