@@ -74,7 +74,7 @@ def rotary(query, key, frequency, position=None, layout='halves', magnitude=1.0)
     Returns
     -------
     A pair of tensors, contiguous, of the shapes and type of query and key (None for a key that is None).  Angles are made in float64
-    and do not lose digits far out (positions up to 2**53); products are float32.  Gradients are those of query and key.
+    and do not lose digits far out (positions up to 2**53); products are float32.  Gradients are those of query and key (frequencies have none).
     """
     if layout not in LAYOUTS:
         raise ValueError(f'unknown layout {layout!r}: one of {list(LAYOUTS)}')
@@ -96,7 +96,7 @@ def rotary(query, key, frequency, position=None, layout='halves', magnitude=1.0)
         if position.device != device:
             raise RuntimeError(f'tensors on different devices: {device} and {position.device}')
         position = position.contiguous()
-    return _turn(query, key, frequency.detach().contiguous(), position, LAYOUTS[layout], float(magnitude), 0)
+    return _turn(query, key, frequency.contiguous(), position, LAYOUTS[layout], float(magnitude), 0)
 
 
 def _turn(query, key, *args):
@@ -110,24 +110,31 @@ def _rows(x):
 
 
 def _place(x):
-    """``x`` as the kernel reads it, its heads, the strides of its samples, tokens and heads, and room for the result."""
+    """``x`` as the kernel reads it, its address, its heads, the strides of its samples, tokens and heads, and room for the result."""
     if x is None:
-        return None, 0, 0, 0, 0, None
+        return None, None, 0, 0, 0, 0, None, None
     x = _rows(x)
-    stride = x.stride()
-    return (x, x.shape[-2], *stride[:-1], N.empty_as(x)) if len(stride) == 4 else (x, x.shape[-2], stride[0], 0, stride[1], N.empty_as(x))
+    out = N.empty_as(x)
+    if x.dim() == 4:
+        sample, token, head, _ = x.stride()
+    else:
+        (sample, head, _), token = x.stride(), 0
+    return x, x.data_ptr(), x.shape[-2], sample, token, head, out, out.data_ptr()
 
 
 def _run(query, key, frequency, position, layout, magnitude, inverse):
     given = query if query is not None else key
     shape = given.shape
-    query, query_heads, *query_stride, out_query = _place(query)
-    key, key_heads, *key_stride, out_key = _place(key)
+    query, a, query_heads, qn, qt, qh, out_query, to_query = _place(query)      # (the copies have to live until the launch)
+    key, b, key_heads, kn, kt, kh, out_key, to_key = _place(key)
+    width = each = 0
+    if position is not None:
+        width, each = position.element_size(), position.dim() == 2
     call = N.Rotary(shape[0], shape[1] if len(shape) == 4 else 1, query_heads, key_heads, shape[-1], 2 * frequency.shape[0],
-                    frequency.data_ptr(), N.ptr(position), 0 if position is None else position.element_size(),
-                    position is not None and position.dim() == 2, layout, N.ELEMENT_TYPES[given.dtype], magnitude, *query_stride, *key_stride)
+                    frequency.data_ptr(), N.ptr(position), width, each, layout, N.ELEMENT_TYPES[given.dtype], magnitude, qn, qt, qh,
+                    kn, kt, kh)
     with N.device_guard(given.device):
-        N.check(N.lib().slayer_rotary(N.ptr(out_query), N.ptr(out_key), N.ptr(query), N.ptr(key), call, inverse, N.stream_handle()))
+        N.check(N.lib().slayer_rotary(to_query, to_key, a, b, call, inverse, N.stream_handle()))
     return out_query, out_key
 
 
