@@ -237,3 +237,28 @@ def test_a_zero_row_and_module():
     half = x.detach().to(torch.bfloat16)
     y, total = m(half, x.detach(), half)
     assert y.dtype == torch.bfloat16 and total.dtype == torch.float32
+
+
+def test_gradients_are_differences():
+    """The derivative along a random direction from results h = 2^-6 to either side.  The difference is off by h^2 / 6 of third derivatives, which are
+    some ten times the magnitudes at most where rows are of unit size (2^-12 * 10 / 6 < 2^-10), and by the results' rounding, 80 * 2^-24 / h = 2^-12:
+    2^-9 of the sum of the terms' magnitudes."""
+    import lava_dl_amd.slayer as slayer
+    gen = torch.Generator().manual_seed(8)
+    for c in (30, 300):
+        d = make(gen, (4, c), torch.float32, torch.float32)
+        d['residual'] = d['residual'] / 2
+        got = run(d, 'silu')
+        g, gt = d['gy'].double(), d['gt'].double()
+        for k in ('input', 'residual', 'gate', 'outer', 'inner', 'scale'):
+            v = torch.randn(d[k].shape, generator=gen)
+
+            def value(sign):
+                e = {n: None if t is None else t.to(DEV) for n, t in dict(d, **{k: d[k] + sign * 2.0 ** -6 * v}).items()}
+                y, total = slayer.neuron.norm.residual_norm(e['input'], e['residual'], e['outer'], e['inner'], e['gate'], e['scale'], 'silu')
+                return y.cpu().double() * g, total.cpu().double() * gt
+            (a, b), (p, q) = value(1), value(-1)
+            slope = float((a - p).sum() + (b - q).sum()) * 2 ** 5
+            terms = got[k].cpu().double() * v.double()
+            size = float(terms.abs().sum() + a.abs().sum() + b.abs().sum())
+            assert abs(slope - float(terms.sum())) <= 2.0 ** -9 * size, (k, slope, float(terms.sum()))

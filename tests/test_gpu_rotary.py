@@ -178,3 +178,21 @@ def test_values_that_are_not_finite_stay_in_their_pair(bad):
         hit = torch.zeros_like(x, dtype=torch.bool)
         hit[0, 2, 1, list(pair)] = True
         assert torch.equal(torch.where(hit, 0, got), torch.where(hit, 0, clean)) and not torch.isfinite(got[hit]).any()
+
+
+def test_gradients_are_differences():
+    """A turn is linear, so a difference of results is the turn of the difference, and its product with any g is that of the gradient for g with the
+    difference: within 12 * 2^-24 of the magnitudes on either side, and 2^-24 of the results that are subtracted."""
+    import lava_dl_amd.slayer as slayer
+    gen = torch.Generator().manual_seed(9)
+    f = slayer.synapse.rotary_frequencies(24, device=DEV)
+    for layout in ('halves', 'pairs'):
+        x, v, g = (torch.randn(2, 30, 3, 29, generator=gen).to(DEV) for _ in range(3))
+        leaf = x.clone().requires_grad_()
+        y = slayer.synapse.rotary(leaf, None, f, layout=layout)[0]
+        grad, = torch.autograd.grad(y, leaf, g)
+        moved = slayer.synapse.rotary(x + v, None, f, layout=layout)[0]
+        difference = ((moved.double() - y.detach().double()) * g).sum()
+        step = (x + v).double() - x.double()
+        size = ((x.abs() + (x + v).abs()).double().sum(-1) * g.abs().double().amax(-1)).sum() * 2
+        assert float((difference - (grad.double() * step).sum()).abs()) <= 2 * 13 * U * float(size)
