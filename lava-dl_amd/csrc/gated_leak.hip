@@ -497,7 +497,8 @@ __global__ __launch_bounds__(256) void leak_step_kernel(LeakArgs a, int quads) {
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Channels of a lane: two bfloat16 where there are two, so that a wave reads 256 bytes of a row.
+// Channels of a lane: two bfloat16 where there are two, so that a wave reads 256 bytes of a row.  (One: [16,1450,1021], ragged, 43 us forward and 67
+// backward where two take 30 and 45 to 52; the prompt above 49, and 44.)
 int lane_of(const slayer_gated_leak* s) { return s->dtype == SLAYER_BFLOAT16 && s->channels > 1 ? 2 : 1; }
 // Tokens of a wave, of the eight waves of a workgroup: as many as leave registers for a second workgroup on a compute unit (backward, pairs of
 // bfloat16, sixteen tokens: 54 us where eight take 46).

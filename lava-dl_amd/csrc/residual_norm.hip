@@ -117,12 +117,12 @@ template <int W> __device__ __forceinline__ void parameters(float (&x)[W], const
     for (int e = 0; e < W; ++e) x[e] = p ? x[e] * factor : factor;
 }
 
-// T: x, gate and y.  R: the residual stream.  LANES threads a row, IT accesses of 16 bytes of x each.  The loop over the rows is the same for
+// T: x, gate and y.  R: the residual stream.  LANES threads a row, eight channels each in one or two accesses of 16 bytes of x.  The loop over the rows is the same for
 // all threads of a workgroup.
 template <int LANES> constexpr int rows_of() { return LANES <= 64 ? 256 / LANES : 1; }
-template <typename T, typename R, int LANES, int IT>
+template <typename T, typename R, int LANES>
 __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_fwd_kernel(ResidualArgs a) {
-    constexpr int W = Elements<T>::kVec, kRows = rows_of<LANES>();
+    constexpr int W = Elements<T>::kVec, IT = 8 / W, kRows = rows_of<LANES>();
     __shared__ float shared[16];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const float inv = 1.f / (float)a.channels;
@@ -211,9 +211,9 @@ __device__ __forceinline__ void write_part(float* part, const float (&x)[IT][W],
     }
 }
 
-template <typename T, typename R, int LANES, int IT>
+template <typename T, typename R, int LANES>
 __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel(ResidualArgs a) {
-    constexpr int W = Elements<T>::kVec, kRows = rows_of<LANES>();
+    constexpr int W = Elements<T>::kVec, IT = 8 / W, kRows = rows_of<LANES>();
     constexpr bool kAgain = LANES == 1024;     // parameters are read for every row: of 128 registers there are none to keep them in
     __shared__ float shared[kRows > 1 ? 256 * IT * W : 16];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
@@ -327,17 +327,14 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 constexpr int64_t kMostChannels = 8192;
 
-// Threads of a row and accesses of a thread: eight channels a thread, four of short float32 rows, which leaves fewer threads idle.
-struct Shape { int lanes, its, rows; int64_t fwd_blocks, bwd_blocks; };     // rows: of a workgroup at a time
-Shape shape_of(int64_t rows, int64_t channels, int dtype) {
-    const int w = dtype == SLAYER_FLOAT32 ? 4 : 8;
-    const int64_t all = (channels + w - 1) / w;
+// Threads of a row: eight channels a thread.  (Four a thread in short float32 rows: 129 us where eight take 123, [250000,128], forward.)
+struct Shape { int lanes; int64_t fwd_blocks, bwd_blocks; };
+Shape shape_of(int64_t rows, int64_t channels) {
     Shape s;
-    s.its = all <= 64 || w == 8 ? 1 : 2;
     s.lanes = 8;
-    while (s.lanes < 1024 && s.lanes * s.its < all) s.lanes *= 2;
-    s.rows = s.lanes <= 64 ? 256 / s.lanes : 1;
-    const int64_t groups = (rows + s.rows - 1) / s.rows;
+    while (s.lanes * 8 < channels) s.lanes *= 2;
+    const int together = s.lanes <= 64 ? 256 / s.lanes : 1;        // rows of a workgroup at a time
+    const int64_t groups = (rows + together - 1) / together;
     // as many workgroups as run at a time; of the backward kernel, which leaves a part of each sum for every one of them, twelve waves a
     // compute unit
     const int64_t fwd = s.lanes <= 64 ? 2048 : 524288 / s.lanes, bwd = s.lanes <= 64 ? 768 : s.lanes < 512 ? 196608 / s.lanes : 256;
@@ -365,29 +362,21 @@ ResidualArgs args_of(const slayer_residual_norm* p) {
     return a;
 }
 
-// The shapes there are: eight to 64 threads with one access, then with eight channels a thread.
-#define SHORT(T, R, LAUNCH)                          \
-    if (s.lanes == 8) LAUNCH(T, R, 8, 1);            \
-    else if (s.lanes == 16) LAUNCH(T, R, 16, 1);     \
-    else if (s.lanes == 32) LAUNCH(T, R, 32, 1);     \
-    else LAUNCH(T, R, 64, 1)
-#define LONG(T, R, IT, LAUNCH)                       \
-    if (s.lanes == 64) LAUNCH(T, R, 64, IT);         \
-    else if (s.lanes == 128) LAUNCH(T, R, 128, IT);  \
-    else if (s.lanes == 256) LAUNCH(T, R, 256, IT);  \
-    else if (s.lanes == 512) LAUNCH(T, R, 512, IT);  \
-    else LAUNCH(T, R, 1024, IT)
-#define BY_TYPE(LAUNCH)                                                          \
-    if (p->dtype == SLAYER_FLOAT32) {                                            \
-        if (s.its == 1) { SHORT(float, float, LAUNCH); }                         \
-        else { LONG(float, float, 2, LAUNCH); }                                  \
-    } else if (p->residual_dtype == SLAYER_FLOAT32) {                            \
-        if (s.lanes <= 64) { SHORT(bf16, float, LAUNCH); }                       \
-        else { LONG(bf16, float, 1, LAUNCH); }                                   \
-    } else {                                                                     \
-        if (s.lanes <= 64) { SHORT(bf16, bf16, LAUNCH); }                        \
-        else { LONG(bf16, bf16, 1, LAUNCH); }                                    \
+#define BY_LANES(T, R, LAUNCH)             \
+    switch (s.lanes) {                     \
+        case 8: LAUNCH(T, R, 8); break;    \
+        case 16: LAUNCH(T, R, 16); break;  \
+        case 32: LAUNCH(T, R, 32); break;  \
+        case 64: LAUNCH(T, R, 64); break;  \
+        case 128: LAUNCH(T, R, 128); break; \
+        case 256: LAUNCH(T, R, 256); break; \
+        case 512: LAUNCH(T, R, 512); break; \
+        default: LAUNCH(T, R, 1024);       \
     }
+#define BY_TYPE(LAUNCH)                                                          \
+    if (p->dtype == SLAYER_FLOAT32) BY_LANES(float, float, LAUNCH)               \
+    else if (p->residual_dtype == SLAYER_FLOAT32) BY_LANES(bf16, float, LAUNCH)  \
+    else BY_LANES(bf16, bf16, LAUNCH)
 
 }  // namespace
 }  // namespace slayer
@@ -396,7 +385,7 @@ using namespace slayer;
 
 extern "C" int64_t slayer_residual_norm_workspace(const slayer_residual_norm* p) {
     if (int e = check_residual(p)) return e;
-    const Shape s = shape_of(p->rows, p->channels, p->dtype);
+    const Shape s = shape_of(p->rows, p->channels);
     return 3 * s.bwd_blocks * p->channels;
 }
 
@@ -408,9 +397,9 @@ extern "C" int slayer_residual_norm_fwd(void* out, void* total, float* stats, co
         return SLAYER_ENULL;
     ResidualArgs a = args_of(p);
     a.out = out; a.total = total; a.stats = stats; a.in = input; a.residual = residual; a.gate = gate;
-    const Shape s = shape_of(p->rows, p->channels, p->dtype);
-#define LAUNCH(T, R, LANES, IT) \
-    hipLaunchKernelGGL((residual_fwd_kernel<T, R, LANES, IT>), dim3((unsigned)s.fwd_blocks), dim3(LANES <= 64 ? 256 : LANES), 0, \
+    const Shape s = shape_of(p->rows, p->channels);
+#define LAUNCH(T, R, LANES) \
+    hipLaunchKernelGGL((residual_fwd_kernel<T, R, LANES>), dim3((unsigned)s.fwd_blocks), dim3(LANES <= 64 ? 256 : LANES), 0, \
                        (hipStream_t)stream, a)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
@@ -440,13 +429,13 @@ extern "C" int slayer_residual_norm_bwd(void* grad_input, void* grad_residual, v
     ResidualArgs a = args_of(p);
     a.grad_in = grad_input; a.grad_residual = grad_residual; a.grad_gate = grad_gate; a.grad_out = grad_out; a.grad_total = grad_total;
     a.stats = (float*)stats; a.in = input; a.residual = residual; a.gate = gate;
-    const Shape s = shape_of(p->rows, p->channels, p->dtype);
+    const Shape s = shape_of(p->rows, p->channels);
     const int64_t size = s.bwd_blocks * p->channels;
     a.part_inner = grad_inner ? workspace : nullptr;
     a.part_outer = grad_outer ? workspace + size : nullptr;
     a.part_scale = grad_scale ? workspace + 2 * size : nullptr;
-#define LAUNCH(T, R, LANES, IT) \
-    hipLaunchKernelGGL((residual_bwd_kernel<T, R, LANES, IT>), dim3((unsigned)s.bwd_blocks), dim3(LANES <= 64 ? 256 : LANES), 0, \
+#define LAUNCH(T, R, LANES) \
+    hipLaunchKernelGGL((residual_bwd_kernel<T, R, LANES>), dim3((unsigned)s.bwd_blocks), dim3(LANES <= 64 ? 256 : LANES), 0, \
                        (hipStream_t)stream, a)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
