@@ -52,11 +52,11 @@ template <int DRIVE> __device__ __forceinline__ Drive drive_of(float leak, float
     return {square * r, keep * r};
 }
 
-// What a lane reads and writes of a row: one float32 or bfloat16, or two bfloat16 at any address that suits one of them.
+// What a lane reads and writes of a row: one float32 or bfloat16, or two bfloat16 at any address that suits one of them.  closed(): gates of -inf.
 template <typename T, int V> struct Piece;
-template <> struct Piece<float, 1> { typedef float Raw; };
-template <> struct Piece<bf16, 1> { typedef unsigned short Raw; };
-template <> struct Piece<bf16, 2> { typedef unsigned Raw; };
+template <> struct Piece<float, 1> { typedef float Raw; static __device__ Raw closed() { return -__builtin_inff(); } };
+template <> struct Piece<bf16, 1> { typedef unsigned short Raw; static __device__ Raw closed() { return 0xff80; } };
+template <> struct Piece<bf16, 2> { typedef unsigned Raw; static __device__ Raw closed() { return 0xff80ff80; } };
 typedef unsigned unsigned_any __attribute__((aligned(2)));
 template <int V> __device__ __forceinline__ typename Piece<bf16, V>::Raw load_piece(const bf16* p) {
     if constexpr (V == 1) return *reinterpret_cast<const unsigned short*>(p);
@@ -96,6 +96,15 @@ template <int V> struct Lane {
 // Keeps the compiler from holding on to what it has made of x: that is made again instead of taking up registers.
 __device__ __forceinline__ void forget(float& x) { asm volatile("" : "+v"(x)); }
 
+// What a few tokens keep of the state in front of them, the product of 1 - leak, and what they lose of it, by itself: each 1 - leak is a multiple
+// of 2^-24, off by the same amount at every token of a steady gate, which would add up along a sample (a leak of 2e-5 at each of 32768 tokens:
+// states 1e-3 off).  (As one float64 product: the backward walk spills.)
+__device__ __forceinline__ void hold(float& kept, float& lost, float leak, float keep) {
+    lost += fmaf(-leak, lost, leak);
+    kept *= keep;
+}
+__device__ __forceinline__ double held(float kept, float lost) { return kept < 0.5f ? (double)kept : 1.0 - (double)lost; }
+
 __device__ __forceinline__ int64_t length_of(const LeakArgs& a, int64_t n) {
     if (!a.lengths) return a.tokens;
     const int64_t length = a.lengths_bytes == 4 ? ((const int*)a.lengths)[n] : ((const int64_t*)a.lengths)[n];
@@ -111,6 +120,8 @@ __device__ __forceinline__ int64_t length_of(const LeakArgs& a, int64_t n) {
 // reads those of the tiles before it in its window, and the state in front of the window; the last tile of a window leaves the state
 // behind it.  Which values are joined, and in which order, depends on the sizes alone and not on who comes first, so that a call computed
 // again has the same bits.
+//   Spans are joined in float64 and states go from wave to wave and tile to tile in it; they are rounded where a wave walks its tokens, so that
+// a result carries the roundings of at most 16 tokens, however many there are.
 //   What is left is a word of 64 bits that says itself that it is there (the workspace is zeroed before), read and written with relaxed
 // atomics of the whole device: no other memory hangs on it, so no fences are needed.
 //   Windows of sixteen: of 32 tiles the words a thread waits for take the registers of a workgroup (backward, [16,1450,1021]: 53 us, and 46), of
@@ -124,33 +135,43 @@ struct Chains {
     int chains;
 };
 
-__device__ __forceinline__ Word pair_word(float A, float H) {      // A is no NaN of the bits that would make the upper half 0
-    const unsigned a = A != A ? 0x7fc00000u : __float_as_uint(A);
-    return (Word)~a << 32 | __float_as_uint(H);
+// A's 32 bits: from a half on those of 1 - A, the leak, with the last bit set; below a half its own, with the last bit cleared.  Either is
+// within 2^-23 of itself.  A NaN has bits that do not make the upper half 0.
+__device__ __forceinline__ Word pair_word(double A, float H) {
+    const bool slow = A >= 0.5;
+    const float f = (float)(slow ? 1.0 - A : A);
+    const unsigned a = f != f ? 0x7fc00000u : __float_as_uint(f);
+    return (Word)~((a & ~1u) | slow) << 32 | __float_as_uint(H);
 }
-__device__ __forceinline__ Word state_word(float h) { return (Word)1 << 32 | __float_as_uint(h); }
+__device__ __forceinline__ double kept_of(Word w) {
+    const unsigned a = ~(unsigned)(w >> 32);
+    const double f = (double)__uint_as_float(a & ~1u);
+    return a & 1 ? 1.0 - f : f;
+}
+__device__ __forceinline__ Word state_word(double h) { return h != h ? ~0x7ff8000000000000ull : ~(Word)__double_as_longlong(h); }
+__device__ __forceinline__ double state_of(Word w) { return __longlong_as_double((long long)~w); }
 __device__ __forceinline__ void leave(Word* p, Word w) { __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ Word look(const Word* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-struct Pair { float a, h; };
-__device__ __forceinline__ Pair then(Pair first, Pair second) { return {first.a * second.a, fmaf(second.a, first.h, second.h)}; }
+struct Pair { double a, h; };
+__device__ __forceinline__ Pair then(Pair first, Pair second) { return {first.a * second.a, fma(second.a, first.h, second.h)}; }
 
 // The pair of all tiles before tile `index` (counted in the order of the pass) in its window, and the state in front of the window
 // (`initial` in front of the first one), for channel threadIdx.x % CH: for the first CH threads.  All threads of the workgroup call it.
-struct Before { Pair pair; float state; };
+struct Before { Pair pair; double state; };
 template <int THREADS, int CH>
-__device__ __forceinline__ Before look_back(Pair (*parts)[CH], const Chains& k, int64_t index, unsigned chain, float initial) {
+__device__ __forceinline__ Before look_back(Pair (*parts)[CH], const Chains& k, int64_t index, unsigned chain, double initial) {
     constexpr int kShares = THREADS / CH, kMost = kWindow / kShares;
     const int channel = threadIdx.x % CH, share = threadIdx.x / CH;
     const int64_t window = index / kWindow, first = window * kWindow;
     const int count = (int)(index - first);                        // less than kWindow
     const int per = (count + kShares - 1) / kShares, from = share * per, mine = count - from < per ? count - from : per;
-    Before b = {{1.f, 0.f}, initial};
+    Before b = {{1.0, 0.0}, initial};
     if (count > 0) {
         const Word* pairs = k.pairs + ((first + from) * k.chains + chain) * CH + channel;
         Word words[kMost];
 #pragma unroll
-        for (int i = 0; i < kMost; ++i) words[i] = i < mine ? 0 : pair_word(1.f, 0.f);
+        for (int i = 0; i < kMost; ++i) words[i] = i < mine ? 0 : pair_word(1.0, 0.f);
         for (bool all = false; !all;) {
             all = true;
 #pragma unroll
@@ -162,7 +183,7 @@ __device__ __forceinline__ Before look_back(Pair (*parts)[CH], const Chains& k, 
         }
 #pragma unroll
         for (int i = 0; i < kMost; ++i)
-            if (i < mine) b.pair = then(b.pair, {__uint_as_float(~(unsigned)(words[i] >> 32)), __uint_as_float((unsigned)words[i])});
+            if (i < mine) b.pair = then(b.pair, {kept_of(words[i]), (double)__uint_as_float((unsigned)words[i])});
         parts[share][channel] = b.pair;
         __syncthreads();
     }
@@ -171,11 +192,11 @@ __device__ __forceinline__ Before look_back(Pair (*parts)[CH], const Chains& k, 
     if (window > 0) {
         const Word* state = k.states + (window * k.chains + chain) * CH + channel;
         Word w = look(state);
-        while (!(w >> 32)) {
+        while (w == 0) {
             __builtin_amdgcn_s_sleep(1);
             w = look(state);
         }
-        b.state = __uint_as_float((unsigned)w);
+        b.state = state_of(w);
     }
     return b;
 }
@@ -198,8 +219,8 @@ template <typename T, int V, int DRIVE, int S, int WAVES, bool LOOK>
 __global__ __launch_bounds__(64 * WAVES, 4) void leak_fwd_kernel(LeakArgs a, Chains k) {
     constexpr int CH = 64 * V, kTile = S * WAVES;
     static_assert(kKept % S == 0 && kTile % kKept == 0, "a wave begins where a state is kept");
-    __shared__ Pair total[WAVES][CH];
-    __shared__ float front[WAVES][CH];                              // the state in front of each wave
+    __shared__ double total_a[WAVES][CH];
+    __shared__ float total_h[WAVES][CH], front[WAVES][CH];          // front: the state in front of each wave
     __shared__ Pair parts[LOOK ? 64 * WAVES / CH : 1][CH];
     const Span span = span_of<LOOK>(a, k);
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -214,14 +235,16 @@ __global__ __launch_bounds__(64 * WAVES, 4) void leak_fwd_kernel(LeakArgs a, Cha
     T* out = (T*)a.out + n * a.tokens * a.channels;
     const int channel = strip * CH + threadIdx.x;                  // of the first CH threads
     const bool keeps = threadIdx.x < CH && channel < a.channels;
-    float carry = keeps && a.state ? a.state[n * a.channels + channel] : 0.f;
+    double carry = keeps && a.state ? a.state[n * a.channels + channel] : 0.f;
     for (int64_t tile = span.first; tile < span.end; ++tile) {
         const int64_t t0 = tile * kTile + wave * S;
         const int count = length - t0 < S ? (length > t0 ? (int)(length - t0) : 0) : S;
-        float keep[S][V], add[S][V];
-        Pair p[V];
+        float keep[S][V], add[S][V], kept[V], lost[V], h[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) p[v] = {1.f, 0.f};
+        for (int v = 0; v < V; ++v) {
+            kept[v] = 1;
+            lost[v] = h[v] = 0;
+        }
         if (count > 0) {
             typename Piece<T, V>::Raw x[S], z[S];
 #pragma unroll
@@ -230,6 +253,14 @@ __global__ __launch_bounds__(64 * WAVES, 4) void leak_fwd_kernel(LeakArgs a, Cha
                 x[s] = load_piece<V>(in + t * a.in_stride[1] + own.from);
                 z[s] = load_piece<V>(gate + t * a.gate_stride[1] + own.from);
             }
+            if (count < S) {                                       // what is not there leaks nothing
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+                    if (s >= count) {
+                        x[s] = 0;
+                        z[s] = Piece<T, V>::closed();
+                    }
+            }
 #pragma unroll
             for (int s = 0; s < S; ++s)
 #pragma unroll
@@ -237,50 +268,40 @@ __global__ __launch_bounds__(64 * WAVES, 4) void leak_fwd_kernel(LeakArgs a, Cha
                     const float leak = d[v] * open_gate(value_of(z[s], v));
                     keep[s][v] = 1.f - leak;
                     add[s][v] = drive_of<DRIVE>(leak, keep[s][v]).value * value_of(x[s], v);
+                    hold(kept[v], lost[v], leak, keep[s][v]);
+                    h[v] = fmaf(keep[s][v], h[v], add[s][v]);
                 }
-            if (count < S) {
-#pragma unroll
-                for (int s = 0; s < S; ++s)
-#pragma unroll
-                    for (int v = 0; v < V; ++v)
-                        if (s >= count) {
-                            keep[s][v] = 1.f;
-                            add[s][v] = 0.f;
-                        }
-            }
-#pragma unroll
-            for (int s = 0; s < S; ++s)
-#pragma unroll
-                for (int v = 0; v < V; ++v) p[v] = then(p[v], {keep[s][v], add[s][v]});
         }
 #pragma unroll
-        for (int v = 0; v < V; ++v) total[wave][own.at(v)] = p[v];
+        for (int v = 0; v < V; ++v) {
+            total_a[wave][own.at(v)] = held(kept[v], lost[v]);
+            total_h[wave][own.at(v)] = h[v];
+        }
         __syncthreads();
         if (LOOK) {
             if (threadIdx.x < CH && (tile + 1) % kWindow != 0 && tile + 1 < a.tiles) {
-                Pair all = {1.f, 0.f};
+                Pair p = {1, 0};
 #pragma unroll
-                for (int w = 0; w < WAVES; ++w) all = then(all, total[w][threadIdx.x]);
-                leave(k.pairs + (tile * k.chains + span.chain) * CH + threadIdx.x, pair_word(all.a, all.h));
+                for (int w = 0; w < WAVES; ++w) p = then(p, {total_a[w][threadIdx.x], total_h[w][threadIdx.x]});
+                leave(k.pairs + (tile * k.chains + span.chain) * CH + threadIdx.x, pair_word(p.a, (float)p.h));
             }
             const Before b = look_back<64 * WAVES, CH>(parts, k, tile, span.chain, carry);
-            carry = tile % kWindow == 0 ? b.state : fmaf(b.pair.a, b.state, b.pair.h);
+            carry = tile % kWindow == 0 ? b.state : fma(b.pair.a, b.state, b.pair.h);
         }
         if (threadIdx.x < CH) {
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                front[w][threadIdx.x] = carry;
+                front[w][threadIdx.x] = (float)carry;
                 const int64_t start = tile * (kTile / kKept) + w * S / kKept;
-                if (w * S % kKept == 0 && a.starts && keeps && start < a.kept) a.starts[(n * a.kept + start) * a.channels + channel] = carry;
-                carry = fmaf(total[w][threadIdx.x].a, carry, total[w][threadIdx.x].h);
+                if (w * S % kKept == 0 && a.starts && keeps && start < a.kept) a.starts[(n * a.kept + start) * a.channels + channel] = (float)carry;
+                carry = fma(total_a[w][threadIdx.x], carry, (double)total_h[w][threadIdx.x]);
             }
-            if (a.last && keeps && tile == a.tiles - 1) a.last[n * a.channels + channel] = carry;
+            if (a.last && keeps && tile == a.tiles - 1) a.last[n * a.channels + channel] = (float)carry;
             if (LOOK && (tile + 1) % kWindow == 0 && tile + 1 < a.tiles)
                 leave(k.states + ((tile + 1) / kWindow * k.chains + span.chain) * CH + threadIdx.x, state_word(carry));
         }
         __syncthreads();
         if (!own.on) continue;
-        float h[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = front[wave][own.at(v)];
 #pragma unroll
@@ -299,13 +320,14 @@ __global__ __launch_bounds__(64 * WAVES, 4) void leak_fwd_kernel(LeakArgs a, Cha
 
 // ---- backward -------------------------------------------------------------------------------------------------------------------
 // The same chains, their tiles from the last to the first.  Inside a tile the states go forwards, from the kept one, and G backwards.
-// LOOK: 80 registers, a third workgroup on a compute unit ([32,1500,256] float32: 48 us, and 50 with 82 registers and two).
+// LOOK: 80 registers, a third workgroup on a compute unit ([32,1500,256] float32, drive none and root: 44 and 47 us; with 84 registers and two
+// workgroups 47 and 50).  G and the states in front of the waves run through threads of their own at the same time ([256,4,4096] bfloat16: 73 us, and 79).
 template <typename T, int V, int DRIVE, int S, int WAVES, bool LOOK>
 __global__ __launch_bounds__(64 * WAVES, LOOK ? 6 : 4) void leak_bwd_kernel(LeakArgs a, Chains k) {
     constexpr int CH = 64 * V, kTile = S * WAVES;
     static_assert(kTile % kKept == 0, "a tile begins where a state is kept");
-    __shared__ Pair total[WAVES][CH];
-    __shared__ float total_g[WAVES][CH];
+    __shared__ double total_a[WAVES][CH];
+    __shared__ float total_h[WAVES][CH], total_g[WAVES][CH];
     __shared__ float front[WAVES][CH], behind[WAVES][CH];           // the state in front of each wave, G behind it
     __shared__ Pair parts[LOOK ? 64 * WAVES / CH : 1][CH];
     const Span span = span_of<LOOK>(a, k);
@@ -324,22 +346,22 @@ __global__ __launch_bounds__(64 * WAVES, LOOK ? 6 : 4) void leak_bwd_kernel(Leak
     const T* grad = (const T*)a.grad + n * a.grad_stride[0];
     T* grad_in = (T*)a.grad_in + n * a.tokens * a.channels;
     T* grad_gate = (T*)a.grad_gate + n * a.tokens * a.channels;
-    const int channel = strip * CH + threadIdx.x;                  // of the first CH threads
-    const bool keeps = threadIdx.x < CH && channel < a.channels;
-    float carry = keeps && a.grad_last ? a.grad_last[n * a.channels + channel] : 0.f;
+    // the first CH threads have a channel of G each, the next ones a channel of the states
+    const int at = threadIdx.x % CH, role = threadIdx.x / CH, channel = strip * CH + at;
+    const bool keeps = role == 0 && channel < a.channels;
+    double carry = keeps && a.grad_last ? a.grad_last[n * a.channels + channel] : 0.f;
     for (int64_t index = span.first; index < span.end; ++index) {   // counted from the last tile
         const int64_t tile = a.tiles - 1 - index, t0 = tile * kTile + wave * S;
         const int count = length - t0 < S ? (length > t0 ? (int)(length - t0) : 0) : S;
-        float start = 0;
-        if (keeps) start = a.starts[(n * a.kept + tile * (kTile / kKept)) * a.channels + channel];
+        double start = 0;
+        if (role == 1 && channel < a.channels) start = a.starts[(n * a.kept + tile * (kTile / kKept)) * a.channels + channel];
         float open[S][V];
         typename Piece<T, V>::Raw x[S], dy[S];
-        Pair p[V];
-        float g[V];
+        float kept[V], lost[V], h[V], g[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            p[v] = {1.f, 0.f};
-            g[v] = 0;
+            kept[v] = 1;
+            lost[v] = h[v] = g[v] = 0;
         }
         if (count > 0) {
             typename Piece<T, V>::Raw z[S];
@@ -368,7 +390,9 @@ __global__ __launch_bounds__(64 * WAVES, LOOK ? 6 : 4) void leak_bwd_kernel(Leak
 #pragma unroll
                 for (int s = 0; s < S; ++s) {
                     const float leak = d[v] * open[s][v], keep = 1.f - leak;
-                    p[v] = then(p[v], {keep, drive_of<DRIVE>(leak, keep).value * value_of(x[s], v)});
+                    h[v] = fmaf(keep, h[v], drive_of<DRIVE>(leak, keep).value * value_of(x[s], v));
+                    hold(kept[v], lost[v], leak, keep);
+                    forget(kept[v]);
                 }
 #pragma unroll
                 for (int s = S - 1; s >= 0; --s) g[v] = fmaf(-d[v], open[s][v], 1.f) * (value_of(dy[s], v) + g[v]);
@@ -376,33 +400,35 @@ __global__ __launch_bounds__(64 * WAVES, LOOK ? 6 : 4) void leak_bwd_kernel(Leak
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            total[wave][own.at(v)] = p[v];
+            total_a[wave][own.at(v)] = held(kept[v], lost[v]);
+            total_h[wave][own.at(v)] = h[v];
             total_g[wave][own.at(v)] = g[v];
         }
         __syncthreads();
         if (LOOK) {
-            if (threadIdx.x < CH && (index + 1) % kWindow != 0 && index + 1 < a.tiles) {
-                Pair all = {1.f, 0.f};
+            if (role == 0 && (index + 1) % kWindow != 0 && index + 1 < a.tiles) {
+                Pair p = {1, 0};
 #pragma unroll
-                for (int w = WAVES - 1; w >= 0; --w) all = then(all, {total[w][threadIdx.x].a, total_g[w][threadIdx.x]});
-                leave(k.pairs + (index * k.chains + span.chain) * CH + threadIdx.x, pair_word(all.a, all.h));
+                for (int w = WAVES - 1; w >= 0; --w) p = then(p, {total_a[w][at], total_g[w][at]});
+                leave(k.pairs + (index * k.chains + span.chain) * CH + at, pair_word(p.a, (float)p.h));
             }
             const Before b = look_back<64 * WAVES, CH>(parts, k, index, span.chain, carry);
-            carry = index % kWindow == 0 ? b.state : fmaf(b.pair.a, b.state, b.pair.h);
+            carry = index % kWindow == 0 ? b.state : fma(b.pair.a, b.state, b.pair.h);
         }
-        if (threadIdx.x < CH) {
+        if (role == 0) {
 #pragma unroll
             for (int w = WAVES - 1; w >= 0; --w) {
-                behind[w][threadIdx.x] = carry;
-                carry = fmaf(total[w][threadIdx.x].a, carry, total_g[w][threadIdx.x]);
+                behind[w][at] = (float)carry;
+                carry = fma(total_a[w][at], carry, (double)total_g[w][at]);
             }
-            if (a.grad_state && keeps && tile == 0) a.grad_state[n * a.channels + channel] = carry;
+            if (a.grad_state && keeps && tile == 0) a.grad_state[n * a.channels + channel] = (float)carry;
             if (LOOK && (index + 1) % kWindow == 0 && index + 1 < a.tiles)
-                leave(k.states + ((index + 1) / kWindow * k.chains + span.chain) * CH + threadIdx.x, state_word(carry));
+                leave(k.states + ((index + 1) / kWindow * k.chains + span.chain) * CH + at, state_word(carry));
+        } else if (role == 1) {
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                front[w][threadIdx.x] = start;
-                start = fmaf(total[w][threadIdx.x].a, start, total[w][threadIdx.x].h);
+                front[w][at] = (float)start;
+                start = fma(total_a[w][at], start, (double)total_h[w][at]);
             }
         }
         __syncthreads();
@@ -411,13 +437,13 @@ __global__ __launch_bounds__(64 * WAVES, LOOK ? 6 : 4) void leak_bwd_kernel(Leak
             float before[S][V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                float h = front[wave][own.at(v)];
+                h[v] = front[wave][own.at(v)];
 #pragma unroll
                 for (int s = 0; s < S; ++s) {
                     forget(open[s][v]);
-                    before[s][v] = h;
+                    before[s][v] = h[v];
                     const float leak = d[v] * open[s][v], keep = 1.f - leak;
-                    h = fmaf(keep, h, drive_of<DRIVE>(leak, keep).value * value_of(x[s], v));
+                    h[v] = fmaf(keep, h[v], drive_of<DRIVE>(leak, keep).value * value_of(x[s], v));
                 }
                 g[v] = behind[wave][own.at(v)];
             }
@@ -487,8 +513,8 @@ __global__ __launch_bounds__(256) void leak_step_kernel(LeakArgs a, int quads) {
     f4 h = load_four(a.last + n * a.channels + c, left);
 #pragma unroll
     for (int v = 0; v < 4; ++v) {
-        const float leak = d[v] * open_gate((float)z[v]), keep = 1.f - leak;
-        h[v] = fmaf(keep, h[v], drive_of<DRIVE>(leak, keep).value * (float)x[v]);
+        const float leak = d[v] * open_gate((float)z[v]), add = drive_of<DRIVE>(leak, 1.f - leak).value * (float)x[v];
+        h[v] = (float)fma(1.0 - (double)leak, (double)h[v], (double)add);
     }
     store_four(a.last + n * a.channels + c, h, left);
     store_four((T*)a.out + n * a.channels + c, h, left);

@@ -71,7 +71,7 @@ def gated_leak_step(input, gate, decay, state, drive='gain'):
         float32 or bfloat16 GPU tensors [N, C] of one type.
     decay, drive : as for ``gated_leak``.
     state : torch.Tensor
-        float32 [N, C], contiguous.
+        float32 [N, C], contiguous.  It is rounded at every call: a leak below 2**-25 leaves it as it is.
 
     Returns
     -------
