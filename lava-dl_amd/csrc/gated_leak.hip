@@ -335,7 +335,8 @@ __global__ __launch_bounds__(64 * WAVES, LOOK ? 6 : 4) void leak_bwd_kernel(Leak
     const int strip = span.chain % (unsigned)a.strips;
     const int64_t n = span.chain / (unsigned)a.strips, length = length_of(a, n);
     const Lane<V> own(strip, lane, a.channels);
-    float d[V], slopes[V];                                          // slopes: sum of dleak * open
+    float d[V];
+    double slopes[V];                                               // sum of dleak * open: of a tile in float32, of the tiles of a walk in float64
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         d[v] = a.decay[a.decays == 1 ? 0 : own.from + v] * (1.f / 4096.f);
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(64 * WAVES, LOOK ? 6 : 4) void leak_bwd_kernel(Leak
         __syncthreads();
         if (!own.on) continue;
         if (count > 0) {
-            float before[S][V];
+            float before[S][V], slope[V] = {};
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 h[v] = front[wave][own.at(v)];
@@ -460,12 +461,14 @@ __global__ __launch_bounds__(64 * WAVES, LOOK ? 6 : 4) void leak_bwd_kernel(Leak
                     const float dleak = D * fmaf(drive.slope, value_of(x[s], v), -before[s][v]);
                     dx[v] = drive.value * D;
                     dz[v] = dleak * leak * (1.f - open[s][v]);
-                    slopes[v] = fmaf(dleak, open[s][v], slopes[v]);
+                    slope[v] = fmaf(dleak, open[s][v], slope[v]);
                     g[v] = keep * D;
                 }
                 own.store(grad_in + (t0 + s) * a.channels, dx);
                 own.store(grad_gate + (t0 + s) * a.channels, dz);
             }
+#pragma unroll
+            for (int v = 0; v < V; ++v) slopes[v] += slope[v];
         }
 #pragma unroll
         for (int s = 0; s < S; ++s)
@@ -479,7 +482,7 @@ __global__ __launch_bounds__(64 * WAVES, LOOK ? 6 : 4) void leak_bwd_kernel(Leak
     // the decays' gradient of this workgroup's tiles: a row of `parts` for all workgroups of a sample's strips, or one number a workgroup
     __syncthreads();                                                // (front has been read)
 #pragma unroll
-    for (int v = 0; v < V; ++v) front[wave][own.at(v)] = slopes[v];
+    for (int v = 0; v < V; ++v) front[wave][own.at(v)] = (float)slopes[v];
     __syncthreads();
     if (threadIdx.x >= CH) return;
     float sum = 0;
