@@ -698,7 +698,8 @@ int slayer_dropout(void *out, const void *in, int dtype, int64_t n, int64_t step
 /* Gated leak: the leaky integrator whose leak a token's gate opens, for every sample and channel
  *     leak[t] = decay / 4096 * sigmoid(gate[t]),   h[t] = (1 - leak[t]) h[t-1] + drive(leak[t]) * input[t],   h[-1] = state,
  * drive 0: 1, 1: leak, 2: sqrt(leak (2 - leak)).  input and gate are [samples][tokens][channels] with strides (in elements) of their first
- * two axes and neighbouring elements on the last; out and the gradients are contiguous.  Lengths as for leaky attention. */
+ * two axes and neighbouring elements on the last; out and the gradients are contiguous.  Lengths as for leaky attention.  Samples times strips
+ * of 64 channels (of 128 for bfloat16) are fewer than 2^23, of all calls: SLAYER_ERANGE. */
 typedef struct slayer_gated_leak {
     int64_t samples, tokens, channels;
     int64_t num_decays;                             /* 1 or channels */
@@ -721,7 +722,8 @@ int slayer_gated_leak_fwd(void *out, float *last, float *starts, const void *inp
 int slayer_gated_leak_bwd(void *grad_input, void *grad_gate, float *grad_decay, float *grad_state, const void *grad_out,
                           const float *grad_last, const void *input, const void *gate, const float *starts,
                           const slayer_gated_leak *a, float *workspace, int64_t workspace_floats, void *stream);
-/* One token a sample (tokens, lengths and the token strides are not looked at): state is updated in place. */
+/* One token a sample: state is updated in place.  tokens, lengths and the token strides are not used, but the structure is checked as for
+ * the other calls (tokens 1, lengths NULL will do). */
 int slayer_gated_leak_step(void *out, float *state, const void *input, const void *gate, const slayer_gated_leak *a, void *stream);
 
 /* Rotary positions: pairs of a head's first `turned` features turned by position * frequency[i], i < turned / 2, and scaled by

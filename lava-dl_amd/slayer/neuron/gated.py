@@ -15,8 +15,8 @@ def gated_leak(input, gate, decay, state=None, lengths=None, drive='gain', retur
     Parameters
     ----------
     input, gate : torch.Tensor
-        float32 or bfloat16 GPU tensors [N, T, C] of one type.  Any strides: what has neighbouring elements along the last axis is
-        read where it lies (two views of one projection, say), what has not is copied first.
+        float32 or bfloat16 GPU tensors [N, T, C] of one type, N * ceil(C / 64) below 2**23 (C / 128 for bfloat16).  Any strides: what
+        has neighbouring elements along the last axis is read where it lies (two views of one projection, say), what has not is copied first.
     decay : torch.Tensor
         float32, one value or one for each channel: the 12-bit decay of an open gate, 0 to 4096 (a state that an open gate
         replaces).  Need not be whole; may be trained.  1 - decay / 4096 is the least that a token keeps of the state.
@@ -68,7 +68,7 @@ def gated_leak_step(input, gate, decay, state, drive='gain'):
     Parameters
     ----------
     input, gate : torch.Tensor
-        float32 or bfloat16 GPU tensors [N, C] of one type.
+        float32 or bfloat16 GPU tensors [N, C] of one type, N and C as for ``gated_leak``.
     decay, drive : as for ``gated_leak``.
     state : torch.Tensor
         float32 [N, C], contiguous.  It is rounded at every call: a leak below 2**-25 leaves it as it is.
