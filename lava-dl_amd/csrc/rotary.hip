@@ -3,7 +3,8 @@
 // (c x - s y, c y + s x); the pairs are (i, i + turned / 2) or (2i, 2i + 1), features behind the first `turned` are copied.  The gradient is
 // the same call with the angle's sign changed.
 //   Angles: the whole turns are taken off in float64, with what the roundings of the products leave, so that a far position costs no
-// digits; sine and cosine of the rest are float32.  All heads of a token share them: a workgroup makes those of its tokens once, in LDS.
+// digits; sine and cosine are those of the rest in float32, turned on by what its rounding leaves.  All heads of a token share them: a
+// workgroup makes those of its tokens once, in LDS.
 //   Bound: memory, each tensor read and written once.  [64,1000,8,64] bfloat16, queries and keys from a projection: 52 us (5.0 TB/s); [16,1450,8,80]
 // float32 with 48 features turned: 42 (5.7 TB/s).  One token of 256 samples, 16 heads of 128: 4.2 us, a launch and two steps that wait for memory.
 #include "common.h"
@@ -108,10 +109,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         constexpr double kHigh = 0x1.45f306dc9c883p-3, kLow = -0x1.6b01ec5417056p-57;           // 1 / (2 pi)
         const double radians = a.frequency[i - t * a.pairs], f = radians * kHigh, turns = positions[t] * f;
         const double rest = (turns - rint(turns)) + (fma(positions[t], f, -turns) + positions[t] * fma(radians, kLow, fma(radians, kHigh, -f)));
+        const float near = (float)rest, left = (float)((rest - (double)near) * 6.283185307179586);
         float s, c;
-        sincospif(2.f * (float)rest, &s, &c);
-        cosines[i] = a.magnitude * c;
-        sines[i] = a.sign * a.magnitude * s;
+        sincospif(2.f * near, &s, &c);
+        cosines[i] = a.magnitude * fmaf(-left, s, c);
+        sines[i] = a.sign * a.magnitude * fmaf(left, c, s);
     }
     __syncthreads();
     while (token < count) {

@@ -1,0 +1,33 @@
+"""The sines and cosines of rotary positions to float32's digits, of small values too.
+
+Tolerance, relative.  U = 2^-24.  Sine and cosine of the angle's nearest float32 are within two units in the last place, 4 U; what that rounding
+leaves of the angle, at most 2 U, is taken in with one rounding more, and terms of second order are 4 U^2 absolute: 5 U and 2^-45, with 2^-50 for the
+reference's own angle in float64."""
+import pytest
+import torch
+
+from tests.test_gpu_rotary import angles
+
+pytestmark = pytest.mark.gpu
+
+DEV, U = 'cuda:0', 2.0 ** -24
+
+
+@pytest.mark.parametrize('inverse', [False, True])
+def test_sines_and_cosines(inverse):
+    import lava_dl_amd.slayer as slayer
+    gen = torch.Generator().manual_seed(51)
+    frequency = torch.cat([slayer.synapse.rotary_frequencies(64), torch.tensor([3.1415, 1.5708, 0.7854, 2.3562], dtype=torch.float64)])
+    position = torch.cat([torch.arange(300), torch.randint(0, 1 << 40, (100,), generator=gen)])
+    angle = angles(position, frequency)
+    f = len(frequency)
+    x = torch.zeros(1, 400, 1, 2 * f)
+    x[..., :f] = 1                                                        # (1, 0) becomes (cosine, sine)
+    x = x.to(DEV).requires_grad_()
+    y, _ = slayer.synapse.rotary(x, None, frequency.to(DEV), position[None].to(DEV))
+    if inverse:
+        y, = torch.autograd.grad(y, x, x.detach())
+    got = y.detach()[0, :, 0].cpu().double()
+    want = torch.cat([angle.cos(), -angle.sin() if inverse else angle.sin()], -1)
+    over = (got - want).abs() - (5 * U * want.abs() + 2.0 ** -45 + 2.0 ** -50)
+    assert float(over.max()) <= 0, (float(over.max() / U), float(((got - want) / want / U)[want != 0].abs().max()))
