@@ -6,7 +6,7 @@
 //     dt = dtotal + (dy outer - hat mean(dy outer hat)) / rms(total),  dr = dt,  db = dt factor scale,  dz = db inner u act'(z),
 //     d = db act(z) inner,  dx = (d - u mean(d u)) / rms(x);  sums over the rows: dscale of dt factor b, dinner of db act(z) u, douter of dy hat.
 //   The norms see the sum as it is, not the one that is rounded to the stream's type.  A row lies in the registers of a part of a wave, a wave, or
-// a workgroup where it is longer, eight channels a thread, so that each tensor is read or written once; the backward pass makes the row
+// a workgroup where it is longer, four or eight channels a thread, so that each tensor is read or written once; the backward pass makes the row
 // again and takes the reciprocals of the two rms from the forward pass.  Parameters stay in registers from row to row, as do the sums of
 // their gradients; rows are summed up without LDS inside a wave.
 //   Bound: memory.  [48000,256] bfloat16, all there is: forward 23 us (5.3 TB/s), backward 39 (5.0), its sums 4.  [8192,4096] bfloat16 on a float32 stream,
@@ -117,12 +117,12 @@ template <int W> __device__ __forceinline__ void parameters(float (&x)[W], const
     for (int e = 0; e < W; ++e) x[e] = p ? x[e] * factor : factor;
 }
 
-// T: x, gate and y.  R: the residual stream.  LANES threads a row, eight channels each in one or two accesses of 16 bytes of x.  The loop over the rows is the same for
+// T: x, gate and y.  R: the residual stream.  LANES threads a row, IT accesses of 16 bytes of x each.  The loop over the rows is the same for
 // all threads of a workgroup.
 template <int LANES> constexpr int rows_of() { return LANES <= 64 ? 256 / LANES : 1; }
-template <typename T, typename R, int LANES>
+template <typename T, typename R, int LANES, int IT>
 __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_fwd_kernel(ResidualArgs a) {
-    constexpr int W = Elements<T>::kVec, IT = 8 / W, kRows = rows_of<LANES>();
+    constexpr int W = Elements<T>::kVec, kRows = rows_of<LANES>();
     __shared__ float shared[16];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
     const float inv = 1.f / (float)a.channels;
@@ -211,9 +211,9 @@ __device__ __forceinline__ void write_part(float* part, const float (&x)[IT][W],
     }
 }
 
-template <typename T, typename R, int LANES>
+template <typename T, typename R, int LANES, int IT>
 __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel(ResidualArgs a) {
-    constexpr int W = Elements<T>::kVec, IT = 8 / W, kRows = rows_of<LANES>();
+    constexpr int W = Elements<T>::kVec, kRows = rows_of<LANES>();
     constexpr bool kAgain = LANES == 1024;     // parameters are read for every row: of 128 registers there are none to keep them in
     __shared__ float shared[kRows > 1 ? 256 * IT * W : 16];
     const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
@@ -327,19 +327,24 @@ __global__ __launch_bounds__(LANES <= 64 ? 256 : LANES) void residual_bwd_kernel
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 constexpr int64_t kMostChannels = 8192;
 
-// Threads of a row: eight channels a thread.  (Four a thread in short float32 rows: 129 us where eight take 123, [250000,128], forward.)
-struct Shape { int lanes; int64_t fwd_blocks, bwd_blocks; };
-Shape shape_of(int64_t rows, int64_t channels) {
+// Threads of a row and accesses of a thread: eight channels a thread.  Four in float32 rows of up to 256 channels, which leaves fewer threads idle and
+// less to do before a row's sum: forward / forward and backward, us, four and eight: [800,128] 3.4 / 11.4 and 4.4 / 13.7, [20000,128] 9.8 / 30.5 and
+// 10.5 / 33.3, [60000,256] 51.1 / 155 and 51.0 / 159.  Forward passes over more than the last-level cache holds take eight: [250000,100] 106 and 103,
+// [250000,128] 129 and 125.
+struct Shape { int lanes, its; int64_t blocks; };
+Shape shape_of(const slayer_residual_norm* p, bool backward) {
+    const bool four = p->dtype == SLAYER_FLOAT32 && p->channels <= 256 && (backward || p->rows * p->channels < 20000000);
+    const int each = four ? 4 : 8;
     Shape s;
+    s.its = p->dtype == SLAYER_FLOAT32 && !four ? 2 : 1;
     s.lanes = 8;
-    while (s.lanes * 8 < channels) s.lanes *= 2;
+    while (s.lanes * each < p->channels) s.lanes *= 2;
     const int together = s.lanes <= 64 ? 256 / s.lanes : 1;        // rows of a workgroup at a time
-    const int64_t groups = (rows + together - 1) / together;
+    const int64_t groups = (p->rows + together - 1) / together;
     // as many workgroups as run at a time; of the backward kernel, which leaves a part of each sum for every one of them, twelve waves a
     // compute unit
-    const int64_t fwd = s.lanes <= 64 ? 2048 : 524288 / s.lanes, bwd = s.lanes <= 64 ? 768 : s.lanes < 512 ? 196608 / s.lanes : 256;
-    s.fwd_blocks = groups < fwd ? groups : fwd;
-    s.bwd_blocks = groups < bwd ? groups : bwd;
+    const int64_t most = backward ? (s.lanes <= 64 ? 768 : s.lanes < 512 ? 196608 / s.lanes : 256) : s.lanes <= 64 ? 2048 : 524288 / s.lanes;
+    s.blocks = groups < most ? groups : most;
     return s;
 }
 
@@ -362,21 +367,32 @@ ResidualArgs args_of(const slayer_residual_norm* p) {
     return a;
 }
 
-#define BY_LANES(T, R, LAUNCH)             \
-    switch (s.lanes) {                     \
-        case 8: LAUNCH(T, R, 8); break;    \
-        case 16: LAUNCH(T, R, 16); break;  \
-        case 32: LAUNCH(T, R, 32); break;  \
-        case 64: LAUNCH(T, R, 64); break;  \
-        case 128: LAUNCH(T, R, 128); break; \
-        case 256: LAUNCH(T, R, 256); break; \
-        case 512: LAUNCH(T, R, 512); break; \
-        default: LAUNCH(T, R, 1024);       \
+#define SHORT(T, R, IT, LAUNCH)                 \
+    switch (s.lanes) {                          \
+        case 8: LAUNCH(T, R, 8, IT); break;     \
+        case 16: LAUNCH(T, R, 16, IT); break;   \
+        case 32: LAUNCH(T, R, 32, IT); break;   \
+        default: LAUNCH(T, R, 64, IT);          \
     }
-#define BY_TYPE(LAUNCH)                                                          \
-    if (p->dtype == SLAYER_FLOAT32) BY_LANES(float, float, LAUNCH)               \
-    else if (p->residual_dtype == SLAYER_FLOAT32) BY_LANES(bf16, float, LAUNCH)  \
-    else BY_LANES(bf16, bf16, LAUNCH)
+#define LONG(T, R, IT, LAUNCH)                  \
+    switch (s.lanes) {                          \
+        case 128: LAUNCH(T, R, 128, IT); break; \
+        case 256: LAUNCH(T, R, 256, IT); break; \
+        case 512: LAUNCH(T, R, 512, IT); break; \
+        default: LAUNCH(T, R, 1024, IT);        \
+    }
+#define BY_TYPE(LAUNCH)                                                       \
+    if (p->dtype == SLAYER_FLOAT32) {                                         \
+        if (s.its == 1) SHORT(float, float, 1, LAUNCH)                        \
+        else if (s.lanes <= 64) SHORT(float, float, 2, LAUNCH)                \
+        else LONG(float, float, 2, LAUNCH)                                    \
+    } else if (p->residual_dtype == SLAYER_FLOAT32) {                         \
+        if (s.lanes <= 64) SHORT(bf16, float, 1, LAUNCH)                      \
+        else LONG(bf16, float, 1, LAUNCH)                                     \
+    } else {                                                                  \
+        if (s.lanes <= 64) SHORT(bf16, bf16, 1, LAUNCH)                       \
+        else LONG(bf16, bf16, 1, LAUNCH)                                      \
+    }
 
 }  // namespace
 }  // namespace slayer
@@ -385,8 +401,7 @@ using namespace slayer;
 
 extern "C" int64_t slayer_residual_norm_workspace(const slayer_residual_norm* p) {
     if (int e = check_residual(p)) return e;
-    const Shape s = shape_of(p->rows, p->channels);
-    return 3 * s.bwd_blocks * p->channels;
+    return 3 * shape_of(p, true).blocks * p->channels;
 }
 
 extern "C" int slayer_residual_norm_fwd(void* out, void* total, float* stats, const void* input, const void* residual, const void* gate,
@@ -397,9 +412,9 @@ extern "C" int slayer_residual_norm_fwd(void* out, void* total, float* stats, co
         return SLAYER_ENULL;
     ResidualArgs a = args_of(p);
     a.out = out; a.total = total; a.stats = stats; a.in = input; a.residual = residual; a.gate = gate;
-    const Shape s = shape_of(p->rows, p->channels);
-#define LAUNCH(T, R, LANES) \
-    hipLaunchKernelGGL((residual_fwd_kernel<T, R, LANES>), dim3((unsigned)s.fwd_blocks), dim3(LANES <= 64 ? 256 : LANES), 0, \
+    const Shape s = shape_of(p, false);
+#define LAUNCH(T, R, LANES, IT) \
+    hipLaunchKernelGGL((residual_fwd_kernel<T, R, LANES, IT>), dim3((unsigned)s.blocks), dim3(LANES <= 64 ? 256 : LANES), 0, \
                        (hipStream_t)stream, a)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
@@ -429,13 +444,13 @@ extern "C" int slayer_residual_norm_bwd(void* grad_input, void* grad_residual, v
     ResidualArgs a = args_of(p);
     a.grad_in = grad_input; a.grad_residual = grad_residual; a.grad_gate = grad_gate; a.grad_out = grad_out; a.grad_total = grad_total;
     a.stats = (float*)stats; a.in = input; a.residual = residual; a.gate = gate;
-    const Shape s = shape_of(p->rows, p->channels);
-    const int64_t size = s.bwd_blocks * p->channels;
+    const Shape s = shape_of(p, true);
+    const int64_t size = s.blocks * p->channels;
     a.part_inner = grad_inner ? workspace : nullptr;
     a.part_outer = grad_outer ? workspace + size : nullptr;
     a.part_scale = grad_scale ? workspace + 2 * size : nullptr;
-#define LAUNCH(T, R, LANES) \
-    hipLaunchKernelGGL((residual_bwd_kernel<T, R, LANES>), dim3((unsigned)s.bwd_blocks), dim3(LANES <= 64 ? 256 : LANES), 0, \
+#define LAUNCH(T, R, LANES, IT) \
+    hipLaunchKernelGGL((residual_bwd_kernel<T, R, LANES, IT>), dim3((unsigned)s.blocks), dim3(LANES <= 64 ? 256 : LANES), 0, \
                        (hipStream_t)stream, a)
     BY_TYPE(LAUNCH)
 #undef LAUNCH
@@ -447,6 +462,6 @@ extern "C" int slayer_residual_norm_bwd(void* grad_input, void* grad_residual, v
             c.out[count] = wanted[i];
             c.parts[count++] = workspace + i * size;
         }
-    c.rows = s.bwd_blocks; c.columns = c.pitch = p->channels; c.factor = 1.f;
+    c.rows = s.blocks; c.columns = c.pitch = p->channels; c.factor = 1.f;
     return launch_column_sums(c, count, (hipStream_t)stream);
 }
