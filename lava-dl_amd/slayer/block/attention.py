@@ -2,12 +2,12 @@
 position, group norm of each head's result with an activation, dropout from a counter, between two dense projections."""
 import torch
 
-from .types import KeepsTypes
 from ..neuron.base import P_SCALE
 from ..neuron.dropout import CounterDropout
 from ..neuron.norm import GroupNorm
 from ..synapse.attention import leaky_attention, leaky_attention_step
 from ..synapse.rotary import rotary
+from ..utils.types import KeepsTypes
 
 
 class LeakyAttention(KeepsTypes):

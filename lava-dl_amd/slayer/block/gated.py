@@ -1,9 +1,9 @@
 """A token-mixing layer of gated leaky integrators between two dense projections."""
 import torch
 
-from .types import KeepsTypes
 from ..neuron.base import P_SCALE
 from ..neuron.gated import gated_leak, gated_leak_step
+from ..utils.types import KeepsTypes
 
 
 class GatedLeak(KeepsTypes):

@@ -11,6 +11,7 @@ slayer_residual_norm_fwd / bwd."""
 import torch
 
 from .. import _native as N
+from ..utils.types import KeepsTypes
 
 
 def _identity(x, descale=False):
@@ -379,9 +380,10 @@ class _ResidualNorm(torch.autograd.Function):
         return (*grads, *sums, None, None, None, None)
 
 
-class ResidualNorm(torch.nn.Module):
+class ResidualNorm(KeepsTypes):
     """:func:`residual_norm` with trained weights: ``inner`` and ``outer`` say which of the two norms there are, ``scale`` is the residual
-    scale that every channel starts with (None: there is none), ``activation`` that of the gate, where ``forward`` is given one."""
+    scale that every channel starts with (None: there is none), ``activation`` that of the gate, where ``forward`` is given one.  The
+    weights are float32 whatever the type of the module (``.to(torch.bfloat16)``)."""
 
     def __init__(self, num_channels, inner=True, outer=True, scale=None, activation='sigmoid', eps=1e-5):
         super().__init__()
