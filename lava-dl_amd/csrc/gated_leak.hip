@@ -10,9 +10,11 @@
 // behind the other, make a tile; their pairs meet in LDS, where one thread a channel runs through them, and with the state in front of it each
 // wave walks its tokens again in its registers.  The backward pass makes the states of a tile again from the one in front of it, which the
 // forward pass has kept (one in 64 tokens), so that it reads neither the results nor anything rounded.
-//   Bound: memory, three tensors forward and five backward, at 4.2 to 5.5 TB/s (a copy reaches 5.1).  [32,1500,256] float32: forward 26 us, backward 48;
-// [16,1450,1021] bfloat16, ragged: 30 and 45 to 52; one sample of 32768 tokens of 1024 channels, bfloat16: 44.  The forms before: lanes of four channels
-// with tokens across the lanes, 43 and 74, 53 and 122, 69 (joining across lanes takes as many instructions as the recurrence).
+//   Bound: memory, three tensors forward and five backward (a copy reaches 5.1 TB/s).  [32,1500,256] float32: forward 30 us (5.0 TB/s), backward 48 (5.1);
+// one sample of 32768 tokens of 1024 channels, bfloat16: 47 (4.3).  Not so samples of different lengths, where what lies behind an end is written and not
+// read: [16,1450,1021] bfloat16, half of it behind ends, 34 and 53 us, 2.8 and 3.1 TB/s (likely tiles that wait for each other; vector instructions
+// 46 and 69 % of the cycles); nor a few tokens, which leave waves of a tile idle: [256,4,4096] bfloat16 77 and 74 us.  The forms before: lanes of four channels with
+// tokens across the lanes, 43 and 74, 53 and 122, prompt 69 (joining across lanes takes as many instructions as the recurrence).
 #include "common.h"
 #include "elements.h"
 
@@ -129,8 +131,8 @@ __device__ __forceinline__ int64_t length_of(const LeakArgs& a, int64_t n) {
 // a result carries the roundings of at most 16 tokens, however many there are.
 //   What is left is a word of 64 bits that says itself that it is there (the workspace is zeroed before), read and written with relaxed
 // atomics of the whole device: no other memory hangs on it, so no fences are needed.
-//   Windows of sixteen: of 32 tiles the words a thread waits for take the registers of a workgroup (backward, [16,1450,1021]: 53 us, and 46), of
-// eight the states have too far to go (one sample of 65536 tokens of 256 channels: forward 67 us, and 43).
+//   Windows of sixteen: of 32 tiles the words a thread waits for take the registers of a workgroup (backward, [16,1450,1021]: 57 us, and 51; one sample of
+// 65536 tokens of 256 float32 channels gains, forward 44 us, and 49), of eight the states have too far to go (that sample: 69 us).
 typedef unsigned long long Word;
 constexpr int kWindow = 16;                    // tiles of a window
 constexpr int kApart = 16;                     // words from one chain's ticket to the next: a cache line each
@@ -531,11 +533,11 @@ __global__ __launch_bounds__(256) void leak_step_kernel(LeakArgs a, int quads) {
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Channels of a lane: two bfloat16 where there are two, so that a wave reads 256 bytes of a row.  (One: [16,1450,1021], ragged, 43 us forward and 67
-// backward where two take 30 and 45 to 52; the prompt above 49, and 44.)
+// Channels of a lane: two bfloat16 where there are two, so that a wave reads 256 bytes of a row.  (One: [16,1450,1021], ragged, 42 us forward and 67
+// backward where two take 33 and 51; the prompt above 52 and 98 where two take 50 and 102.)
 int lane_of(const slayer_gated_leak* s) { return s->dtype == SLAYER_BFLOAT16 && s->channels > 1 ? 2 : 1; }
 // Tokens of a wave, of the eight waves of a workgroup: as many as leave registers for a second workgroup on a compute unit (backward, pairs of
-// bfloat16, sixteen tokens: 54 us where eight take 46).
+// bfloat16, sixteen tokens: [16,1450,1021] 109 us where eight take 51).
 constexpr int tokens_of(int lane, bool backward) { return lane == 2 && backward ? 8 : 16; }
 constexpr int kWaves = 8;
 constexpr int64_t kMostBlocks = (int64_t)1 << 23;                  // of 512 threads: fewer than 2^32 threads in a launch
@@ -566,9 +568,11 @@ Plan plan_of(const slayer_gated_leak* s, bool backward) {
     p.strips = ceil_div(s->channels, 64 * lane);
     p.chains = s->samples * p.strips;
     // A workgroup for each tile where chains are fewer than compute units; with more, walking saves the words and the launch that zeroes
-    // them.  Forward / backward, us, a workgroup for each tile and a walk: [32,512,512] bfloat16, 128 chains, 15 / 29 and 19 / 34; [48,512,512], 192
-    // chains, 22 / 37 and 20 / 36; [64,512,512], 256 chains, 25 / 43 and 24 / 39; float32, 256 chains, 20 / 33 and 20 / 35; ragged samples alike.
-    // Two tiles, [4,200,128] float32: 8.2 / 11.6 and 7.7 / 13.5.
+    // them.  Forward / backward, us, a workgroup for each tile and a walk: [32,512,512] bfloat16, 128 chains, 15 / 27 and 19 / 36; [48,512,512], 192
+    // chains, 22 / 34 and 21 / 38; [64,512,512], 256 chains, 25 / 39 and 22 / 39; 400 chains, 37 / 60 and 31 / 63; float32, 200 chains, 30 / 47 and 28 / 47.
+    // One rule for both directions: between 192 and 300 chains bfloat16 backward passes would gain up to a fifth from the other form (272 chains:
+    // 40 and 50).  Two tiles, [4,200,128] float32: 7.7 / 11.1 and 8.3 / 13.6, but such calls wait for the host, where a launch and an allocation
+    // more cost 4.5 us (11.3 us a call with the walk, 15.8 without).
     p.look = p.tiles > 2 && p.chains < 192 && p.tiles * p.chains < kMostBlocks;
     p.blocks = p.look ? p.tiles * p.chains : p.chains;
     if (p.look) {

@@ -5,8 +5,8 @@
 //   Angles: the whole turns are taken off in float64, with what the roundings of the products leave, so that a far position costs no
 // digits; sine and cosine are those of the rest in float32, turned on by what its rounding leaves.  All heads of a token share them: a
 // workgroup makes those of its tokens once, in LDS.
-//   Bound: memory, each tensor read and written once.  [64,1000,8,64] bfloat16, queries and keys from a projection: 52 us (5.0 TB/s); [16,1450,8,80]
-// float32 with 48 features turned: 42 (5.7 TB/s).  One token of 256 samples, 16 heads of 128: 4.2 us, a launch and two steps that wait for memory.
+//   Bound: memory, each tensor read and written once.  [64,1000,8,64] bfloat16, queries and keys from a projection: 53 us (4.9 TB/s); [16,1450,8,80]
+// float32 with 48 features turned: 42 (5.7 TB/s).  One token of 256 samples, 16 heads of 128: 4.4 us, a launch and two steps that wait for memory.
 #include "common.h"
 #include "elements.h"
 
