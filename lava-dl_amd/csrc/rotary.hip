@@ -3,8 +3,8 @@
 // (c x - s y, c y + s x); the pairs are (i, i + turned / 2) or (2i, 2i + 1), features behind the first `turned` are copied.  The gradient is
 // the same call with the angle's sign changed.
 //   Angles: the whole turns are taken off in float64, with what the roundings of the products leave, so that a far position costs no
-// digits; sine and cosine are those of the rest in float32, turned on by what its rounding leaves.  All heads of a token share them: a
-// workgroup makes those of its tokens once, in LDS.
+// digits; sine and cosine of the rest are made in float64 as well and rounded once.  All heads of a token share them: a workgroup makes those of
+// its tokens once, in LDS.
 //   Bound: memory, each tensor read and written once.  [64,1000,8,64] bfloat16, queries and keys from a projection: 53 us (4.9 TB/s); [16,1450,8,80]
 // float32 with 48 features turned: 42 (5.7 TB/s).  One token of 256 samples, 16 heads of 128: 4.4 us, a launch and two steps that wait for memory.
 #include "common.h"
@@ -70,6 +70,18 @@ __device__ __forceinline__ Place<T> place_of(const RotaryArgs& a, const int64_t 
     return p;
 }
 
+// Cosine and sine of a part of a turn between -1/2 and 1/2: quarters are taken off, and Taylor's series of the angle that is left, at most pi / 4, stop
+// where the next term is below 2^-28 of the sum.  float64 fused multiply-adds run at float32's rate here, so this costs what float32's functions do.
+struct Turn { double cosine, sine; };
+__device__ __forceinline__ Turn turn_of(double rest) {
+    const double quarters = rint(4 * rest), x = (rest - 0.25 * quarters) * 6.283185307179586, z = x * x;
+    const double s = fma(fma(fma(fma(1.0 / 362880, z, -1.0 / 5040), z, 1.0 / 120), z, -1.0 / 6) * z, x, x);
+    const double c = fma(fma(fma(fma(fma(-1.0 / 3628800, z, 1.0 / 40320), z, -1.0 / 720), z, 1.0 / 24), z, -0.5), z, 1.0);
+    const int q = (int)quarters;
+    const double first = q & 1 ? s : c, second = q & 1 ? c : s;
+    return {(q + 1) & 2 ? -first : first, q & 2 ? -second : second};
+}
+
 // Angles of a workgroup's tokens, then its accesses: for each token and head the pairs, W at a time, and what is copied.  The last access of
 // either, where there are W, ends with the last feature and so may do some of the one before it again, with the same values: no access is
 // cut.  The angles are being made while the first features are on their way.
@@ -109,11 +121,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         constexpr double kHigh = 0x1.45f306dc9c883p-3, kLow = -0x1.6b01ec5417056p-57;           // 1 / (2 pi)
         const double radians = a.frequency[i - t * a.pairs], f = radians * kHigh, turns = positions[t] * f;
         const double rest = (turns - rint(turns)) + (fma(positions[t], f, -turns) + positions[t] * fma(radians, kLow, fma(radians, kHigh, -f)));
-        const float near = (float)rest, left = (float)((rest - (double)near) * 6.283185307179586);
-        float s, c;
-        sincospif(2.f * near, &s, &c);
-        cosines[i] = a.magnitude * fmaf(-left, s, c);
-        sines[i] = a.sign * a.magnitude * fmaf(left, c, s);
+        const Turn turn = turn_of(rest);
+        cosines[i] = (float)(a.magnitude * turn.cosine);
+        sines[i] = (float)(a.sign * a.magnitude * turn.sine);
     }
     __syncthreads();
     while (token < count) {

@@ -31,3 +31,21 @@ def test_sines_and_cosines(inverse):
     want = torch.cat([angle.cos(), -angle.sin() if inverse else angle.sin()], -1)
     over = (got - want).abs() - (5 * U * want.abs() + 2.0 ** -45 + 2.0 ** -50)
     assert float(over.max()) <= 0, (float(over.max() / U), float(((got - want) / want / U)[want != 0].abs().max()))
+
+
+def test_rounded_once():
+    """Sine and cosine times the magnitude are float64 and rounded to float32 once, U; the series stop within U / 16 of the sum, the reference's own angle is
+    within 2^-50."""
+    import lava_dl_amd.slayer as slayer
+    gen = torch.Generator().manual_seed(52)
+    frequency = slayer.synapse.rotary_frequencies(64, 500000.0)
+    position = torch.randint(-(1 << 30), 1 << 30, (500,), generator=gen)
+    angle = angles(position, frequency)
+    magnitude = 1.1
+    x = torch.zeros(1, 500, 1, 64)
+    x[..., :32] = 1
+    y, _ = slayer.synapse.rotary(x.to(DEV), None, frequency.to(DEV), position[None].to(DEV), magnitude=magnitude)
+    got = y[0, :, 0].cpu().double()
+    want = float(torch.tensor(magnitude)) * torch.cat([angle.cos(), angle.sin()], -1)
+    over = (got - want).abs() - ((1 + 1 / 16) * U * want.abs() + 2.0 ** -49)
+    assert float(over.max()) <= 0, float(((got - want) / want / U).abs().max())
