@@ -1,8 +1,8 @@
 """The sines and cosines of rotary positions to float32's digits, of small values too.
 
-Tolerance, relative.  U = 2^-24.  Sine and cosine of the angle's nearest float32 are within two units in the last place, 4 U; what that rounding
-leaves of the angle, at most 2 U, is taken in with one rounding more, and terms of second order are 4 U^2 absolute: 5 U and 2^-45, with 2^-50 for the
-reference's own angle in float64."""
+Tolerance, relative.  U = 2^-24.  Functions of the angle in float32 that are right to two units in the last place, 4 U, and take in what the
+angle's rounding leaves, U, have 5 U and 2^-45 for terms of second order, with 2^-50 for the reference's own angle in float64; functions in
+float64 that are rounded once have U."""
 import pytest
 import torch
 
